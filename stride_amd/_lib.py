@@ -1,4 +1,5 @@
-"""ctypes binding of libstride_tc.so (the C ABI declared in include/stride_tc.h).
+"""ctypes binding of libstride_tc.so (the C ABI declared in include/stride_tc.h,
+include/stride_exact.h and include/stride_serve.h).
 
 The Structure classes mirror the reference's POD parameter blocks byte for byte
 (src/kernels.h:23-46, 79-98, 125-128; src/kernels_tc.h:10-77); ``check_layout`` asserts
@@ -193,6 +194,50 @@ EXPORTS = (
 ) + tuple(EXACT_ENTRIES)
 
 
+# Serving operators (include/stride_serve.h).
+class WindowAttentionParams(C.Structure):
+    _fields_ = [("l", Lanes), ("q", C.c_void_p), ("q_stride", C.c_int64), ("out", C.c_void_p), ("kv", KvRef),
+                ("row_slot", C.c_void_p), ("row_pos", C.c_void_p), ("scratch", C.c_void_p), ("scratch_floats", C.c_int64),
+                ("out_cols", C.c_int32), ("max_pages", C.c_int32), ("layer", C.c_int32), ("n_kv", C.c_int32),
+                ("n_q", C.c_int32), ("head_dim", C.c_int32), ("window", C.c_int32), ("sinks", C.c_int32),
+                ("runs", C.c_int32), ("scale", C.c_float)]
+
+
+class KvPoolParams(C.Structure):
+    _fields_ = [("kv", KvRef), ("refs", C.c_void_p), ("free_bits", C.c_void_p), ("errors", C.c_void_p),
+                ("work", C.c_void_p), ("work_ints", C.c_int64), ("pages", C.c_int32), ("slots", C.c_int32),
+                ("layers", C.c_int32), ("n_kv", C.c_int32), ("elem_bytes", C.c_int32)]
+
+
+class LogitsParams(C.Structure):
+    _fields_ = [("l", Lanes), ("logits", C.c_void_p), ("out", C.c_void_p), ("row_slot", C.c_void_p),
+                ("counts", C.c_void_p), ("seen", C.c_void_p), ("penalties", C.c_void_p), ("bias_offsets", C.c_void_p),
+                ("bias_tokens", C.c_void_p), ("bias_values", C.c_void_p), ("mask", C.c_void_p),
+                ("mask_row", C.c_void_p), ("best", C.c_void_p), ("scratch", C.c_void_p), ("vocab", C.c_int32),
+                ("slots", C.c_int32), ("masks", C.c_int32)]
+
+
+class TokenCountsParams(C.Structure):
+    _fields_ = [("counts", C.c_void_p), ("seen", C.c_void_p), ("slots", C.c_int32), ("vocab", C.c_int32)]
+
+
+_VP, _I32, _I64 = C.c_void_p, C.c_int32, C.c_int64
+SERVE_ENTRIES = {  # name -> (result, argument types)
+    "stride_serve_window_attention": (C.c_int, [_VP, _VP]),
+    "stride_serve_window_attention_scratch": (_I64, [_VP]),
+    "stride_kv_work_ints": (_I64, [_I32, _I32, _I32]),
+    "stride_kv_reserve": (C.c_int, [_VP, _VP, _VP, _VP, _I32, _VP]),
+    "stride_kv_release": (C.c_int, [_VP, _VP, _VP, _VP, _I32, _VP]),
+    "stride_kv_fork": (C.c_int, [_VP, _VP, _VP, _VP, _I32, _VP]),
+    "stride_kv_compact": (C.c_int, [_VP, _VP, _VP, _VP, _VP, _I64, _I32, _I32, _VP]),
+    "stride_kv_copy": (C.c_int, [_VP, _VP, _VP, _VP, _VP, _I32, _VP]),
+    "stride_logits_process": (C.c_int, [_VP, _VP]),
+    "stride_logits_scratch": (_I64, [_I32]),
+    "stride_logits_record": (C.c_int, [_VP, _VP, _VP, _I32, _I32, _I32, _VP]),
+    "stride_logits_reset": (C.c_int, [_VP, _VP, _VP, _I32, _VP]),
+}
+
+
 def check_layout() -> None:
     """Sizes and offsets the C++ side static_asserts (reference PODs on x86-64)."""
     assert C.sizeof(GemmMat) == 16
@@ -210,6 +255,10 @@ def check_layout() -> None:
     assert C.sizeof(EmbedParams) == 48 and C.sizeof(NormParams) == 48
     assert QkvParams.kv.offset == 88 and QkvParams.rope.offset == 144 and C.sizeof(QkvParams) == 176
     assert C.sizeof(GemmResidualParams) == 48 and C.sizeof(Mlp13Params) == 64 and C.sizeof(CompactParams) == 56
+    assert WindowAttentionParams.kv.offset == 40 and WindowAttentionParams.out_cols.offset == 128
+    assert C.sizeof(WindowAttentionParams) == 168
+    assert KvPoolParams.refs.offset == 56 and KvPoolParams.pages.offset == 96 and C.sizeof(KvPoolParams) == 120
+    assert LogitsParams.vocab.offset == 120 and C.sizeof(LogitsParams) == 136 and C.sizeof(TokenCountsParams) == 24
     assert LmGreedyParams.best.offset == 48 and C.sizeof(LmGreedyParams) == 56 and C.sizeof(LmFullParams) == 48
 
 
@@ -255,6 +304,9 @@ def load(path: str = LIB_PATH) -> C.CDLL:
         fn = getattr(lib, name)
         fn.argtypes = [C.POINTER(ptype), C.c_int32, vp] if with_j else [C.POINTER(ptype), vp]
         fn.restype = C.c_int
+    for name, (result, args) in SERVE_ENTRIES.items():
+        fn = getattr(lib, name)
+        fn.argtypes, fn.restype = args, result
     lib.stride_tc_set_stream_config.argtypes = [C.c_int32]
     lib.stride_tc_set_stream_config.restype = C.c_int
     lib.stride_tc_stream_config_count.argtypes = []
@@ -292,6 +344,9 @@ def packed() -> C.CDLL:
             fn = getattr(lib, "stride_tc_" + name)
             fn.argtypes = [C.c_char_p] + [C.c_int] * ints + [C.c_void_p]
             fn.restype = C.c_int
+        for name, (result, args) in SERVE_ENTRIES.items():
+            fn = getattr(lib, name)
+            fn.argtypes, fn.restype = [C.c_char_p] + args[1:] if args[0] is _VP else args, result
         _packed = lib
     return _packed
 

@@ -20,7 +20,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_obj")
 SOURCES = [os.path.join(CSRC, f) for f in ("tc_gemm.hip", "tc_gemm_mlp13.hip", "tc_gemm_qkv.hip", "tc_gemm_lm_full.hip",
-                                            "tc_gemm_lm_greedy.hip", "tc_aux.hip", "exact.hip")]
+                                            "tc_gemm_lm_greedy.hip", "tc_aux.hip", "exact.hip", "serve_attn.hip", "serve_kv.hip",
+                                            "serve_logits.hip")]
 # (source, object name, extra flags): the entry points, then each epilogue's
 # configuration table of each kernel family in an object of its own.
 UNITS = [(s, os.path.basename(s) + ".o", []) for s in SOURCES] + [

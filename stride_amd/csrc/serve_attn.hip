@@ -1,0 +1,476 @@
+// Grouped-query attention of new rows over a paged bf16 cache, all positions or the last
+// `window` and the first `sinks` ones (include/stride_serve.h).
+//
+// The order of every sum is fixed by absolute positions, so that a row's bits do not depend
+// on its batch or on the form that computes it. Positions fall into leaves of 256, a leaf
+// into four chunks of 64. With s the scores times log2(e) and exp2 for exp:
+//   in a leaf   a reference r starts at -inf; chunk by chunk r becomes the chunk's maximum
+//               where that exceeds r + 8 (and what is summed so far is scaled by
+//               exp2(old r - r)); p = exp2(s - r), rounded to bf16, enters
+//               acc = sum p V and l = sum p, MFMA chains in ascending order
+//   over leaves R' = max(R, r), G = G exp2(R - R') + acc exp2(r - R'), L alike
+// The slack of 8 keeps p below 2^8 and saves nearly all rescaling: a reference need not be
+// the maximum, only near it. A chunk or leaf that a row does not see changes nothing (p = 0,
+// r as it was), so forms may skip it or not.
+//
+// Roundings to fewer than 32 bits: p to bf16 (2^-9 relative, random over the positions; l
+// sums the rounded ones, so the weights still add up to one) and the result to bf16. The
+// query is scale * log2(e) * q in fp32, split into two bf16 whose sum has 16 bits (2^-16
+// relative): the scores keep nearly fp32 queries' accuracy (bf16 queries alone would add an
+// error of the size of p's) for twice the score products.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cstddef>
+#include <string>
+
+#include "../../include/stride_serve.h"
+#include "tc_common.hpp"
+
+namespace stride_tc {
+
+int fail(int code, const std::string& msg);  // tc_gemm.hip
+
+namespace {
+
+constexpr int kLeaf = 256;
+constexpr int kChunk = 64;
+constexpr float kSlack = 8.0f;
+constexpr float kLog2e = 1.44269504088896341f;
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float neg_inf() { return f32_of(0xFF800000u); }
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// What a row sees: [0, sink_end) and [lo, pos].
+struct Sight {
+  int pos, lo, sink_end;
+  __device__ __forceinline__ bool sees(int t) const { return t <= pos && (t >= lo || t < sink_end); }
+};
+__device__ __forceinline__ Sight sight_of(const StrideWindowAttentionParams& p, int pos, int limit) {
+  Sight s;
+  s.pos = min(pos, limit - 1);
+  s.lo = p.window > 0 ? max(0, s.pos - p.window + 1) : 0;
+  s.sink_end = p.window > 0 ? max(0, min(p.sinks, s.pos + 1)) : 0;
+  return s;
+}
+
+// The leaves that a row sees, ascending: `head` of them from 0, then those from `rest` on.
+struct Leaves {
+  int head, rest, count;
+  __device__ __forceinline__ int at(int i) const { return i < head ? i : rest + i - head; }
+};
+__device__ __forceinline__ Leaves leaves_of(const Sight& s) {
+  Leaves v;
+  v.head = (s.sink_end + kLeaf - 1) / kLeaf;
+  v.rest = max(s.lo / kLeaf, v.head);
+  v.count = s.pos < 0 ? 0 : v.head + max(0, s.pos / kLeaf - v.rest + 1);
+  return v;
+}
+
+// A score row's query as MFMA operand: 8 dims from `q`, times c, as two bf16 that add up to
+// it to 16 bits. Both have its sign and neither is 0 where it is not (2^-24 of it does no
+// harm), so that a key's infinity makes one infinity of the two products.
+__device__ __forceinline__ void split_query(const float* q, float c, bool live, u32x4& hi, u32x4& lo) {
+  f32x4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+  if (live) {
+    a = reinterpret_cast<const f32x4*>(q)[0];
+    b = reinterpret_cast<const f32x4*>(q)[1];
+  }
+  bf16x8 h, l;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float v = (i < 4 ? a[i & 3] : b[i & 3]) * c;
+    const float top = f32_of(u32_of(v) & 0xFFFF0000u);
+    h[i] = static_cast<__bf16>(top);
+    l[i] = static_cast<__bf16>(v == top ? v * 0x1p-24f : v - top);
+  }
+  hi = __builtin_bit_cast(u32x4, h);
+  lo = __builtin_bit_cast(u32x4, l);
+}
+
+// V rows lie in LDS as [position][D] with their 64-byte blocks permuted so that the four
+// rows of a transposing read fall into different banks (four rows of 64 bytes fill them).
+template <int D>
+__device__ __forceinline__ int v_at(int row, int dim) {
+  constexpr int kBlocks = D / 32;  // 64-byte blocks of a row
+  const int turn = kBlocks == 1 ? 0 : (kBlocks == 2 ? (row >> 1) & 1 : row & 3);
+  return row * D + (((dim >> 5) ^ turn) << 5) + (dim & 31);
+}
+// Element (row + r, dim + i) for r = 0 .. 3 in lane i of each 16 lanes, whose lane i must
+// pass (row + i / 4, dim + 4 * (i % 4)).
+__device__ __forceinline__ u32x2 read_transposed(const uint16_t* at) {
+  auto p = (__attribute__((address_space(3))) s16x4*)(at);
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
+}
+__device__ __forceinline__ u32x4 both(u32x2 a, u32x2 b) { return u32x4{a[0], a[1], b[0], b[1]}; }
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  bf16x2 v;
+  v[0] = static_cast<__bf16>(a);
+  v[1] = static_cast<__bf16>(b);
+  return __builtin_bit_cast(uint32_t, v);
+}
+
+constexpr uint32_t kOnes = 0x3F803F80u;  // two bf16 ones
+
+// The fold over leaves for one column: the running reference and sum, and the factors that
+// scale what is there and what comes. A leaf with l = 0 (nothing seen) changes nothing.
+struct Fold {
+  float ref, sum;
+  __device__ __forceinline__ void take(float r, float l, float& a, float& b) {
+    a = 1.0f;
+    b = 0.0f;
+    if (!(l == 0.0f)) {
+      const float m = r > ref ? r : ref;
+      a = exp2_of(ref - m);
+      b = exp2_of(r - m);
+      if (sum == 0.0f) a = 0.0f;  // the first leaf: -inf - -inf where its scores are NaN
+      sum = __builtin_fmaf(l, b, sum * a);
+      ref = m;
+    }
+  }
+};
+// (a, b) as above; NaN sums stay NaN.
+__device__ __forceinline__ f32x4 folded(f32x4 g, f32x4 acc, float a, float b) {
+  f32x4 o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(acc[e], b, g[e] * a);
+  return o;
+}
+
+// Four neighbouring dims of head h of group g, row j, as bf16; + 0 makes one zero of both.
+__device__ __forceinline__ void put_out(const StrideWindowAttentionParams& p, int j, int g, int h, int d, f32x4 acc, float sum) {
+  const int idx = (g * p.n_q + h) * p.head_dim + d;
+  uint16_t* at = p.out + (static_cast<int64_t>(j >> 4) * (p.out_cols >> 4) + (idx >> 4)) * kTileElems + (j & 15) * 16 + (idx & 15);
+  f32x4 v = {0, 0, 0, 0};
+  if (!(sum == 0.0f)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = acc[e] / sum + 0.0f;
+  }
+  *reinterpret_cast<u32x2*>(at) = u32x2{pack2(v[0], v[1]), pack2(v[2], v[3])};
+}
+
+// A split row's leaf record: acc [n_q][D], then (reference, l) per head.
+__device__ __forceinline__ int record_floats(int n_q, int d) { return (n_q * (d + 2) + 3) / 4 * 4; }
+
+// ---------------------------------------------------------------------------
+// Rows one by one: a workgroup has a row and a KV group, its heads are the columns of the
+// matrix products. Wave w scores chunk w of a leaf (keys straight from memory: the 16 x 32
+// operand is 16 rows of 64 bytes), the four maxima give every wave the leaf's references,
+// the weights go through LDS, and each wave sums its quarter of the dims over the leaf. The
+// next leaf's loads are in flight meanwhile.
+// SPLIT: one leaf a workgroup, its record to scratch (few rows, long contexts).
+template <int D, bool SPLIT>
+__global__ __launch_bounds__(256) void k_rows(StrideWindowAttentionParams p, int page_shift, int limit, int span) {
+  constexpr int kKey = D / 32;           // operands of a key row
+  constexpr int kRow = D / 8;            // 16-byte pieces of a row
+  constexpr int kPer = kChunk * kRow / 64;
+  constexpr int kOut = (D + 63) / 64;    // 16-dim blocks of a wave
+  __shared__ __align__(16) uint16_t vs[kLeaf * D];
+  __shared__ __align__(16) u32x4 weights[kLeaf / 32][64];
+  __shared__ float maxima[4][16];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
+  const int g = blockIdx.x % p.n_kv;
+  const int unit = blockIdx.x / p.n_kv;
+  const int j = SPLIT ? unit / span : unit;
+  const int slot = p.row_slot[j];
+  const Sight sight = sight_of(p, p.row_pos[j], limit);
+  const Leaves leaves = leaves_of(sight);
+  const int begin = SPLIT ? unit % span : 0, end = SPLIT ? begin + 1 : leaves.count;
+  if (SPLIT && begin >= leaves.count) return;
+
+  const uint16_t* base = static_cast<const uint16_t*>(p.kv.arena) + p.layer * p.kv.layer_elems + g * p.kv.group_elems;
+  const int32_t* table = p.kv.table + static_cast<int64_t>(slot) * p.kv.max_blocks;
+  const int in_page = (1 << page_shift) - 1;
+
+  u32x4 kr[4][kKey], vr[kPer];
+  int block;        // of position 64 * wave + lane of the leaf; below 0: not seen, or not held
+  uint64_t seen;    // bit i: position 64 * wave + i is seen
+  auto look = [&](int leaf) {
+    const int t = leaf * kLeaf + wave * kChunk + lane;
+    const bool s = sight.sees(t);
+    block = s ? table[t >> page_shift] : -1;
+    seen = __ballot(s);
+  };
+  const u32x4 zero = {0, 0, 0, 0};
+  auto fetch_k = [&](int leaf) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int i = 16 * t + col, b = __shfl(block, i);
+      const uint16_t* at = base + max(b, 0) * p.kv.block_elems + ((leaf * kLeaf + wave * kChunk + i) & in_page) * D + 8 * quarter;
+#pragma unroll
+      for (int k = 0; k < kKey; ++k) {
+        kr[t][k] = load16(at + 32 * k);
+        if (b < 0) kr[t][k] = zero;
+      }
+    }
+  };
+  auto fetch_v = [&](int leaf) {
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const int piece = u * 64 + lane, i = piece / kRow, b = __shfl(block, i);
+      vr[u] = ld_kv(base + p.kv.which_elems + max(b, 0) * p.kv.block_elems +
+                    ((leaf * kLeaf + wave * kChunk + i) & in_page) * D + (piece % kRow) * 8);
+      if (b < 0) vr[u] = zero;
+    }
+  };
+
+  u32x4 qh[kKey], ql[kKey];
+  {
+    const float* q = p.q + j * p.q_stride + (static_cast<int64_t>(g) * p.n_q + col) * D + 8 * quarter;
+#pragma unroll
+    for (int k = 0; k < kKey; ++k) split_query(q + 32 * k, p.scale * kLog2e, col < p.n_q, qh[k], ql[k]);
+  }
+
+  f32x4 total[kOut];
+#pragma unroll
+  for (int b = 0; b < kOut; ++b) total[b] = f32x4{0, 0, 0, 0};
+  Fold fold = {neg_inf(), 0.0f};
+
+  if (begin < end) {
+    look(leaves.at(begin));
+    fetch_k(leaves.at(begin));
+    fetch_v(leaves.at(begin));
+  }
+  for (int it = begin; it < end; ++it) {
+    f32x4 s[4];
+    float most = neg_inf();
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      s[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int k = 0; k < kKey; ++k) {
+        s[t] = mfma(kr[t][k], qh[k], s[t]);
+        s[t] = mfma(kr[t][k], ql[k], s[t]);
+      }
+    }
+    const uint64_t mine = seen;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (!((mine >> (16 * t + 4 * quarter + e)) & 1)) s[t][e] = neg_inf();
+        most = fmaxf(most, s[t][e]);
+      }
+    most = fmaxf(most, __shfl_xor(most, 16));
+    most = fmaxf(most, __shfl_xor(most, 32));
+    if (lane < 16) maxima[wave][lane] = most;
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const int piece = u * 64 + lane;
+      *reinterpret_cast<u32x4*>(vs + v_at<D>(wave * kChunk + piece / kRow, (piece % kRow) * 8)) = vr[u];
+    }
+    if (!SPLIT && it + 1 < end) look(leaves.at(it + 1));
+    lds_barrier();
+    if (!SPLIT && it + 1 < end) {
+      fetch_k(leaves.at(it + 1));
+      fetch_v(leaves.at(it + 1));
+    }
+    // the leaf's references, the same in every wave
+    float ref = neg_inf(), own_ref = neg_inf(), alpha[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float m = maxima[c][col];
+      alpha[c] = 1.0f;
+      if (m > ref + kSlack) {
+        alpha[c] = exp2_of(ref - m);
+        ref = m;
+      }
+      if (c == wave) own_ref = ref;
+    }
+    const float at = own_ref == neg_inf() ? 0.0f : own_ref;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      u32x4 w;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const f32x4 v = s[2 * half + x];
+        w[2 * x] = pack2(exp2_of(v[0] - at), exp2_of(v[1] - at));
+        w[2 * x + 1] = pack2(exp2_of(v[2] - at), exp2_of(v[3] - at));
+      }
+      weights[2 * wave + half][lane] = w;
+    }
+    lds_barrier();
+    f32x4 acc[kOut], l = {0, 0, 0, 0};
+#pragma unroll
+    for (int b = 0; b < kOut; ++b) acc[b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        l[e] *= alpha[c];
+#pragma unroll
+        for (int b = 0; b < kOut; ++b) acc[b][e] *= alpha[c];
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const u32x4 w = weights[2 * c + half][lane];
+        const int row = c * kChunk + 32 * half + 4 * quarter + (col >> 2);
+        l = mfma(u32x4{kOnes, kOnes, kOnes, kOnes}, w, l);
+#pragma unroll
+        for (int b = 0; b < kOut; ++b) {
+          const int dim = (wave * kOut + b) * 16;
+          if (dim < D)
+            acc[b] = mfma(both(read_transposed(vs + v_at<D>(row, dim + 4 * (col & 3))),
+                               read_transposed(vs + v_at<D>(row + 16, dim + 4 * (col & 3)))),
+                          w, acc[b]);
+        }
+      }
+    }
+    if constexpr (SPLIT) {
+      if (col < p.n_q) {
+        float* rec = p.scratch + ((static_cast<int64_t>(j) * p.n_kv + g) * span + it) * record_floats(p.n_q, D);
+#pragma unroll
+        for (int b = 0; b < kOut; ++b) {
+          const int dim = (wave * kOut + b) * 16 + 4 * quarter;
+          if (dim < D) *reinterpret_cast<f32x4*>(rec + col * D + dim) = acc[b];
+        }
+        if (threadIdx.x < 16) *reinterpret_cast<f32x2*>(rec + p.n_q * D + 2 * col) = f32x2{ref, l[0]};
+      }
+      return;
+    }
+    float a, b;
+    fold.take(ref, l[0], a, b);
+#pragma unroll
+    for (int x = 0; x < kOut; ++x) total[x] = folded(total[x], acc[x], a, b);
+    lds_barrier();  // the staging is written again
+  }
+  if (!SPLIT && col < p.n_q) {
+#pragma unroll
+    for (int b = 0; b < kOut; ++b) {
+      const int dim = (wave * kOut + b) * 16 + 4 * quarter;
+      if (dim < D) put_out(p, j, g, col, dim, total[b], fold.sum);
+    }
+  }
+}
+
+// Joins a split row's records in ascending order. A thread has four dims of a head.
+template <int D>
+__global__ __launch_bounds__(256) void k_join(StrideWindowAttentionParams p, int limit, int span) {
+  const int g = blockIdx.x % p.n_kv, j = blockIdx.x / p.n_kv;
+  const int count = leaves_of(sight_of(p, p.row_pos[j], limit)).count;
+  const int rf = record_floats(p.n_q, D);
+  const float* recs = p.scratch + (static_cast<int64_t>(j) * p.n_kv + g) * span * rf;
+  for (int u = threadIdx.x; u < p.n_q * (D / 4); u += 256) {
+    const int h = u / (D / 4), d = u % (D / 4) * 4;
+    f32x4 total = {0, 0, 0, 0};
+    Fold fold = {neg_inf(), 0.0f};
+    for (int i0 = 0; i0 < count; i0 += 8) {
+      f32x4 acc[8];
+      f32x2 rl[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float* rec = recs + min(i0 + i, count - 1) * rf;
+        acc[i] = *reinterpret_cast<const f32x4*>(rec + h * D + d);
+        rl[i] = *reinterpret_cast<const f32x2*>(rec + p.n_q * D + 2 * h);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i0 + i >= count) break;
+        float a, b;
+        fold.take(rl[i][0], rl[i][1], a, b);
+        total = folded(total, acc[i], a, b);
+      }
+    }
+    put_out(p, j, g, h, d, total, fold.sum);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+
+struct Plan {
+  int page_shift, limit, span;
+  bool split;
+  int64_t scratch;
+};
+
+const char* plan_of(const StrideWindowAttentionParams& p, Plan& plan) {
+  const int D = p.head_dim;
+  if (p.l.rows < 0 || p.l.lane_groups != (static_cast<int64_t>(p.l.rows) + 15) / 16) return "need rows >= 0 and lane_groups = ceil(rows/16)";
+  if ((D != 32 && D != 64 && D != 128) || p.kv.head_dim != D) return "head_dim must be 32, 64 or 128 and match kv.head_dim";
+  if (p.n_q < 1 || p.n_q > 16) return "1 to 16 query heads per KV head";
+  if (p.n_kv < 1 || p.layer < 0 || p.max_pages < 1 || p.sinks < 0 || p.runs < 0 || p.kv.max_blocks < 1)
+    return "bad n_kv, layer, max_pages, sinks, runs or max_blocks";
+  const int64_t tokens = p.kv.group_elems > 0 && p.kv.group_elems % D == 0 ? p.kv.group_elems / D : 0;
+  if (tokens < 8 || (tokens & (tokens - 1)) || tokens > (int64_t{1} << 30)) return "the KV page (group_elems / head_dim) must be a power of two from 8 up";
+  if (p.kv.block_elems % 8 || p.kv.layer_elems % 8 || p.kv.which_elems % 8) return "KV strides must be multiples of 8 elements";
+  const int64_t heads = static_cast<int64_t>(p.n_kv) * p.n_q * D;
+  if (heads > INT_MAX || p.out_cols % 16 || p.out_cols < heads) return "out_cols must be a multiple of 16 covering every head";
+  if (p.l.rows > 1 && (p.q_stride % 4 || p.q_stride < heads)) return "q_stride must be a multiple of 4 covering every head";
+  plan.page_shift = 0;
+  while ((int64_t{1} << plan.page_shift) < tokens) ++plan.page_shift;
+  plan.limit = static_cast<int>(std::min<int64_t>(std::min<int64_t>(int64_t{64} * p.max_pages, tokens * p.kv.max_blocks), INT_MAX - kLeaf));
+  // leaves that a row can see
+  int64_t span = (static_cast<int64_t>(plan.limit) + kLeaf - 1) / kLeaf;
+  if (p.window > 0) {
+    const int64_t head = (std::min<int64_t>(p.sinks, plan.limit) + kLeaf - 1) / kLeaf, rest = (static_cast<int64_t>(p.window) + kLeaf - 2) / kLeaf + 1;
+    span = std::min(span, head + rest);
+  }
+  plan.span = static_cast<int>(span);
+  const int64_t units = static_cast<int64_t>(p.l.rows) * p.n_kv;
+  if (units * span > INT_MAX) return "rows, n_kv and the context are too large together";
+  plan.split = span > 1 && units < 512;
+  plan.scratch = plan.split ? units * span * ((p.n_q * (D + 2) + 3) / 4 * 4) : 0;
+  return nullptr;
+}
+
+int launched(const char* what) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(static_cast<int>(e), std::string(what) + " launch failed: " + hipGetErrorString(e));
+  return 0;
+}
+
+template <int D>
+int run(const StrideWindowAttentionParams& p, const Plan& plan, hipStream_t st) {
+  const int units = p.l.rows * p.n_kv;
+  if (plan.split) {
+    hipLaunchKernelGGL((k_rows<D, true>), dim3(units * plan.span), dim3(256), 0, st, p, plan.page_shift, plan.limit, plan.span);
+    if (int rc = launched("window_attention (leaves)")) return rc;
+    hipLaunchKernelGGL((k_join<D>), dim3(units), dim3(256), 0, st, p, plan.limit, plan.span);
+    return launched("window_attention (join)");
+  }
+  hipLaunchKernelGGL((k_rows<D, false>), dim3(units), dim3(256), 0, st, p, plan.page_shift, plan.limit, plan.span);
+  return launched("window_attention");
+}
+
+}  // namespace
+}  // namespace stride_tc
+
+using namespace stride_tc;
+
+static_assert(offsetof(StrideWindowAttentionParams, kv) == 40 && offsetof(StrideWindowAttentionParams, out_cols) == 128 &&
+                  sizeof(StrideWindowAttentionParams) == 168,
+              "WindowAttentionParams layout");
+
+extern "C" {
+
+int64_t stride_serve_window_attention_scratch(const StrideWindowAttentionParams* p) {
+  Plan plan;
+  if (!p || plan_of(*p, plan)) return -1;
+  return plan.scratch;
+}
+
+int stride_serve_window_attention(const StrideWindowAttentionParams* p, void* stream) {
+  if (!p) return fail(STRIDE_TC_EINVAL, "window_attention: null parameters");
+  Plan plan;
+  if (const char* why = plan_of(*p, plan)) return fail(STRIDE_TC_EINVAL, std::string("window_attention: ") + why);
+  if (p->l.rows == 0) return 0;
+  if (!p->q || !p->out || !p->kv.arena || !p->kv.table || !p->row_slot || !p->row_pos)
+    return fail(STRIDE_TC_EINVAL, "window_attention: missing pointer");
+  if ((reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->kv.arena) | reinterpret_cast<uintptr_t>(p->scratch)) % 16 ||
+      reinterpret_cast<uintptr_t>(p->out) % 8)
+    return fail(STRIDE_TC_EINVAL, "window_attention: q, the arena and scratch must be 16-byte aligned, out 8");
+  if (plan.scratch > 0 && (!p->scratch || p->scratch_floats < plan.scratch))
+    return fail(STRIDE_TC_EINVAL, "window_attention: scratch is smaller than stride_serve_window_attention_scratch()");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (p->head_dim == 32) return run<32>(*p, plan, st);
+  if (p->head_dim == 64) return run<64>(*p, plan, st);
+  return run<128>(*p, plan, st);
+}
+
+}  // extern "C"

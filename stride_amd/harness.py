@@ -26,6 +26,7 @@ _ATTENTION = Struct("<4iQi4xQi4x56s3Qi4xQ6if4x").pack
 _RESIDUAL = _LM_FULL = Struct("<4iQQ2iQ").pack
 _MLP13 = Struct("<4iQQ2iQ2iQ").pack
 _LM_GREEDY = Struct("<4iQQ2ii4xQ").pack
+_WINDOW_ATTENTION = Struct("<4iQqQ56sQQQq9if").pack
 
 
 def _check(rc: int) -> None:
@@ -130,6 +131,23 @@ class PagedKv:
         arena = torch.zeros(nblocks * block, dtype=U16, device=device)
         ref = KvRef(ptr(arena), ptr(table), block, layer, which, group, max_blocks, head_dim)
         return PagedKv(arena, table, ref, page_tokens, max_blocks)
+
+    @staticmethod
+    def over(arena, table, kv_heads: int, head_dim: int, layers: int, page_tokens: int) -> "PagedKv":
+        """An arena (int16 bits, any shape, contiguous) and table [slots][max_blocks] int32 that
+        exist already."""
+        if arena.dtype != U16 or table.dtype != torch.int32 or table.dim() != 2:
+            raise ValueError("the arena holds int16 bits, the table int32 [slots][max_blocks]")
+        if not (arena.is_contiguous() and table.is_contiguous()) or arena.device != table.device:
+            raise ValueError("arena and table must be contiguous and on one device")
+        group = page_tokens * head_dim
+        which = group * kv_heads
+        layer = which * 2
+        block = layer * layers
+        if block <= 0 or arena.numel() % block:
+            raise ValueError("the arena is not a whole number of pages")
+        ref = KvRef(ptr(arena), ptr(table), block, layer, which, group, int(table.shape[1]), head_dim)
+        return PagedKv(arena, table, ref, page_tokens, int(table.shape[1]))
 
     @property
     def slots(self) -> int:
@@ -278,3 +296,70 @@ def qkv(wq_tiles, wk_tiles, wv_tiles, x_tiles, rows: int, head_dim: int, rope, r
              layer, head_dim)
     _check(_lib.packed().stride_tc_qkv(p, tc.kernel_stream()))
     return q_out
+
+
+def here(t) -> None:
+    """Refuses tensors of another device than the current one, where the launch would go."""
+    if t.get_device() != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors are on {t.device}, the current device is {torch._C._cuda_getDevice()}")
+
+
+def window_attention_scratch(rows: int, n_kv: int, n_q: int, head_dim: int, window: int, sinks: int, max_pages: int,
+                             device):
+    """The scratch that window_attention wants for calls of these sizes (None: none). It may
+    be larger than a call's; its contents need no preparation."""
+    p = _lib.WindowAttentionParams()
+    p.l = lanes(rows)
+    p.q_stride = p.out_cols = n_kv * n_q * head_dim
+    p.max_pages, p.n_kv, p.n_q, p.head_dim, p.window, p.sinks = max_pages, n_kv, n_q, head_dim, window, sinks
+    p.kv.head_dim, p.kv.group_elems, p.kv.max_blocks = head_dim, 64 * head_dim, max_pages
+    import ctypes
+
+    n = _lib.load().stride_serve_window_attention_scratch(ctypes.byref(p))
+    if n < 0:
+        raise ValueError("window_attention does not serve these sizes")
+    return torch.empty(n, dtype=torch.float32, device=device) if n else None
+
+
+def window_attention(q, kv: PagedKv, row_slot, row_pos, n_kv: int, n_q: int, head_dim: int, scale: float, window: int = 0,
+                     sinks: int = 0, layer: int = 0, max_pages: int | None = None, out_tiles=None, scratch=None,
+                     runs: int = 0):
+    """Attention of rows (row_slot, row_pos) over the paged cache: every position up to the
+    row's own (window 0), or the last `window` and the first `sinks` ones. q: [rows][n_kv *
+    n_q * head_dim] fp32 (rows may be strided). A row with row_pos < 0 gets zeros. max_pages:
+    no row lies behind position 64 * max_pages - 1 (default: the slots' capacity). runs: a
+    hint, how many neighbouring rows are of one sequence at most (1: decode; 0: not known).
+    scratch: window_attention_scratch() (default: allocated here, on torch's current stream).
+    Returns bf16 x tiles."""
+    rows, cols = int(q.shape[0]), n_kv * n_q * head_dim
+    here(q)
+    if q.dtype != torch.float32 or q.dim() != 2 or q.shape[1] != cols or (cols > 1 and q.stride(1) != 1):
+        raise ValueError("q must be fp32 [rows][n_kv * n_q * head_dim], its rows contiguous")
+    if row_slot.dtype != torch.int32 or row_pos.dtype != torch.int32 or row_slot.numel() < rows or row_pos.numel() < rows:
+        raise ValueError("row_slot and row_pos must be int32, one for each row")
+    if not (row_slot.is_contiguous() and row_pos.is_contiguous()):
+        raise ValueError("row_slot and row_pos must be contiguous")
+    if not 0 <= layer < kv.ref.block_elems // kv.ref.layer_elems or kv.ref.which_elems != n_kv * kv.ref.group_elems:
+        raise ValueError("layer or n_kv is not the cache's")
+    T = (rows + 15) // 16
+    if out_tiles is None:
+        out_tiles = torch.zeros((T, cols // 16, 16, 16), dtype=U16, device=q.device)
+    elif (out_tiles.dtype != U16 and out_tiles.dtype != torch.bfloat16) or not out_tiles.is_contiguous() \
+            or out_tiles.numel() < T * 16 * cols or (out_tiles.dim() == 4 and out_tiles.shape[1] * 16 != cols):
+        raise ValueError("out_tiles must be contiguous 16-bit x tiles of n_kv * n_q * head_dim columns")
+    if max_pages is None:
+        max_pages = (kv.capacity + 63) // 64
+    if scratch is None:
+        if tc._stream is not None:
+            raise ValueError("with a stream set by set_kernel_stream, pass scratch (window_attention_scratch)")
+        scratch = window_attention_scratch(rows, n_kv, n_q, head_dim, window, sinks, max_pages, q.device)
+    floats = 0
+    if scratch is not None:
+        if scratch.dtype != torch.float32 or not scratch.is_contiguous():
+            raise ValueError("scratch must be contiguous fp32")
+        floats = scratch.numel()
+    p = _WINDOW_ATTENTION(rows, T, 0, 0, _ptr(q), q.stride(0) if rows > 1 else cols, _ptr(out_tiles), bytes(kv.ref),
+                          _ptr(row_slot), _ptr(row_pos), _ptr(scratch), floats, cols, max_pages, layer, n_kv, n_q,
+                          head_dim, window, sinks, runs, scale)
+    _check(_lib.packed().stride_serve_window_attention(p, tc.kernel_stream()))
+    return out_tiles
