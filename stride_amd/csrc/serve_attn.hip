@@ -165,7 +165,7 @@ __device__ __forceinline__ int record_floats(int n_q, int d) { return (n_q * (d 
 // next leaf's loads are in flight meanwhile.
 // SPLIT: one leaf a workgroup, its record to scratch (few rows, long contexts).
 template <int D, bool SPLIT>
-__global__ __launch_bounds__(256) void k_rows(StrideWindowAttentionParams p, int page_shift, int limit, int span) {
+__device__ __forceinline__ void one_row(const StrideWindowAttentionParams& p, int page_shift, int limit, int span, int g, int j, int begin) {
   constexpr int kKey = D / 32;           // operands of a key row
   constexpr int kRow = D / 8;            // 16-byte pieces of a row
   constexpr int kPer = kChunk * kRow / 64;
@@ -174,13 +174,10 @@ __global__ __launch_bounds__(256) void k_rows(StrideWindowAttentionParams p, int
   __shared__ __align__(16) u32x4 weights[kLeaf / 32][64];
   __shared__ float maxima[4][16];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
-  const int g = blockIdx.x % p.n_kv;
-  const int unit = blockIdx.x / p.n_kv;
-  const int j = SPLIT ? unit / span : unit;
   const int slot = p.row_slot[j];
   const Sight sight = sight_of(p, p.row_pos[j], limit);
   const Leaves leaves = leaves_of(sight);
-  const int begin = SPLIT ? unit % span : 0, end = SPLIT ? begin + 1 : leaves.count;
+  const int end = SPLIT ? begin + 1 : leaves.count;
   if (SPLIT && begin >= leaves.count) return;
 
   const uint16_t* base = static_cast<const uint16_t*>(p.kv.arena) + p.layer * p.kv.layer_elems + g * p.kv.group_elems;
@@ -348,6 +345,293 @@ __global__ __launch_bounds__(256) void k_rows(StrideWindowAttentionParams p, int
   }
 }
 
+template <int D>
+__global__ __launch_bounds__(256) void k_leaves(StrideWindowAttentionParams p, int page_shift, int limit, int span) {
+  const int unit = blockIdx.x / p.n_kv;
+  one_row<D, true>(p, page_shift, limit, span, blockIdx.x % p.n_kv, unit / span, unit % span);
+}
+
+// `per` rows one after the other; those of tiles that k_tile has done (done: its marks, or
+// NULL) are skipped.
+template <int D>
+__global__ __launch_bounds__(256) void k_rows(StrideWindowAttentionParams p, int page_shift, int limit, int per, const int32_t* done,
+                                              int tile_rows) {
+  const int g = blockIdx.x % p.n_kv, j0 = blockIdx.x / p.n_kv * per;
+  for (int j = j0; j < min(j0 + per, p.l.rows); ++j) {
+    if (done && done[j / tile_rows * p.n_kv + g]) continue;
+    one_row<D, false>(p, page_shift, limit, 0, g, j, 0);
+    if (per > 1) lds_barrier();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Prompts: a workgroup has a tile of 128 score columns, (row, head) pairs of neighbouring
+// rows, and a KV group, so that a chunk of keys and values is fetched once for all of them.
+// Four waves of 32 columns each, v_mfma_f32_32x32x16_bf16 (two give the bits of one
+// 16x16x32, k halves in order), the transposed product first: S^T = K Q^T leaves a column's
+// scores in a lane pair, so that references, weights and sums are lane-local, and S^T's
+// registers are P^T's operand as they are, with the value rows taken in the same order.
+//
+// A chunk goes through LDS, the next one's loads in flight meanwhile. Key rows have their
+// 16-byte pieces permuted by the row, so that the 32 rows of an operand read spread over the
+// banks; value rows as v_at has them.
+//
+// Rows of several sequences meet in a tile where prompts end: the tile goes through the
+// sequences one after the other, each column taking part in its own. A tile of many short
+// runs is left to k_rows, and so is one with a value that is not finite in a chunk that some
+// of its columns must not see (0 times it is NaN). done[tile * n_kv + g]: whether it was done.
+template <int D>
+__device__ __forceinline__ int k_at(int row, int piece) {
+  constexpr int kPieces = D / 8;
+  return row * D + ((piece ^ ((row * D / 128) & (kPieces - 1))) << 3);
+}
+__device__ __forceinline__ bool has_nonfinite(u32x4 v) {
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) bad |= (v[e] & 0x7F80u) == 0x7F80u || (v[e] & 0x7F800000u) == 0x7F800000u;
+  return bad;
+}
+
+constexpr int kColumns = 128;
+
+template <int D>
+__global__ __launch_bounds__(256, D == 128 ? 1 : 2) void k_tile(StrideWindowAttentionParams p, int page_shift, int limit, int tile_rows, int32_t* done) {
+  constexpr int kRow = D / 8;              // 16-byte pieces of a row
+  constexpr int kPer = kChunk * kRow / 256;  // pieces of K (and of V) a thread moves
+  constexpr int kDims = D / 32;
+  __shared__ __align__(16) uint16_t ks[2][kChunk * D];
+  __shared__ __align__(16) uint16_t vs[2][kChunk * D];
+  __shared__ int slots[kColumns], poss[kColumns];
+  __shared__ uint64_t starts[2];  // bit i: row i begins a run
+  __shared__ int bad[2][4];
+  const int t = threadIdx.x, wave = t >> 6, lane = t & 63, c32 = lane & 31, half = lane >> 5;
+  const int g = blockIdx.x % p.n_kv;
+  const int tiles = gridDim.x / p.n_kv, tile = tiles - 1 - blockIdx.x / p.n_kv;  // later rows see more: first
+  const int j0 = tile * tile_rows, nr = min(tile_rows, p.l.rows - j0);
+  int32_t* mark = done + tile * p.n_kv + g;
+
+  if (t < kColumns) {
+    const int j = j0 + min(t, nr - 1);
+    const int slot = p.row_slot[j], pos = t < nr ? min(p.row_pos[j], limit - 1) : -1;
+    slots[t] = slot;
+    poss[t] = pos;
+  }
+  __syncthreads();
+  if (t < kColumns) {
+    const uint64_t b = __ballot(t < nr && (t == 0 || slots[t] != slots[t - 1]));
+    if (lane == 0) starts[wave] = b;
+  }
+  __syncthreads();
+  const uint64_t first = starts[0], second = starts[1];
+  const int runs = __popcll(first) + __popcll(second);
+  if (nr < 4 * runs) {
+    if (t == 0) *mark = 0;
+    return;
+  }
+
+  // this lane's column
+  const int col = wave * 32 + c32, row = col / p.n_q, head = col - row * p.n_q;
+  const bool live = row < nr;
+  const int my_pos = live ? poss[row] : -1;
+  const Sight sight = sight_of(p, my_pos, limit);
+  u32x4 qh[D / 16], ql[D / 16];
+  {
+    const float* q = p.q + (j0 + (live ? row : 0)) * p.q_stride + (static_cast<int64_t>(g) * p.n_q + head) * D + 8 * half;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) split_query(q + 16 * k, p.scale * kLog2e, live, qh[k], ql[k]);
+  }
+
+  const uint16_t* base = static_cast<const uint16_t*>(p.kv.arena) + p.layer * p.kv.layer_elems + g * p.kv.group_elems;
+  const int in_page = (1 << page_shift) - 1;
+  f32x16 total[kDims];
+#pragma unroll
+  for (int d = 0; d < kDims; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) total[d][i] = 0.0f;
+  Fold fold = {neg_inf(), 0.0f};
+
+  int buf = 0;
+  for (int r0 = 0; r0 < nr;) {
+    // the run [r0, r1): its sequence, and what its rows see together
+    int r1 = nr;
+    {
+      const uint64_t lo = r0 < 63 ? first & (~uint64_t{0} << (r0 + 1)) : 0;
+      const uint64_t hi = r0 < 63 ? second : (r0 < 127 ? second & (~uint64_t{0} << (r0 + 1 - 64)) : 0);
+      if (lo) r1 = __builtin_ctzll(lo);
+      else if (hi) r1 = 64 + __builtin_ctzll(hi);
+    }
+    int low = INT_MAX, high = -1;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int r = lane + 64 * x, pos = poss[r];
+      if (r >= r0 && r < r1 && pos >= 0) {
+        low = min(low, pos);
+        high = max(high, pos);
+      }
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      low = min(low, __shfl_xor(low, d));
+      high = max(high, __shfl_xor(high, d));
+    }
+    low = __builtin_amdgcn_readfirstlane(low);
+    high = __builtin_amdgcn_readfirstlane(high);
+    const bool mine = row >= r0 && row < r1;
+    const int slot = __builtin_amdgcn_readfirstlane(slots[r0]);
+    const bool whole = r0 == 0 && r1 == nr;
+    r0 = r1;
+    if (high < 0) continue;
+    const Sight near = sight_of(p, low, limit), far = sight_of(p, high, limit);
+    // chunks: [0, head) and [rest, last]
+    const int head_chunks = (far.sink_end + kChunk - 1) / kChunk, rest = max(near.lo / kChunk, head_chunks);
+    const int chunks = head_chunks + max(0, high / kChunk - rest + 1);
+    const int32_t* table = p.kv.table + static_cast<int64_t>(slot) * p.kv.max_blocks;
+    auto chunk_at = [&](int i) { return i < head_chunks ? i : rest + i - head_chunks; };
+
+    int block[kPer];
+    u32x4 kr[kPer], vr[kPer];
+    const u32x4 zero = {0, 0, 0, 0};
+    auto look = [&](int i) {
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) {
+        const int pos = chunk_at(i) * kChunk + (t + 256 * u) / kRow;
+        const bool s = pos <= high && (pos >= near.lo || pos < far.sink_end);
+        block[u] = s ? table[pos >> page_shift] : -1;
+      }
+    };
+    auto fetch = [&](int i) {
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) {
+        const int piece = t + 256 * u, pos = chunk_at(i) * kChunk + piece / kRow, b = block[u];
+        const uint16_t* at = base + max(b, 0) * p.kv.block_elems + (pos & in_page) * D + piece % kRow * 8;
+        kr[u] = load16(at);
+        vr[u] = load16(at + p.kv.which_elems);
+        if (b < 0) kr[u] = vr[u] = zero;
+      }
+    };
+
+    f32x16 acc[kDims], l;
+    float ref = neg_inf();
+    auto fresh = [&]() {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        l[i] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) acc[d][i] = 0.0f;
+      }
+      ref = neg_inf();
+    };
+    fresh();
+    look(0);
+    fetch(0);
+    if (chunks > 1) look(1);
+    for (int i = 0; i < chunks; ++i) {
+      const int a = chunk_at(i) * kChunk;
+      // do all columns see all of it?
+      const bool full = whole && a + kChunk - 1 <= low && (a >= far.lo || a + kChunk <= near.sink_end);
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) {
+        const int piece = t + 256 * u;
+        *reinterpret_cast<u32x4*>(&ks[buf][k_at<D>(piece / kRow, piece % kRow)]) = kr[u];
+        *reinterpret_cast<u32x4*>(&vs[buf][v_at<D>(piece / kRow, piece % kRow * 8)]) = vr[u];
+      }
+      if (!full) {
+        bool b = false;
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) b |= has_nonfinite(vr[u]);
+        const bool any = __any(b);
+        if (lane == 0) bad[buf][wave] = any;
+      }
+      lds_barrier();
+      if (!full && (bad[buf][0] | bad[buf][1] | bad[buf][2] | bad[buf][3])) {
+        if (t == 0) *mark = 0;
+        return;
+      }
+      if (i + 1 < chunks) {
+        fetch(i + 1);
+        if (i + 2 < chunks) look(i + 2);
+      }
+      f32x16 s[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) {
+          const u32x4 k0 = *reinterpret_cast<const u32x4*>(&ks[buf][k_at<D>(32 * b + c32, 4 * k + half)]);
+          const u32x4 k1 = *reinterpret_cast<const u32x4*>(&ks[buf][k_at<D>(32 * b + c32, 4 * k + 2 + half)]);
+          s[b] = mfma32(k0, qh[2 * k], s[b]);
+          s[b] = mfma32(k1, qh[2 * k + 1], s[b]);
+          s[b] = mfma32(k0, ql[2 * k], s[b]);
+          s[b] = mfma32(k1, ql[2 * k + 1], s[b]);
+        }
+      }
+      if (!full) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (!(mine && sight.sees(a + 32 * b + 8 * (e / 4) + 4 * half + e % 4))) s[b][e] = neg_inf();
+      }
+      float most = s[0][0];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) most = fmaxf(most, s[b][e]);
+      most = fmaxf(most, __shfl_xor(most, 32));
+      if (__any(most > ref + kSlack)) {
+        const bool up = most > ref + kSlack;
+        const float alpha = up ? exp2_of(ref - most) : 1.0f;
+        if (up) ref = most;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          l[e] *= alpha;
+#pragma unroll
+          for (int d = 0; d < kDims; ++d) acc[d][e] *= alpha;
+        }
+      }
+      const float at = ref == neg_inf() ? 0.0f : ref;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        uint32_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = pack2(exp2_of(s[b][2 * e] - at), exp2_of(s[b][2 * e + 1] - at));
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const u32x4 pw = {w[2 * x], w[2 * x + 1], w[2 * x + 4], w[2 * x + 5]};
+          l = mfma32(u32x4{kOnes, kOnes, kOnes, kOnes}, pw, l);
+          const int r = 32 * b + 8 * x + 4 * half + ((lane & 15) >> 2);
+#pragma unroll
+          for (int d = 0; d < kDims; ++d) {
+            const int dim = 32 * d + (lane & 16) + 4 * (lane & 3);
+            acc[d] = mfma32(both(read_transposed(&vs[buf][v_at<D>(r, dim)]), read_transposed(&vs[buf][v_at<D>(r + 16, dim)])), pw, acc[d]);
+          }
+        }
+      }
+      buf ^= 1;
+      if (i + 1 == chunks || chunk_at(i + 1) / (kLeaf / kChunk) != a / kLeaf) {
+        float fa, fb;
+        fold.take(ref, l[0], fa, fb);
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) total[d][e] = __builtin_fmaf(acc[d][e], fb, total[d][e] * fa);
+        fresh();
+      }
+    }
+  }
+  if (live) {
+    const float sum = my_pos < 0 ? 0.0f : fold.sum;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        put_out(p, j0 + row, g, head, 32 * d + 8 * e + 4 * half,
+                f32x4{total[d][4 * e], total[d][4 * e + 1], total[d][4 * e + 2], total[d][4 * e + 3]}, sum);
+  }
+  if (t == 0) *mark = 1;
+}
+
 // Joins a split row's records in ascending order. A thread has four dims of a head.
 template <int D>
 __global__ __launch_bounds__(256) void k_join(StrideWindowAttentionParams p, int limit, int span) {
@@ -385,6 +669,7 @@ __global__ __launch_bounds__(256) void k_join(StrideWindowAttentionParams p, int
 
 struct Plan {
   int page_shift, limit, span;
+  int tile_rows;  // 0: no tiles
   bool split;
   int64_t scratch;
 };
@@ -415,7 +700,9 @@ const char* plan_of(const StrideWindowAttentionParams& p, Plan& plan) {
   const int64_t units = static_cast<int64_t>(p.l.rows) * p.n_kv;
   if (units * span > INT_MAX) return "rows, n_kv and the context are too large together";
   plan.split = span > 1 && units < 512;
+  plan.tile_rows = plan.split || p.runs == 1 ? 0 : kColumns / p.n_q;
   plan.scratch = plan.split ? units * span * ((p.n_q * (D + 2) + 3) / 4 * 4) : 0;
+  if (plan.tile_rows) plan.scratch = static_cast<int64_t>(p.l.rows + plan.tile_rows - 1) / plan.tile_rows * p.n_kv;
   return nullptr;
 }
 
@@ -429,12 +716,21 @@ template <int D>
 int run(const StrideWindowAttentionParams& p, const Plan& plan, hipStream_t st) {
   const int units = p.l.rows * p.n_kv;
   if (plan.split) {
-    hipLaunchKernelGGL((k_rows<D, true>), dim3(units * plan.span), dim3(256), 0, st, p, plan.page_shift, plan.limit, plan.span);
+    hipLaunchKernelGGL((k_leaves<D>), dim3(units * plan.span), dim3(256), 0, st, p, plan.page_shift, plan.limit, plan.span);
     if (int rc = launched("window_attention (leaves)")) return rc;
     hipLaunchKernelGGL((k_join<D>), dim3(units), dim3(256), 0, st, p, plan.limit, plan.span);
     return launched("window_attention (join)");
   }
-  hipLaunchKernelGGL((k_rows<D, false>), dim3(units), dim3(256), 0, st, p, plan.page_shift, plan.limit, plan.span);
+  int32_t* done = nullptr;
+  int per = 1;
+  if (plan.tile_rows) {
+    done = reinterpret_cast<int32_t*>(p.scratch);
+    hipLaunchKernelGGL((k_tile<D>), dim3(static_cast<unsigned>(plan.scratch)), dim3(256), 0, st, p, plan.page_shift, plan.limit, plan.tile_rows, done);
+    if (int rc = launched("window_attention (tiles)")) return rc;
+    per = std::max(1, std::min(8, units / 2048));  // most of them only find that nothing is left
+  }
+  hipLaunchKernelGGL((k_rows<D>), dim3((p.l.rows + per - 1) / per * p.n_kv), dim3(256), 0, st, p, plan.page_shift, plan.limit, per, done,
+                     std::max(1, plan.tile_rows));
   return launched("window_attention");
 }
 

@@ -305,13 +305,14 @@ def here(t) -> None:
 
 
 def window_attention_scratch(rows: int, n_kv: int, n_q: int, head_dim: int, window: int, sinks: int, max_pages: int,
-                             device):
+                             device, runs: int = 0):
     """The scratch that window_attention wants for calls of these sizes (None: none). It may
     be larger than a call's; its contents need no preparation."""
     p = _lib.WindowAttentionParams()
     p.l = lanes(rows)
     p.q_stride = p.out_cols = n_kv * n_q * head_dim
     p.max_pages, p.n_kv, p.n_q, p.head_dim, p.window, p.sinks = max_pages, n_kv, n_q, head_dim, window, sinks
+    p.runs = runs
     p.kv.head_dim, p.kv.group_elems, p.kv.max_blocks = head_dim, 64 * head_dim, max_pages
     import ctypes
 
@@ -352,7 +353,7 @@ def window_attention(q, kv: PagedKv, row_slot, row_pos, n_kv: int, n_q: int, hea
     if scratch is None:
         if tc._stream is not None:
             raise ValueError("with a stream set by set_kernel_stream, pass scratch (window_attention_scratch)")
-        scratch = window_attention_scratch(rows, n_kv, n_q, head_dim, window, sinks, max_pages, q.device)
+        scratch = window_attention_scratch(rows, n_kv, n_q, head_dim, window, sinks, max_pages, q.device, runs)
     floats = 0
     if scratch is not None:
         if scratch.dtype != torch.float32 or not scratch.is_contiguous():

@@ -102,7 +102,7 @@ def test_attention_empty_and_null():
 
 def test_attention_scratch_is_bounded_by_the_sight():
     """A window bounds the leaves that a row sees, and with them the scratch."""
-    size = lambda **o: _lib.load().stride_serve_window_attention_scratch(C.byref(attention(**o)))
+    size = lambda **o: _lib.load().stride_serve_window_attention_scratch(C.byref(attention(runs=1, **o)))
     everything = size(max_pages=512, kv__max_blocks=2048)
     assert everything > 0 and everything % (4 * 8 * 128) == 0  # 32768 positions: 128 leaves of 4 rows and 8 groups
     one = everything // 128
