@@ -24,6 +24,7 @@
 #include <climits>
 #include <cstddef>
 #include <string>
+#include <type_traits>
 
 #include "../../include/stride_serve.h"
 #include "tc_common.hpp"
@@ -358,7 +359,16 @@ __global__ __launch_bounds__(256) void k_rows(StrideWindowAttentionParams p, int
                                               int tile_rows) {
   const int g = blockIdx.x % p.n_kv, j0 = blockIdx.x / p.n_kv * per;
   for (int j = j0; j < min(j0 + per, p.l.rows); ++j) {
-    if (done && done[j / tile_rows * p.n_kv + g]) continue;
+    if (done) {
+      const int tile = j / tile_rows;
+      const int32_t* mark = done + (tile * p.n_kv + g) * 2;
+      if (mark[0] && mark[1]) continue;
+      if (mark[0] || mark[1]) {  // one part: is the row of the tile's first run?
+        int part = 0;
+        for (int i = tile * tile_rows + 1; i <= j; ++i) part |= p.row_slot[i] != p.row_slot[i - 1];
+        if (mark[part]) continue;
+      }
+    }
     one_row<D, false>(p, page_shift, limit, 0, g, j, 0);
     if (per > 1) lds_barrier();
   }
@@ -367,24 +377,43 @@ __global__ __launch_bounds__(256) void k_rows(StrideWindowAttentionParams p, int
 // ---------------------------------------------------------------------------
 // Prompts: a workgroup has a tile of 128 score columns, (row, head) pairs of neighbouring
 // rows, and a KV group, so that a chunk of keys and values is fetched once for all of them.
-// Four waves of 32 columns each, v_mfma_f32_32x32x16_bf16 (two give the bits of one
-// 16x16x32, k halves in order), the transposed product first: S^T = K Q^T leaves a column's
-// scores in a lane pair, so that references, weights and sums are lane-local, and S^T's
-// registers are P^T's operand as they are, with the value rows taken in the same order.
+// A wave has COLS of the columns: 32 with v_mfma_f32_32x32x16_bf16 (two, k halves in order,
+// give the bits of one 16x16x32), or 16 at head_dim 128, where 32 would take over 256
+// registers and leave one wave on a SIMD. The transposed product first: S^T = K Q^T leaves a
+// column's scores in a few lanes, so that references, weights and sums are lane-local, and
+// S^T's registers are P^T's operand as they are, with the value rows taken in the same order.
 //
-// A chunk goes through LDS, the next one's loads in flight meanwhile. Key rows have their
-// 16-byte pieces permuted by the row, so that the 32 rows of an operand read spread over the
-// banks; value rows as v_at has them.
+// Chunks are copied memory -> LDS two ahead, into three buffers. Key rows have their 16-byte
+// pieces permuted by the row and value rows their COLS * 2-byte blocks, so that an operand
+// read spreads over the banks; the copy lands in order, so its source is permuted.
 //
-// Rows of several sequences meet in a tile where prompts end: the tile goes through the
-// sequences one after the other, each column taking part in its own. A tile of many short
-// runs is left to k_rows, and so is one with a value that is not finite in a chunk that some
-// of its columns must not see (0 times it is NaN). done[tile * n_kv + g]: whether it was done.
-template <int D>
-__device__ __forceinline__ int k_at(int row, int piece) {
-  constexpr int kPieces = D / 8;
-  return row * D + ((piece ^ ((row * D / 128) & (kPieces - 1))) << 3);
-}
+// Rows of several sequences meet in a tile where prompts end: one workgroup takes the first
+// run of a tile, another the rest, run by run, each column taking part in its own. A tile of
+// many short runs is left to k_rows, and so is one with a value that is not finite in a chunk
+// that some of its columns must not see (0 times it is NaN). done[(tile * n_kv + g) * 2 +
+// part]: whether it was done.
+constexpr int kColumns = 128;
+
+template <int D, int COLS>
+struct Lay {
+  static constexpr int kRow = D / 8;  // 16-byte pieces of a row
+  static constexpr int kBlock = COLS == 32 ? 4 : 2;  // pieces of a value row's block
+  // what the row adds to a key's piece and a value's block
+  __device__ static __forceinline__ int k_turn(int row) { return (row * D / 128) & (kRow - 1); }
+  __device__ static __forceinline__ int v_turn(int row) {
+    constexpr int kBlocks = kRow / kBlock;
+    if constexpr (COLS == 32) return kBlocks == 1 ? 0 : (kBlocks == 2 ? (row >> 1) & 1 : row & 3);
+    else return (row * D / 128) & (kBlocks - 1);
+  }
+  __device__ static __forceinline__ int k_at(int row, int piece) { return row * D + ((piece ^ k_turn(row)) << 3); }
+  __device__ static __forceinline__ int v_at(int row, int dim) {
+    return row * D + (((dim / (kBlock * 8)) ^ v_turn(row)) * kBlock * 8) + (dim & (kBlock * 8 - 1));
+  }
+  // the pieces that slot `at` of a row gets
+  __device__ static __forceinline__ int k_from(int row, int at) { return at ^ k_turn(row); }
+  __device__ static __forceinline__ int v_from(int row, int at) { return ((at / kBlock) ^ v_turn(row)) * kBlock + at % kBlock; }
+};
+
 __device__ __forceinline__ bool has_nonfinite(u32x4 v) {
   bool bad = false;
 #pragma unroll
@@ -392,29 +421,45 @@ __device__ __forceinline__ bool has_nonfinite(u32x4 v) {
   return bad;
 }
 
-constexpr int kColumns = 128;
+__device__ __align__(16) uint32_t zeros16[4];  // what unseen and unheld positions are copied from
 
-template <int D>
-__global__ __launch_bounds__(256, D == 128 ? 1 : 2) void k_tile(StrideWindowAttentionParams p, int page_shift, int limit, int tile_rows, int32_t* done) {
-  constexpr int kRow = D / 8;              // 16-byte pieces of a row
-  constexpr int kPer = kChunk * kRow / 256;  // pieces of K (and of V) a thread moves
-  constexpr int kDims = D / 32;
-  __shared__ __align__(16) uint16_t ks[2][kChunk * D];
-  __shared__ __align__(16) uint16_t vs[2][kChunk * D];
+// 64 lanes' 16 bytes each, memory -> LDS, in lane order from `to`. Written as assembly because
+// the compiler, not knowing which buffer a transposing read reads, would have every such read
+// wait for all copies under way; the kernel counts them itself (nothing else of its loop is
+// counted by vmcnt). The instruction has no register that it writes.
+__device__ __forceinline__ void copy_to_lds(const uint16_t* from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)(p)));
+}
+
+template <int D, int COLS>
+__global__ __launch_bounds__(64 * kColumns / COLS, 2) void k_tile(StrideWindowAttentionParams p, int page_shift, int limit, int tile_rows,
+                                                                   int32_t* done) {
+  using L = Lay<D, COLS>;
+  constexpr int kWavesHere = kColumns / COLS;
+  constexpr int kPer = kChunk * L::kRow / 64 / kWavesHere;  // copies of K (and of V) a wave makes
+  constexpr int kSub = COLS == 32 ? 2 : 4;                  // position blocks of a chunk
+  constexpr int kReg = COLS == 32 ? 16 : 4;                 // accumulator registers of a block
+  constexpr int kDims = D / COLS;
+  constexpr int kStep = COLS == 32 ? 16 : 32;               // dims of a score product
+  using Acc = typename std::conditional<COLS == 32, f32x16, f32x4>::type;
+  __shared__ __align__(16) uint16_t ks[3][kChunk * D];
+  __shared__ __align__(16) uint16_t vs[3][kChunk * D];
   __shared__ int slots[kColumns], poss[kColumns];
   __shared__ uint64_t starts[2];  // bit i: row i begins a run
-  __shared__ int bad[2][4];
-  const int t = threadIdx.x, wave = t >> 6, lane = t & 63, c32 = lane & 31, half = lane >> 5;
-  const int g = blockIdx.x % p.n_kv;
-  const int tiles = gridDim.x / p.n_kv, tile = tiles - 1 - blockIdx.x / p.n_kv;  // later rows see more: first
+  __shared__ int bad[2][kWavesHere];
+  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, cl = lane & (COLS - 1), quarter = lane / COLS;
+  const int g = blockIdx.x % p.n_kv, part = blockIdx.x / p.n_kv & 1;
+  const int tiles = gridDim.x / p.n_kv / 2, tile = tiles - 1 - blockIdx.x / p.n_kv / 2;  // later rows see more: first
   const int j0 = tile * tile_rows, nr = min(tile_rows, p.l.rows - j0);
-  int32_t* mark = done + tile * p.n_kv + g;
+  int32_t* mark = done + (tile * p.n_kv + g) * 2 + part;
 
   if (t < kColumns) {
     const int j = j0 + min(t, nr - 1);
-    const int slot = p.row_slot[j], pos = t < nr ? min(p.row_pos[j], limit - 1) : -1;
-    slots[t] = slot;
-    poss[t] = pos;
+    slots[t] = p.row_slot[j];
+    poss[t] = t < nr ? min(p.row_pos[j], limit - 1) : -1;
   }
   __syncthreads();
   if (t < kColumns) {
@@ -424,42 +469,47 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void k_tile(StrideWindowAtte
   __syncthreads();
   const uint64_t first = starts[0], second = starts[1];
   const int runs = __popcll(first) + __popcll(second);
-  if (nr < 4 * runs) {
-    if (t == 0) *mark = 0;
+  if (nr < 4 * runs || runs <= part) {
+    if (t == 0) *mark = nr < 4 * runs ? 0 : 1;
     return;
   }
+  // the row after row r at which another run begins
+  auto next_run = [&](int r) {
+    const uint64_t lo = r < 63 ? first & (~uint64_t{0} << (r + 1)) : 0;
+    const uint64_t hi = r < 63 ? second : (r < 127 ? second & (~uint64_t{0} << (r + 1 - 64)) : 0);
+    return lo ? __builtin_ctzll(lo) : (hi ? 64 + __builtin_ctzll(hi) : nr);
+  };
 
   // this lane's column
-  const int col = wave * 32 + c32, row = col / p.n_q, head = col - row * p.n_q;
+  const int col = wave * COLS + cl, row = col / p.n_q, head = col - row * p.n_q;
   const bool live = row < nr;
   const int my_pos = live ? poss[row] : -1;
   const Sight sight = sight_of(p, my_pos, limit);
-  u32x4 qh[D / 16], ql[D / 16];
+  u32x4 qh[D / kStep], ql[D / kStep];
   {
-    const float* q = p.q + (j0 + (live ? row : 0)) * p.q_stride + (static_cast<int64_t>(g) * p.n_q + head) * D + 8 * half;
+    const float* q = p.q + (j0 + (live ? row : 0)) * p.q_stride + (static_cast<int64_t>(g) * p.n_q + head) * D + 8 * quarter;
 #pragma unroll
-    for (int k = 0; k < D / 16; ++k) split_query(q + 16 * k, p.scale * kLog2e, live, qh[k], ql[k]);
+    for (int k = 0; k < D / kStep; ++k) split_query(q + kStep * k, p.scale * kLog2e, live, qh[k], ql[k]);
   }
 
   const uint16_t* base = static_cast<const uint16_t*>(p.kv.arena) + p.layer * p.kv.layer_elems + g * p.kv.group_elems;
   const int in_page = (1 << page_shift) - 1;
-  f32x16 total[kDims];
+  Acc total[kDims];
 #pragma unroll
   for (int d = 0; d < kDims; ++d)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) total[d][i] = 0.0f;
+    for (int i = 0; i < kReg; ++i) total[d][i] = 0.0f;
   Fold fold = {neg_inf(), 0.0f};
 
-  int buf = 0;
-  for (int r0 = 0; r0 < nr;) {
+  auto mma = [](u32x4 a, u32x4 b, Acc c) __attribute__((always_inline)) {
+    if constexpr (COLS == 32) return mfma32(a, b, c);
+    else return mfma(a, b, c);
+  };
+
+  const int begin = part ? next_run(0) : 0, end = part ? nr : next_run(0);
+  for (int r0 = begin; r0 < end;) {
     // the run [r0, r1): its sequence, and what its rows see together
-    int r1 = nr;
-    {
-      const uint64_t lo = r0 < 63 ? first & (~uint64_t{0} << (r0 + 1)) : 0;
-      const uint64_t hi = r0 < 63 ? second : (r0 < 127 ? second & (~uint64_t{0} << (r0 + 1 - 64)) : 0);
-      if (lo) r1 = __builtin_ctzll(lo);
-      else if (hi) r1 = 64 + __builtin_ctzll(hi);
-    }
+    const int r1 = next_run(r0);
     int low = INT_MAX, high = -1;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -485,148 +535,189 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void k_tile(StrideWindowAtte
     // chunks: [0, head) and [rest, last]
     const int head_chunks = (far.sink_end + kChunk - 1) / kChunk, rest = max(near.lo / kChunk, head_chunks);
     const int chunks = head_chunks + max(0, high / kChunk - rest + 1);
-    const int32_t* table = p.kv.table + static_cast<int64_t>(slot) * p.kv.max_blocks;
+    const auto table = (const __attribute__((address_space(4))) int32_t*)(p.kv.table + static_cast<int64_t>(slot) * p.kv.max_blocks);
     auto chunk_at = [&](int i) { return i < head_chunks ? i : rest + i - head_chunks; };
 
+    // Table entries one chunk ahead of the copies, which are two ahead of the products. A copy's
+    // rows lie in one page, so its entry comes through the scalar cache. Past the last chunk it
+    // is copied again, so that the waits can count.
     int block[kPer];
-    u32x4 kr[kPer], vr[kPer];
-    const u32x4 zero = {0, 0, 0, 0};
     auto look = [&](int i) {
+      const int c = chunk_at(min(i, chunks - 1)) * kChunk;
 #pragma unroll
       for (int u = 0; u < kPer; ++u) {
-        const int pos = chunk_at(i) * kChunk + (t + 256 * u) / kRow;
-        const bool s = pos <= high && (pos >= near.lo || pos < far.sink_end);
-        block[u] = s ? table[pos >> page_shift] : -1;
+        // an entry that no row sees is not looked at: the run's own last one stands for it
+        const int a = c + (wave * kPer + u) * 64 / L::kRow, z = a + 64 / L::kRow - 1;
+        const bool s = a <= high && (z >= near.lo || a < far.sink_end);
+        block[u] = table[__builtin_amdgcn_readfirstlane((s ? a : high) >> page_shift)];
       }
     };
-    auto fetch = [&](int i) {
+    auto copy = [&](int i, int buf) {
+      const int c = chunk_at(min(i, chunks - 1)) * kChunk;
 #pragma unroll
       for (int u = 0; u < kPer; ++u) {
-        const int piece = t + 256 * u, pos = chunk_at(i) * kChunk + piece / kRow, b = block[u];
-        const uint16_t* at = base + max(b, 0) * p.kv.block_elems + (pos & in_page) * D + piece % kRow * 8;
-        kr[u] = load16(at);
-        vr[u] = load16(at + p.kv.which_elems);
-        if (b < 0) kr[u] = vr[u] = zero;
+        const int at = (wave * kPer + u) * 64, r = (at + lane) / L::kRow, slot_in = (at + lane) % L::kRow, pos = c + r;
+        const bool seen = block[u] >= 0 && pos <= high && (pos >= near.lo || pos < far.sink_end);
+        const uint16_t* from = base + block[u] * p.kv.block_elems + (pos & in_page) * D;
+        const uint16_t* zero = reinterpret_cast<const uint16_t*>(zeros16);
+        copy_to_lds(seen ? from + L::k_from(r, slot_in) * 8 : zero, lds_offset(&ks[buf][at * 8]));
+        copy_to_lds(seen ? from + p.kv.which_elems + L::v_from(r, slot_in) * 8 : zero, lds_offset(&vs[buf][at * 8]));
       }
     };
-
-    f32x16 acc[kDims], l;
-    float ref = neg_inf();
-    auto fresh = [&]() {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        l[i] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < kDims; ++d) acc[d][i] = 0.0f;
-      }
-      ref = neg_inf();
-    };
-    fresh();
     look(0);
-    fetch(0);
-    if (chunks > 1) look(1);
-    for (int i = 0; i < chunks; ++i) {
-      const int a = chunk_at(i) * kChunk;
-      // do all columns see all of it?
-      const bool full = whole && a + kChunk - 1 <= low && (a >= far.lo || a + kChunk <= near.sink_end);
+    copy(0, 0);
+    look(1);
+    copy(1, 1);
+    look(2);
+    int buf = 0;
+    for (int i = 0; i < chunks;) {
+      const int leaf = chunk_at(i) / (kLeaf / kChunk);
+      Acc acc[kDims], l;
+      float ref = neg_inf();
 #pragma unroll
-      for (int u = 0; u < kPer; ++u) {
-        const int piece = t + 256 * u;
-        *reinterpret_cast<u32x4*>(&ks[buf][k_at<D>(piece / kRow, piece % kRow)]) = kr[u];
-        *reinterpret_cast<u32x4*>(&vs[buf][v_at<D>(piece / kRow, piece % kRow * 8)]) = vr[u];
+      for (int e = 0; e < kReg; ++e) {
+        l[e] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) acc[d][e] = 0.0f;
       }
-      if (!full) {
-        bool b = false;
+      do {
+        const int a = chunk_at(i) * kChunk;
+        // do all columns see all of it?
+        const bool full = whole && a + kChunk - 1 <= low && (a >= far.lo || a + kChunk <= near.sink_end);
+        // this chunk has arrived (the next one's copies may be under way), and every wave has
+        // read the one before, whose buffer is filled next
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kPer) : "memory");
+        lds_barrier();
+        if (!full) {
+          bool b = false;
 #pragma unroll
-        for (int u = 0; u < kPer; ++u) b |= has_nonfinite(vr[u]);
-        const bool any = __any(b);
-        if (lane == 0) bad[buf][wave] = any;
-      }
-      lds_barrier();
-      if (!full && (bad[buf][0] | bad[buf][1] | bad[buf][2] | bad[buf][3])) {
-        if (t == 0) *mark = 0;
-        return;
-      }
-      if (i + 1 < chunks) {
-        fetch(i + 1);
-        if (i + 2 < chunks) look(i + 2);
-      }
-      f32x16 s[2];
+          for (int u = 0; u < kPer; ++u) b |= has_nonfinite(*reinterpret_cast<const u32x4*>(&vs[buf][((wave * kPer + u) * 64 + lane) * 8]));
+          const bool any = __any(b);
+          if (lane == 0) bad[i & 1][wave] = any;
+          lds_barrier();
+          int sum = 0;
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < D / 32; ++k) {
-          const u32x4 k0 = *reinterpret_cast<const u32x4*>(&ks[buf][k_at<D>(32 * b + c32, 4 * k + half)]);
-          const u32x4 k1 = *reinterpret_cast<const u32x4*>(&ks[buf][k_at<D>(32 * b + c32, 4 * k + 2 + half)]);
-          s[b] = mfma32(k0, qh[2 * k], s[b]);
-          s[b] = mfma32(k1, qh[2 * k + 1], s[b]);
-          s[b] = mfma32(k0, ql[2 * k], s[b]);
-          s[b] = mfma32(k1, ql[2 * k + 1], s[b]);
-        }
-      }
-      if (!full) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (!(mine && sight.sees(a + 32 * b + 8 * (e / 4) + 4 * half + e % 4))) s[b][e] = neg_inf();
-      }
-      float most = s[0][0];
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) most = fmaxf(most, s[b][e]);
-      most = fmaxf(most, __shfl_xor(most, 32));
-      if (__any(most > ref + kSlack)) {
-        const bool up = most > ref + kSlack;
-        const float alpha = up ? exp2_of(ref - most) : 1.0f;
-        if (up) ref = most;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          l[e] *= alpha;
-#pragma unroll
-          for (int d = 0; d < kDims; ++d) acc[d][e] *= alpha;
-        }
-      }
-      const float at = ref == neg_inf() ? 0.0f : ref;
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        uint32_t w[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = pack2(exp2_of(s[b][2 * e] - at), exp2_of(s[b][2 * e + 1] - at));
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const u32x4 pw = {w[2 * x], w[2 * x + 1], w[2 * x + 4], w[2 * x + 5]};
-          l = mfma32(u32x4{kOnes, kOnes, kOnes, kOnes}, pw, l);
-          const int r = 32 * b + 8 * x + 4 * half + ((lane & 15) >> 2);
-#pragma unroll
-          for (int d = 0; d < kDims; ++d) {
-            const int dim = 32 * d + (lane & 16) + 4 * (lane & 3);
-            acc[d] = mfma32(both(read_transposed(&vs[buf][v_at<D>(r, dim)]), read_transposed(&vs[buf][v_at<D>(r + 16, dim)])), pw, acc[d]);
+          for (int w = 0; w < kWavesHere; ++w) sum |= bad[i & 1][w];
+          if (sum) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (t == 0) *mark = 0;
+            return;
           }
         }
-      }
-      buf ^= 1;
-      if (i + 1 == chunks || chunk_at(i + 1) / (kLeaf / kChunk) != a / kLeaf) {
-        float fa, fb;
-        fold.take(ref, l[0], fa, fb);
+        copy(i + 2, buf == 0 ? 2 : buf - 1);
+        look(i + 3);
+        Acc s[kSub];
 #pragma unroll
-        for (int d = 0; d < kDims; ++d)
+        for (int b = 0; b < kSub; ++b) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) total[d][e] = __builtin_fmaf(acc[d][e], fb, total[d][e] * fa);
-        fresh();
-      }
+          for (int e = 0; e < kReg; ++e) s[b][e] = 0.0f;
+#pragma unroll
+          for (int k = 0; k < D / 32; ++k) {
+            if constexpr (COLS == 32) {
+              const u32x4 k0 = *reinterpret_cast<const u32x4*>(&ks[buf][L::k_at(32 * b + cl, 4 * k + quarter)]);
+              const u32x4 k1 = *reinterpret_cast<const u32x4*>(&ks[buf][L::k_at(32 * b + cl, 4 * k + 2 + quarter)]);
+              s[b] = mma(k0, qh[2 * k], s[b]);
+              s[b] = mma(k1, qh[2 * k + 1], s[b]);
+              s[b] = mma(k0, ql[2 * k], s[b]);
+              s[b] = mma(k1, ql[2 * k + 1], s[b]);
+            } else {
+              const u32x4 k0 = *reinterpret_cast<const u32x4*>(&ks[buf][L::k_at(16 * b + cl, 4 * k + quarter)]);
+              s[b] = mma(k0, qh[k], s[b]);
+              s[b] = mma(k0, ql[k], s[b]);
+            }
+          }
+        }
+        // register e of block b is position b * COLS + 8 * (e / 4) + 4 * quarter + e % 4 of the chunk
+        if (!full) {
+          const int from = a + 4 * quarter;
+          if (a >= far.sink_end) {
+            const uint32_t wide = mine && sight.pos >= sight.lo ? sight.pos - sight.lo : 0;
+            const int shift = mine && sight.pos >= sight.lo ? from - sight.lo : INT_MIN / 2;  // far below: unseen
+#pragma unroll
+            for (int b = 0; b < kSub; ++b)
+#pragma unroll
+              for (int e = 0; e < kReg; ++e)
+                if (static_cast<uint32_t>(shift + b * COLS + 8 * (e / 4) + e % 4) > wide) s[b][e] = neg_inf();
+          } else {
+#pragma unroll
+            for (int b = 0; b < kSub; ++b)
+#pragma unroll
+              for (int e = 0; e < kReg; ++e)
+                if (!(mine && sight.sees(from + b * COLS + 8 * (e / 4) + e % 4))) s[b][e] = neg_inf();
+          }
+        }
+        float most = s[0][0];
+#pragma unroll
+        for (int b = 0; b < kSub; ++b)
+#pragma unroll
+          for (int e = 0; e < kReg; ++e) most = fmaxf(most, s[b][e]);
+        if constexpr (COLS == 16) most = fmaxf(most, __shfl_xor(most, 16));
+        most = fmaxf(most, __shfl_xor(most, 32));
+        if (__any(most > ref + kSlack)) {
+          const bool up = most > ref + kSlack;
+          const float alpha = up ? exp2_of(ref - most) : 1.0f;
+          if (up) ref = most;
+#pragma unroll
+          for (int e = 0; e < kReg; ++e) {
+            l[e] *= alpha;
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) acc[d][e] *= alpha;
+          }
+        }
+        const float at = ref == neg_inf() ? 0.0f : ref;
+#pragma unroll
+        for (int b = 0; b < kSub; ++b)
+#pragma unroll
+          for (int e = 0; e < kReg; ++e) s[b][e] = exp2_of(s[b][e] - at);
+        // 32 positions: the products in the order of the 16 x 16 x 32 form's k
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if constexpr (COLS == 32) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const u32x4 pw = {pack2(s[h][4 * x], s[h][4 * x + 1]), pack2(s[h][4 * x + 2], s[h][4 * x + 3]),
+                                pack2(s[h][4 * x + 8], s[h][4 * x + 9]), pack2(s[h][4 * x + 10], s[h][4 * x + 11])};
+              l = mma(u32x4{kOnes, kOnes, kOnes, kOnes}, pw, l);
+              const int r = 32 * h + 8 * x + 4 * quarter + ((lane & 15) >> 2);
+#pragma unroll
+              for (int d = 0; d < kDims; ++d) {
+                const int dim = 32 * d + (lane & 16) + 4 * (lane & 3);
+                acc[d] = mma(both(read_transposed(&vs[buf][L::v_at(r, dim)]), read_transposed(&vs[buf][L::v_at(r + 16, dim)])), pw, acc[d]);
+              }
+            }
+          } else {
+            const u32x4 pw = {pack2(s[2 * h][0], s[2 * h][1]), pack2(s[2 * h][2], s[2 * h][3]), pack2(s[2 * h + 1][0], s[2 * h + 1][1]),
+                              pack2(s[2 * h + 1][2], s[2 * h + 1][3])};
+            l = mma(u32x4{kOnes, kOnes, kOnes, kOnes}, pw, l);
+            const int r = 32 * h + 4 * quarter + ((lane & 15) >> 2);
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) {
+              const int dim = 16 * d + 4 * (lane & 3);
+              acc[d] = mma(both(read_transposed(&vs[buf][L::v_at(r, dim)]), read_transposed(&vs[buf][L::v_at(r + 16, dim)])), pw, acc[d]);
+            }
+          }
+        }
+        buf = buf == 2 ? 0 : buf + 1;
+        ++i;
+      } while (i < chunks && chunk_at(i) / (kLeaf / kChunk) == leaf);
+      float fa, fb;
+      fold.take(ref, l[0], fa, fb);
+#pragma unroll
+      for (int d = 0; d < kDims; ++d)
+#pragma unroll
+        for (int e = 0; e < kReg; ++e) total[d][e] = __builtin_fmaf(acc[d][e], fb, total[d][e] * fa);
     }
+    // nothing is on its way to the buffers when another run, or the end, comes
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();
   }
-  if (live) {
+  if (live && row >= begin && row < end) {
     const float sum = my_pos < 0 ? 0.0f : fold.sum;
 #pragma unroll
     for (int d = 0; d < kDims; ++d)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        put_out(p, j0 + row, g, head, 32 * d + 8 * e + 4 * half,
+      for (int e = 0; e < kReg / 4; ++e)
+        put_out(p, j0 + row, g, head, COLS * d + 8 * e + 4 * quarter,
                 f32x4{total[d][4 * e], total[d][4 * e + 1], total[d][4 * e + 2], total[d][4 * e + 3]}, sum);
   }
   if (t == 0) *mark = 1;
@@ -700,9 +791,10 @@ const char* plan_of(const StrideWindowAttentionParams& p, Plan& plan) {
   const int64_t units = static_cast<int64_t>(p.l.rows) * p.n_kv;
   if (units * span > INT_MAX) return "rows, n_kv and the context are too large together";
   plan.split = span > 1 && units < 512;
-  plan.tile_rows = plan.split || p.runs == 1 ? 0 : kColumns / p.n_q;
+  // (a tile's copies of 64 / (head_dim / 8) rows lie in one page)
+  plan.tile_rows = plan.split || p.runs == 1 || tokens < 512 / D ? 0 : kColumns / p.n_q;
   plan.scratch = plan.split ? units * span * ((p.n_q * (D + 2) + 3) / 4 * 4) : 0;
-  if (plan.tile_rows) plan.scratch = static_cast<int64_t>(p.l.rows + plan.tile_rows - 1) / plan.tile_rows * p.n_kv;
+  if (plan.tile_rows) plan.scratch = (static_cast<int64_t>(p.l.rows) + plan.tile_rows - 1) / plan.tile_rows * p.n_kv * 2;
   return nullptr;
 }
 
@@ -725,7 +817,8 @@ int run(const StrideWindowAttentionParams& p, const Plan& plan, hipStream_t st) 
   int per = 1;
   if (plan.tile_rows) {
     done = reinterpret_cast<int32_t*>(p.scratch);
-    hipLaunchKernelGGL((k_tile<D>), dim3(static_cast<unsigned>(plan.scratch)), dim3(256), 0, st, p, plan.page_shift, plan.limit, plan.tile_rows, done);
+    constexpr int kCols = D == 128 ? 16 : 32;
+    hipLaunchKernelGGL((k_tile<D, kCols>), dim3(static_cast<unsigned>(plan.scratch)), dim3(64 * kColumns / kCols), 0, st, p, plan.page_shift, plan.limit, plan.tile_rows, done);
     if (int rc = launched("window_attention (tiles)")) return rc;
     per = std::max(1, std::min(8, units / 2048));  // most of them only find that nothing is left
   }

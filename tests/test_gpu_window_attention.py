@@ -115,11 +115,11 @@ def test_pages(page, window):
 
 @pytest.mark.parametrize("seqs,rows,past", [(1, 2, 0), (1, 33, 0), (1, 130, 70), (3, 40, 250), (2, 65, 500), (5, 7, 300), (40, 3, 90)])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (50, 4), (300, 0)])
-@pytest.mark.parametrize("D,n_q", [(64, 4), (128, 8), (32, 1), (64, 3)])
-def test_chunks_of_prompts(seqs, rows, past, window, sinks, D, n_q):
+@pytest.mark.parametrize("n_kv,D,n_q", [(2, 64, 4), (2, 128, 8), (2, 32, 1), (2, 64, 3), (16, 64, 4), (16, 128, 3), (16, 32, 2)])
+def test_chunks_of_prompts(seqs, rows, past, window, sinks, n_kv, D, n_q):
     """Neighbouring rows of one sequence, and tiles in which several sequences meet."""
-    say("chunks", seqs, rows, past, window, sinks, D, n_q)
-    c = Case(seqs * rows + past, seqs, past + rows, 2, n_q, D, 16)
+    say("chunks", seqs, rows, past, window, sinks, n_kv, D, n_q)
+    c = Case(seqs * rows + past, seqs, past + rows, n_kv, n_q, D, 16)
     slot = [s for s in range(seqs) for _ in range(rows)]
     pos = [past + i for _ in range(seqs) for i in range(rows)]
     q = c.queries(len(slot))
@@ -164,14 +164,14 @@ def test_larger_capacity_changes_nothing(rows):
     assert torch.equal(a, c.run(q, slot, pos, max_pages=1 << 20))
 
 
-@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("rows,n_kv", [(1, 2), (40, 2), (40, 16)])
 @pytest.mark.parametrize("poison", [float("nan"), float("inf"), -float("inf")])
-def test_masked_places_have_no_influence(rows, poison):
+def test_masked_places_have_no_influence(rows, n_kv, poison):
     """Poison in every position that a row must not see: behind it, between sinks and window,
     in released pages; and in its neighbours' sights in the same tile."""
-    say("poison", rows, poison)
+    say("poison", rows, n_kv, poison)
     window, sinks = 90, 3
-    c = Case(7, 1, 700, 2, 4, 64, 16)
+    c = Case(7, 1, 700, n_kv, 4, 64, 16)
     pos = [560 + i for i in range(rows)]
     q = c.queries(rows)
     clean = c.run(q, [0] * rows, pos, window, sinks)
@@ -186,14 +186,15 @@ def test_masked_places_have_no_influence(rows, poison):
     assert torch.equal(clean, c.run(q, [0] * rows, pos, window, sinks))
 
 
+@pytest.mark.parametrize("n_kv", [2, 8])
 @pytest.mark.parametrize("which", [0, 1])
 @pytest.mark.parametrize("poison", [float("nan"), float("inf"), -float("inf")])
-def test_a_bad_token_reaches_only_the_rows_that_see_it(which, poison):
+def test_a_bad_token_reaches_only_the_rows_that_see_it(n_kv, which, poison):
     """A key or value that is not finite: rows before it and rows whose window has passed it
     are as they were, in tiles too, and for those that see it the plain formula decides what is
     not finite."""
     window, sinks, rows, at = 20, 0, 64, 330
-    c = Case(8, 1, 500, 2, 4, 64, 16)
+    c = Case(8, 1, 500, n_kv, 4, 64, 16)
     pos = [300 + i for i in range(rows)]
     q = c.queries(rows)
     clean = layout.untile_lanes(c.run(q, [0] * rows, pos, window, sinks), rows)
@@ -201,8 +202,9 @@ def test_a_bad_token_reaches_only_the_rows_that_see_it(which, poison):
     got = layout.untile_lanes(c.run(q, [0] * rows, pos, window, sinks, runs=rows), rows)
     sees = torch.tensor([at <= p < at + window for p in pos], device=DEV)
     assert torch.equal(got[~sees], clean[~sees])
-    heads = got.reshape(rows, 2, 4, 64).view(torch.bfloat16)
-    assert torch.equal(got.reshape(rows, 2, -1)[:, 0], clean.reshape(rows, 2, -1)[:, 0])  # the other group
+    heads = got.reshape(rows, n_kv, 4, 64).view(torch.bfloat16)
+    others = [g for g in range(n_kv) if g != 1]
+    assert torch.equal(got.reshape(rows, n_kv, -1)[:, others], clean.reshape(rows, n_kv, -1)[:, others])
     if which == 1:  # a value: its dim alone
         assert torch.isfinite(heads[sees][:, 1, :, :5]).all() and torch.isfinite(heads[sees][:, 1, :, 6:]).all()
         assert not torch.isfinite(heads[sees][:, 1, :, 5]).any()
@@ -213,12 +215,32 @@ def test_a_bad_token_reaches_only_the_rows_that_see_it(which, poison):
     elif poison != poison:  # a key: every dim of its heads
         assert torch.isnan(heads[sees][:, 1]).all()
     else:  # a score of +inf takes inf - inf, one of -inf is a weight of 0
-        sign = torch.sign(q.reshape(rows, 2, 4, 64)[sees][:, 1, :, 5]) * (1 if poison > 0 else -1)
+        sign = torch.sign(q.reshape(rows, n_kv, 4, 64)[sees][:, 1, :, 5]) * (1 if poison > 0 else -1)
         assert torch.isnan(heads[sees][:, 1][sign > 0]).all() and torch.isfinite(heads[sees][:, 1][sign < 0]).all()
     for j in range(rows):  # and the same bits, or the same kind of value, row by row
         one = layout.untile_lanes(c.run(q[j:j + 1], [0], [pos[j]], window, sinks), 1)[0]
         a, b = one.view(torch.bfloat16), got[j].view(torch.bfloat16)
         assert torch.equal(a.nan_to_num(7e7), b.nan_to_num(7e7)), j
+
+
+def test_a_bad_token_where_two_prompts_meet():
+    """A tile of two sequences, the bad value in either, at an edge: its part alone is done
+    another way, and no other row changes."""
+    for at_slot in (0, 1):
+        c = Case(20 + at_slot, 2, 400, 8, 4, 64, 16)
+        slot = [0] * 80 + [1] * 80
+        pos = [200 + i for i in range(80)] + [300 + i for i in range(80)]
+        q = c.queries(160)
+        clean = layout.untile_lanes(c.run(q, slot, pos, 150, 4, runs=80), 160)
+        at = (230, 330)[at_slot]
+        c.arena[int(c.table[at_slot, at // 16]), 1, 1, 3, at % 16, 40] = float("inf")
+        got = layout.untile_lanes(c.run(q, slot, pos, 150, 4, runs=80), 160)
+        touched = torch.tensor([s == at_slot and p >= at for s, p in zip(slot, pos)], device=DEV)
+        assert torch.equal(got[~touched], clean[~touched])
+        heads = got.reshape(160, 8, 4, 64).view(torch.bfloat16)
+        assert torch.isinf(heads[touched][:, 3, :, 40]).all()
+        heads[:, 3, :, 40] = clean.reshape(160, 8, 4, 64).view(torch.bfloat16)[:, 3, :, 40]
+        assert torch.equal(heads.view(torch.int16).reshape(160, -1), clean)
 
 
 def test_large_scores():
