@@ -352,26 +352,34 @@ __global__ __launch_bounds__(256) void k_leaves(StrideWindowAttentionParams p, i
   one_row<D, true>(p, page_shift, limit, span, blockIdx.x % p.n_kv, unit / span, unit % span);
 }
 
-// `per` rows one after the other; those of tiles that k_tile has done (done: its marks, or
-// NULL) are skipped.
+// A workgroup a unit (row, group); with tiles that k_tile may have done (done: its marks), a
+// workgroup looks at up to 256 units, spread over the batch, and takes those that are left.
+__device__ __forceinline__ bool unit_done(const StrideWindowAttentionParams& p, int unit, const int32_t* done, int tile_rows) {
+  const int j = unit / p.n_kv, tile = j / tile_rows;
+  const int32_t* mark = done + (tile * p.n_kv + unit % p.n_kv) * 2;
+  if (mark[0] == mark[1]) return mark[0];
+  int part = 0;  // is the row of the tile's first run?
+  for (int i = tile * tile_rows + 1; i <= j; ++i) part |= p.row_slot[i] != p.row_slot[i - 1];
+  return mark[part];
+}
 template <int D>
-__global__ __launch_bounds__(256) void k_rows(StrideWindowAttentionParams p, int page_shift, int limit, int per, const int32_t* done,
-                                              int tile_rows) {
-  const int g = blockIdx.x % p.n_kv, j0 = blockIdx.x / p.n_kv * per;
-  for (int j = j0; j < min(j0 + per, p.l.rows); ++j) {
-    if (done) {
-      const int tile = j / tile_rows;
-      const int32_t* mark = done + (tile * p.n_kv + g) * 2;
-      if (mark[0] && mark[1]) continue;
-      if (mark[0] || mark[1]) {  // one part: is the row of the tile's first run?
-        int part = 0;
-        for (int i = tile * tile_rows + 1; i <= j; ++i) part |= p.row_slot[i] != p.row_slot[i - 1];
-        if (mark[part]) continue;
-      }
-    }
-    one_row<D, false>(p, page_shift, limit, 0, g, j, 0);
-    if (per > 1) lds_barrier();
+__global__ __launch_bounds__(256) void k_rows(StrideWindowAttentionParams p, int page_shift, int limit, const int32_t* done, int tile_rows) {
+  if (!done) {
+    one_row<D, false>(p, page_shift, limit, 0, blockIdx.x % p.n_kv, blockIdx.x / p.n_kv, 0);
+    return;
   }
+  __shared__ uint64_t left[4];
+  const int units = p.l.rows * p.n_kv, mine = threadIdx.x * gridDim.x + blockIdx.x;
+  const uint64_t b = __ballot(mine < units && !unit_done(p, mine, done, tile_rows));
+  if ((threadIdx.x & 63) == 0) left[threadIdx.x >> 6] = b;
+  __syncthreads();
+#pragma unroll 1
+  for (int w = 0; w < 4; ++w)
+#pragma unroll 1
+    for (uint64_t todo = left[w]; todo; todo &= todo - 1) {
+      const int unit = __builtin_amdgcn_readfirstlane((w * 64 + __builtin_ctzll(todo)) * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x));
+      one_row<D, false>(p, page_shift, limit, 0, unit % p.n_kv, unit / p.n_kv, 0);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -451,8 +459,11 @@ __global__ __launch_bounds__(64 * kColumns / COLS, 2) void k_tile(StrideWindowAt
   __shared__ uint64_t starts[2];  // bit i: row i begins a run
   __shared__ int bad[2][kWavesHere];
   const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, cl = lane & (COLS - 1), quarter = lane / COLS;
-  const int g = blockIdx.x % p.n_kv, part = blockIdx.x / p.n_kv & 1;
-  const int tiles = gridDim.x / p.n_kv / 2, tile = tiles - 1 - blockIdx.x / p.n_kv / 2;  // later rows see more: first
+  // The first runs' workgroups first (most of the others only leave; taken in turn with them,
+  // they left whole CUs idle: 2048 rows of window 512 70 us against 41), and later rows, which
+  // see more, before earlier ones.
+  const int tiles = gridDim.x / p.n_kv / 2, unit = blockIdx.x / p.n_kv;
+  const int g = blockIdx.x % p.n_kv, part = unit >= tiles ? 1 : 0, tile = tiles - 1 - (part ? unit - tiles : unit);
   const int j0 = tile * tile_rows, nr = min(tile_rows, p.l.rows - j0);
   int32_t* mark = done + (tile * p.n_kv + g) * 2 + part;
 
@@ -814,16 +825,16 @@ int run(const StrideWindowAttentionParams& p, const Plan& plan, hipStream_t st) 
     return launched("window_attention (join)");
   }
   int32_t* done = nullptr;
-  int per = 1;
+  int groups = units;
   if (plan.tile_rows) {
     done = reinterpret_cast<int32_t*>(p.scratch);
     constexpr int kCols = D == 128 ? 16 : 32;
-    hipLaunchKernelGGL((k_tile<D, kCols>), dim3(static_cast<unsigned>(plan.scratch)), dim3(64 * kColumns / kCols), 0, st, p, plan.page_shift, plan.limit, plan.tile_rows, done);
+    hipLaunchKernelGGL((k_tile<D, kCols>), dim3(static_cast<unsigned>(plan.scratch)), dim3(64 * kColumns / kCols), 0, st, p, plan.page_shift, plan.limit,
+                       plan.tile_rows, done);
     if (int rc = launched("window_attention (tiles)")) return rc;
-    per = std::max(1, std::min(8, units / 2048));  // most of them only find that nothing is left
+    groups = std::max(std::min(units, 1024), (units + 255) / 256);  // most of them only find that nothing is left
   }
-  hipLaunchKernelGGL((k_rows<D>), dim3((p.l.rows + per - 1) / per * p.n_kv), dim3(256), 0, st, p, plan.page_shift, plan.limit, per, done,
-                     std::max(1, plan.tile_rows));
+  hipLaunchKernelGGL((k_rows<D>), dim3(groups), dim3(256), 0, st, p, plan.page_shift, plan.limit, done, std::max(1, plan.tile_rows));
   return launched("window_attention");
 }
 
