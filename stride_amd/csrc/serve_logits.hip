@@ -23,7 +23,9 @@ namespace {
 constexpr int kTiles = 32;             // row tiles of a workgroup
 constexpr int kTokens = kTiles * 16;
 constexpr int kWords = kTokens / 32;
-constexpr int kSteps = kTiles / 4;     // a wave takes every fourth tile
+constexpr int kThreads = 512;
+constexpr int kWaves = kThreads / 64;
+constexpr int kSteps = kTiles / kWaves;  // a wave takes every eighth tile
 
 // (value, lowest index first) as a key whose unsigned order is the choice's, 0 below all.
 // + 0 joins the zeros, which compare equal.
@@ -35,6 +37,27 @@ __device__ __forceinline__ uint64_t key_of(float v, int index) {
 __device__ __forceinline__ float key_value(uint64_t k) {
   const uint32_t order = static_cast<uint32_t>(k >> 32);
   return f32_of(order & 0x80000000u ? order & 0x7FFFFFFFu : ~order);
+}
+
+// Scratch of a lane tile: kSubs + 1 units of 16 keys and a count, 256 bytes each.
+constexpr int kSubs = 16;
+constexpr int kUnit = 32;
+
+// A wave's keys (lane t's: row t) enter a unit; true in the last of `members` workgroups, whose
+// k are then the largest of all.
+__device__ __forceinline__ bool join(unsigned long long* unit, bool live, uint64_t& k, int members) {
+  if (live && k) {
+    const unsigned long long before = __hip_atomic_fetch_max(unit + threadIdx.x, static_cast<unsigned long long>(k), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("" ::"v"(before));
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // they have been performed
+  int ended = 0;
+  if (threadIdx.x == 0)
+    ended = __hip_atomic_fetch_add(unit + 16, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == static_cast<unsigned long long>(members - 1);
+  if (!__builtin_amdgcn_readfirstlane(ended)) return false;
+  if (live) k = __hip_atomic_exchange(unit + threadIdx.x, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (threadIdx.x == 0) __hip_atomic_exchange(unit + 16, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return true;
 }
 
 // First entry of the ascending list t[lo, hi) that is not below x.
@@ -50,11 +73,10 @@ __device__ __forceinline__ int lower_bound(const int32_t* t, int lo, int hi, int
 // Workgroup: lane tile lt, tokens [t0, t0 + kTokens). Thread: four lanes of a token in each
 // of its steps, as the tiles lie. Lane tiles of a chunk have neighbouring workgroups.
 template <bool COUNTS, bool BIAS>
-__global__ __launch_bounds__(256) void k_process(StrideLogitsParams p, int row_tiles, int chunks) {
+__global__ __launch_bounds__(kThreads) void k_process(StrideLogitsParams p, int row_tiles, int chunks) {
   __shared__ __align__(16) uint32_t seen[kWords][16], allowed[kWords][16], biased[kWords][16];
   __shared__ float bias[BIAS ? kTokens : 1][16];
-  __shared__ uint64_t best[4][16];
-  __shared__ int last;
+  __shared__ uint64_t best[kWaves][16];
   const int lt = blockIdx.x % p.l.lane_groups, chunk = blockIdx.x / p.l.lane_groups;
   const int t0 = chunk * kTokens;
   const int t = threadIdx.x, wave = t >> 6, lane = t & 63, quad = t & 3, tok = (t >> 2) & 15;
@@ -66,67 +88,66 @@ __global__ __launch_bounds__(256) void k_process(StrideLogitsParams p, int row_t
   const int64_t step = static_cast<int64_t>(p.l.lane_groups) * kTileElems;
   const float* in = p.logits + rt0 * step + lt * kTileElems + tok * 16 + quad * 4;
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    const int tile = 4 * i + wave;
-    v[i] = f32x4{0, 0, 0, 0};
-    if (rt0 + tile < row_tiles) v[i] = *reinterpret_cast<const f32x4*>(in + tile * step);
-  }
-  {  // a word a thread: lane t % 16, word t / 16
-    const int row = lt * 16 + (t & 15), w = (t0 >> 5) + (t >> 4);
-    uint32_t s = 0, a = 0xFFFFFFFFu;
-    if (row < p.l.rows && w < words) {
+  for (int i = 0; i < kSteps; ++i)
+    v[i] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(in + min(kWaves * i + wave, row_tiles - 1 - rt0) * step));
+  // A word a thread, lane t % 16 and word t / 16 % 16: the first half of the workgroup the
+  // seen bits, the second the mask's. Sixteen threads a lane look for its biases in the range.
+  uint32_t bits = t < 256 ? 0u : 0xFFFFFFFFu;
+  const int row = lt * 16 + (t & 15), w = (t0 >> 5) + ((t >> 4) & 15);
+  if (row < p.l.rows && w < words) {
+    if (t < 256) {
       if constexpr (COUNTS) {
         const int slot = p.row_slot[row];
-        if (slot >= 0 && slot < p.slots) s = p.seen[static_cast<int64_t>(slot) * words + w];
+        if (slot >= 0 && slot < p.slots) bits = p.seen[static_cast<int64_t>(slot) * words + w];
       }
-      if (p.mask) {
-        const int m = p.mask_row[row];
-        if (m >= 0 && m < p.masks) a = p.mask[static_cast<int64_t>(m) * words + w];
-      }
+    } else if (p.mask) {
+      const int m = p.mask_row[row];
+      if (m >= 0 && m < p.masks) bits = p.mask[static_cast<int64_t>(m) * words + w];
     }
-    seen[t >> 4][t & 15] = s;
-    allowed[t >> 4][t & 15] = a;
-    biased[t >> 4][t & 15] = 0;
   }
-  __syncthreads();
-  if constexpr (BIAS) {  // sixteen threads a lane look for its entries in the range
-    const int ln = t >> 4, row = lt * 16 + ln;
-    if (row < p.l.rows) {
-      int lo = p.bias_offsets[row], hi = p.bias_offsets[row + 1];
+  float rep[4], pres[4], freq[4];
+  const int32_t* counts[4];
+  if constexpr (COUNTS) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = min(lt * 16 + quad * 4 + e, p.l.rows - 1);
+      rep[e] = p.penalties[3 * r];
+      pres[e] = p.penalties[3 * r + 1];
+      freq[e] = p.penalties[3 * r + 2];
+      const int slot = p.row_slot[r];
+      counts[e] = p.counts + static_cast<int64_t>(slot >= 0 && slot < p.slots ? slot : 0) * p.vocab;
+    }
+  }
+  if constexpr (BIAS) {
+    if (t < 256) biased[t >> 4][t & 15] = 0;
+    __syncthreads();
+    const int ln = t >> 5, r = lt * 16 + ln;
+    if (r < p.l.rows) {
+      int lo = p.bias_offsets[r], hi = p.bias_offsets[r + 1];
       const int end = hi;
       if (hi - lo > 256) {
         lo = lower_bound(p.bias_tokens, lo, hi, t0);
         hi = lower_bound(p.bias_tokens, lo, hi, t0 + kTokens);
       }
-      for (int e = lo + (t & 15); e < hi; e += 16) {
-        const int token = p.bias_tokens[e], at = token - t0;
-        if (at < 0 || at >= kTokens || token >= p.vocab || (e + 1 < end && p.bias_tokens[e + 1] == token)) continue;
-        bias[at][ln] = p.bias_values[e];
+      for (int e = lo + (t & 31); e < hi; e += 32) {
+        const int token = p.bias_tokens[e], next = p.bias_tokens[min(e + 1, end - 1)], at = token - t0;
+        const float b = p.bias_values[e];
+        if (at < 0 || at >= kTokens || token >= p.vocab || (e + 1 < end && next == token)) continue;
+        bias[at][ln] = b;
         atomicOr(&biased[at >> 5][ln], 1u << (at & 31));
       }
     }
-    __syncthreads();
   }
+  if (t < 256) seen[(t >> 4) & 15][t & 15] = bits;
+  else allowed[(t >> 4) & 15][t & 15] = bits;
+  __syncthreads();
 
-  float rep[4] = {1, 1, 1, 1}, pres[4] = {0, 0, 0, 0}, freq[4] = {0, 0, 0, 0};
-  const int32_t* counts[4] = {nullptr, nullptr, nullptr, nullptr};
-  if constexpr (COUNTS) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int row = min(lt * 16 + quad * 4 + e, p.l.rows - 1);
-      rep[e] = p.penalties[3 * row];
-      pres[e] = p.penalties[3 * row + 1];
-      freq[e] = p.penalties[3 * row + 2];
-      const int slot = p.row_slot[row];
-      counts[e] = p.counts + static_cast<int64_t>(slot >= 0 && slot < p.slots ? slot : 0) * p.vocab;
-    }
-  }
   // every wanted count is under way before the first is used
   int n[kSteps][4];
   if constexpr (COUNTS) {
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      const int at = (4 * i + wave) * 16 + tok;
+      const int at = (kWaves * i + wave) * 16 + tok;
       const u32x4 s = *reinterpret_cast<const u32x4*>(&seen[at >> 5][4 * quad]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -137,10 +158,11 @@ __global__ __launch_bounds__(256) void k_process(StrideLogitsParams p, int row_t
   }
   float top[4] = {f32_of(0xFF800000u), f32_of(0xFF800000u), f32_of(0xFF800000u), f32_of(0xFF800000u)};
   int who[4] = {-1, -1, -1, -1};
+  const int rows = p.l.rows - (lt * 16 + quad * 4);
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
-    const int tile = 4 * i + wave, at = tile * 16 + tok, token = t0 + at;
-    if (token >= p.vocab) continue;
+    const int tile = kWaves * i + wave, at = tile * 16 + tok, token = t0 + at;
+    const bool real = token < p.vocab;
     const u32x4 a = *reinterpret_cast<const u32x4*>(&allowed[at >> 5][4 * quad]);
     u32x4 b = {0, 0, 0, 0};
     if constexpr (BIAS) b = *reinterpret_cast<const u32x4*>(&biased[at >> 5][4 * quad]);
@@ -162,15 +184,14 @@ __global__ __launch_bounds__(256) void k_process(StrideLogitsParams p, int row_t
       }
       if (!((a[e] >> (at & 31)) & 1u)) l = f32_of(0xFF800000u);
       v[i][e] = l;
-      if (l > top[e]) {
+      if (real && l > top[e]) {
         top[e] = l;
         who[e] = token;
       }
     }
-    if (p.out) {
+    if (p.out && real) {
       float* out = p.out + (rt0 + tile) * step + lt * kTileElems + tok * 16 + quad * 4;
-      const int rows = p.l.rows - (lt * 16 + quad * 4);
-      if (rows >= 4) *reinterpret_cast<f32x4*>(out) = v[i];
+      if (rows >= 4) __builtin_nontemporal_store(v[i], reinterpret_cast<f32x4*>(out));
       else
         for (int e = 0; e < 3; ++e)
           if (e < rows) out[e] = v[i][e];
@@ -188,32 +209,28 @@ __global__ __launch_bounds__(256) void k_process(StrideLogitsParams p, int row_t
     if (lane < 4) best[wave][4 * quad + e] = k;
   }
   __syncthreads();
-  // Joined in scratch; the lane tile's last workgroup writes the result and leaves zeros.
-  unsigned long long* keys = reinterpret_cast<unsigned long long*>(p.scratch) + lt * 16;
-  unsigned long long* arrived = reinterpret_cast<unsigned long long*>(p.scratch) + p.l.lane_groups * 16 + lt;
-  if (t < 16) {
-    uint64_t k = best[0][t];
+  // Joined in scratch by atomics alone, which are performed where all workgroups see them; a
+  // fence would write back the L2's dirty lines, the logits among them (128 rows 110 us with
+  // fences, 45 without). In two stages of at most kSubs and 1 / kSubs of the workgroups each,
+  // since atomics on one address queue up. The last workgroup of a stage takes its keys out,
+  // which leaves zeros, and the very last one writes the result.
+  if (t >= 64) return;
+  const int row_of_key = lt * 16 + t;
+  const bool live = t < 16 && row_of_key < p.l.rows;
+  uint64_t k = 0;
+  if (live)
 #pragma unroll
-    for (int w = 1; w < 4; ++w) k = best[w][t] > k ? best[w][t] : k;
-    if (k) atomicMax(&keys[t], static_cast<unsigned long long>(k));
-    __threadfence();
+    for (int x = 0; x < kWaves; ++x) k = best[x][t] > k ? best[x][t] : k;
+  unsigned long long* unit = reinterpret_cast<unsigned long long*>(p.scratch) + static_cast<int64_t>(lt) * (kSubs + 1) * kUnit;
+  const int sub = chunk % kSubs;
+  if (!join(unit + (1 + sub) * kUnit, live, k, (chunks - sub + kSubs - 1) / kSubs)) return;
+  if (!join(unit, live, k, min(kSubs, chunks))) return;
+  if (live) {
+    StrideBestEntry e;
+    e.value = k ? key_value(k) : f32_of(0xFF800000u);
+    e.index = k ? static_cast<int32_t>(~static_cast<uint32_t>(k)) : -1;
+    p.best[row_of_key] = e;
   }
-  __syncthreads();
-  if (t == 0) last = atomicAdd(arrived, 1ull) == static_cast<unsigned long long>(chunks - 1);
-  __syncthreads();
-  if (!last) return;
-  __threadfence();
-  if (t < 16) {
-    const uint64_t k = atomicExch(&keys[t], 0ull);
-    const int row = lt * 16 + t;
-    if (row < p.l.rows) {
-      StrideBestEntry e;
-      e.value = k ? key_value(k) : f32_of(0xFF800000u);
-      e.index = k ? static_cast<int32_t>(~static_cast<uint32_t>(k)) : -1;
-      p.best[row] = e;
-    }
-  }
-  if (t == 0) atomicExch(arrived, 0ull);
 }
 
 __global__ __launch_bounds__(256) void k_record(StrideTokenCounts p, const int32_t* slots, const int32_t* tokens, int token_stride, int n,
@@ -272,7 +289,7 @@ static_assert(sizeof(StrideTokenCounts) == 24, "TokenCounts layout");
 
 extern "C" {
 
-int64_t stride_logits_scratch(int32_t rows) { return rows < 0 ? -1 : (static_cast<int64_t>(rows) + 15) / 16 * 17; }
+int64_t stride_logits_scratch(int32_t rows) { return rows < 0 ? -1 : (static_cast<int64_t>(rows) + 15) / 16 * (kSubs + 1) * kUnit; }
 
 int stride_logits_process(const StrideLogitsParams* p, void* stream) {
   const char* what = "logits_process";
@@ -288,7 +305,7 @@ int stride_logits_process(const StrideLogitsParams* p, void* stream) {
   const int row_tiles = (p->vocab + 15) / 16, chunks = (row_tiles + kTiles - 1) / kTiles;
   const int64_t groups = static_cast<int64_t>(chunks) * p->l.lane_groups;
   if (groups > INT_MAX) return refused(what, "rows and vocab are too large together");
-  const dim3 grid(static_cast<unsigned>(groups)), block(256);
+  const dim3 grid(static_cast<unsigned>(groups)), block(kThreads);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (p->counts && p->bias_offsets) hipLaunchKernelGGL((k_process<true, true>), grid, block, 0, st, *p, row_tiles, chunks);
   else if (p->counts) hipLaunchKernelGGL((k_process<true, false>), grid, block, 0, st, *p, row_tiles, chunks);

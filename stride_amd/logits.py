@@ -25,12 +25,8 @@ from . import _lib, tc
 from .harness import here
 
 _LOGITS = Struct("<4i13Q3i4x").pack
+UNIT = 17 * 32  # scratch of a lane tile, int64
 IN_PROMPT = -(1 << 31)  # TokenCounts.counts: the token is in the prompt
-
-
-def _run(rc: int) -> None:
-    if rc:
-        _lib.check(rc)
 
 
 def words(vocab: int) -> int:
@@ -53,6 +49,7 @@ class TokenCounts:
         self.slots, self.vocab = (int(x) for x in counts.shape)
         self._params = _lib.TokenCountsParams(tc.ptr(counts), tc.ptr(seen), self.slots, self.vocab)
         self._at = C.addressof(self._params)
+        self._counts_at, self._seen_at, self._device = tc.ptr(counts), tc.ptr(seen), counts.get_device()
         self._scratch = {}
 
     @staticmethod
@@ -60,29 +57,30 @@ class TokenCounts:
         return TokenCounts(torch.zeros((slots, vocab), dtype=torch.int32, device=device),
                            torch.zeros((slots, words(vocab)), dtype=torch.int32, device=device))
 
-    def _items(self, *items) -> int:
-        for t in items:
-            if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != items[0].shape[0] or t.device != self.counts.device:
-                raise ValueError("items are int32 vectors of one length on the counts' device")
-        here(self.counts)
-        return items[0].shape[0]
-
     def record(self, slot, tokens, prompt: bool = False) -> None:
         """Counts tokens[i] for slot[i] (int32 vectors; tokens may be strided, as the indices of
         a BestEntry buffer are); those out of range, -1 among them, are ignored."""
-        n = self._items(slot, tokens)
-        if not slot.is_contiguous():
-            raise ValueError("slot must be contiguous")
-        _run(_lib.load().stride_logits_record(self._at, slot.data_ptr(), tokens.data_ptr(), tokens.stride(0) if n > 1 else 1, n,
-                                              1 if prompt else 0, tc.kernel_stream()))
+        n = slot.numel()
+        if slot.dtype != torch.int32 or tokens.dtype != torch.int32 or tokens.dim() != 1 or tokens.numel() != n \
+                or slot.get_device() != self._device or tokens.get_device() != self._device or not slot.is_contiguous():
+            raise ValueError("slot (contiguous) and tokens are int32 vectors of one length on the counts' device")
+        here(slot)
+        rc = _lib.load().stride_logits_record(self._at, slot.data_ptr(), tokens.data_ptr(), tokens.stride(0) if n > 1 else 1, n,
+                                              1 if prompt else 0, tc.kernel_stream())
+        if rc:
+            _lib.check(rc)
 
     def reset(self, slot, src=None) -> None:
         """slot[i] forgets its tokens, or takes over those of src[i]. A slot to be changed comes
         up once and is no source."""
-        n = self._items(slot) if src is None else self._items(slot, src)
-        if not slot.is_contiguous() or (src is not None and not src.is_contiguous()):
-            raise ValueError("slot and src must be contiguous")
-        _run(_lib.load().stride_logits_reset(self._at, slot.data_ptr(), 0 if src is None else src.data_ptr(), n, tc.kernel_stream()))
+        n = slot.numel()
+        for t in (slot,) if src is None else (slot, src):
+            if t.dtype != torch.int32 or t.numel() != n or t.get_device() != self._device or not t.is_contiguous():
+                raise ValueError("slot and src are contiguous int32 vectors of one length on the counts' device")
+        here(slot)
+        rc = _lib.load().stride_logits_reset(self._at, slot.data_ptr(), 0 if src is None else src.data_ptr(), n, tc.kernel_stream())
+        if rc:
+            _lib.check(rc)
 
 
 def scratch(rows: int, device):
@@ -130,56 +128,63 @@ def process(logits, rows: int, vocab: int, counts: TokenCounts | None = None, ro
     [masks][words], with mask_row int32 [rows] (below 0: no mask). out: receives the processed
     tiles (may be `logits`). work: scratch(rows) (default: one that `counts` keeps for this
     stream, or a new one)."""
+    i32, f32 = torch.int32, torch.float32
     here(logits)
     T = (rows + 15) // 16
-    if logits.dtype != torch.float32 or not logits.is_contiguous() or logits.dim() != 4 or logits.shape[1] != T \
-            or logits.shape[0] * 16 < vocab:
+    shape = logits.shape
+    if logits.dtype != f32 or len(shape) != 4 or shape[1] != T or shape[0] * 16 < vocab or shape[2] != 16 or shape[3] != 16 \
+            or not logits.is_contiguous():
         raise ValueError("logits must be contiguous fp32 tiles [ceil(vocab / 16)][ceil(rows / 16)][16][16]")
-    if out is not None and (out.dtype != torch.float32 or not out.is_contiguous() or out.shape != logits.shape):
-        raise ValueError("out must be tiles like logits")
+    o_at = 0
+    if out is not None:
+        if out.dtype != f32 or out.shape != shape or not out.is_contiguous():
+            raise ValueError("out must be tiles like logits")
+        o_at = out.data_ptr()
     if best is None:
-        best = torch.empty((rows, 2), dtype=torch.int32, device=logits.device)
-    elif best.dtype != torch.int32 or not best.is_contiguous() or best.numel() < 2 * rows:
+        best = torch.empty((rows, 2), dtype=i32, device=logits.device)
+    elif best.dtype != i32 or best.numel() < 2 * rows or not best.is_contiguous():
         raise ValueError("best must be contiguous int32 [rows][2]")
-    c = s = sl = pen = 0
-    slots = 0
+    c = s = sl = pen = slots = 0
     if counts is not None:
-        if counts.vocab != vocab or counts.counts.device != logits.device:
+        if counts.vocab != vocab or counts.counts.get_device() != logits.get_device():
             raise ValueError("the counts are of another vocabulary or device")
         if row_slot is None or penalties is None:
             raise ValueError("counts need row_slot and penalties")
-        if row_slot.dtype != torch.int32 or row_slot.numel() < rows or not row_slot.is_contiguous():
+        if row_slot.dtype != i32 or row_slot.numel() < rows or not row_slot.is_contiguous():
             raise ValueError("row_slot must be contiguous int32 [rows]")
-        if penalties.dtype != torch.float32 or penalties.numel() < 3 * rows or not penalties.is_contiguous():
+        if penalties.dtype != f32 or penalties.numel() < 3 * rows or not penalties.is_contiguous():
             raise ValueError("penalties must be contiguous fp32 [rows][3]")
-        c, s, sl, pen, slots = counts.counts.data_ptr(), counts.seen.data_ptr(), row_slot.data_ptr(), penalties.data_ptr(), counts.slots
+        c, s, sl, pen, slots = counts._counts_at, counts._seen_at, row_slot.data_ptr(), penalties.data_ptr(), counts.slots
     bo = bt = bv = 0
     if bias is not None:
         o, t, v = bias
-        if o.dtype != torch.int32 or t.dtype != torch.int32 or v.dtype != torch.float32 or o.numel() < rows + 1 \
-                or v.numel() != t.numel() or not (o.is_contiguous() and t.is_contiguous() and v.is_contiguous()):
+        n = t.numel()
+        if o.dtype != i32 or t.dtype != i32 or v.dtype != f32 or o.numel() < rows + 1 or v.numel() != n \
+                or not (o.is_contiguous() and t.is_contiguous() and v.is_contiguous()):
             raise ValueError("bias is (offsets int32 [rows + 1], tokens int32, values fp32), contiguous")
-        if t.numel():  # without entries there is nothing to add
+        if n:  # without entries there is nothing to add
             bo, bt, bv = o.data_ptr(), t.data_ptr(), v.data_ptr()
     mk = mr = masks = 0
     if mask is not None:
-        if mask.dtype != torch.int32 or mask.dim() != 2 or mask.shape[1] != words(vocab) or not mask.is_contiguous():
+        if mask.dtype != i32 or mask.dim() != 2 or mask.size(1) != (vocab + 31) // 32 or not mask.is_contiguous():
             raise ValueError("mask must be contiguous int32 [masks][ceil(vocab / 32)]")
-        if mask_row is None or mask_row.dtype != torch.int32 or mask_row.numel() < rows or not mask_row.is_contiguous():
+        if mask_row is None or mask_row.dtype != i32 or mask_row.numel() < rows or not mask_row.is_contiguous():
             raise ValueError("a mask needs mask_row, contiguous int32 [rows]")
-        mk, mr, masks = mask.data_ptr(), mask_row.data_ptr(), mask.shape[0]
+        mk, mr, masks = mask.data_ptr(), mask_row.data_ptr(), mask.size(0)
     stream = tc.kernel_stream()
     if work is None:
-        work = _work_of(counts, rows, stream, logits.device)
-    elif work.dtype != torch.int64 or work.numel() < T * 17 or not work.is_contiguous():
+        work = _work_of(counts, T, rows, stream, logits.device)
+    elif work.dtype != torch.int64 or work.numel() < T * UNIT or not work.is_contiguous():
         raise ValueError("work must be scratch(rows)")
-    p = _LOGITS(rows, T, 0, 0, logits.data_ptr(), 0 if out is None else out.data_ptr(), sl, c, s, pen, bo, bt, bv, mk, mr,
-                best.data_ptr(), work.data_ptr(), vocab, slots, masks)
-    _run(_lib.packed().stride_logits_process(p, stream))
+    p = _LOGITS(rows, T, 0, 0, logits.data_ptr(), o_at, sl, c, s, pen, bo, bt, bv, mk, mr, best.data_ptr(), work.data_ptr(),
+                vocab, slots, masks)
+    rc = _lib.packed().stride_logits_process(p, stream)
+    if rc:
+        _lib.check(rc)
     return best
 
 
-def _work_of(counts, rows: int, stream: int, device):
+def _work_of(counts, T: int, rows: int, stream: int, device):
     """A scratch of its own for each stream that uses the counts, kept with them. A captured
     graph must not find it in eager use on another stream: it gets one that is its own."""
     if tc._stream is not None:
@@ -187,6 +192,6 @@ def _work_of(counts, rows: int, stream: int, device):
     if counts is None or torch.cuda.is_current_stream_capturing():
         return scratch(rows, device)
     kept = counts._scratch.get(stream)
-    if kept is None or kept.numel() < (rows + 15) // 16 * 17:
+    if kept is None or kept.numel() < T * UNIT:
         kept = counts._scratch[stream] = scratch(rows, device)
     return kept

@@ -205,7 +205,7 @@ def test_logits_empty_and_sizes():
     p = process(l__rows=0, l__lane_groups=0, logits=0)
     assert lib.stride_logits_process(C.byref(p), None) == 0
     assert lib.stride_logits_process(None, None) == _lib.EINVAL
-    assert [lib.stride_logits_scratch(n) for n in (-1, 0, 1, 16, 17)] == [-1, 0, 17, 17, 34]
+    assert [lib.stride_logits_scratch(n) for n in (-1, 0, 1, 16, 17)] == [-1, 0, logits.UNIT, logits.UNIT, 2 * logits.UNIT]
     c = _lib.TokenCountsParams(BUF, BUF, 4, 1000)
     assert lib.stride_logits_record(C.byref(c), None, None, 1, 0, 0, None) == 0
     assert lib.stride_logits_record(C.byref(c), BUF, BUF, -1, 1, 0, None) == _lib.EINVAL
