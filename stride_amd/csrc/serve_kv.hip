@@ -58,9 +58,9 @@ __device__ __forceinline__ int before_me(int v, int* lds, int& sum) {
     const int o = __shfl_up(x, d);
     if (lane >= d) x += o;
   }
-  __syncthreads();
+  lds_barrier();
   if (lane == 63) lds[wave] = x;
-  __syncthreads();
+  lds_barrier();
   int base = 0;
   sum = 0;
 #pragma unroll
@@ -70,19 +70,43 @@ __device__ __forceinline__ int before_me(int v, int* lds, int& sum) {
   }
   return base + x - v;
 }
+// The same of truth values.
+__device__ __forceinline__ int count_before_me(bool v, int* lds, int& sum) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint64_t all = __ballot(v);
+  lds_barrier();
+  if (lane == 0) lds[wave] = __popcll(all);
+  lds_barrier();
+  int base = 0;
+  sum = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) base += lds[w];
+    sum += lds[w];
+  }
+  return base + __popcll(all & ((uint64_t{1} << lane) - 1));
+}
 
-// The lowest `want` free pages, in order, to free_list. False: there are fewer.
-__device__ __forceinline__ bool list_free(const StrideKvPool& p, int want, int* lds) {
+// Word w of the free pages' bit map, no bits behind the last page.
+__device__ __forceinline__ uint32_t free_word(const StrideKvPool& p, int w) {
+  const int words = (p.pages + 31) / 32;
+  uint32_t bits = w < words ? p.free_bits[w] : 0u;
+  if (w == words - 1 && (p.pages & 31)) bits &= (1u << (p.pages & 31)) - 1u;
+  return bits;
+}
+
+// The lowest `want` free pages, in order, to `list`; `head` is the thread's own first word,
+// which a plan fetches before anything else. False: there are fewer.
+__device__ __forceinline__ bool list_free(const StrideKvPool& p, uint32_t head, int want, int32_t* list, int* lds) {
   const int words = (p.pages + 31) / 32;
   int have = 0;
   for (int w0 = 0; w0 < words && have < want; w0 += kPlan) {
     const int w = w0 + threadIdx.x;
-    uint32_t bits = w < words ? p.free_bits[w] : 0u;
-    if (w == words - 1 && (p.pages & 31)) bits &= (1u << (p.pages & 31)) - 1u;
+    uint32_t bits = w0 == 0 ? head : free_word(p, w);
     int sum;
-    int at = have + before_me(__popc(bits), lds, sum);
+    int at = have + before_me(static_cast<int>(__popc(bits)), lds, sum);
     while (bits && at < want) {
-      free_list(p)[at++] = w * 32 + __ffs(bits) - 1;
+      list[at++] = w * 32 + __ffs(bits) - 1;
       bits &= bits - 1;
     }
     have += sum;
@@ -103,25 +127,86 @@ __device__ __forceinline__ bool mark(uint32_t* bits, int slot) {
 }
 __device__ __forceinline__ bool marked(const uint32_t* bits, int slot) { return (bits[slot >> 5] >> (slot & 31)) & 1u; }
 
-// Ends a plan's checks: the workgroup's errors together. True: none.
+// Ends a plan's checks. True: no thread found anything bad. (Else the call ends here: work[0]
+// is 0 since the plan's start.)
 __device__ __forceinline__ bool agree(const StrideKvPool& p, int bad, int* lds) {
-  __syncthreads();
-  if (threadIdx.x == 0) lds[0] = 0;
-  __syncthreads();
-  if (bad) atomicOr(&lds[0], bad);
-  __syncthreads();
-  const int all = lds[0];
-  if (all && threadIdx.x == 0) atomicOr(p.errors, all);
-  if (threadIdx.x == 0) p.work[0] = all ? 0 : 1;
-  __syncthreads();
-  return all == 0;
+  if (bad) atomicOr(p.errors, bad);
+  int sum;
+  count_before_me(bad != 0, lds, sum);
+  return sum == 0;
 }
 
-// The plan of reserve and compact: items i with table ranges [lo, hi) whose entries want a
-// page where `wants(row, b)`; `give(i, b, page)` takes it. Wave per item, counts first.
+// What a plan workgroup keeps of a call of few items: their table ranges, and the pages that
+// it hands out.
+constexpr int kFewItems = kPlan;
+constexpr int kFewEach = 4;  // table entries a thread
+constexpr int kFewPages = 2048;
+struct Few {
+  int slot[kFewItems], lo[kFewItems], before[kFewItems];  // before: entries of the items before
+  int32_t pages[kFewPages];
+};
+
+// The plan of reserve and compact, for item i with table range [lo, hi) of `slot` (the thread's
+// own one: item threadIdx.x, and `range` for any): an entry wants a page where `wants(entry)`,
+// and `give(i, b, page)` takes it (page < 0: the entry stays). Two ways to the same outcome.
+// Few items and entries: the entries of all items in a row over the threads, each read once and
+// kept (64 items of one entry: 13.7 us the other way, which reads them twice and waits for one
+// item after the other). Else a wave an item, counts first.
 template <class Range, class Wants, class Give>
-__device__ __forceinline__ void share_out(const StrideKvPool& p, int n, int* lds, Range range, Wants wants, Give give) {
+__device__ __forceinline__ void share_out(const StrideKvPool& p, int n, uint32_t head, int* lds, Few& few, int slot0, int lo0, int hi0, Range range,
+                                          Wants wants, Give give) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (n <= kFewItems) {
+    constexpr int kMost = kPlan * kFewEach;
+    int entries;
+    const int size = static_cast<int>(threadIdx.x) < n ? max(0, min(hi0 - lo0, kMost + 1)) : 0;  // exact where they are few
+    const int before = before_me(size, lds, entries);
+    few.slot[threadIdx.x] = slot0, few.lo[threadIdx.x] = lo0, few.before[threadIdx.x] = before;
+    lds_barrier();
+    if (entries <= kMost) {
+      int item[kFewEach], at[kFewEach], entry[kFewEach], place[kFewEach], total = 0;
+      bool want[kFewEach];
+      const int rounds = (entries + kPlan - 1) / kPlan;
+#pragma unroll
+      for (int x = 0; x < kFewEach; ++x) {
+        const int e = x * kPlan + threadIdx.x;
+        item[x] = -1;
+        if (x >= rounds || e >= entries) continue;
+        int a = 0, z = n;  // the last item with before <= e
+        while (z - a > 1) {
+          const int m = (a + z) / 2;
+          if (few.before[m] <= e) a = m;
+          else z = m;
+        }
+        item[x] = a;
+        at[x] = few.lo[a] + e - few.before[a];
+        entry[x] = table_row(p, few.slot[a])[at[x]];
+      }
+#pragma unroll
+      for (int x = 0; x < kFewEach; ++x) want[x] = item[x] >= 0 && wants(entry[x]);
+#pragma unroll
+      for (int x = 0; x < kFewEach; ++x) {
+        if (x >= rounds) continue;
+        int sum;
+        place[x] = total + count_before_me(want[x], lds, sum);
+        total += sum;
+      }
+      int32_t* list = total <= kFewPages ? few.pages : free_list(p);
+      if (total > 0 && !list_free(p, head, total, list, lds)) {
+        if (threadIdx.x == 0) atomicOr(p.errors, STRIDE_KV_NO_PAGES);
+        return;
+      }
+      if (threadIdx.x == 0) p.work[0] = 1;
+#pragma unroll
+      for (int x = 0; x < kFewEach; ++x) {
+        if (item[x] < 0) continue;
+        const int page = want[x] ? list[place[x]] : -1;
+        if (page >= 0) take(p, page);
+        give(item[x], at[x], page);
+      }
+      return;
+    }
+  }
   int32_t* first_of = item_work(p);  // [n]: the item's first place in the list
   for (int i = wave; i < n; i += kWaves) {
     int slot, lo, hi, count = 0;
@@ -142,8 +227,11 @@ __device__ __forceinline__ void share_out(const StrideKvPool& p, int n, int* lds
     total += sum;
   }
   __syncthreads();
-  const bool enough = total == 0 || list_free(p, total, lds);
-  if (!agree(p, enough ? 0 : STRIDE_KV_NO_PAGES, lds)) return;
+  if (total > 0 && !list_free(p, head, total, free_list(p), lds)) {
+    if (threadIdx.x == 0) atomicOr(p.errors, STRIDE_KV_NO_PAGES);
+    return;
+  }
+  if (threadIdx.x == 0) p.work[0] = 1;
   for (int i = wave; i < n; i += kWaves) {
     int slot, lo, hi;
     range(i, slot, lo, hi);
@@ -164,20 +252,24 @@ __device__ __forceinline__ void share_out(const StrideKvPool& p, int n, int* lds
 __global__ __launch_bounds__(kPlan) void k_reserve(StrideKvPool p, const int32_t* slots, const int32_t* first, const int32_t* end, int n) {
   __shared__ uint32_t bits[kMaxSlots / 32];
   __shared__ int lds[kWaves];
+  __shared__ Few few;
+  const uint32_t head = free_word(p, threadIdx.x);
+  int slot0 = 0, lo0 = 0, hi0 = 0;
+  auto range = [&](int i, int& s, int& lo, int& hi) { s = slots[i], lo = first[i], hi = end[i]; };
+  if (static_cast<int>(threadIdx.x) < n) range(threadIdx.x, slot0, lo0, hi0);
   for (int i = threadIdx.x; i < (p.slots + 31) / 32; i += kPlan) bits[i] = 0;
-  __syncthreads();
+  lds_barrier();
   int bad = 0;
   for (int i = threadIdx.x; i < n; i += kPlan) {
-    const int s = slots[i];
-    if (s < 0 || s >= p.slots || first[i] < 0 || end[i] > p.kv.max_blocks) bad |= STRIDE_KV_BAD_ITEM;
+    int s = slot0, lo = lo0, hi = hi0;
+    if (i >= kPlan) range(i, s, lo, hi);
+    if (s < 0 || s >= p.slots || lo < 0 || hi > p.kv.max_blocks) bad |= STRIDE_KV_BAD_ITEM;
     else if (mark(bits, s)) bad |= STRIDE_KV_TWICE;
   }
   if (!agree(p, bad, lds)) return;
-  share_out(
-      p, n, lds, [&](int i, int& s, int& lo, int& hi) { s = slots[i], lo = first[i], hi = end[i]; }, [](int b) { return b < 0; },
-      [&](int i, int b, int page) {
-        if (page >= 0) table_row(p, slots[i])[b] = page;
-      });
+  share_out(p, n, head, lds, few, slot0, lo0, hi0, range, [](int b) { return b < 0; }, [&](int i, int b, int page) {
+    if (page >= 0) table_row(p, slots[i])[b] = page;
+  });
 }
 
 __global__ __launch_bounds__(256) void k_release(StrideKvPool p, const int32_t* slots, const int32_t* first, const int32_t* end) {
@@ -200,33 +292,43 @@ __global__ __launch_bounds__(kPlan) void k_fork_plan(StrideKvPool p, const int32
                                                      int n, int page_shift) {
   __shared__ uint32_t to[kMaxSlots / 32];
   __shared__ int lds[kWaves];
+  const uint32_t head = free_word(p, threadIdx.x);
+  int a0 = 0, b0 = 0, len0 = 0;
+  if (static_cast<int>(threadIdx.x) < n) a0 = src[threadIdx.x], b0 = dst[threadIdx.x], len0 = length[threadIdx.x];
   for (int i = threadIdx.x; i < (p.slots + 31) / 32; i += kPlan) to[i] = 0;
-  __syncthreads();
+  if (threadIdx.x == 0) p.work[0] = 0;
+  lds_barrier();
   int bad = 0;
   for (int i = threadIdx.x; i < n; i += kPlan) {
-    const int a = src[i], b = dst[i], len = length[i];
+    int a = a0, b = b0, len = len0;
+    if (i >= kPlan) a = src[i], b = dst[i], len = length[i];
     if (a < 0 || a >= p.slots || b < 0 || b >= p.slots || len < 0 || len > static_cast<int64_t>(p.kv.max_blocks) << page_shift)
       bad |= STRIDE_KV_BAD_ITEM;
     else if (mark(to, b)) bad |= STRIDE_KV_TWICE;
   }
-  __syncthreads();
+  lds_barrier();
   for (int i = threadIdx.x; i < n; i += kPlan) {
-    const int a = src[i];
+    const int a = i >= kPlan ? src[i] : a0;
     if (a >= 0 && a < p.slots && marked(to, a)) bad |= STRIDE_KV_TWICE;
   }
   if (!agree(p, bad, lds)) return;
-  auto wants = [&](int i) { return (length[i] & ((1 << page_shift) - 1)) && is_page(p, table_row(p, src[i])[length[i] >> page_shift]); };
   int total = 0;
   for (int i0 = 0; i0 < n; i0 += kPlan) {
     const int i = i0 + threadIdx.x;
-    const bool w = i < n && wants(i);
+    int a = a0, len = len0;
+    if (i0 > 0 && i < n) a = src[i], len = length[i];
+    const bool w = i < n && (len & ((1 << page_shift) - 1)) && is_page(p, table_row(p, a)[len >> page_shift]);
     int sum;
-    const int at = total + before_me(w ? 1 : 0, lds, sum);
+    const int at = total + count_before_me(w, lds, sum);
     if (i < n) item_work(p)[i] = w ? at : -1;
     total += sum;
   }
+  if (total > 0 && !list_free(p, head, total, free_list(p), lds)) {
+    if (threadIdx.x == 0) atomicOr(p.errors, STRIDE_KV_NO_PAGES);
+    return;
+  }
   __syncthreads();
-  if (!agree(p, total == 0 || list_free(p, total, lds) ? 0 : STRIDE_KV_NO_PAGES, lds)) return;
+  if (threadIdx.x == 0) p.work[0] = 1;
   for (int i = threadIdx.x; i < n; i += kPlan) {
     const int at = item_work(p)[i];
     if (at < 0) continue;
@@ -296,74 +398,113 @@ __global__ __launch_bounds__(kPlan) void k_compact_plan(StrideKvPool p, const in
                                                         int n, int page_shift, int width) {
   __shared__ uint32_t bits[kMaxSlots / 32];
   __shared__ int lds[kWaves];
+  __shared__ Few few;
+  const uint32_t head = free_word(p, threadIdx.x);
+  // the pages that kept positions move into
+  auto pages = [&](int f, int c, int& lo, int& hi) {
+    lo = f >> page_shift;
+    hi = c ? (f + c + (1 << page_shift) - 1) >> page_shift : lo;
+  };
+  int slot0 = 0, f0 = 0, c0 = 0;
+  if (static_cast<int>(threadIdx.x) < n) slot0 = slots[threadIdx.x], f0 = first[threadIdx.x], c0 = count[threadIdx.x];
   for (int i = threadIdx.x; i < (p.slots + 31) / 32; i += kPlan) bits[i] = 0;
-  __syncthreads();
+  if (threadIdx.x == 0) p.work[0] = 0;
+  lds_barrier();
   int bad = 0;
   for (int i = threadIdx.x; i < n; i += kPlan) {
-    const int s = slots[i];
-    if (s < 0 || s >= p.slots || first[i] < 0 || count[i] < 0 || count[i] > width ||
-        static_cast<int64_t>(first[i]) + count[i] > static_cast<int64_t>(p.kv.max_blocks) << page_shift)
+    int s = slot0, f = f0, c = c0;
+    if (i >= kPlan) s = slots[i], f = first[i], c = count[i];
+    if (s < 0 || s >= p.slots || f < 0 || c < 0 || c > width || static_cast<int64_t>(f) + c > static_cast<int64_t>(p.kv.max_blocks) << page_shift)
       bad |= STRIDE_KV_BAD_ITEM;
     else if (mark(bits, s)) bad |= STRIDE_KV_TWICE;
   }
   if (!agree(p, bad, lds)) return;
+  int lo0, hi0;
+  pages(f0, c0, lo0, hi0);
   share_out(
-      p, n, lds,
+      p, n, head, lds, few, slot0, lo0, hi0,
       [&](int i, int& s, int& lo, int& hi) {
         s = slots[i];
-        lo = first[i] >> page_shift;
-        hi = count[i] ? (first[i] + count[i] + (1 << page_shift) - 1) >> page_shift : lo;
+        pages(first[i], count[i], lo, hi);
       },
       [&](int b) { return !is_page(p, b) || p.refs[b] > 1; }, [&](int i, int b, int page) { new_row(p, n, i)[b] = page; });
 }
 
-// Moves one run (a layer, K or V, a group) of an item's kept positions. In place it must not
-// write what is still to be read: positions ascend and each comes from its own place or a
-// later one, so a workgroup that takes them in ascending steps, loads a step whole before it
-// writes it, overwrites only what it has read.
-template <int U>
+// Moves runs (a layer, K or V, a group) of an item's kept positions: `group` runs a workgroup,
+// `step` positions at a time, at most kHold 16-byte pieces a thread. In place it must not write
+// what is still to be read: positions ascend and each comes from its own place or a later one,
+// so a workgroup that takes them in ascending steps, loads a step whole before it writes it,
+// overwrites only what it has read. While a step's pieces are on their way the next one's pages
+// are looked up, one position a thread, and left in LDS for the threads that share it.
+constexpr int kHold = 8;
+constexpr int kStepMax = 256;
+
 __global__ __launch_bounds__(256) void k_compact_move(StrideKvPool p, const int32_t* slots, const int32_t* first, const int32_t* count,
-                                                      const int32_t* keep, int64_t keep_stride, int n, int page_shift, int pieces) {
+                                                      const int32_t* keep, int64_t keep_stride, int n, int page_shift, int pieces, int step,
+                                                      int group) {
   if (p.work[0] == 0) return;
+  __shared__ int64_t from[2][kStepMax], to[2][kStepMax];  // byte offsets of a position in its run's arena; below 0: nothing
   const Runs runs = runs_of(p);
-  const int i = blockIdx.x / runs.count, run = blockIdx.x % runs.count, t = threadIdx.x;
+  const int groups = (runs.count + group - 1) / group;
+  const int i = blockIdx.x / groups, run0 = blockIdx.x % groups * group, t = threadIdx.x;
   const int begin = first[i], many = count[i], in_page = (1 << page_shift) - 1;
   if (many == 0) return;
   const int32_t* row = table_row(p, slots[i]);
   const int32_t* fresh = new_row(p, n, i);
   const int32_t* list = keep + i * keep_stride;
-  char* base = static_cast<char*>(p.kv.arena) + runs.at(run);
+  char* arena = static_cast<char*>(p.kv.arena);
   const int64_t block = p.kv.block_elems * p.elem_bytes;
   const int cap = p.kv.max_blocks << page_shift, row_bytes = pieces * 16;
   // a page that is replaced takes along what it holds before `begin`
   const int lead = fresh[begin >> page_shift] >= 0 ? begin & in_page : 0;
-  const int per = 256 / pieces;  // positions of a load
-  const int in = t % pieces * 16, at = t / pieces;
   int bad = 0;
-  for (int k0 = -lead; k0 < many; k0 += per * U) {
-    u32x4 v[U];
-    bool ok[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = k0 + u * per + at;
-      ok[u] = at < per && k < many;
-      if (!ok[u]) continue;
-      const int from = k < 0 ? begin + k : list[k];
-      if (from < begin + k || from >= cap || (k > 0 && list[k - 1] >= from)) bad |= STRIDE_KV_BAD_KEEP;
-      const int page = from >= 0 && from < cap ? row[from >> page_shift] : -1;
-      ok[u] = is_page(p, page);
-      if (ok[u]) v[u] = load16(base + page * block + static_cast<int64_t>(from & in_page) * row_bytes + in);
-      else if (k >= 0) bad |= STRIDE_KV_MISSING;
+  auto look = [&](int k0, int b) {
+    const int k = k0 + t;
+    if (t >= step) return;
+    int64_t f = -1, d = -1;
+    if (k < many) {
+      const int pos = begin + k, src = k < 0 ? pos : list[k];
+      const int here = row[pos >> page_shift], other = fresh[pos >> page_shift];
+      if (src < pos || src >= cap || (k > 0 && list[k - 1] >= src)) bad |= STRIDE_KV_BAD_KEEP;
+      const int page = src >= 0 && src < cap ? row[src >> page_shift] : -1;
+      if (is_page(p, page)) {
+        f = page * block + static_cast<int64_t>(src & in_page) * row_bytes;
+        d = (other >= 0 ? other : here) * block + static_cast<int64_t>(pos & in_page) * row_bytes;
+      } else if (k >= 0) {
+        bad |= STRIDE_KV_MISSING;
+      }
     }
+    from[b][t] = f;
+    to[b][t] = d;
+  };
+  // this thread's pieces: of run run0 + r, position q of a step, piece `in`
+  const int all = min(group, runs.count - run0) * step * pieces;
+  int64_t base[kHold];
+  int place[kHold];
+#pragma unroll
+  for (int u = 0; u < kHold; ++u) {
+    const int e = u * 256 + t, r = e / (step * pieces), q = e / pieces % step;
+    place[u] = e < all ? q : -1;
+    base[u] = e < all ? runs.at(run0 + r) + e % pieces * 16 : 0;
+  }
+  look(-lead, 0);
+  __syncthreads();
+  int b = 0;
+  for (int k0 = -lead; k0 < many; k0 += step, b ^= 1) {
+    u32x4 v[kHold];
+    int64_t d[kHold];  // taken before the barrier: after it the other waves write the next step's
+#pragma unroll
+    for (int u = 0; u < kHold; ++u) {
+      const int64_t f = place[u] >= 0 ? from[b][place[u]] : -1;
+      d[u] = f >= 0 ? to[b][place[u]] : -1;
+      if (f >= 0) v[u] = load16(arena + base[u] + f);
+    }
+    if (k0 + step < many) look(k0 + step, b ^ 1);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the step is read before any wave writes it
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (!ok[u]) continue;
-      const int to = begin + k0 + u * per + at;
-      const int page = fresh[to >> page_shift] >= 0 ? fresh[to >> page_shift] : row[to >> page_shift];
-      *reinterpret_cast<u32x4*>(base + page * block + static_cast<int64_t>(to & in_page) * row_bytes + in) = v[u];
-    }
+    for (int u = 0; u < kHold; ++u)
+      if (d[u] >= 0) *reinterpret_cast<u32x4*>(arena + base[u] + d[u]) = v[u];
   }
   if (bad) atomicOr(p.errors, bad);
 }
@@ -394,6 +535,7 @@ __global__ __launch_bounds__(kPlan) void k_copy_plan(StrideKvPool p, const int32
                                                      int to_pages, int same, int page_tokens) {
   __shared__ int lds[kWaves];
   uint32_t* bits = reinterpret_cast<uint32_t*>(free_list(p));
+  if (threadIdx.x == 0) p.work[0] = 0;
   for (int i = threadIdx.x; i < (to_pages + 31) / 32; i += kPlan) bits[i] = 0;
   __syncthreads();
   int bad = 0;
@@ -406,7 +548,7 @@ __global__ __launch_bounds__(kPlan) void k_copy_plan(StrideKvPool p, const int32
   if (same)
     for (int i = threadIdx.x; i < n; i += kPlan)
       if (is_page(p, src[i]) && src[i] < to_pages && marked(bits, src[i])) bad |= STRIDE_KV_TWICE;
-  agree(p, bad, lds);
+  if (agree(p, bad, lds) && threadIdx.x == 0) p.work[0] = 1;
 }
 
 __global__ __launch_bounds__(256) void k_copy(StrideKvPool p, char* to, const int32_t* src, const int32_t* dst, const int32_t* tokens,
@@ -521,8 +663,13 @@ int stride_kv_compact(const StrideKvPool* p, const int32_t* slot, const int32_t*
   hipStream_t st = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(k_compact_plan, dim3(1), dim3(kPlan), 0, st, *p, slot, first, count, n, shift, width);
   if (int rc = launched("kv_compact (plan)")) return rc;
-  hipLaunchKernelGGL((k_compact_move<4>), dim3(static_cast<unsigned>(runs * n)), dim3(256), 0, st, *p, slot, first, count, keep, keep_stride, n,
-                     shift, p->kv.head_dim * p->elem_bytes / 16);
+  // Positions a step and runs a workgroup: short lists (a few accepted tokens) share a
+  // workgroup's threads, and its lookups, between runs.
+  const int pieces = p->kv.head_dim * p->elem_bytes / 16, most = 256 * kHold / pieces;
+  const int step = static_cast<int>(std::min<int64_t>(std::min(kStepMax, most), std::max<int64_t>(1, static_cast<int64_t>(width) + (1 << shift) - 1)));
+  const int group = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(runs, most / step)));
+  hipLaunchKernelGGL(k_compact_move, dim3(static_cast<unsigned>((runs + group - 1) / group * n)), dim3(256), 0, st, *p, slot, first, count, keep,
+                     keep_stride, n, shift, pieces, step, group);
   if (int rc = launched("kv_compact (move)")) return rc;
   hipLaunchKernelGGL(k_compact_finish, dim3(n), dim3(256), 0, st, *p, slot, first, count, n, shift);
   return launched("kv_compact");
