@@ -96,8 +96,9 @@ __device__ __forceinline__ uint32_t free_word(const StrideKvPool& p, int w) {
 }
 
 // The lowest `want` free pages, in order, to `list`; `head` is the thread's own first word,
-// which a plan fetches before anything else. False: there are fewer.
-__device__ __forceinline__ bool list_free(const StrideKvPool& p, uint32_t head, int want, int32_t* list, int* lds) {
+// which a plan fetches before anything else, and `left` what remains of it. False: there are
+// fewer.
+__device__ __forceinline__ bool list_free(const StrideKvPool& p, uint32_t head, int want, int32_t* list, int* lds, uint32_t& left) {
   const int words = (p.pages + 31) / 32;
   int have = 0;
   for (int w0 = 0; w0 < words && have < want; w0 += kPlan) {
@@ -109,16 +110,21 @@ __device__ __forceinline__ bool list_free(const StrideKvPool& p, uint32_t head, 
       list[at++] = w * 32 + __ffs(bits) - 1;
       bits &= bits - 1;
     }
+    if (w0 == 0) left = bits;
     have += sum;
   }
   __syncthreads();
   return have >= want;
 }
 
-// A page of the list is taken: its first reference.
+// A page of the list is taken: its first reference. The first words' bits are cleared by the
+// threads that hold them (close_head), not one by one.
 __device__ __forceinline__ void take(const StrideKvPool& p, int page) {
   p.refs[page] = 1;
-  atomicAnd(&p.free_bits[page >> 5], ~(1u << (page & 31)));
+  if (page >= kPlan * 32) atomicAnd(&p.free_bits[page >> 5], ~(1u << (page & 31)));
+}
+__device__ __forceinline__ void close_head(const StrideKvPool& p, uint32_t head, uint32_t left) {
+  if (left != head) p.free_bits[threadIdx.x] = left;
 }
 
 // Marks slot in the bit map of an LDS array; true where it was marked before.
@@ -148,7 +154,7 @@ struct Few {
 
 // The plan of reserve and compact, for item i with table range [lo, hi) of `slot` (the thread's
 // own one: item threadIdx.x, and `range` for any): an entry wants a page where `wants(entry)`,
-// and `give(i, b, page)` takes it (page < 0: the entry stays). Two ways to the same outcome.
+// and `give(i, slot, b, page)` takes it (page < 0: the entry stays). Two ways to the same outcome.
 // Few items and entries: the entries of all items in a row over the threads, each read once and
 // kept (64 items of one entry: 13.7 us the other way, which reads them twice and waits for one
 // item after the other). Else a wave an item, counts first.
@@ -192,17 +198,19 @@ __device__ __forceinline__ void share_out(const StrideKvPool& p, int n, uint32_t
         total += sum;
       }
       int32_t* list = total <= kFewPages ? few.pages : free_list(p);
-      if (total > 0 && !list_free(p, head, total, list, lds)) {
+      uint32_t left = head;
+      if (total > 0 && !list_free(p, head, total, list, lds, left)) {
         if (threadIdx.x == 0) atomicOr(p.errors, STRIDE_KV_NO_PAGES);
         return;
       }
+      close_head(p, head, left);
       if (threadIdx.x == 0) p.work[0] = 1;
 #pragma unroll
       for (int x = 0; x < kFewEach; ++x) {
         if (item[x] < 0) continue;
         const int page = want[x] ? list[place[x]] : -1;
         if (page >= 0) take(p, page);
-        give(item[x], at[x], page);
+        give(item[x], few.slot[item[x]], at[x], page);
       }
       return;
     }
@@ -227,10 +235,12 @@ __device__ __forceinline__ void share_out(const StrideKvPool& p, int n, uint32_t
     total += sum;
   }
   __syncthreads();
-  if (total > 0 && !list_free(p, head, total, free_list(p), lds)) {
+  uint32_t left = head;
+  if (total > 0 && !list_free(p, head, total, free_list(p), lds, left)) {
     if (threadIdx.x == 0) atomicOr(p.errors, STRIDE_KV_NO_PAGES);
     return;
   }
+  close_head(p, head, left);
   if (threadIdx.x == 0) p.work[0] = 1;
   for (int i = wave; i < n; i += kWaves) {
     int slot, lo, hi;
@@ -243,7 +253,7 @@ __device__ __forceinline__ void share_out(const StrideKvPool& p, int n, uint32_t
       const uint64_t all = __ballot(w);
       const int page = w ? free_list(p)[at + __popcll(all & ((uint64_t{1} << lane) - 1))] : -1;
       if (w) take(p, page);
-      if (b < hi) give(i, b, page);
+      if (b < hi) give(i, slot, b, page);
       at += __popcll(all);
     }
   }
@@ -267,8 +277,8 @@ __global__ __launch_bounds__(kPlan) void k_reserve(StrideKvPool p, const int32_t
     else if (mark(bits, s)) bad |= STRIDE_KV_TWICE;
   }
   if (!agree(p, bad, lds)) return;
-  share_out(p, n, head, lds, few, slot0, lo0, hi0, range, [](int b) { return b < 0; }, [&](int i, int b, int page) {
-    if (page >= 0) table_row(p, slots[i])[b] = page;
+  share_out(p, n, head, lds, few, slot0, lo0, hi0, range, [](int b) { return b < 0; }, [&](int, int s, int b, int page) {
+    if (page >= 0) table_row(p, s)[b] = page;
   });
 }
 
@@ -323,10 +333,12 @@ __global__ __launch_bounds__(kPlan) void k_fork_plan(StrideKvPool p, const int32
     if (i < n) item_work(p)[i] = w ? at : -1;
     total += sum;
   }
-  if (total > 0 && !list_free(p, head, total, free_list(p), lds)) {
+  uint32_t left = head;
+  if (total > 0 && !list_free(p, head, total, free_list(p), lds, left)) {
     if (threadIdx.x == 0) atomicOr(p.errors, STRIDE_KV_NO_PAGES);
     return;
   }
+  close_head(p, head, left);
   __syncthreads();
   if (threadIdx.x == 0) p.work[0] = 1;
   for (int i = threadIdx.x; i < n; i += kPlan) {
@@ -427,7 +439,7 @@ __global__ __launch_bounds__(kPlan) void k_compact_plan(StrideKvPool p, const in
         s = slots[i];
         pages(first[i], count[i], lo, hi);
       },
-      [&](int b) { return !is_page(p, b) || p.refs[b] > 1; }, [&](int i, int b, int page) { new_row(p, n, i)[b] = page; });
+      [&](int b) { return !is_page(p, b) || p.refs[b] > 1; }, [&](int i, int, int b, int page) { new_row(p, n, i)[b] = page; });
 }
 
 // Moves runs (a layer, K or V, a group) of an item's kept positions: `group` runs a workgroup,
@@ -444,6 +456,7 @@ __global__ __launch_bounds__(256) void k_compact_move(StrideKvPool p, const int3
                                                       int group) {
   if (p.work[0] == 0) return;
   __shared__ int64_t from[2][kStepMax], to[2][kStepMax];  // byte offsets of a position in its run's arena; below 0: nothing
+  __shared__ int64_t run_at[256];
   const Runs runs = runs_of(p);
   const int groups = (runs.count + group - 1) / group;
   const int i = blockIdx.x / groups, run0 = blockIdx.x % groups * group, t = threadIdx.x;
@@ -477,15 +490,19 @@ __global__ __launch_bounds__(256) void k_compact_move(StrideKvPool p, const int3
     from[b][t] = f;
     to[b][t] = d;
   };
-  // this thread's pieces: of run run0 + r, position q of a step, piece `in`
-  const int all = min(group, runs.count - run0) * step * pieces;
+  // this thread's pieces: of rows m, m + per, .. of the workgroup's (run, position) rows
+  const int per = 256 / pieces, in = t % pieces * 16, row0 = t / pieces;
+  const int rows = row0 < per ? min(group, runs.count - run0) * step : 0;
+  const float rcp = 1.0f / static_cast<float>(step);
+  if (t < min(group, runs.count - run0)) run_at[t] = runs.at(run0 + t);
+  __syncthreads();
   int64_t base[kHold];
   int place[kHold];
 #pragma unroll
   for (int u = 0; u < kHold; ++u) {
-    const int e = u * 256 + t, r = e / (step * pieces), q = e / pieces % step;
-    place[u] = e < all ? q : -1;
-    base[u] = e < all ? runs.at(run0 + r) + e % pieces * 16 : 0;
+    const int m = row0 + u * per, r = static_cast<int>((static_cast<float>(m) + 0.5f) * rcp);  // m < 2048: exact
+    place[u] = m < rows ? m - r * step : -1;
+    base[u] = m < rows ? run_at[r] + in : 0;
   }
   look(-lead, 0);
   __syncthreads();
@@ -665,9 +682,9 @@ int stride_kv_compact(const StrideKvPool* p, const int32_t* slot, const int32_t*
   if (int rc = launched("kv_compact (plan)")) return rc;
   // Positions a step and runs a workgroup: short lists (a few accepted tokens) share a
   // workgroup's threads, and its lookups, between runs.
-  const int pieces = p->kv.head_dim * p->elem_bytes / 16, most = 256 * kHold / pieces;
+  const int pieces = p->kv.head_dim * p->elem_bytes / 16, most = 256 / pieces * kHold;
   const int step = static_cast<int>(std::min<int64_t>(std::min(kStepMax, most), std::max<int64_t>(1, static_cast<int64_t>(width) + (1 << shift) - 1)));
-  const int group = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(runs, most / step)));
+  const int group = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(runs, 256), most / step)));
   hipLaunchKernelGGL(k_compact_move, dim3(static_cast<unsigned>((runs + group - 1) / group * n)), dim3(256), 0, st, *p, slot, first, count, keep,
                      keep_stride, n, shift, pieces, step, group);
   if (int rc = launched("kv_compact (move)")) return rc;

@@ -76,6 +76,7 @@ class KvPool:
         self._params = _lib.KvPoolParams(ref, tc.ptr(refs), tc.ptr(self.free_bits), tc.ptr(self.errors), tc.ptr(self.work),
                                          ints, pages, slots, layers, kv_heads, elem)
         self._at = C.addressof(self._params)
+        self._device = table.get_device()
 
     @staticmethod
     def create(slots: int, max_ctx: int, pages: int, kv_heads: int, head_dim: int, layers: int, page_tokens: int, device,
@@ -103,14 +104,12 @@ class KvPool:
         """How many pages are free (waits for the device)."""
         return int((self.refs == 0).sum())
 
-    def _items(self, first, *more) -> int:
-        n = first.numel()
-        for t in (first, *more):
-            if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
-                raise ValueError("items are contiguous int32 tensors of one length")
-            if t.device != self.table.device:
-                raise ValueError("items must be on the pool's device")
-        here(self.table)
+    def _items(self, *items) -> int:
+        n, dev = items[0].numel(), self._device
+        for t in items:
+            if t.dtype != torch.int32 or t.get_device() != dev or t.numel() != n or not t.is_contiguous():
+                raise ValueError("items are contiguous int32 tensors of one length on the pool's device")
+        here(items[0])
         return n
 
     def reserve(self, slot, first, end) -> None:
@@ -136,7 +135,7 @@ class KvPool:
         n = self._items(slot, first, count)
         if keep.dtype != torch.int32 or keep.dim() != 2 or keep.shape[0] != n or (keep.shape[1] > 1 and keep.stride(1) != 1):
             raise ValueError("keep must be int32 [n][width], its rows contiguous")
-        if keep.device != self.table.device:
+        if keep.get_device() != self._device:
             raise ValueError("items must be on the pool's device")
         _run(_lib.load().stride_kv_compact(self._at, slot.data_ptr(), first.data_ptr(), count.data_ptr(), keep.data_ptr(),
                                            keep.stride(0) if n > 1 else keep.shape[1], keep.shape[1], n, tc.kernel_stream()))
