@@ -171,6 +171,10 @@ __device__ __forceinline__ void one_row(const StrideWindowAttentionParams& p, in
   constexpr int kRow = D / 8;            // 16-byte pieces of a row
   constexpr int kPer = kChunk * kRow / 64;
   constexpr int kOut = (D + 63) / 64;    // 16-dim blocks of a wave
+  // At head_dim 128 two leaves' registers would leave one workgroup a CU; two that take turns
+  // loading do better (128 rows of 1024 positions, 8 groups: 187 us with the next leaf's loads
+  // in flight).
+  constexpr bool kNext = !SPLIT && D < 128;
   __shared__ __align__(16) uint16_t vs[kLeaf * D];
   __shared__ __align__(16) u32x4 weights[kLeaf / 32][64];
   __shared__ float maxima[4][16];
@@ -229,12 +233,17 @@ __device__ __forceinline__ void one_row(const StrideWindowAttentionParams& p, in
   for (int b = 0; b < kOut; ++b) total[b] = f32x4{0, 0, 0, 0};
   Fold fold = {neg_inf(), 0.0f};
 
-  if (begin < end) {
+  if (kNext && begin < end) {
     look(leaves.at(begin));
     fetch_k(leaves.at(begin));
     fetch_v(leaves.at(begin));
   }
   for (int it = begin; it < end; ++it) {
+    if constexpr (!kNext) {
+      look(leaves.at(it));
+      fetch_k(leaves.at(it));
+      fetch_v(leaves.at(it));
+    }
     f32x4 s[4];
     float most = neg_inf();
 #pragma unroll
@@ -262,9 +271,9 @@ __device__ __forceinline__ void one_row(const StrideWindowAttentionParams& p, in
       const int piece = u * 64 + lane;
       *reinterpret_cast<u32x4*>(vs + v_at<D>(wave * kChunk + piece / kRow, (piece % kRow) * 8)) = vr[u];
     }
-    if (!SPLIT && it + 1 < end) look(leaves.at(it + 1));
+    if (kNext && it + 1 < end) look(leaves.at(it + 1));
     lds_barrier();
-    if (!SPLIT && it + 1 < end) {
+    if (kNext && it + 1 < end) {
       fetch_k(leaves.at(it + 1));
       fetch_v(leaves.at(it + 1));
     }
@@ -347,7 +356,7 @@ __device__ __forceinline__ void one_row(const StrideWindowAttentionParams& p, in
 }
 
 template <int D>
-__global__ __launch_bounds__(256) void k_leaves(StrideWindowAttentionParams p, int page_shift, int limit, int span) {
+__global__ __launch_bounds__(256, 2) void k_leaves(StrideWindowAttentionParams p, int page_shift, int limit, int span) {
   const int unit = blockIdx.x / p.n_kv;
   one_row<D, true>(p, page_shift, limit, span, blockIdx.x % p.n_kv, unit / span, unit % span);
 }
@@ -363,7 +372,7 @@ __device__ __forceinline__ bool unit_done(const StrideWindowAttentionParams& p, 
   return mark[part];
 }
 template <int D>
-__global__ __launch_bounds__(256) void k_rows(StrideWindowAttentionParams p, int page_shift, int limit, const int32_t* done, int tile_rows) {
+__global__ __launch_bounds__(256, 2) void k_rows(StrideWindowAttentionParams p, int page_shift, int limit, const int32_t* done, int tile_rows) {
   if (!done) {
     one_row<D, false>(p, page_shift, limit, 0, blockIdx.x % p.n_kv, blockIdx.x / p.n_kv, 0);
     return;
@@ -734,36 +743,83 @@ __global__ __launch_bounds__(64 * kColumns / COLS, 2) void k_tile(StrideWindowAt
   if (t == 0) *mark = 1;
 }
 
-// Joins a split row's records in ascending order. A thread has four dims of a head.
+// Joins a split row's records in ascending order. The factors of a head's leaves follow from
+// the references' running maximum, which a wave finds for 64 leaves at once; what is left in
+// order is one product and one FMA a leaf and value, a thread a value, with the values of up to
+// 32 records on their way. (With the factors formed leaf by leaf in every thread, 4 rows of 128
+// leaves at 8 heads of 128 took 17.8 us.)
 template <int D>
-__global__ __launch_bounds__(256) void k_join(StrideWindowAttentionParams p, int limit, int span) {
-  const int g = blockIdx.x % p.n_kv, j = blockIdx.x / p.n_kv;
+__global__ __launch_bounds__(256) void k_join(StrideWindowAttentionParams p, int limit, int span, int parts) {
+  constexpr int kHeads = 256 / D;  // of a workgroup
+  constexpr int kBlock = 256;      // leaves whose factors are in LDS
+  __shared__ f32x4 factor[kHeads][kBlock];  // a, b, l
+  const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+  const int part = blockIdx.x % parts, unit = blockIdx.x / parts, g = unit % p.n_kv, j = unit / p.n_kv;
   const int count = leaves_of(sight_of(p, p.row_pos[j], limit)).count;
   const int rf = record_floats(p.n_q, D);
   const float* recs = p.scratch + (static_cast<int64_t>(j) * p.n_kv + g) * span * rf;
-  for (int u = threadIdx.x; u < p.n_q * (D / 4); u += 256) {
-    const int h = u / (D / 4), d = u % (D / 4) * 4;
-    f32x4 total = {0, 0, 0, 0};
-    Fold fold = {neg_inf(), 0.0f};
-    for (int i0 = 0; i0 < count; i0 += 8) {
-      f32x4 acc[8];
-      f32x2 rl[8];
+  const int mine = t / D, h = part * kHeads + mine;  // a wave's values are of one head, or, at D = 32, of two
+  float total = 0.0f, sum = 0.0f;
+  const float* values = recs + min(h, p.n_q - 1) * D + t % D;
+  // running reference of head part * kHeads + wave + 4 k, the same in all lanes of its wave
+  float run[(kHeads + 3) / 4];
+  bool any[(kHeads + 3) / 4];  // has a leaf had weights
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float* rec = recs + min(i0 + i, count - 1) * rf;
-        acc[i] = *reinterpret_cast<const f32x4*>(rec + h * D + d);
-        rl[i] = *reinterpret_cast<const f32x2*>(rec + p.n_q * D + 2 * h);
-      }
+  for (int k = 0; k < (kHeads + 3) / 4; ++k) run[k] = neg_inf(), any[k] = false;
+  for (int i0 = 0; i0 < count; i0 += kBlock) {
+    const int n = min(kBlock, count - i0);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i0 + i >= count) break;
-        float a, b;
-        fold.take(rl[i][0], rl[i][1], a, b);
-        total = folded(total, acc[i], a, b);
+    for (int k = 0; k < (kHeads + 3) / 4; ++k) {
+      const int head = wave + 4 * k;
+      if (head >= kHeads) continue;
+      const float* rl = recs + static_cast<int64_t>(i0) * rf + p.n_q * D + 2 * min(part * kHeads + head, p.n_q - 1);
+      for (int i = 0; i < n; i += 64) {
+        const int at = min(i + lane, n - 1);
+        const f32x2 v = *reinterpret_cast<const f32x2*>(rl + static_cast<int64_t>(at) * rf);
+        const bool has = i + lane < n && !(v[1] == 0.0f);
+        float m = has ? v[0] : neg_inf();
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+          const float o = __shfl_up(m, d);
+          if (lane >= d && o > m) m = o;
+        }
+        if (run[k] > m) m = run[k];
+        float before = __shfl_up(m, 1);
+        if (lane == 0) before = run[k];
+        const uint64_t all = __ballot(has);
+        const bool first = !any[k] && (all & ((uint64_t{1} << lane) - 1)) == 0;
+        // (behind the last leaf, too, up to where values are read in one go: nothing changes there)
+        factor[head][i + lane] = has ? f32x4{first ? 0.0f : exp2_of(before - m), exp2_of(v[0] - m), v[1], 0} : f32x4{1, 0, 0, 0};
+        run[k] = __shfl(m, 63);
+        any[k] = any[k] || all;
       }
     }
-    put_out(p, j, g, h, d, total, fold.sum);
+    __syncthreads();
+    const float* at = values + static_cast<int64_t>(i0) * rf;
+    auto take = [&](auto ahead) __attribute__((always_inline)) {
+      constexpr int A = decltype(ahead)::value;
+      for (int i = 0; i < n; i += A) {
+        float v[A];
+#pragma unroll
+        for (int x = 0; x < A; ++x) v[x] = at[static_cast<int64_t>(min(i + x, n - 1)) * rf];
+        __builtin_amdgcn_sched_barrier(0);  // all of them before the first is used
+#pragma unroll
+        for (int x = 0; x < A; ++x) {
+          const f32x4 f = factor[mine][i + x];
+          total = __builtin_fmaf(i + x < n ? v[x] : 0.0f, f[1], total * f[0]);  // (0 times an infinity is NaN)
+          sum = __builtin_fmaf(f[2], f[1], sum * f[0]);
+        }
+      }
+    };
+    if (n <= 8) take(std::integral_constant<int, 8>{});
+    else take(std::integral_constant<int, 32>{});
+    __syncthreads();
   }
+  // four neighbouring values to the lane of the first
+  f32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = __shfl(total, (lane & ~3) + e);
+  if (h < p.n_q && (t & 3) == 0) put_out(p, j, g, h, t % D, v, sum);
 }
 
 // ---------------------------------------------------------------------------
@@ -821,7 +877,8 @@ int run(const StrideWindowAttentionParams& p, const Plan& plan, hipStream_t st) 
   if (plan.split) {
     hipLaunchKernelGGL((k_leaves<D>), dim3(units * plan.span), dim3(256), 0, st, p, plan.page_shift, plan.limit, plan.span);
     if (int rc = launched("window_attention (leaves)")) return rc;
-    hipLaunchKernelGGL((k_join<D>), dim3(units), dim3(256), 0, st, p, plan.limit, plan.span);
+    const int parts = (p.n_q * D + 255) / 256;
+    hipLaunchKernelGGL((k_join<D>), dim3(units * parts), dim3(256), 0, st, p, plan.limit, plan.span, parts);
     return launched("window_attention (join)");
   }
   int32_t* done = nullptr;
