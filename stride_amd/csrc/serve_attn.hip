@@ -393,42 +393,39 @@ __global__ __launch_bounds__(256, 2) void k_rows(StrideWindowAttentionParams p, 
 
 // ---------------------------------------------------------------------------
 // Prompts: a workgroup has a tile of 128 score columns, (row, head) pairs of neighbouring
-// rows, and a KV group, so that a chunk of keys and values is fetched once for all of them.
-// A wave has COLS of the columns: 32 with v_mfma_f32_32x32x16_bf16 (two, k halves in order,
-// give the bits of one 16x16x32), or 16 at head_dim 128, where 32 would take over 256
-// registers and leave one wave on a SIMD. The transposed product first: S^T = K Q^T leaves a
-// column's scores in a few lanes, so that references, weights and sums are lane-local, and
-// S^T's registers are P^T's operand as they are, with the value rows taken in the same order.
+// rows, and a KV group, so that keys and values are fetched once for all of them. Eight waves
+// of 16 columns each, v_mfma_f32_16x16x32_bf16, the transposed product first: S^T = K Q^T
+// leaves a column's scores in four lanes, so that references, weights and sums are lane-local,
+// and S^T's registers are P^T's operand as they are, with the value rows taken in the same
+// order. (Waves of 32 columns and the 32x32x16 form halve the LDS reads, but leave one wave a
+// SIMD at head_dim 128: 2048 rows of window 1984 195 us against 155, and 84 against 80 at 64.)
 //
-// Chunks are copied memory -> LDS two ahead, into three buffers. Key rows have their 16-byte
-// pieces permuted by the row and value rows their COLS * 2-byte blocks, so that an operand
+// C chunks at a time, a span. With two, a wave has two of each latency's work between two
+// barriers; with one, at head_dim 64, two workgroups fit on a CU (128 registers) and fill each
+// other's waits. So two at head_dim 128, or where there is at most a workgroup a CU (1024 rows
+// of one sequence at 8192, 8 groups, head_dim 64: 153 us against 183; 4096 rows: 440 against
+// 386). Spans are copied memory -> LDS one (C = 2) or two (C = 1) ahead. Key rows have their
+// 16-byte pieces permuted by the row and value rows their 32-byte blocks, so that an operand
 // read spreads over the banks; the copy lands in order, so its source is permuted.
 //
 // Rows of several sequences meet in a tile where prompts end: one workgroup takes the first
 // run of a tile, another the rest, run by run, each column taking part in its own. A tile of
-// many short runs is left to k_rows, and so is one with a value that is not finite in a chunk
-// that some of its columns must not see (0 times it is NaN). done[(tile * n_kv + g) * 2 +
-// part]: whether it was done.
+// many short runs is left to k_rows, and so is one with a value that is not finite among
+// positions that some of its columns must not see (0 times it is NaN). done[(tile * n_kv + g) *
+// 2 + part]: whether it was done.
 constexpr int kColumns = 128;
 
-template <int D, int COLS>
+template <int D>
 struct Lay {
   static constexpr int kRow = D / 8;  // 16-byte pieces of a row
-  static constexpr int kBlock = COLS == 32 ? 4 : 2;  // pieces of a value row's block
-  // what the row adds to a key's piece and a value's block
+  // what the row adds to a key's piece and a value's block of two
   __device__ static __forceinline__ int k_turn(int row) { return (row * D / 128) & (kRow - 1); }
-  __device__ static __forceinline__ int v_turn(int row) {
-    constexpr int kBlocks = kRow / kBlock;
-    if constexpr (COLS == 32) return kBlocks == 1 ? 0 : (kBlocks == 2 ? (row >> 1) & 1 : row & 3);
-    else return (row * D / 128) & (kBlocks - 1);
-  }
+  __device__ static __forceinline__ int v_turn(int row) { return (row * D / 128) & (kRow / 2 - 1); }
   __device__ static __forceinline__ int k_at(int row, int piece) { return row * D + ((piece ^ k_turn(row)) << 3); }
-  __device__ static __forceinline__ int v_at(int row, int dim) {
-    return row * D + (((dim / (kBlock * 8)) ^ v_turn(row)) * kBlock * 8) + (dim & (kBlock * 8 - 1));
-  }
-  // the pieces that slot `at` of a row gets
+  __device__ static __forceinline__ int v_at(int row, int dim) { return row * D + (((dim >> 4) ^ v_turn(row)) << 4) + (dim & 15); }
+  // the piece that slot `at` of a row gets
   __device__ static __forceinline__ int k_from(int row, int at) { return at ^ k_turn(row); }
-  __device__ static __forceinline__ int v_from(int row, int at) { return ((at / kBlock) ^ v_turn(row)) * kBlock + at % kBlock; }
+  __device__ static __forceinline__ int v_from(int row, int at) { return (((at >> 1) ^ v_turn(row)) << 1) + (at & 1); }
 };
 
 __device__ __forceinline__ bool has_nonfinite(u32x4 v) {
@@ -438,12 +435,21 @@ __device__ __forceinline__ bool has_nonfinite(u32x4 v) {
   return bad;
 }
 
+// The maximum over the four lanes of a column (16 apart): the row swaps leave a lane's own and
+// its partner's value.
+__device__ __forceinline__ float column_max(float m) {
+  const auto a = __builtin_amdgcn_permlane16_swap(u32_of(m), u32_of(m), false, false);
+  m = fmaxf(f32_of(a[0]), f32_of(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(u32_of(m), u32_of(m), false, false);
+  return fmaxf(f32_of(b[0]), f32_of(b[1]));
+}
+
 __device__ __align__(16) uint32_t zeros16[4];  // what unseen and unheld positions are copied from
 
 // 64 lanes' 16 bytes each, memory -> LDS, in lane order from `to`. Written as assembly because
 // the compiler, not knowing which buffer a transposing read reads, would have every such read
-// wait for all copies under way; the kernel counts them itself (nothing else of its loop is
-// counted by vmcnt). The instruction has no register that it writes.
+// wait for all copies under way; the kernel waits for them itself. The instruction has no
+// register that it writes.
 __device__ __forceinline__ void copy_to_lds(const uint16_t* from, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory", "m0");
 }
@@ -451,23 +457,21 @@ __device__ __forceinline__ uint32_t lds_offset(const void* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)(p)));
 }
 
-template <int D, int COLS>
-__global__ __launch_bounds__(64 * kColumns / COLS, 2) void k_tile(StrideWindowAttentionParams p, int page_shift, int limit, int tile_rows,
-                                                                   int32_t* done) {
-  using L = Lay<D, COLS>;
-  constexpr int kWavesHere = kColumns / COLS;
-  constexpr int kPer = kChunk * L::kRow / 64 / kWavesHere;  // copies of K (and of V) a wave makes
-  constexpr int kSub = COLS == 32 ? 2 : 4;                  // position blocks of a chunk
-  constexpr int kReg = COLS == 32 ? 16 : 4;                 // accumulator registers of a block
-  constexpr int kDims = D / COLS;
-  constexpr int kStep = COLS == 32 ? 16 : 32;               // dims of a score product
-  using Acc = typename std::conditional<COLS == 32, f32x16, f32x4>::type;
-  __shared__ __align__(16) uint16_t ks[3][kChunk * D];
-  __shared__ __align__(16) uint16_t vs[3][kChunk * D];
+template <int D, int C>
+__global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttentionParams p, int page_shift, int limit, int tile_rows, int32_t* done) {
+  using L = Lay<D>;
+  constexpr int kWaves = kColumns / 16;
+  constexpr int kSpan = C * kChunk;
+  constexpr int kBufs = C == 2 ? 2 : 3;
+  constexpr int kPer = kSpan * L::kRow / 64 / kWaves;  // copies of K (and of V) a wave makes
+  static_assert(kPer > 0, "every wave copies");
+  constexpr int kDims = D / 16;
+  __shared__ __align__(16) uint16_t ks[kBufs][kSpan * D];
+  __shared__ __align__(16) uint16_t vs[kBufs][kSpan * D];
   __shared__ int slots[kColumns], poss[kColumns];
   __shared__ uint64_t starts[2];  // bit i: row i begins a run
-  __shared__ int bad[2][kWavesHere];
-  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, cl = lane & (COLS - 1), quarter = lane / COLS;
+  __shared__ int bad[2][kWaves];
+  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, cl = lane & 15, quarter = lane >> 4;
   // The first runs' workgroups first (most of the others only leave; taken in turn with them,
   // they left whole CUs idle: 2048 rows of window 512 70 us against 41), and later rows, which
   // see more, before earlier ones.
@@ -501,30 +505,23 @@ __global__ __launch_bounds__(64 * kColumns / COLS, 2) void k_tile(StrideWindowAt
   };
 
   // this lane's column
-  const int col = wave * COLS + cl, row = col / p.n_q, head = col - row * p.n_q;
+  const int col = wave * 16 + cl, row = col / p.n_q, head = col - row * p.n_q;
   const bool live = row < nr;
   const int my_pos = live ? poss[row] : -1;
   const Sight sight = sight_of(p, my_pos, limit);
-  u32x4 qh[D / kStep], ql[D / kStep];
+  u32x4 qh[D / 32], ql[D / 32];
   {
     const float* q = p.q + (j0 + (live ? row : 0)) * p.q_stride + (static_cast<int64_t>(g) * p.n_q + head) * D + 8 * quarter;
 #pragma unroll
-    for (int k = 0; k < D / kStep; ++k) split_query(q + kStep * k, p.scale * kLog2e, live, qh[k], ql[k]);
+    for (int k = 0; k < D / 32; ++k) split_query(q + 32 * k, p.scale * kLog2e, live, qh[k], ql[k]);
   }
 
   const uint16_t* base = static_cast<const uint16_t*>(p.kv.arena) + p.layer * p.kv.layer_elems + g * p.kv.group_elems;
   const int in_page = (1 << page_shift) - 1;
-  Acc total[kDims];
+  f32x4 total[kDims];
 #pragma unroll
-  for (int d = 0; d < kDims; ++d)
-#pragma unroll
-    for (int i = 0; i < kReg; ++i) total[d][i] = 0.0f;
+  for (int d = 0; d < kDims; ++d) total[d] = f32x4{0, 0, 0, 0};
   Fold fold = {neg_inf(), 0.0f};
-
-  auto mma = [](u32x4 a, u32x4 b, Acc c) __attribute__((always_inline)) {
-    if constexpr (COLS == 32) return mfma32(a, b, c);
-    else return mfma(a, b, c);
-  };
 
   const int begin = part ? next_run(0) : 0, end = part ? nr : next_run(0);
   for (int r0 = begin; r0 < end;) {
@@ -552,18 +549,18 @@ __global__ __launch_bounds__(64 * kColumns / COLS, 2) void k_tile(StrideWindowAt
     r0 = r1;
     if (high < 0) continue;
     const Sight near = sight_of(p, low, limit), far = sight_of(p, high, limit);
-    // chunks: [0, head) and [rest, last]
-    const int head_chunks = (far.sink_end + kChunk - 1) / kChunk, rest = max(near.lo / kChunk, head_chunks);
-    const int chunks = head_chunks + max(0, high / kChunk - rest + 1);
+    // spans: [0, head) and [rest, last]
+    const int head_spans = (far.sink_end + kSpan - 1) / kSpan, rest = max(near.lo / kSpan, head_spans);
+    const int spans = head_spans + max(0, high / kSpan - rest + 1);
     const auto table = (const __attribute__((address_space(4))) int32_t*)(p.kv.table + static_cast<int64_t>(slot) * p.kv.max_blocks);
-    auto chunk_at = [&](int i) { return i < head_chunks ? i : rest + i - head_chunks; };
+    auto span_at = [&](int i) { return i < head_spans ? i : rest + i - head_spans; };
 
-    // Table entries one chunk ahead of the copies, which are two ahead of the products. A copy's
-    // rows lie in one page, so its entry comes through the scalar cache. Past the last chunk it
-    // is copied again, so that the waits can count.
+    // Table entries one span ahead of the copies, which are kBufs - 1 ahead of the products. A
+    // copy's rows lie in one page, so its entry comes through the scalar cache. Past the last
+    // span it is copied again, so that the waits can count.
     int block[kPer];
     auto look = [&](int i) {
-      const int c = chunk_at(min(i, chunks - 1)) * kChunk;
+      const int c = span_at(min(i, spans - 1)) * kSpan;
 #pragma unroll
       for (int u = 0; u < kPer; ++u) {
         // an entry that no row sees is not looked at: the run's own last one stands for it
@@ -573,7 +570,7 @@ __global__ __launch_bounds__(64 * kColumns / COLS, 2) void k_tile(StrideWindowAt
       }
     };
     auto copy = [&](int i, int buf) {
-      const int c = chunk_at(min(i, chunks - 1)) * kChunk;
+      const int c = span_at(min(i, spans - 1)) * kSpan;
 #pragma unroll
       for (int u = 0; u < kPer; ++u) {
         const int at = (wave * kPer + u) * 64, r = (at + lane) / L::kRow, slot_in = (at + lane) % L::kRow, pos = c + r;
@@ -584,29 +581,26 @@ __global__ __launch_bounds__(64 * kColumns / COLS, 2) void k_tile(StrideWindowAt
         copy_to_lds(seen ? from + p.kv.which_elems + L::v_from(r, slot_in) * 8 : zero, lds_offset(&vs[buf][at * 8]));
       }
     };
-    look(0);
-    copy(0, 0);
-    look(1);
-    copy(1, 1);
-    look(2);
+#pragma unroll
+    for (int x = 0; x < kBufs - 1; ++x) {
+      look(x);
+      copy(x, x);
+    }
+    look(kBufs - 1);
     int buf = 0;
-    for (int i = 0; i < chunks;) {
-      const int leaf = chunk_at(i) / (kLeaf / kChunk);
-      Acc acc[kDims], l;
+    for (int i = 0; i < spans;) {
+      const int leaf = span_at(i) / (kLeaf / kSpan);
+      f32x4 acc[kDims], l = {0, 0, 0, 0};
       float ref = neg_inf();
 #pragma unroll
-      for (int e = 0; e < kReg; ++e) {
-        l[e] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < kDims; ++d) acc[d][e] = 0.0f;
-      }
+      for (int d = 0; d < kDims; ++d) acc[d] = f32x4{0, 0, 0, 0};
       do {
-        const int a = chunk_at(i) * kChunk;
+        const int a = span_at(i) * kSpan;
         // do all columns see all of it?
-        const bool full = whole && a + kChunk - 1 <= low && (a >= far.lo || a + kChunk <= near.sink_end);
-        // this chunk has arrived (the next one's copies may be under way), and every wave has
-        // read the one before, whose buffer is filled next
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kPer) : "memory");
+        const bool full = whole && a + kSpan - 1 <= low && (a >= far.lo || a + kSpan <= near.sink_end);
+        // this span has arrived, and every wave has read the one before, whose buffer is filled next
+        // (the copies of the next may be under way)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kBufs - 2) * 2 * kPer) : "memory");
         lds_barrier();
         if (!full) {
           bool b = false;
@@ -617,128 +611,103 @@ __global__ __launch_bounds__(64 * kColumns / COLS, 2) void k_tile(StrideWindowAt
           lds_barrier();
           int sum = 0;
 #pragma unroll
-          for (int w = 0; w < kWavesHere; ++w) sum |= bad[i & 1][w];
+          for (int w = 0; w < kWaves; ++w) sum |= bad[i & 1][w];
           if (sum) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             if (t == 0) *mark = 0;
             return;
           }
         }
-        copy(i + 2, buf == 0 ? 2 : buf - 1);
-        look(i + 3);
-        Acc s[kSub];
+        copy(i + kBufs - 1, buf == 0 ? kBufs - 1 : buf - 1);
+        look(i + kBufs);
+        f32x4 s[4 * C];
 #pragma unroll
-        for (int b = 0; b < kSub; ++b) {
-#pragma unroll
-          for (int e = 0; e < kReg; ++e) s[b][e] = 0.0f;
+        for (int b = 0; b < 4 * C; ++b) {
+          s[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
           for (int k = 0; k < D / 32; ++k) {
-            if constexpr (COLS == 32) {
-              const u32x4 k0 = *reinterpret_cast<const u32x4*>(&ks[buf][L::k_at(32 * b + cl, 4 * k + quarter)]);
-              const u32x4 k1 = *reinterpret_cast<const u32x4*>(&ks[buf][L::k_at(32 * b + cl, 4 * k + 2 + quarter)]);
-              s[b] = mma(k0, qh[2 * k], s[b]);
-              s[b] = mma(k1, qh[2 * k + 1], s[b]);
-              s[b] = mma(k0, ql[2 * k], s[b]);
-              s[b] = mma(k1, ql[2 * k + 1], s[b]);
-            } else {
-              const u32x4 k0 = *reinterpret_cast<const u32x4*>(&ks[buf][L::k_at(16 * b + cl, 4 * k + quarter)]);
-              s[b] = mma(k0, qh[k], s[b]);
-              s[b] = mma(k0, ql[k], s[b]);
-            }
+            const u32x4 key = *reinterpret_cast<const u32x4*>(&ks[buf][L::k_at(16 * b + cl, 4 * k + quarter)]);
+            s[b] = mfma(key, qh[k], s[b]);
+            s[b] = mfma(key, ql[k], s[b]);
           }
         }
-        // register e of block b is position b * COLS + 8 * (e / 4) + 4 * quarter + e % 4 of the chunk
+        // register e of block b is position 16 b + 4 quarter + e of the span
         if (!full) {
           const int from = a + 4 * quarter;
           if (a >= far.sink_end) {
-            const uint32_t wide = mine && sight.pos >= sight.lo ? sight.pos - sight.lo : 0;
-            const int shift = mine && sight.pos >= sight.lo ? from - sight.lo : INT_MIN / 2;  // far below: unseen
+            const bool some = mine && sight.pos >= sight.lo;
+            const uint32_t wide = some ? sight.pos - sight.lo : 0;
+            const int shift = some ? from - sight.lo : INT_MIN / 2;  // far below: unseen
 #pragma unroll
-            for (int b = 0; b < kSub; ++b)
+            for (int b = 0; b < 4 * C; ++b)
 #pragma unroll
-              for (int e = 0; e < kReg; ++e)
-                if (static_cast<uint32_t>(shift + b * COLS + 8 * (e / 4) + e % 4) > wide) s[b][e] = neg_inf();
+              for (int e = 0; e < 4; ++e)
+                if (static_cast<uint32_t>(shift + 16 * b + e) > wide) s[b][e] = neg_inf();
           } else {
 #pragma unroll
-            for (int b = 0; b < kSub; ++b)
+            for (int b = 0; b < 4 * C; ++b)
 #pragma unroll
-              for (int e = 0; e < kReg; ++e)
-                if (!(mine && sight.sees(from + b * COLS + 8 * (e / 4) + e % 4))) s[b][e] = neg_inf();
+              for (int e = 0; e < 4; ++e)
+                if (!(mine && sight.sees(from + 16 * b + e))) s[b][e] = neg_inf();
           }
         }
-        float most = s[0][0];
+        float most[C];
 #pragma unroll
-        for (int b = 0; b < kSub; ++b)
+        for (int h = 0; h < C; ++h) {
+          most[h] = s[4 * h][0];
 #pragma unroll
-          for (int e = 0; e < kReg; ++e) most = fmaxf(most, s[b][e]);
-        if constexpr (COLS == 16) most = fmaxf(most, __shfl_xor(most, 16));
-        most = fmaxf(most, __shfl_xor(most, 32));
-        if (__any(most > ref + kSlack)) {
-          const bool up = most > ref + kSlack;
-          const float alpha = up ? exp2_of(ref - most) : 1.0f;
-          if (up) ref = most;
+          for (int b = 0; b < 4; ++b)
 #pragma unroll
-          for (int e = 0; e < kReg; ++e) {
-            l[e] *= alpha;
-#pragma unroll
-            for (int d = 0; d < kDims; ++d) acc[d][e] *= alpha;
-          }
+            for (int e = 0; e < 4; ++e) most[h] = fmaxf(most[h], s[4 * h + b][e]);
+          most[h] = column_max(most[h]);
         }
-        const float at = ref == neg_inf() ? 0.0f : ref;
 #pragma unroll
-        for (int b = 0; b < kSub; ++b)
+        for (int h = 0; h < C; ++h) {
+          if (__any(most[h] > ref + kSlack)) {
+            const bool up = most[h] > ref + kSlack;
+            const float alpha = up ? exp2_of(ref - most[h]) : 1.0f;
+            if (up) ref = most[h];
 #pragma unroll
-          for (int e = 0; e < kReg; ++e) s[b][e] = exp2_of(s[b][e] - at);
-        // 32 positions: the products in the order of the 16 x 16 x 32 form's k
+            for (int e = 0; e < 4; ++e) {
+              l[e] *= alpha;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if constexpr (COLS == 32) {
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const u32x4 pw = {pack2(s[h][4 * x], s[h][4 * x + 1]), pack2(s[h][4 * x + 2], s[h][4 * x + 3]),
-                                pack2(s[h][4 * x + 8], s[h][4 * x + 9]), pack2(s[h][4 * x + 10], s[h][4 * x + 11])};
-              l = mma(u32x4{kOnes, kOnes, kOnes, kOnes}, pw, l);
-              const int r = 32 * h + 8 * x + 4 * quarter + ((lane & 15) >> 2);
-#pragma unroll
-              for (int d = 0; d < kDims; ++d) {
-                const int dim = 32 * d + (lane & 16) + 4 * (lane & 3);
-                acc[d] = mma(both(read_transposed(&vs[buf][L::v_at(r, dim)]), read_transposed(&vs[buf][L::v_at(r + 16, dim)])), pw, acc[d]);
-              }
+              for (int d = 0; d < kDims; ++d) acc[d][e] *= alpha;
             }
-          } else {
-            const u32x4 pw = {pack2(s[2 * h][0], s[2 * h][1]), pack2(s[2 * h][2], s[2 * h][3]), pack2(s[2 * h + 1][0], s[2 * h + 1][1]),
-                              pack2(s[2 * h + 1][2], s[2 * h + 1][3])};
-            l = mma(u32x4{kOnes, kOnes, kOnes, kOnes}, pw, l);
-            const int r = 32 * h + 4 * quarter + ((lane & 15) >> 2);
+          }
+          const float at = ref == neg_inf() ? 0.0f : ref;
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * h + b][e] = exp2_of(s[4 * h + b][e] - at);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const f32x4 s0 = s[4 * h + 2 * x], s1 = s[4 * h + 2 * x + 1];
+            const u32x4 pw = {pack2(s0[0], s0[1]), pack2(s0[2], s0[3]), pack2(s1[0], s1[1]), pack2(s1[2], s1[3])};
+            l = mfma(u32x4{kOnes, kOnes, kOnes, kOnes}, pw, l);
+            const int r = 64 * h + 32 * x + 4 * quarter + (cl >> 2);
 #pragma unroll
             for (int d = 0; d < kDims; ++d) {
               const int dim = 16 * d + 4 * (lane & 3);
-              acc[d] = mma(both(read_transposed(&vs[buf][L::v_at(r, dim)]), read_transposed(&vs[buf][L::v_at(r + 16, dim)])), pw, acc[d]);
+              acc[d] = mfma(both(read_transposed(&vs[buf][L::v_at(r, dim)]), read_transposed(&vs[buf][L::v_at(r + 16, dim)])), pw, acc[d]);
             }
           }
         }
-        buf = buf == 2 ? 0 : buf + 1;
+        buf = buf == kBufs - 1 ? 0 : buf + 1;
         ++i;
-      } while (i < chunks && chunk_at(i) / (kLeaf / kChunk) == leaf);
+      } while (i < spans && span_at(i) / (kLeaf / kSpan) == leaf);
       float fa, fb;
       fold.take(ref, l[0], fa, fb);
 #pragma unroll
-      for (int d = 0; d < kDims; ++d)
-#pragma unroll
-        for (int e = 0; e < kReg; ++e) total[d][e] = __builtin_fmaf(acc[d][e], fb, total[d][e] * fa);
+      for (int d = 0; d < kDims; ++d) total[d] = folded(total[d], acc[d], fa, fb);
     }
-    // nothing is on its way to the buffers when another run, or the end, comes
+    // nothing is on its way to the buffers, and every wave has read them, when another run comes
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     lds_barrier();
   }
   if (live && row >= begin && row < end) {
     const float sum = my_pos < 0 ? 0.0f : fold.sum;
 #pragma unroll
-    for (int d = 0; d < kDims; ++d)
-#pragma unroll
-      for (int e = 0; e < kReg / 4; ++e)
-        put_out(p, j0 + row, g, head, COLS * d + 8 * e + 4 * quarter,
-                f32x4{total[d][4 * e], total[d][4 * e + 1], total[d][4 * e + 2], total[d][4 * e + 3]}, sum);
+    for (int d = 0; d < kDims; ++d) put_out(p, j0 + row, g, head, 16 * d + 4 * quarter, total[d], sum);
   }
   if (t == 0) *mark = 1;
 }
@@ -885,9 +854,11 @@ int run(const StrideWindowAttentionParams& p, const Plan& plan, hipStream_t st) 
   int groups = units;
   if (plan.tile_rows) {
     done = reinterpret_cast<int32_t*>(p.scratch);
-    constexpr int kCols = D == 128 ? 16 : 32;
-    hipLaunchKernelGGL((k_tile<D, kCols>), dim3(static_cast<unsigned>(plan.scratch)), dim3(64 * kColumns / kCols), 0, st, p, plan.page_shift, plan.limit,
-                       plan.tile_rows, done);
+    const dim3 grid(static_cast<unsigned>(plan.scratch)), block(512);
+    if (D != 64 || plan.scratch <= 2 * 256)
+      hipLaunchKernelGGL((k_tile<D, 2>), grid, block, 0, st, p, plan.page_shift, plan.limit, plan.tile_rows, done);
+    else
+      hipLaunchKernelGGL((k_tile<64, 1>), grid, block, 0, st, p, plan.page_shift, plan.limit, plan.tile_rows, done);
     if (int rc = launched("window_attention (tiles)")) return rc;
     groups = std::max(std::min(units, 1024), (units + 255) / 256);  // most of them only find that nothing is left
   }
