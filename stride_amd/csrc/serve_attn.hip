@@ -149,8 +149,9 @@ __device__ __forceinline__ void put_out(const StrideWindowAttentionParams& p, in
   uint16_t* at = p.out + (static_cast<int64_t>(j >> 4) * (p.out_cols >> 4) + (idx >> 4)) * kTileElems + (j & 15) * 16 + (idx & 15);
   f32x4 v = {0, 0, 0, 0};
   if (!(sum == 0.0f)) {
+    const float r = 1.0f / sum;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = acc[e] / sum + 0.0f;
+    for (int e = 0; e < 4; ++e) v[e] = acc[e] * r + 0.0f;
   }
   *reinterpret_cast<u32x2*>(at) = u32x2{pack2(v[0], v[1]), pack2(v[2], v[3])};
 }
@@ -429,10 +430,12 @@ struct Lay {
 };
 
 __device__ __forceinline__ bool has_nonfinite(u32x4 v) {
-  bool bad = false;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) bad |= (v[e] & 0x7F80u) == 0x7F80u || (v[e] & 0x7F800000u) == 0x7F800000u;
-  return bad;
+  typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  const u16x8 e = __builtin_bit_cast(u16x8, v & u32x4{0x7F807F80u, 0x7F807F80u, 0x7F807F80u, 0x7F807F80u});
+  const u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(u16x2{e[0], e[1]}, u16x2{e[2], e[3]}),
+                                            __builtin_elementwise_max(u16x2{e[4], e[5]}, u16x2{e[6], e[7]}));
+  return m[0] == 0x7F80 || m[1] == 0x7F80;
 }
 
 // The maximum over the four lanes of a column (16 apart): the row swaps leave a lane's own and
@@ -444,14 +447,33 @@ __device__ __forceinline__ float column_max(float m) {
   return fmaxf(f32_of(b[0]), f32_of(b[1]));
 }
 
+// The largest over a wave, in every lane: DPP within rows of 16, then the row swaps.
+template <int CTRL>
+__device__ __forceinline__ int larger_by(int v) {
+  return max(v, __builtin_amdgcn_update_dpp(v, v, CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ int wave_most(int v) {
+  v = larger_by<0xB1>(v);   // quad_perm [1,0,3,2]
+  v = larger_by<0x4E>(v);   // quad_perm [2,3,0,1]
+  v = larger_by<0x124>(v);  // row_ror:4
+  v = larger_by<0x128>(v);  // row_ror:8
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(static_cast<int>(a[0]), static_cast<int>(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return __builtin_amdgcn_readfirstlane(max(static_cast<int>(b[0]), static_cast<int>(b[1])));
+}
+
 __device__ __align__(16) uint32_t zeros16[4];  // what unseen and unheld positions are copied from
 
 // 64 lanes' 16 bytes each, memory -> LDS, in lane order from `to`. Written as assembly because
 // the compiler, not knowing which buffer a transposing read reads, would have every such read
 // wait for all copies under way; the kernel waits for them itself. The instruction has no
-// register that it writes.
+// register that it writes. The second form takes a base for the wave and a byte offset a lane.
 __device__ __forceinline__ void copy_to_lds(const uint16_t* from, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory", "m0");
+}
+__device__ __forceinline__ void copy_to_lds(const uint16_t* base, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory", "m0");
 }
 __device__ __forceinline__ uint32_t lds_offset(const void* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)(p)));
@@ -510,18 +532,23 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
   const int my_pos = live ? poss[row] : -1;
   const Sight sight = sight_of(p, my_pos, limit);
   u32x4 qh[D / 32], ql[D / 32];
-  {
-    const float* q = p.q + (j0 + (live ? row : 0)) * p.q_stride + (static_cast<int64_t>(g) * p.n_q + head) * D + 8 * quarter;
-#pragma unroll
-    for (int k = 0; k < D / 32; ++k) split_query(q + 32 * k, p.scale * kLog2e, live, qh[k], ql[k]);
-  }
-
   const uint16_t* base = static_cast<const uint16_t*>(p.kv.arena) + p.layer * p.kv.layer_elems + g * p.kv.group_elems;
   const int in_page = (1 << page_shift) - 1;
   f32x4 total[kDims];
 #pragma unroll
   for (int d = 0; d < kDims; ++d) total[d] = f32x4{0, 0, 0, 0};
   Fold fold = {neg_inf(), 0.0f};
+
+  const uint16_t* zero = reinterpret_cast<const uint16_t*>(zeros16);
+  asm("" : "+s"(zero));  // kept, not looked up again for each copy
+  // a lane's bytes in a copy, from the first of its rows
+  uint32_t k_off[kPer], v_off[kPer];
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
+    const int at = (wave * kPer + u) * 64, r = (at + lane) / L::kRow, slot_in = (at + lane) % L::kRow;
+    k_off[u] = (lane / L::kRow * D + L::k_from(r, slot_in) * 8) * 2;
+    v_off[u] = (lane / L::kRow * D + L::v_from(r, slot_in) * 8) * 2;
+  }
 
   const int begin = part ? next_run(0) : 0, end = part ? nr : next_run(0);
   for (int r0 = begin; r0 < end;) {
@@ -536,13 +563,8 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
         high = max(high, pos);
       }
     }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      low = min(low, __shfl_xor(low, d));
-      high = max(high, __shfl_xor(high, d));
-    }
-    low = __builtin_amdgcn_readfirstlane(low);
-    high = __builtin_amdgcn_readfirstlane(high);
+    low = -1 - wave_most(-1 - low);
+    high = wave_most(high);
     const bool mine = row >= r0 && row < r1;
     const int slot = __builtin_amdgcn_readfirstlane(slots[r0]);
     const bool whole = r0 == 0 && r1 == nr;
@@ -571,14 +593,22 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
     };
     auto copy = [&](int i, int buf) {
       const int c = span_at(min(i, spans - 1)) * kSpan;
+      // Does some row see each position? Then a lane's place in a copy's page is all it needs.
+      const bool inside = c + kSpan - 1 <= high && (c >= near.lo || c + kSpan <= far.sink_end);
 #pragma unroll
       for (int u = 0; u < kPer; ++u) {
-        const int at = (wave * kPer + u) * 64, r = (at + lane) / L::kRow, slot_in = (at + lane) % L::kRow, pos = c + r;
-        const bool seen = block[u] >= 0 && pos <= high && (pos >= near.lo || pos < far.sink_end);
-        const uint16_t* from = base + block[u] * p.kv.block_elems + (pos & in_page) * D;
-        const uint16_t* zero = reinterpret_cast<const uint16_t*>(zeros16);
-        copy_to_lds(seen ? from + L::k_from(r, slot_in) * 8 : zero, lds_offset(&ks[buf][at * 8]));
-        copy_to_lds(seen ? from + p.kv.which_elems + L::v_from(r, slot_in) * 8 : zero, lds_offset(&vs[buf][at * 8]));
+        const int at = (wave * kPer + u) * 64, row0 = at / L::kRow;
+        const uint16_t* page = base + block[u] * p.kv.block_elems + ((c + row0) & in_page) * D;
+        const uint32_t k_to = lds_offset(&ks[buf][at * 8]), v_to = lds_offset(&vs[buf][at * 8]);
+        if (inside && block[u] >= 0) {
+          copy_to_lds(page, k_off[u], k_to);
+          copy_to_lds(page + p.kv.which_elems, v_off[u], v_to);
+        } else {
+          const int pos = c + row0 + lane / L::kRow;
+          const bool seen = block[u] >= 0 && pos <= high && (pos >= near.lo || pos < far.sink_end);
+          copy_to_lds(seen ? page + k_off[u] / 2 : zero, k_to);
+          copy_to_lds(seen ? page + p.kv.which_elems + v_off[u] / 2 : zero, v_to);
+        }
       }
     };
 #pragma unroll
@@ -587,6 +617,11 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
       copy(x, x);
     }
     look(kBufs - 1);
+    {  // beside the first copies
+      const float* q = p.q + (j0 + (live ? row : 0)) * p.q_stride + (static_cast<int64_t>(g) * p.n_q + head) * D + 8 * quarter;
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) split_query(q + 32 * k, p.scale * kLog2e, live, qh[k], ql[k]);
+    }
     int buf = 0;
     for (int i = 0; i < spans;) {
       const int leaf = span_at(i) / (kLeaf / kSpan);
@@ -674,22 +709,33 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
               for (int d = 0; d < kDims; ++d) acc[d][e] *= alpha;
             }
           }
-          const float at = ref == neg_inf() ? 0.0f : ref;
-#pragma unroll
-          for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[4 * h + b][e] = exp2_of(s[4 * h + b][e] - at);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const f32x4 s0 = s[4 * h + 2 * x], s1 = s[4 * h + 2 * x + 1];
-            const u32x4 pw = {pack2(s0[0], s0[1]), pack2(s0[2], s0[3]), pack2(s1[0], s1[1]), pack2(s1[2], s1[3])};
-            l = mfma(u32x4{kOnes, kOnes, kOnes, kOnes}, pw, l);
+          // value operands of 32 positions; the first half's are read beside the exponentials, the
+          // second's beside the first's products
+          u32x4 v[2][kDims];
+          auto read = [&](int x) __attribute__((always_inline)) {
             const int r = 64 * h + 32 * x + 4 * quarter + (cl >> 2);
 #pragma unroll
             for (int d = 0; d < kDims; ++d) {
               const int dim = 16 * d + 4 * (lane & 3);
-              acc[d] = mfma(both(read_transposed(&vs[buf][L::v_at(r, dim)]), read_transposed(&vs[buf][L::v_at(r + 16, dim)])), pw, acc[d]);
+              v[x][d] = both(read_transposed(&vs[buf][L::v_at(r, dim)]), read_transposed(&vs[buf][L::v_at(r + 16, dim)]));
             }
+            __builtin_amdgcn_sched_barrier(0);
+          };
+          read(0);
+          const float at = ref == neg_inf() ? 0.0f : ref;
+          u32x4 pw[2];
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const f32x4 z = s[4 * h + b];
+            pw[b >> 1][2 * (b & 1)] = pack2(exp2_of(z[0] - at), exp2_of(z[1] - at));
+            pw[b >> 1][2 * (b & 1) + 1] = pack2(exp2_of(z[2] - at), exp2_of(z[3] - at));
+          }
+          read(1);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            l = mfma(u32x4{kOnes, kOnes, kOnes, kOnes}, pw[x], l);
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) acc[d] = mfma(v[x][d], pw[x], acc[d]);
           }
         }
         buf = buf == kBufs - 1 ? 0 : buf + 1;
