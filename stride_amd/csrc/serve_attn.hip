@@ -655,6 +655,7 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
         }
         copy(i + kBufs - 1, buf == 0 ? kBufs - 1 : buf - 1);
         look(i + kBufs);
+        __builtin_amdgcn_s_setprio(1);
         f32x4 s[4 * C];
 #pragma unroll
         for (int b = 0; b < 4 * C; ++b) {
@@ -666,6 +667,7 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
             s[b] = mfma(key, ql[k], s[b]);
           }
         }
+        __builtin_amdgcn_s_setprio(0);
         // register e of block b is position 16 b + 4 quarter + e of the span
         if (!full) {
           const int from = a + 4 * quarter;
@@ -731,12 +733,14 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
             pw[b >> 1][2 * (b & 1) + 1] = pack2(exp2_of(z[2] - at), exp2_of(z[3] - at));
           }
           read(1);
+          __builtin_amdgcn_s_setprio(1);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             l = mfma(u32x4{kOnes, kOnes, kOnes, kOnes}, pw[x], l);
 #pragma unroll
             for (int d = 0; d < kDims; ++d) acc[d] = mfma(v[x][d], pw[x], acc[d]);
           }
+          __builtin_amdgcn_s_setprio(0);
         }
         buf = buf == kBufs - 1 ? 0 : buf + 1;
         ++i;
