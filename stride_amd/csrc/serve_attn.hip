@@ -51,6 +51,8 @@ struct Sight {
   int pos, lo, sink_end;
   __device__ __forceinline__ bool sees(int t) const { return t <= pos && (t >= lo || t < sink_end); }
 };
+// a row of no sequence is one without a position
+__device__ __forceinline__ int pos_of(const StrideWindowAttentionParams& p, int j) { return p.row_slot[j] < 0 ? -1 : p.row_pos[j]; }
 __device__ __forceinline__ Sight sight_of(const StrideWindowAttentionParams& p, int pos, int limit) {
   Sight s;
   s.pos = min(pos, limit - 1);
@@ -181,7 +183,7 @@ __device__ __forceinline__ void one_row(const StrideWindowAttentionParams& p, in
   __shared__ float maxima[4][16];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
   const int slot = p.row_slot[j];
-  const Sight sight = sight_of(p, p.row_pos[j], limit);
+  const Sight sight = sight_of(p, pos_of(p, j), limit);
   const Leaves leaves = leaves_of(sight);
   const int end = SPLIT ? begin + 1 : leaves.count;
   if (SPLIT && begin >= leaves.count) return;
@@ -357,9 +359,14 @@ __device__ __forceinline__ void one_row(const StrideWindowAttentionParams& p, in
 }
 
 template <int D>
-__global__ __launch_bounds__(256, 2) void k_leaves(StrideWindowAttentionParams p, int page_shift, int limit, int span) {
-  const int unit = blockIdx.x / p.n_kv;
-  one_row<D, true>(p, page_shift, limit, span, blockIdx.x % p.n_kv, unit / span, unit % span);
+__global__ __launch_bounds__(256, 2) void k_leaves(StrideWindowAttentionParams p, int page_shift, int limit, int span, const int32_t* done,
+                                                   int tile_rows, int parts) {
+  const int unit = blockIdx.x / p.n_kv, g = blockIdx.x % p.n_kv, j = unit / span, at = unit % span;
+  if (done) {
+    const Leaves leaves = leaves_of(sight_of(p, pos_of(p, j), limit));
+    if (at >= leaves.count || done[(j / tile_rows * p.n_kv + g) * parts + leaves.at(at) % parts]) return;
+  }
+  one_row<D, true>(p, page_shift, limit, span, g, j, at);
 }
 
 // A workgroup a unit (row, group); with tiles that k_tile may have done (done: its marks), a
@@ -409,11 +416,16 @@ __global__ __launch_bounds__(256, 2) void k_rows(StrideWindowAttentionParams p, 
 // 16-byte pieces permuted by the row and value rows their 32-byte blocks, so that an operand
 // read spreads over the banks; the copy lands in order, so its source is permuted.
 //
+// SPLIT: few rows over a long context. A workgroup has the leaves of its tile that are its
+// number modulo `parts`, each leaf's sums go to the columns' rows as records, and k_join joins
+// them (64 rows at 8192 positions, 8 groups, head_dim 64: 139 us otherwise, 45 so). There a
+// workgroup takes part in all of its tile's runs, one after the other.
+//
 // Rows of several sequences meet in a tile where prompts end: one workgroup takes the first
 // run of a tile, another the rest, run by run, each column taking part in its own. A tile of
 // many short runs is left to k_rows, and so is one with a value that is not finite among
 // positions that some of its columns must not see (0 times it is NaN). done[(tile * n_kv + g) *
-// 2 + part]: whether it was done.
+// parts + part]: whether it was done; with SPLIT, part = leaf % parts, otherwise parts is 2.
 constexpr int kColumns = 128;
 
 template <int D>
@@ -479,8 +491,9 @@ __device__ __forceinline__ uint32_t lds_offset(const void* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)(p)));
 }
 
-template <int D, int C>
-__global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttentionParams p, int page_shift, int limit, int tile_rows, int32_t* done) {
+template <int D, int C, bool SPLIT>
+__global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttentionParams p, int page_shift, int limit, int tile_rows, int32_t* done,
+                                                              int span, int parts) {
   using L = Lay<D>;
   constexpr int kWaves = kColumns / 16;
   constexpr int kSpan = C * kChunk;
@@ -497,15 +510,15 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
   // The first runs' workgroups first (most of the others only leave; taken in turn with them,
   // they left whole CUs idle: 2048 rows of window 512 70 us against 41), and later rows, which
   // see more, before earlier ones.
-  const int tiles = gridDim.x / p.n_kv / 2, unit = blockIdx.x / p.n_kv;
-  const int g = blockIdx.x % p.n_kv, part = unit >= tiles ? 1 : 0, tile = tiles - 1 - (part ? unit - tiles : unit);
+  const int tiles = gridDim.x / p.n_kv / parts, unit = blockIdx.x / p.n_kv;
+  const int g = blockIdx.x % p.n_kv, part = unit / tiles, tile = tiles - 1 - unit % tiles;
   const int j0 = tile * tile_rows, nr = min(tile_rows, p.l.rows - j0);
-  int32_t* mark = done + (tile * p.n_kv + g) * 2 + part;
+  int32_t* mark = done + (tile * p.n_kv + g) * parts + part;
 
   if (t < kColumns) {
     const int j = j0 + min(t, nr - 1);
     slots[t] = p.row_slot[j];
-    poss[t] = t < nr ? min(p.row_pos[j], limit - 1) : -1;
+    poss[t] = t < nr ? min(pos_of(p, j), limit - 1) : -1;
   }
   __syncthreads();
   if (t < kColumns) {
@@ -515,8 +528,9 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
   __syncthreads();
   const uint64_t first = starts[0], second = starts[1];
   const int runs = __popcll(first) + __popcll(second);
-  if (nr < 4 * runs || runs <= part) {
-    if (t == 0) *mark = nr < 4 * runs ? 0 : 1;
+  const bool left = nr < 4 * runs;
+  if (left || (!SPLIT && runs <= part)) {
+    if (t == 0) *mark = left ? 0 : 1;
     return;
   }
   // the row after row r at which another run begins
@@ -550,7 +564,7 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
     v_off[u] = (lane / L::kRow * D + L::v_from(r, slot_in) * 8) * 2;
   }
 
-  const int begin = part ? next_run(0) : 0, end = part ? nr : next_run(0);
+  const int begin = !SPLIT && part ? next_run(0) : 0, end = SPLIT || part ? nr : next_run(0);
   for (int r0 = begin; r0 < end;) {
     // the run [r0, r1): its sequence, and what its rows see together
     const int r1 = next_run(r0);
@@ -571,190 +585,217 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
     r0 = r1;
     if (high < 0) continue;
     const Sight near = sight_of(p, low, limit), far = sight_of(p, high, limit);
-    // spans: [0, head) and [rest, last]
-    const int head_spans = (far.sink_end + kSpan - 1) / kSpan, rest = max(near.lo / kSpan, head_spans);
-    const int spans = head_spans + max(0, high / kSpan - rest + 1);
+    // spans: [0, all_head) and [all_rest, all_last]
+    const int all_head = (far.sink_end + kSpan - 1) / kSpan, all_rest = max(near.lo / kSpan, all_head), all_last = high / kSpan;
     const auto table = (const __attribute__((address_space(4))) int32_t*)(p.kv.table + static_cast<int64_t>(slot) * p.kv.max_blocks);
-    auto span_at = [&](int i) { return i < head_spans ? i : rest + i - head_spans; };
+    // One pass over all of them, or over the workgroup's leaves one by one: the spans
+    // [0, head_spans) and those from `rest` on, `spans` in all.
+    for (int part_leaf = SPLIT ? part : 0; part_leaf <= (SPLIT ? high / kLeaf : 0); part_leaf += SPLIT ? parts : 1) {
+      int head_spans = all_head, rest = all_rest, last = all_last;
+      if constexpr (SPLIT) {
+        // from the first to the last span of the leaf that a row sees
+        head_spans = 0, rest = part_leaf * (kLeaf / kSpan), last = min(rest + kLeaf / kSpan - 1, all_last);
+        if (rest >= all_head) rest = max(rest, all_rest);
+        if (last < all_rest) last = min(last, all_head - 1);
+        if (rest > last) continue;
+      }
+      const int spans = head_spans + max(0, last - rest + 1);
+      auto span_at = [&](int i) { return i < head_spans ? i : rest + i - head_spans; };
 
-    // Table entries one span ahead of the copies, which are kBufs - 1 ahead of the products. A
-    // copy's rows lie in one page, so its entry comes through the scalar cache. Past the last
-    // span it is copied again, so that the waits can count.
-    int block[kPer];
-    auto look = [&](int i) {
-      const int c = span_at(min(i, spans - 1)) * kSpan;
+      // Table entries one span ahead of the copies, which are kBufs - 1 ahead of the products. A
+      // copy's rows lie in one page, so its entry comes through the scalar cache. Past the last
+      // span it is copied again, so that the waits can count.
+      int block[kPer];
+      auto look = [&](int i) {
+        const int c = span_at(min(i, spans - 1)) * kSpan;
 #pragma unroll
-      for (int u = 0; u < kPer; ++u) {
-        // an entry that no row sees is not looked at: the run's own last one stands for it
-        const int a = c + (wave * kPer + u) * 64 / L::kRow, z = a + 64 / L::kRow - 1;
-        const bool s = a <= high && (z >= near.lo || a < far.sink_end);
-        block[u] = table[__builtin_amdgcn_readfirstlane((s ? a : high) >> page_shift)];
-      }
-    };
-    auto copy = [&](int i, int buf) {
-      const int c = span_at(min(i, spans - 1)) * kSpan;
-      // Does some row see each position? Then a lane's place in a copy's page is all it needs.
-      const bool inside = c + kSpan - 1 <= high && (c >= near.lo || c + kSpan <= far.sink_end);
-#pragma unroll
-      for (int u = 0; u < kPer; ++u) {
-        const int at = (wave * kPer + u) * 64, row0 = at / L::kRow;
-        const uint16_t* page = base + block[u] * p.kv.block_elems + ((c + row0) & in_page) * D;
-        const uint32_t k_to = lds_offset(&ks[buf][at * 8]), v_to = lds_offset(&vs[buf][at * 8]);
-        if (inside && block[u] >= 0) {
-          copy_to_lds(page, k_off[u], k_to);
-          copy_to_lds(page + p.kv.which_elems, v_off[u], v_to);
-        } else {
-          const int pos = c + row0 + lane / L::kRow;
-          const bool seen = block[u] >= 0 && pos <= high && (pos >= near.lo || pos < far.sink_end);
-          copy_to_lds(seen ? page + k_off[u] / 2 : zero, k_to);
-          copy_to_lds(seen ? page + p.kv.which_elems + v_off[u] / 2 : zero, v_to);
+        for (int u = 0; u < kPer; ++u) {
+          // an entry that no row sees is not looked at: the run's own last one stands for it
+          const int a = c + (wave * kPer + u) * 64 / L::kRow, z = a + 64 / L::kRow - 1;
+          const bool s = a <= high && (z >= near.lo || a < far.sink_end);
+          block[u] = table[__builtin_amdgcn_readfirstlane((s ? a : high) >> page_shift)];
         }
-      }
-    };
+      };
+      auto copy = [&](int i, int buf) {
+        const int c = span_at(min(i, spans - 1)) * kSpan;
+        // Does some row see each position? Then a lane's place in a copy's page is all it needs.
+        const bool inside = c + kSpan - 1 <= high && (c >= near.lo || c + kSpan <= far.sink_end);
 #pragma unroll
-    for (int x = 0; x < kBufs - 1; ++x) {
-      look(x);
-      copy(x, x);
-    }
-    look(kBufs - 1);
-    {  // beside the first copies
-      const float* q = p.q + (j0 + (live ? row : 0)) * p.q_stride + (static_cast<int64_t>(g) * p.n_q + head) * D + 8 * quarter;
-#pragma unroll
-      for (int k = 0; k < D / 32; ++k) split_query(q + 32 * k, p.scale * kLog2e, live, qh[k], ql[k]);
-    }
-    int buf = 0;
-    for (int i = 0; i < spans;) {
-      const int leaf = span_at(i) / (kLeaf / kSpan);
-      f32x4 acc[kDims], l = {0, 0, 0, 0};
-      float ref = neg_inf();
-#pragma unroll
-      for (int d = 0; d < kDims; ++d) acc[d] = f32x4{0, 0, 0, 0};
-      do {
-        const int a = span_at(i) * kSpan;
-        // do all columns see all of it?
-        const bool full = whole && a + kSpan - 1 <= low && (a >= far.lo || a + kSpan <= near.sink_end);
-        // this span has arrived, and every wave has read the one before, whose buffer is filled next
-        // (the copies of the next may be under way)
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kBufs - 2) * 2 * kPer) : "memory");
-        lds_barrier();
-        if (!full) {
-          bool b = false;
-#pragma unroll
-          for (int u = 0; u < kPer; ++u) b |= has_nonfinite(*reinterpret_cast<const u32x4*>(&vs[buf][((wave * kPer + u) * 64 + lane) * 8]));
-          const bool any = __any(b);
-          if (lane == 0) bad[i & 1][wave] = any;
-          lds_barrier();
-          int sum = 0;
-#pragma unroll
-          for (int w = 0; w < kWaves; ++w) sum |= bad[i & 1][w];
-          if (sum) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            if (t == 0) *mark = 0;
-            return;
-          }
-        }
-        copy(i + kBufs - 1, buf == 0 ? kBufs - 1 : buf - 1);
-        look(i + kBufs);
-        __builtin_amdgcn_s_setprio(1);
-        f32x4 s[4 * C];
-#pragma unroll
-        for (int b = 0; b < 4 * C; ++b) {
-          s[b] = f32x4{0, 0, 0, 0};
-#pragma unroll
-          for (int k = 0; k < D / 32; ++k) {
-            const u32x4 key = *reinterpret_cast<const u32x4*>(&ks[buf][L::k_at(16 * b + cl, 4 * k + quarter)]);
-            s[b] = mfma(key, qh[k], s[b]);
-            s[b] = mfma(key, ql[k], s[b]);
-          }
-        }
-        __builtin_amdgcn_s_setprio(0);
-        // register e of block b is position 16 b + 4 quarter + e of the span
-        if (!full) {
-          const int from = a + 4 * quarter;
-          if (a >= far.sink_end) {
-            const bool some = mine && sight.pos >= sight.lo;
-            const uint32_t wide = some ? sight.pos - sight.lo : 0;
-            const int shift = some ? from - sight.lo : INT_MIN / 2;  // far below: unseen
-#pragma unroll
-            for (int b = 0; b < 4 * C; ++b)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (static_cast<uint32_t>(shift + 16 * b + e) > wide) s[b][e] = neg_inf();
+        for (int u = 0; u < kPer; ++u) {
+          const int at = (wave * kPer + u) * 64, row0 = at / L::kRow;
+          const uint16_t* page = base + block[u] * p.kv.block_elems + ((c + row0) & in_page) * D;
+          const uint32_t k_to = lds_offset(&ks[buf][at * 8]), v_to = lds_offset(&vs[buf][at * 8]);
+          if (inside && block[u] >= 0) {
+            copy_to_lds(page, k_off[u], k_to);
+            copy_to_lds(page + p.kv.which_elems, v_off[u], v_to);
           } else {
-#pragma unroll
-            for (int b = 0; b < 4 * C; ++b)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (!(mine && sight.sees(from + 16 * b + e))) s[b][e] = neg_inf();
+            const int pos = c + row0 + lane / L::kRow;
+            const bool seen = block[u] >= 0 && pos <= high && (pos >= near.lo || pos < far.sink_end);
+            copy_to_lds(seen ? page + k_off[u] / 2 : zero, k_to);
+            copy_to_lds(seen ? page + p.kv.which_elems + v_off[u] / 2 : zero, v_to);
           }
         }
-        float most[C];
+      };
 #pragma unroll
-        for (int h = 0; h < C; ++h) {
-          most[h] = s[4 * h][0];
+      for (int x = 0; x < kBufs - 1; ++x) {
+        look(x);
+        copy(x, x);
+      }
+      look(kBufs - 1);
+      {  // beside the first copies
+        const float* q = p.q + (j0 + (live ? row : 0)) * p.q_stride + (static_cast<int64_t>(g) * p.n_q + head) * D + 8 * quarter;
 #pragma unroll
-          for (int b = 0; b < 4; ++b)
+        for (int k = 0; k < D / 32; ++k) split_query(q + 32 * k, p.scale * kLog2e, live, qh[k], ql[k]);
+      }
+      int buf = 0;
+      for (int i = 0; i < spans;) {
+        const int leaf = span_at(i) / (kLeaf / kSpan);
+        f32x4 acc[kDims], l = {0, 0, 0, 0};
+        float ref = neg_inf();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) most[h] = fmaxf(most[h], s[4 * h + b][e]);
-          most[h] = column_max(most[h]);
-        }
+        for (int d = 0; d < kDims; ++d) acc[d] = f32x4{0, 0, 0, 0};
+        do {
+          const int a = span_at(i) * kSpan;
+          // do all columns see all of it?
+          const bool full = whole && a + kSpan - 1 <= low && (a >= far.lo || a + kSpan <= near.sink_end);
+          // this span has arrived, and every wave has read the one before, whose buffer is filled next
+          // (the copies of the next may be under way)
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kBufs - 2) * 2 * kPer) : "memory");
+          lds_barrier();
+          if (!full) {
+            bool b = false;
 #pragma unroll
-        for (int h = 0; h < C; ++h) {
-          if (__any(most[h] > ref + kSlack)) {
-            const bool up = most[h] > ref + kSlack;
-            const float alpha = up ? exp2_of(ref - most[h]) : 1.0f;
-            if (up) ref = most[h];
+            for (int u = 0; u < kPer; ++u) b |= has_nonfinite(*reinterpret_cast<const u32x4*>(&vs[buf][((wave * kPer + u) * 64 + lane) * 8]));
+            const bool any = __any(b);
+            if (lane == 0) bad[i & 1][wave] = any;
+            lds_barrier();
+            int sum = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              l[e] *= alpha;
-#pragma unroll
-              for (int d = 0; d < kDims; ++d) acc[d][e] *= alpha;
+            for (int w = 0; w < kWaves; ++w) sum |= bad[i & 1][w];
+            if (__builtin_amdgcn_readfirstlane(sum)) {
+              asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+              if (t == 0) *mark = 0;
+              // Two ways to leave, for the registers that the compiler gives the loop around them:
+              // head_dim 64, 2048 rows of window 512 take 31.5 us so and 34.4 with the return;
+              // 256 rows of 8192 positions, C == 2, 152 and 141.
+              if constexpr (C == 1) __builtin_amdgcn_endpgm();
+              return;
             }
           }
-          // value operands of 32 positions; the first half's are read beside the exponentials, the
-          // second's beside the first's products
-          u32x4 v[2][kDims];
-          auto read = [&](int x) __attribute__((always_inline)) {
-            const int r = 64 * h + 32 * x + 4 * quarter + (cl >> 2);
-#pragma unroll
-            for (int d = 0; d < kDims; ++d) {
-              const int dim = 16 * d + 4 * (lane & 3);
-              v[x][d] = both(read_transposed(&vs[buf][L::v_at(r, dim)]), read_transposed(&vs[buf][L::v_at(r + 16, dim)]));
-            }
-            __builtin_amdgcn_sched_barrier(0);
-          };
-          read(0);
-          const float at = ref == neg_inf() ? 0.0f : ref;
-          u32x4 pw[2];
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            const f32x4 z = s[4 * h + b];
-            pw[b >> 1][2 * (b & 1)] = pack2(exp2_of(z[0] - at), exp2_of(z[1] - at));
-            pw[b >> 1][2 * (b & 1) + 1] = pack2(exp2_of(z[2] - at), exp2_of(z[3] - at));
-          }
-          read(1);
+          copy(i + kBufs - 1, buf == 0 ? kBufs - 1 : buf - 1);
+          look(i + kBufs);
           __builtin_amdgcn_s_setprio(1);
+          f32x4 s[4 * C];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            l = mfma(u32x4{kOnes, kOnes, kOnes, kOnes}, pw[x], l);
+          for (int b = 0; b < 4 * C; ++b) {
+            s[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int d = 0; d < kDims; ++d) acc[d] = mfma(v[x][d], pw[x], acc[d]);
+            for (int k = 0; k < D / 32; ++k) {
+              const u32x4 key = *reinterpret_cast<const u32x4*>(&ks[buf][L::k_at(16 * b + cl, 4 * k + quarter)]);
+              s[b] = mfma(key, qh[k], s[b]);
+              s[b] = mfma(key, ql[k], s[b]);
+            }
           }
           __builtin_amdgcn_s_setprio(0);
-        }
-        buf = buf == kBufs - 1 ? 0 : buf + 1;
-        ++i;
-      } while (i < spans && span_at(i) / (kLeaf / kSpan) == leaf);
-      float fa, fb;
-      fold.take(ref, l[0], fa, fb);
+          // register e of block b is position 16 b + 4 quarter + e of the span
+          if (!full) {
+            const int from = a + 4 * quarter;
+            if (a >= far.sink_end) {
+              const bool some = mine && sight.pos >= sight.lo;
+              const uint32_t wide = some ? sight.pos - sight.lo : 0;
+              const int shift = some ? from - sight.lo : INT_MIN / 2;  // far below: unseen
 #pragma unroll
-      for (int d = 0; d < kDims; ++d) total[d] = folded(total[d], acc[d], fa, fb);
+              for (int b = 0; b < 4 * C; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (static_cast<uint32_t>(shift + 16 * b + e) > wide) s[b][e] = neg_inf();
+            } else {
+#pragma unroll
+              for (int b = 0; b < 4 * C; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (!(mine && sight.sees(from + 16 * b + e))) s[b][e] = neg_inf();
+            }
+          }
+          float most[C];
+#pragma unroll
+          for (int h = 0; h < C; ++h) {
+            most[h] = s[4 * h][0];
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) most[h] = fmaxf(most[h], s[4 * h + b][e]);
+            most[h] = column_max(most[h]);
+          }
+#pragma unroll
+          for (int h = 0; h < C; ++h) {
+            if (__any(most[h] > ref + kSlack)) {
+              const bool up = most[h] > ref + kSlack;
+              const float alpha = up ? exp2_of(ref - most[h]) : 1.0f;
+              if (up) ref = most[h];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                l[e] *= alpha;
+#pragma unroll
+                for (int d = 0; d < kDims; ++d) acc[d][e] *= alpha;
+              }
+            }
+            // value operands of 32 positions; the first half's are read beside the exponentials, the
+            // second's beside the first's products
+            u32x4 v[2][kDims];
+            auto read = [&](int x) __attribute__((always_inline)) {
+              const int r = 64 * h + 32 * x + 4 * quarter + (cl >> 2);
+#pragma unroll
+              for (int d = 0; d < kDims; ++d) {
+                const int dim = 16 * d + 4 * (lane & 3);
+                v[x][d] = both(read_transposed(&vs[buf][L::v_at(r, dim)]), read_transposed(&vs[buf][L::v_at(r + 16, dim)]));
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            };
+            read(0);
+            const float at = ref == neg_inf() ? 0.0f : ref;
+            u32x4 pw[2];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+              const f32x4 z = s[4 * h + b];
+              pw[b >> 1][2 * (b & 1)] = pack2(exp2_of(z[0] - at), exp2_of(z[1] - at));
+              pw[b >> 1][2 * (b & 1) + 1] = pack2(exp2_of(z[2] - at), exp2_of(z[3] - at));
+            }
+            read(1);
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              l = mfma(u32x4{kOnes, kOnes, kOnes, kOnes}, pw[x], l);
+#pragma unroll
+              for (int d = 0; d < kDims; ++d) acc[d] = mfma(v[x][d], pw[x], acc[d]);
+            }
+            __builtin_amdgcn_s_setprio(0);
+          }
+          buf = buf == kBufs - 1 ? 0 : buf + 1;
+          ++i;
+        } while (i < spans && span_at(i) / (kLeaf / kSpan) == leaf);
+        if constexpr (SPLIT) {
+          const Leaves sees = leaves_of(sight);
+          const int at = leaf < sees.head ? leaf : (leaf >= sees.rest ? sees.head + leaf - sees.rest : sees.count);
+          if (live && mine && at < sees.count) {
+            float* rec = p.scratch + ((static_cast<int64_t>(j0 + row) * p.n_kv + g) * span + at) * record_floats(p.n_q, D);
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) *reinterpret_cast<f32x4*>(rec + head * D + 16 * d + 4 * quarter) = acc[d];
+            if (quarter == 0) *reinterpret_cast<f32x2*>(rec + p.n_q * D + 2 * head) = f32x2{ref, l[0]};
+          }
+        } else {
+          float fa, fb;
+          fold.take(ref, l[0], fa, fb);
+#pragma unroll
+          for (int d = 0; d < kDims; ++d) total[d] = folded(total[d], acc[d], fa, fb);
+        }
+      }
+      // nothing is on its way to the buffers, and every wave has read them, when another pass comes
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      lds_barrier();
     }
-    // nothing is on its way to the buffers, and every wave has read them, when another run comes
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    lds_barrier();
   }
-  if (live && row >= begin && row < end) {
+  if (!SPLIT && live && row >= begin && row < end) {
     const float sum = my_pos < 0 ? 0.0f : fold.sum;
 #pragma unroll
     for (int d = 0; d < kDims; ++d) put_out(p, j0 + row, g, head, 16 * d + 4 * quarter, total[d], sum);
@@ -774,7 +815,7 @@ __global__ __launch_bounds__(256) void k_join(StrideWindowAttentionParams p, int
   __shared__ f32x4 factor[kHeads][kBlock];  // a, b, l
   const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
   const int part = blockIdx.x % parts, unit = blockIdx.x / parts, g = unit % p.n_kv, j = unit / p.n_kv;
-  const int count = leaves_of(sight_of(p, p.row_pos[j], limit)).count;
+  const int count = leaves_of(sight_of(p, pos_of(p, j), limit)).count;
   const int rf = record_floats(p.n_q, D);
   const float* recs = p.scratch + (static_cast<int64_t>(j) * p.n_kv + g) * span * rf;
   const int mine = t / D, h = part * kHeads + mine;  // a wave's values are of one head, or, at D = 32, of two
@@ -847,8 +888,9 @@ __global__ __launch_bounds__(256) void k_join(StrideWindowAttentionParams p, int
 struct Plan {
   int page_shift, limit, span;
   int tile_rows;  // 0: no tiles
+  int parts;      // marks of a tile and group
   bool split;
-  int64_t scratch;
+  int64_t records, scratch;  // floats; the tiles' marks come behind the records
 };
 
 const char* plan_of(const StrideWindowAttentionParams& p, Plan& plan) {
@@ -876,11 +918,24 @@ const char* plan_of(const StrideWindowAttentionParams& p, Plan& plan) {
   plan.span = static_cast<int>(span);
   const int64_t units = static_cast<int64_t>(p.l.rows) * p.n_kv;
   if (units * span > INT_MAX) return "rows, n_kv and the context are too large together";
-  plan.split = span > 1 && units < 512;
-  // (a tile's copies of 64 / (head_dim / 8) rows lie in one page)
-  plan.tile_rows = plan.split || p.runs == 1 || tokens < 512 / D ? 0 : kColumns / p.n_q;
-  plan.scratch = plan.split ? units * span * ((p.n_q * (D + 2) + 3) / 4 * 4) : 0;
-  if (plan.tile_rows) plan.scratch = (static_cast<int64_t>(p.l.rows) + plan.tile_rows - 1) / plan.tile_rows * p.n_kv * 2;
+  // Tiles where neighbouring rows may be of one sequence (a tile's copies of 64 / (head_dim / 8)
+  // rows lie in one page). Leaves in workgroups of their own, and joined, where the rows or
+  // tiles alone would not fill the chip: below 512 workgroups of k_rows; of tiles where rows are
+  // few (2048 units are 512 of them at n_q = 4) and leaves at least eight, for the records and
+  // two launches more (64 rows of 2000 positions, 8 groups, head_dim 64 / 128: 21 / 31 us
+  // against 42 / 64 row by row; of 600 positions 18 / 24 against 21 / 29, but 16 rows 15 / 20
+  // against 13 / 16, and 200 rows 24 / 37 against 22 / 32 in whole tiles).
+  const int64_t records = units * span * ((p.n_q * (D + 2) + 3) / 4 * 4);
+  const bool may_split = span > 1 && records <= int64_t{1} << 28;  // a GiB
+  bool tiles = p.runs != 1 && p.l.rows >= 4 && tokens >= 512 / D;
+  plan.split = may_split && tiles && p.runs > 1 && span >= 8 && units < 2048;
+  if (!plan.split && may_split && units < 512) plan.split = true, tiles = false;
+  plan.tile_rows = tiles ? kColumns / p.n_q : 0;
+  plan.parts = plan.split ? static_cast<int>(std::min<int64_t>((static_cast<int64_t>(plan.limit) + kLeaf - 1) / kLeaf, span + 1)) : 2;
+  plan.records = plan.split ? records : 0;
+  const int64_t marks = tiles ? (static_cast<int64_t>(p.l.rows) + plan.tile_rows - 1) / plan.tile_rows * p.n_kv * plan.parts : 0;
+  if (marks > INT_MAX) return "rows, n_kv and the context are too large together";
+  plan.scratch = plan.records + marks;
   return nullptr;
 }
 
@@ -893,26 +948,27 @@ int launched(const char* what) {
 template <int D>
 int run(const StrideWindowAttentionParams& p, const Plan& plan, hipStream_t st) {
   const int units = p.l.rows * p.n_kv;
+  int32_t* done = plan.tile_rows ? reinterpret_cast<int32_t*>(p.scratch + plan.records) : nullptr;
+  if (done) {
+    const unsigned groups = static_cast<unsigned>(plan.scratch - plan.records);  // a mark each
+    const dim3 grid(groups), block(512);
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, p, plan.page_shift, plan.limit, plan.tile_rows, done, plan.span, plan.parts); };
+    if (plan.split) launch(k_tile<D, 2, true>);
+    else if (D != 64 || groups <= 2 * 256) launch(k_tile<D, 2, false>);
+    else launch(k_tile<64, 1, false>);
+    if (int rc = launched("window_attention (tiles)")) return rc;
+  }
+  const int tile_rows = std::max(1, plan.tile_rows);
   if (plan.split) {
-    hipLaunchKernelGGL((k_leaves<D>), dim3(units * plan.span), dim3(256), 0, st, p, plan.page_shift, plan.limit, plan.span);
+    hipLaunchKernelGGL((k_leaves<D>), dim3(units * plan.span), dim3(256), 0, st, p, plan.page_shift, plan.limit, plan.span, done, tile_rows, plan.parts);
     if (int rc = launched("window_attention (leaves)")) return rc;
     const int parts = (p.n_q * D + 255) / 256;
     hipLaunchKernelGGL((k_join<D>), dim3(units * parts), dim3(256), 0, st, p, plan.limit, plan.span, parts);
     return launched("window_attention (join)");
   }
-  int32_t* done = nullptr;
-  int groups = units;
-  if (plan.tile_rows) {
-    done = reinterpret_cast<int32_t*>(p.scratch);
-    const dim3 grid(static_cast<unsigned>(plan.scratch)), block(512);
-    if (D != 64 || plan.scratch <= 2 * 256)
-      hipLaunchKernelGGL((k_tile<D, 2>), grid, block, 0, st, p, plan.page_shift, plan.limit, plan.tile_rows, done);
-    else
-      hipLaunchKernelGGL((k_tile<64, 1>), grid, block, 0, st, p, plan.page_shift, plan.limit, plan.tile_rows, done);
-    if (int rc = launched("window_attention (tiles)")) return rc;
-    groups = std::max(std::min(units, 1024), (units + 255) / 256);  // most of them only find that nothing is left
-  }
-  hipLaunchKernelGGL((k_rows<D>), dim3(groups), dim3(256), 0, st, p, plan.page_shift, plan.limit, done, std::max(1, plan.tile_rows));
+  // (with tiles most of the workgroups only find that nothing is left)
+  const int groups = done ? std::max(std::min(units, 1024), (units + 255) / 256) : units;
+  hipLaunchKernelGGL((k_rows<D>), dim3(groups), dim3(256), 0, st, p, plan.page_shift, plan.limit, done, tile_rows);
   return launched("window_attention");
 }
 

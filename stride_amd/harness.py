@@ -306,8 +306,8 @@ def here(t) -> None:
 
 def window_attention_scratch(rows: int, n_kv: int, n_q: int, head_dim: int, window: int, sinks: int, max_pages: int,
                              device, runs: int = 0):
-    """The scratch that window_attention wants for calls of these sizes (None: none). It may
-    be larger than a call's; its contents need no preparation."""
+    """The scratch that window_attention wants for calls of these sizes (None: none), with a
+    cache of at least 64 * max_pages positions a slot. Its contents need no preparation."""
     p = _lib.WindowAttentionParams()
     p.l = lanes(rows)
     p.q_stride = p.out_cols = n_kv * n_q * head_dim
@@ -327,8 +327,8 @@ def window_attention(q, kv: PagedKv, row_slot, row_pos, n_kv: int, n_q: int, hea
                      runs: int = 0):
     """Attention of rows (row_slot, row_pos) over the paged cache: every position up to the
     row's own (window 0), or the last `window` and the first `sinks` ones. q: [rows][n_kv *
-    n_q * head_dim] fp32 (rows may be strided). A row with row_pos < 0 gets zeros. max_pages:
-    no row lies behind position 64 * max_pages - 1 (default: the slots' capacity). runs: a
+    n_q * head_dim] fp32 (rows may be strided). A row with row_pos < 0 or row_slot < 0 gets
+    zeros. max_pages: no row lies behind position 64 * max_pages - 1 (default: the slots' capacity). runs: a
     hint, how many neighbouring rows are of one sequence at most (1: decode; 0: not known).
     scratch: window_attention_scratch() (default: allocated here, on torch's current stream).
     Returns bf16 x tiles."""
@@ -348,8 +348,9 @@ def window_attention(q, kv: PagedKv, row_slot, row_pos, n_kv: int, n_q: int, hea
     elif (out_tiles.dtype != U16 and out_tiles.dtype != torch.bfloat16) or not out_tiles.is_contiguous() \
             or out_tiles.numel() < T * 16 * cols or (out_tiles.dim() == 4 and out_tiles.shape[1] * 16 != cols):
         raise ValueError("out_tiles must be contiguous 16-bit x tiles of n_kv * n_q * head_dim columns")
-    if max_pages is None:
-        max_pages = (kv.capacity + 63) // 64
+    most = (kv.capacity + 63) // 64
+    if max_pages is None or max_pages > most:
+        max_pages = most
     if scratch is None:
         if tc._stream is not None:
             raise ValueError("with a stream set by set_kernel_stream, pass scratch (window_attention_scratch)")

@@ -243,6 +243,53 @@ def test_a_bad_token_where_two_prompts_meet():
         assert torch.equal(heads.view(torch.int16).reshape(160, -1), clean)
 
 
+@pytest.mark.parametrize("D,n_q", [(32, 1), (64, 4), (64, 3), (128, 8)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (2100, 300), (2050, 0)])
+@pytest.mark.parametrize("lengths", [(4,), (33,), (40, 25, 3, 30), (130, 7)])
+def test_short_prompts_on_long_caches(D, n_q, window, sinks, lengths):
+    """Few rows of few sequences over many leaves: tiles whose leaves are split among
+    workgroups, short runs in them left to rows; one lane without a sequence, one with no
+    position, capacities that change the split, and every row alone."""
+    say("split tiles", D, n_q, window, sinks, lengths)
+    c = Case(D + sum(lengths), len(lengths), 2900, 3, n_q, D, 16)
+    slot = [s for s, n in enumerate(lengths) for _ in range(n)]
+    pos = [(2899, 2600, 2304, 2047)[s] - n + 1 + i for s, n in enumerate(lengths) for i in range(n)]
+    rows = len(slot)
+    q = c.queries(rows)
+    tiles = c.check(q, slot, pos, window, sinks, runs=max(lengths))
+    a = layout.untile_lanes(tiles, rows)
+    for runs in (0, 1, 2, rows):
+        assert torch.equal(tiles, c.run(q, slot, pos, window, sinks, runs=runs)), runs
+    assert torch.equal(tiles, c.run(q, slot, pos, window, sinks, runs=rows, max_pages=1 << 20))
+    for j in (0, rows // 2, rows - 1):
+        assert torch.equal(layout.untile_lanes(c.run(q[j:j + 1], [slot[j]], [pos[j]], window, sinks), 1)[0], a[j]), j
+    slot[1], pos[2] = -1, -1
+    got = layout.untile_lanes(c.run(q, slot, pos, window, sinks, runs=rows), rows)
+    assert not got[1:3].any()
+    keep = [j for j in range(rows) if j not in (1, 2)]
+    assert torch.equal(got[keep], a[keep])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("at", [5, 700, 2795, 2799])
+@pytest.mark.parametrize("poison", [float("nan"), float("inf")])
+def test_a_bad_token_on_a_long_cache(D, at, poison):
+    """A bad value in one leaf of split tiles: among the sinks, where only some rows' windows
+    begin, where only some rows end. Their leaves alone are done another way."""
+    window, sinks, rows = 2101, 4, 30
+    c = Case(30, 1, 2900, 3, 4, D, 16)
+    pos = [2775 + i for i in range(rows)]
+    q = c.queries(rows)
+    clean = layout.untile_lanes(c.run(q, [0] * rows, pos, window, sinks, runs=rows), rows)
+    c.arena[int(c.table[0, at // 16]), 1, 1, 2, at % 16, 7] = poison
+    got = layout.untile_lanes(c.run(q, [0] * rows, pos, window, sinks, runs=rows), rows)
+    sees = torch.tensor([at <= p < at + window for p in pos], device=DEV)
+    heads, was = (x.reshape(rows, 3, 4, D).view(torch.bfloat16) for x in (got, clean))
+    assert not torch.isfinite(heads[sees][:, 2, :, 7]).any() and torch.equal(got[~sees], clean[~sees])
+    heads[:, 2, :, 7] = was[:, 2, :, 7]
+    assert torch.equal(heads.view(torch.int16).reshape(rows, -1), clean)
+
+
 def test_large_scores():
     """Scores that outrun exp's range, rising and falling along the cache, and weights that
     underflow: the references follow."""
