@@ -98,32 +98,52 @@ class Engine:
             self.max_pages, cfg.head_dim, page_tokens)
         lt = (max_rows + 15) // 16
         H, D = cfg.hidden, cfg.head_dim
-        self.kv = harness.PagedKv.create(slots, max_ctx, cfg.kv_heads, D, cfg.layers, page_tokens, dev,
-                                         shuffle_seed=shuffle_seed)
+        self.kv = self._cache(slots, max_ctx, page_tokens, shuffle_seed)
         self.h = torch.zeros((lt, H // 16, 16, 16), dtype=torch.float32, device=dev)
         self.x = torch.zeros((lt, H // 16, 16, 16), dtype=torch.int16, device=dev)
         self.attn = torch.zeros((lt, cfg.heads * D // 16, 16, 16), dtype=torch.int16, device=dev)
         self.z = torch.zeros((lt, cfg.mlp // 16, 16, 16), dtype=torch.int16, device=dev)
         self.lm_x = torch.zeros((lt, H // 16, 16, 16), dtype=torch.int16, device=dev)
         self.q = torch.zeros((max_rows, cfg.heads * D), dtype=torch.float32, device=dev)
-        self.scratch = torch.zeros(max_rows * cfg.kv_heads * self.max_pages * (4 * D + 8), dtype=torch.float32,
-                                   device=dev)
+        self.scratch = self._attention_scratch()
 
-    def launch(self, n: int, slot, pos, tok, items, greedy=None, best=None) -> None:
+    def _cache(self, slots, max_ctx, page_tokens, shuffle_seed) -> harness.PagedKv:
+        cfg = self.cfg
+        return harness.PagedKv.create(slots, max_ctx, cfg.kv_heads, cfg.head_dim, cfg.layers, page_tokens, self.dev,
+                                      shuffle_seed=shuffle_seed)
+
+    def _attention_scratch(self):
+        cfg = self.cfg
+        return torch.zeros(self.max_rows * cfg.kv_heads * self.max_pages * (4 * cfg.head_dim + 8), dtype=torch.float32,
+                           device=self.dev)
+
+    def _attention(self, n: int, slot, pos, items, runs: int):
+        """A step's attention, a function of the layer."""
+        cfg = self.cfg
+        scale = float(math.pow(cfg.head_dim, -0.5))
+        return lambda layer: harness.attention(
+            self.q[:n], self.kv, slot, pos, cfg.kv_heads, cfg.head_dim, scale, layer=layer, max_pages=self.max_pages,
+            out_tiles=self.attn, items=items, scratch=self.scratch, one_kernel=self.one_kernel)
+
+    def _choose(self, x, count: int, best, rules) -> None:
+        """Tokens of the first `count` lanes of x into best."""
+        harness.best_reset(best)
+        harness.lm_greedy(self.w.lm, x, count, self.cfg.vocab, best=best)
+
+    def launch(self, n: int, slot, pos, tok, items, greedy=None, best=None, rules=None, runs: int = 0) -> None:
         """Enqueue one step over n rows described by device tensors (row slots,
         positions, tokens, attention items); no host synchronization, so it can
         be captured in a HIP graph. `greedy` (device int32 row indices) selects
-        the rows whose token is wanted (None: all n), `best` receives them."""
+        the rows whose token is wanted (None: all n), `best` receives them.
+        `rules` and `runs` are ServingEngine's (stride_amd.serving)."""
         cfg, w = self.cfg, self.w
-        scale = float(math.pow(cfg.head_dim, -0.5))
+        attend = self._attention(n, slot, pos, items, runs)
         harness.embed(w.embed, tok, n, cfg.hidden, h_out=self.h)
         for li, L in enumerate(w.layers):
             harness.norm(self.h, n, L["norm_attn"], cfg.rms_eps, x_out=self.x)
             harness.qkv(L["q"], L["k"], L["v"], self.x, n, cfg.head_dim, w.rope, slot, pos, self.kv, layer=li,
                         q_out=self.q)
-            harness.attention(self.q[:n], self.kv, slot, pos, cfg.kv_heads, cfg.head_dim, scale, layer=li,
-                              max_pages=self.max_pages, out_tiles=self.attn, items=items, scratch=self.scratch,
-                              one_kernel=self.one_kernel)
+            attend(li)
             harness.gemm_residual(L["o"], self.attn, self.h, n)
             harness.norm(self.h, n, L["norm_mlp"], cfg.rms_eps, x_out=self.x)
             harness.mlp13(L["w1"], L["w3"], self.x, n, out=self.z)
@@ -136,8 +156,7 @@ class Engine:
         if greedy is not None:
             harness.compact(self.x, greedy, out_tiles=self.lm_x)
             x = self.lm_x
-        harness.best_reset(best)
-        harness.lm_greedy(w.lm, x, count, cfg.vocab, best=best)
+        self._choose(x, count, best, rules)
 
     def device_rows(self, rows):
         """Device tensors (slot, pos, tok, items) for rows [(slot, pos, token)];
@@ -151,19 +170,20 @@ class Engine:
                              dtype=torch.int32, device=dev).reshape(-1)
         return slot, pos, tok, items
 
-    def step(self, rows, greedy):
+    def step(self, rows, greedy, **how):
         """One step over rows [(slot, pos, token)]; returns (index, value bits) for
-        the rows listed in `greedy` (indices into rows), in that order."""
+        the rows listed in `greedy` (indices into rows), in that order. `how` goes
+        to launch."""
         n = len(rows)
         assert 0 < n <= self.max_rows
         slot, pos, tok, items = self.device_rows(rows)
         if not greedy:
-            self.launch(n, slot, pos, tok, items)
+            self.launch(n, slot, pos, tok, items, **how)
             return []
         count = len(greedy)
         sel = None if count == n else torch.tensor(greedy, dtype=torch.int32, device=self.dev)
         best = torch.empty((count, 2), dtype=torch.int32, device=self.dev)
-        self.launch(n, slot, pos, tok, items, greedy=sel, best=best)
+        self.launch(n, slot, pos, tok, items, greedy=sel, best=best, **how)
         b = best.cpu().numpy().view(np.uint32).reshape(count, 2)
         return [(int(b[i, 1].view(np.int32)), int(b[i, 0])) for i in range(count)]
 

@@ -328,10 +328,10 @@ def window_attention(q, kv: PagedKv, row_slot, row_pos, n_kv: int, n_q: int, hea
     """Attention of rows (row_slot, row_pos) over the paged cache: every position up to the
     row's own (window 0), or the last `window` and the first `sinks` ones. q: [rows][n_kv *
     n_q * head_dim] fp32 (rows may be strided). A row with row_pos < 0 or row_slot < 0 gets
-    zeros. max_pages: no row lies behind position 64 * max_pages - 1 (default: the slots' capacity). runs: a
-    hint, how many neighbouring rows are of one sequence at most (1: decode; 0: not known).
-    scratch: window_attention_scratch() (default: allocated here, on torch's current stream).
-    Returns bf16 x tiles."""
+    zeros. max_pages: no row lies behind position 64 * max_pages - 1 (default: the slots'
+    capacity). runs: a hint, how many neighbouring rows are of one sequence at most (1:
+    decode; 0: not known). scratch: window_attention_scratch() (default: allocated here, on
+    torch's current stream). Returns bf16 x tiles."""
     rows, cols = int(q.shape[0]), n_kv * n_q * head_dim
     here(q)
     if q.dtype != torch.float32 or q.dim() != 2 or q.shape[1] != cols or (cols > 1 and q.stride(1) != 1):
