@@ -371,23 +371,26 @@ __global__ __launch_bounds__(256, 2) void k_leaves(StrideWindowAttentionParams p
 
 // A workgroup a unit (row, group); with tiles that k_tile may have done (done: its marks), a
 // workgroup looks at up to 256 units, spread over the batch, and takes those that are left.
-__device__ __forceinline__ bool unit_done(const StrideWindowAttentionParams& p, int unit, const int32_t* done, int tile_rows) {
+__device__ __forceinline__ bool unit_done(const StrideWindowAttentionParams& p, int unit, const int32_t* done, int tile_rows, int parts) {
   const int j = unit / p.n_kv, tile = j / tile_rows;
-  const int32_t* mark = done + (tile * p.n_kv + unit % p.n_kv) * 2;
-  if (mark[0] == mark[1]) return mark[0];
-  int part = 0;  // is the row of the tile's first run?
-  for (int i = tile * tile_rows + 1; i <= j; ++i) part |= p.row_slot[i] != p.row_slot[i - 1];
-  return mark[part];
+  const int32_t* mark = done + (tile * p.n_kv + unit % p.n_kv) * parts;
+  bool same = true;
+  for (int i = 1; i < parts; ++i) same &= mark[i] == mark[0];
+  if (same) return mark[0];
+  int run = 0;  // the row's, in its tile
+  for (int i = tile * tile_rows + 1; i <= j; ++i) run += p.row_slot[i] != p.row_slot[i - 1];
+  return mark[run % parts];
 }
 template <int D>
-__global__ __launch_bounds__(256, 2) void k_rows(StrideWindowAttentionParams p, int page_shift, int limit, const int32_t* done, int tile_rows) {
+__global__ __launch_bounds__(256, 2) void k_rows(StrideWindowAttentionParams p, int page_shift, int limit, const int32_t* done, int tile_rows,
+                                                 int parts) {
   if (!done) {
     one_row<D, false>(p, page_shift, limit, 0, blockIdx.x % p.n_kv, blockIdx.x / p.n_kv, 0);
     return;
   }
   __shared__ uint64_t left[4];
   const int units = p.l.rows * p.n_kv, mine = threadIdx.x * gridDim.x + blockIdx.x;
-  const uint64_t b = __ballot(mine < units && !unit_done(p, mine, done, tile_rows));
+  const uint64_t b = __ballot(mine < units && !unit_done(p, mine, done, tile_rows, parts));
   if ((threadIdx.x & 63) == 0) left[threadIdx.x >> 6] = b;
   __syncthreads();
 #pragma unroll 1
@@ -421,12 +424,15 @@ __global__ __launch_bounds__(256, 2) void k_rows(StrideWindowAttentionParams p, 
 // them (64 rows at 8192 positions, 8 groups, head_dim 64: 139 us otherwise, 45 so). There a
 // workgroup takes part in all of its tile's runs, one after the other.
 //
-// Rows of several sequences meet in a tile where prompts end: one workgroup takes the first
-// run of a tile, another the rest, run by run, each column taking part in its own. A tile of
-// many short runs is left to k_rows, and so is one with a value that is not finite among
-// positions that some of its columns must not see (0 times it is NaN). done[(tile * n_kv + g) *
-// parts + part]: whether it was done; with SPLIT, part = leaf % parts, otherwise parts is 2.
+// Rows of several sequences meet in a tile where prompts end. `parts` workgroups take its runs
+// in turn, each column taking part in its own; a wave without a column of the run only helps
+// with the copies (64 prompts of 8 rows at 1024 positions, head_dim 64: 37 us; 62 with two parts
+// always, 74 with such waves in the products too; the rows alone 140). A tile of many short runs
+// is left to k_rows, and so is a part with a value that is not finite among positions that some
+// columns of its run must not see (0 times it is NaN). done[(tile * n_kv + g) * parts + part]:
+// whether it was done; with SPLIT, part = leaf % parts, otherwise run % parts.
 constexpr int kColumns = 128;
+constexpr int kRunRows = 4;  // rows a run, on average, below which a tile is left to k_rows
 
 template <int D>
 struct Lay {
@@ -507,7 +513,7 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
   __shared__ uint64_t starts[2];  // bit i: row i begins a run
   __shared__ int bad[2][kWaves];
   const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, cl = lane & 15, quarter = lane >> 4;
-  // The first runs' workgroups first (most of the others only leave; taken in turn with them,
+  // The first runs' workgroups first (many of the others only leave; taken in turn with them,
   // they left whole CUs idle: 2048 rows of window 512 70 us against 41), and later rows, which
   // see more, before earlier ones.
   const int tiles = gridDim.x / p.n_kv / parts, unit = blockIdx.x / p.n_kv;
@@ -528,7 +534,7 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
   __syncthreads();
   const uint64_t first = starts[0], second = starts[1];
   const int runs = __popcll(first) + __popcll(second);
-  const bool left = nr < 4 * runs;
+  const bool left = nr < kRunRows * runs;
   if (left || (!SPLIT && runs <= part)) {
     if (t == 0) *mark = left ? 0 : 1;
     return;
@@ -564,10 +570,13 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
     v_off[u] = (lane / L::kRow * D + L::v_from(r, slot_in) * 8) * 2;
   }
 
-  const int begin = !SPLIT && part ? next_run(0) : 0, end = SPLIT || part ? nr : next_run(0);
-  for (int r0 = begin; r0 < end;) {
+  bool taken = false;  // has this lane's column been in a run of this part's?
+  int turn = SPLIT ? 0 : part;
+  for (int r0 = 0, r1; r0 < nr; r0 = r1) {
+    r1 = next_run(r0);
+    if (!SPLIT && turn-- != 0) continue;
+    turn = parts - 1;
     // the run [r0, r1): its sequence, and what its rows see together
-    const int r1 = next_run(r0);
     int low = INT_MAX, high = -1;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -580,9 +589,8 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
     low = -1 - wave_most(-1 - low);
     high = wave_most(high);
     const bool mine = row >= r0 && row < r1;
+    taken |= mine;
     const int slot = __builtin_amdgcn_readfirstlane(slots[r0]);
-    const bool whole = r0 == 0 && r1 == nr;
-    r0 = r1;
     if (high < 0) continue;
     const Sight near = sight_of(p, low, limit), far = sight_of(p, high, limit);
     // spans: [0, all_head) and [all_rest, all_last]
@@ -647,8 +655,42 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) split_query(q + 32 * k, p.scale * kLog2e, live, qh[k], ql[k]);
       }
-      int buf = 0;
-      for (int i = 0; i < spans;) {
+      // do all of the run's columns see all of the span from a?
+      auto is_full = [&](int a) __attribute__((always_inline)) {
+        return a + kSpan - 1 <= low && (a >= far.lo || a + kSpan <= near.sink_end);
+      };
+      // Waits until span i has arrived, and every wave has read the one before, whose buffer is
+      // filled next (the copies of the next may be under way). False: it holds a value that is not
+      // finite, and not all of the run's columns see it; nothing more is to be done here.
+      auto arrived = [&](int i, bool full, int buf) __attribute__((always_inline)) {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kBufs - 2) * 2 * kPer) : "memory");
+        lds_barrier();
+        if (full) return true;
+        bool b = false;
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) b |= has_nonfinite(*reinterpret_cast<const u32x4*>(&vs[buf][((wave * kPer + u) * 64 + lane) * 8]));
+        const bool any = __any(b);
+        if (lane == 0) bad[i & 1][wave] = any;
+        lds_barrier();
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) sum |= bad[i & 1][w];
+        if (!__builtin_amdgcn_readfirstlane(sum)) return true;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (t == 0) *mark = 0;
+        return false;
+      };
+      int buf = 0, i = 0;
+      // a wave without a column of this run only helps with the copies
+      if (!__any(mine))
+        for (; i < spans; ++i) {
+          const int a = span_at(i) * kSpan;
+          if (!arrived(i, is_full(a), buf)) __builtin_amdgcn_endpgm();
+          copy(i + kBufs - 1, buf == 0 ? kBufs - 1 : buf - 1);
+          look(i + kBufs);
+          buf = buf == kBufs - 1 ? 0 : buf + 1;
+        }
+      while (i < spans) {
         const int leaf = span_at(i) / (kLeaf / kSpan);
         f32x4 acc[kDims], l = {0, 0, 0, 0};
         float ref = neg_inf();
@@ -656,31 +698,14 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
         for (int d = 0; d < kDims; ++d) acc[d] = f32x4{0, 0, 0, 0};
         do {
           const int a = span_at(i) * kSpan;
-          // do all columns see all of it?
-          const bool full = whole && a + kSpan - 1 <= low && (a >= far.lo || a + kSpan <= near.sink_end);
-          // this span has arrived, and every wave has read the one before, whose buffer is filled next
-          // (the copies of the next may be under way)
-          asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kBufs - 2) * 2 * kPer) : "memory");
-          lds_barrier();
-          if (!full) {
-            bool b = false;
-#pragma unroll
-            for (int u = 0; u < kPer; ++u) b |= has_nonfinite(*reinterpret_cast<const u32x4*>(&vs[buf][((wave * kPer + u) * 64 + lane) * 8]));
-            const bool any = __any(b);
-            if (lane == 0) bad[i & 1][wave] = any;
-            lds_barrier();
-            int sum = 0;
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) sum |= bad[i & 1][w];
-            if (__builtin_amdgcn_readfirstlane(sum)) {
-              asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-              if (t == 0) *mark = 0;
-              // Two ways to leave, for the registers that the compiler gives the loop around them:
-              // head_dim 64, 2048 rows of window 512 take 31.5 us so and 34.4 with the return;
-              // 256 rows of 8192 positions, C == 2, 152 and 141.
-              if constexpr (C == 1) __builtin_amdgcn_endpgm();
-              return;
-            }
+          const bool full = is_full(a);
+          if (!arrived(i, full, buf)) {
+            // Two ways to leave, for the registers that the compiler gives the loop around them: 2048
+            // rows of window 512 take 31.5 us so and 34.4 with the return (head_dim 64), 1000 rows of
+            // three sequences of 3000 positions 108 and 116 (128); but 256 rows of 8192 positions,
+            // head_dim 64 and C == 2, 152 and 141.
+            if constexpr (D != 64 || C == 1) __builtin_amdgcn_endpgm();
+            return;
           }
           copy(i + kBufs - 1, buf == 0 ? kBufs - 1 : buf - 1);
           look(i + kBufs);
@@ -784,10 +809,11 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
             if (quarter == 0) *reinterpret_cast<f32x2*>(rec + p.n_q * D + 2 * head) = f32x2{ref, l[0]};
           }
         } else {
+          // (other runs' columns took part with what they do not see)
           float fa, fb;
-          fold.take(ref, l[0], fa, fb);
+          fold.take(mine ? ref : neg_inf(), mine ? l[0] : 0.0f, fa, fb);
 #pragma unroll
-          for (int d = 0; d < kDims; ++d) total[d] = folded(total[d], acc[d], fa, fb);
+          for (int d = 0; d < kDims; ++d) total[d] = folded(total[d], mine ? acc[d] : f32x4{0, 0, 0, 0}, fa, fb);
         }
       }
       // nothing is on its way to the buffers, and every wave has read them, when another pass comes
@@ -795,7 +821,7 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
       lds_barrier();
     }
   }
-  if (!SPLIT && live && row >= begin && row < end) {
+  if (!SPLIT && live && taken) {
     const float sum = my_pos < 0 ? 0.0f : fold.sum;
 #pragma unroll
     for (int d = 0; d < kDims; ++d) put_out(p, j0 + row, g, head, 16 * d + 4 * quarter, total[d], sum);
@@ -889,6 +915,7 @@ struct Plan {
   int page_shift, limit, span;
   int tile_rows;  // 0: no tiles
   int parts;      // marks of a tile and group
+  int64_t runs;   // of tiles and groups together, about
   bool split;
   int64_t records, scratch;  // floats; the tiles' marks come behind the records
 };
@@ -920,20 +947,29 @@ const char* plan_of(const StrideWindowAttentionParams& p, Plan& plan) {
   if (units * span > INT_MAX) return "rows, n_kv and the context are too large together";
   // Tiles where neighbouring rows may be of one sequence (a tile's copies of 64 / (head_dim / 8)
   // rows lie in one page). Leaves in workgroups of their own, and joined, where the rows or
-  // tiles alone would not fill the chip: below 512 workgroups of k_rows; of tiles where rows are
-  // few (2048 units are 512 of them at n_q = 4) and leaves at least eight, for the records and
-  // two launches more (64 rows of 2000 positions, 8 groups, head_dim 64 / 128: 21 / 31 us
-  // against 42 / 64 row by row; of 600 positions 18 / 24 against 21 / 29, but 16 rows 15 / 20
-  // against 13 / 16, and 200 rows 24 / 37 against 22 / 32 in whole tiles).
+  // tiles alone would not fill the chip: below 512 workgroups of k_rows; of tiles below 64, a
+  // quarter of the CUs (192 rows of one sequence at 8192, 48 tiles, head_dim 64 / 128: 118 / 168
+  // us against 143 / 226 in whole tiles; 256 rows, 64 tiles: 154 / 223 against 141 / 225), and
+  // with eight leaves or more, for the records and two launches more (64 rows of 2000 positions:
+  // 21 / 31 us against 42 / 64; of 600 positions 18 / 24 against 21 / 29, but 16 rows 15 / 20
+  // against 13 / 16, and 200 rows 24 / 37 against 22 / 32).
   const int64_t records = units * span * ((p.n_q * (D + 2) + 3) / 4 * 4);
   const bool may_split = span > 1 && records <= int64_t{1} << 28;  // a GiB
   bool tiles = p.runs != 1 && p.l.rows >= 4 && tokens >= 512 / D;
-  plan.split = may_split && tiles && p.runs > 1 && span >= 8 && units < 2048;
+  const int64_t rows_a_tile = kColumns / p.n_q, groups = (p.l.rows + rows_a_tile - 1) / rows_a_tile * p.n_kv;
+  plan.split = may_split && tiles && p.runs > 1 && span >= 8 && groups < 64;
   if (!plan.split && may_split && units < 512) plan.split = true, tiles = false;
-  plan.tile_rows = tiles ? kColumns / p.n_q : 0;
+  plan.tile_rows = tiles ? static_cast<int>(rows_a_tile) : 0;
   plan.parts = plan.split ? static_cast<int>(std::min<int64_t>((static_cast<int64_t>(plan.limit) + kLeaf - 1) / kLeaf, span + 1)) : 2;
+  // As many parts as a tile may have runs, where the chip has room for them at once (128 prompts
+  // of 8 rows at 1024 positions, head_dim 128, 256 tiles: 129 us with two parts, 146 with five).
+  if (tiles && !plan.split) {
+    const int most = plan.tile_rows / kRunRows, room = static_cast<int>((D < 128 ? 1024 : 512) / groups);
+    plan.parts = std::max(2, std::min(room, p.runs > 0 ? std::min(most, (plan.tile_rows - 1) / p.runs + 2) : most));
+  }
+  plan.runs = groups * std::max(1, p.runs > 0 ? plan.tile_rows / p.runs : 1);
   plan.records = plan.split ? records : 0;
-  const int64_t marks = tiles ? (static_cast<int64_t>(p.l.rows) + plan.tile_rows - 1) / plan.tile_rows * p.n_kv * plan.parts : 0;
+  const int64_t marks = tiles ? groups * plan.parts : 0;
   if (marks > INT_MAX) return "rows, n_kv and the context are too large together";
   plan.scratch = plan.records + marks;
   return nullptr;
@@ -954,7 +990,7 @@ int run(const StrideWindowAttentionParams& p, const Plan& plan, hipStream_t st) 
     const dim3 grid(groups), block(512);
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, p, plan.page_shift, plan.limit, plan.tile_rows, done, plan.span, plan.parts); };
     if (plan.split) launch(k_tile<D, 2, true>);
-    else if (D != 64 || groups <= 2 * 256) launch(k_tile<D, 2, false>);
+    else if (D != 64 || plan.runs <= 256) launch(k_tile<D, 2, false>);
     else launch(k_tile<64, 1, false>);
     if (int rc = launched("window_attention (tiles)")) return rc;
   }
@@ -968,7 +1004,7 @@ int run(const StrideWindowAttentionParams& p, const Plan& plan, hipStream_t st) 
   }
   // (with tiles most of the workgroups only find that nothing is left)
   const int groups = done ? std::max(std::min(units, 1024), (units + 255) / 256) : units;
-  hipLaunchKernelGGL((k_rows<D>), dim3(groups), dim3(256), 0, st, p, plan.page_shift, plan.limit, done, tile_rows);
+  hipLaunchKernelGGL((k_rows<D>), dim3(groups), dim3(256), 0, st, p, plan.page_shift, plan.limit, done, tile_rows, plan.parts);
   return launched("window_attention");
 }
 

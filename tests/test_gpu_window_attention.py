@@ -270,6 +270,32 @@ def test_short_prompts_on_long_caches(D, n_q, window, sinks, lengths):
     assert torch.equal(got[keep], a[keep])
 
 
+@pytest.mark.parametrize("D,n_q,each", [(64, 4, 8), (64, 4, 5), (128, 4, 4), (32, 1, 11), (64, 16, 4)])
+@pytest.mark.parametrize("runs", [0, 1, 2])
+def test_a_bad_token_where_many_prompts_meet(D, n_q, each, runs):
+    """Tiles of several short runs, which workgroups take in turn: a bad value that only some
+    rows of one prompt see makes that prompt's rows alone another way's work."""
+    say("many prompts", D, n_q, each, runs)
+    seqs = 24
+    c = Case(D + each, seqs, 500, 2, n_q, D, 16)
+    slot = [s for s in range(seqs) for _ in range(each)]
+    pos = [300 + 7 * s + i for s in range(seqs) for i in range(each)]
+    rows = len(slot)
+    q = c.queries(rows)
+    hint = (0, each, 1)[runs]
+    clean = layout.untile_lanes(c.check(q, slot, pos, 130, 2, runs=hint), rows)
+    assert torch.equal(clean, layout.untile_lanes(c.run(q, slot, pos, 130, 2, runs=1), rows))
+    bad = {5: 300 + 35 + 2, 6: 300 + 42 + each, 13: 300 + 91 - 129, 20: 1}
+    for s, at in bad.items():
+        c.arena[int(c.table[s, at // 16]), 1, 1, 1, at % 16, 9] = float("inf")
+    got = layout.untile_lanes(c.run(q, slot, pos, 130, 2, runs=hint), rows)
+    sees = torch.tensor([s in bad and bad[s] <= p and (p - bad[s] < 130 or bad[s] < 2) for s, p in zip(slot, pos)], device=DEV)
+    heads, was = (x.reshape(rows, 2, n_q, D).view(torch.bfloat16) for x in (got, clean))
+    assert torch.isinf(heads[sees][:, 1, :, 9]).all() and torch.equal(got[~sees], clean[~sees])
+    heads[:, 1, :, 9] = was[:, 1, :, 9]
+    assert torch.equal(heads.view(torch.int16).reshape(rows, -1), clean)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("at", [5, 700, 2795, 2799])
 @pytest.mark.parametrize("poison", [float("nan"), float("inf")])
