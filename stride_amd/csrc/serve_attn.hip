@@ -955,15 +955,19 @@ const char* plan_of(const StrideWindowAttentionParams& p, Plan& plan) {
   // against 13 / 16, and 200 rows 24 / 37 against 22 / 32).
   const int64_t records = units * span * ((p.n_q * (D + 2) + 3) / 4 * 4);
   const bool may_split = span > 1 && records <= int64_t{1} << 28;  // a GiB
-  bool tiles = p.runs != 1 && p.l.rows >= 4 && tokens >= 512 / D;
+  bool tiles = (p.runs == 0 || p.runs >= kRunRows) && p.l.rows >= kRunRows && tokens >= 512 / D;
   const int64_t rows_a_tile = kColumns / p.n_q, groups = (p.l.rows + rows_a_tile - 1) / rows_a_tile * p.n_kv;
-  plan.split = may_split && tiles && p.runs > 1 && span >= 8 && groups < 64;
+  plan.split = may_split && tiles && p.runs > 0 && span >= 8 && groups < 64;
   if (!plan.split && may_split && units < 512) plan.split = true, tiles = false;
   plan.tile_rows = tiles ? static_cast<int>(rows_a_tile) : 0;
   plan.parts = plan.split ? static_cast<int>(std::min<int64_t>((static_cast<int64_t>(plan.limit) + kLeaf - 1) / kLeaf, span + 1)) : 2;
   // As many parts as a tile may have runs, where the chip has room for them at once (128 prompts
   // of 8 rows at 1024 positions, head_dim 128, 256 tiles: 129 us with two parts, 146 with five).
-  if (tiles && !plan.split) {
+  // One where the rows look like one sequence's, for the workgroups that only leave again.
+  const bool one = p.runs >= p.l.rows;
+  if (one && !plan.split) {
+    plan.parts = 1;
+  } else if (tiles && !plan.split) {
     const int most = plan.tile_rows / kRunRows, room = static_cast<int>((D < 128 ? 1024 : 512) / groups);
     plan.parts = std::max(2, std::min(room, p.runs > 0 ? std::min(most, (plan.tile_rows - 1) / p.runs + 2) : most));
   }
@@ -1002,8 +1006,11 @@ int run(const StrideWindowAttentionParams& p, const Plan& plan, hipStream_t st) 
     hipLaunchKernelGGL((k_join<D>), dim3(units * parts), dim3(256), 0, st, p, plan.limit, plan.span, parts);
     return launched("window_attention (join)");
   }
-  // (with tiles most of the workgroups only find that nothing is left)
-  const int groups = done ? std::max(std::min(units, 1024), (units + 255) / 256) : units;
+  // With tiles most of the workgroups only find that nothing is left; the fewer where that is
+  // likely for all of them (2048 rows of one sequence, window 512, head_dim 64: 30.1 us with 1024
+  // of them and parts for two runs, 28.7 so; but 128 sequences of 2 rows that were left 85 us with
+  // 1024 and 126 with 256).
+  const int groups = done ? std::max(std::min(units, p.runs >= p.l.rows ? 256 : 1024), (units + 255) / 256) : units;
   hipLaunchKernelGGL((k_rows<D>), dim3(groups), dim3(256), 0, st, p, plan.page_shift, plan.limit, done, tile_rows, plan.parts);
   return launched("window_attention");
 }
