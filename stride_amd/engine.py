@@ -127,6 +127,8 @@ class Engine:
 
     def _choose(self, x, count: int, best, rules) -> None:
         """Tokens of the first `count` lanes of x into best."""
+        if rules is not None:
+            raise ValueError("rules want a ServingEngine")
         harness.best_reset(best)
         harness.lm_greedy(self.w.lm, x, count, self.cfg.vocab, best=best)
 

@@ -340,6 +340,10 @@ def window_attention(q, kv: PagedKv, row_slot, row_pos, n_kv: int, n_q: int, hea
         raise ValueError("row_slot and row_pos must be int32, one for each row")
     if not (row_slot.is_contiguous() and row_pos.is_contiguous()):
         raise ValueError("row_slot and row_pos must be contiguous")
+    dev = q.get_device()
+    if not row_slot.get_device() == row_pos.get_device() == kv.table.get_device() == dev \
+            or out_tiles is not None and out_tiles.get_device() != dev or scratch is not None and scratch.get_device() != dev:
+        raise ValueError("the arguments are on different devices")
     if not 0 <= layer < kv.ref.block_elems // kv.ref.layer_elems or kv.ref.which_elems != n_kv * kv.ref.group_elems:
         raise ValueError("layer or n_kv is not the cache's")
     T = (rows + 15) // 16

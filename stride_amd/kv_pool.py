@@ -144,6 +144,8 @@ class KvPool:
         """The first tokens[i] (None: all) tokens of page src[i] to page dst[i] of `into` (None:
         this pool). Tables and counts stay as they are."""
         n = self._items(src, dst) if tokens is None else self._items(src, dst, tokens)
+        if into is not None and into._device != self._device:
+            raise ValueError("the pools must be on one device")
         _run(_lib.load().stride_kv_copy(self._at, None if into is None else into._at, src.data_ptr(), dst.data_ptr(),
                                         0 if tokens is None else tokens.data_ptr(), n, tc.kernel_stream()))
 

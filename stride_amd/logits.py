@@ -135,46 +135,46 @@ def process(logits, rows: int, vocab: int, counts: TokenCounts | None = None, ro
     if logits.dtype != f32 or len(shape) != 4 or shape[1] != T or shape[0] * 16 < vocab or shape[2] != 16 or shape[3] != 16 \
             or not logits.is_contiguous():
         raise ValueError("logits must be contiguous fp32 tiles [ceil(vocab / 16)][ceil(rows / 16)][16][16]")
-    o_at = 0
+    dev, o_at = logits.get_device(), 0
     if out is not None:
-        if out.dtype != f32 or out.shape != shape or not out.is_contiguous():
+        if out.get_device() != dev or out.dtype != f32 or out.shape != shape or not out.is_contiguous():
             raise ValueError("out must be tiles like logits")
         o_at = out.data_ptr()
     if best is None:
         best = torch.empty((rows, 2), dtype=i32, device=logits.device)
-    elif best.dtype != i32 or best.numel() < 2 * rows or not best.is_contiguous():
+    elif best.get_device() != dev or best.dtype != i32 or best.numel() < 2 * rows or not best.is_contiguous():
         raise ValueError("best must be contiguous int32 [rows][2]")
     c = s = sl = pen = slots = 0
     if counts is not None:
-        if counts.vocab != vocab or counts.counts.get_device() != logits.get_device():
+        if counts.vocab != vocab or counts._device != dev:
             raise ValueError("the counts are of another vocabulary or device")
         if row_slot is None or penalties is None:
             raise ValueError("counts need row_slot and penalties")
-        if row_slot.dtype != i32 or row_slot.numel() < rows or not row_slot.is_contiguous():
+        if row_slot.get_device() != dev or row_slot.dtype != i32 or row_slot.numel() < rows or not row_slot.is_contiguous():
             raise ValueError("row_slot must be contiguous int32 [rows]")
-        if penalties.dtype != f32 or penalties.numel() < 3 * rows or not penalties.is_contiguous():
+        if penalties.get_device() != dev or penalties.dtype != f32 or penalties.numel() < 3 * rows or not penalties.is_contiguous():
             raise ValueError("penalties must be contiguous fp32 [rows][3]")
         c, s, sl, pen, slots = counts._counts_at, counts._seen_at, row_slot.data_ptr(), penalties.data_ptr(), counts.slots
     bo = bt = bv = 0
     if bias is not None:
         o, t, v = bias
         n = t.numel()
-        if o.dtype != i32 or t.dtype != i32 or v.dtype != f32 or o.numel() < rows + 1 or v.numel() != n \
+        if not o.get_device() == t.get_device() == v.get_device() == dev or o.dtype != i32 or t.dtype != i32 or v.dtype != f32 or o.numel() < rows + 1 or v.numel() != n \
                 or not (o.is_contiguous() and t.is_contiguous() and v.is_contiguous()):
             raise ValueError("bias is (offsets int32 [rows + 1], tokens int32, values fp32), contiguous")
         if n:  # without entries there is nothing to add
             bo, bt, bv = o.data_ptr(), t.data_ptr(), v.data_ptr()
     mk = mr = masks = 0
     if mask is not None:
-        if mask.dtype != i32 or mask.dim() != 2 or mask.size(1) != (vocab + 31) // 32 or not mask.is_contiguous():
+        if mask.get_device() != dev or mask.dtype != i32 or mask.dim() != 2 or mask.size(1) != (vocab + 31) // 32 or not mask.is_contiguous():
             raise ValueError("mask must be contiguous int32 [masks][ceil(vocab / 32)]")
-        if mask_row is None or mask_row.dtype != i32 or mask_row.numel() < rows or not mask_row.is_contiguous():
+        if mask_row is None or mask_row.get_device() != dev or mask_row.dtype != i32 or mask_row.numel() < rows or not mask_row.is_contiguous():
             raise ValueError("a mask needs mask_row, contiguous int32 [rows]")
         mk, mr, masks = mask.data_ptr(), mask_row.data_ptr(), mask.size(0)
     stream = tc.kernel_stream()
     if work is None:
         work = _work_of(counts, T, rows, stream, logits.device)
-    elif work.dtype != torch.int64 or work.numel() < T * UNIT or not work.is_contiguous():
+    elif work.get_device() != dev or work.dtype != torch.int64 or work.numel() < T * UNIT or not work.is_contiguous():
         raise ValueError("work must be scratch(rows)")
     p = _LOGITS(rows, T, 0, 0, logits.data_ptr(), o_at, sl, c, s, pen, bo, bt, bv, mk, mr, best.data_ptr(), work.data_ptr(),
                 vocab, slots, masks)

@@ -24,7 +24,7 @@ import typing
 
 import torch
 
-from . import engine, harness, logits
+from . import engine, harness, logits, tc
 from .kv_pool import KvPool
 
 
@@ -189,6 +189,8 @@ class ServingEngine(engine.Engine):
         return t[0], t[1], t[2], None
 
     def _attention(self, n, slot, pos, items, runs):
+        if tc._stream is not None:
+            raise ValueError("a ServingEngine allocates for its steps, on torch's current stream: none may be set by set_kernel_stream")
         cfg = self.cfg
         scale = float(math.pow(cfg.head_dim, -0.5))
         scratch = harness.window_attention_scratch(n, cfg.kv_heads, cfg.repeat(), cfg.head_dim, self.window, self.sinks,

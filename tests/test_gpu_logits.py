@@ -289,3 +289,20 @@ def test_refusals():
             bad()
     empty = logits.process(torch.zeros((7, 0, 16, 16), device=DEV), 0, 100)
     assert empty.shape == (0, 2)
+
+
+def test_arguments_of_another_device():
+    """Each argument in host memory is refused before anything is launched."""
+    l = tiles_of(np.zeros((5, 100), np.float32))
+    c = logits.TokenCounts.create(2, 100, DEV)
+    slot = torch.zeros(5, dtype=torch.int32, device=DEV)
+    good = dict(logits=l, rows=5, vocab=100, counts=c, row_slot=slot, penalties=torch.ones((5, 3), device=DEV),
+                bias=logits.bias_lists([{1: 2.0}] * 5, DEV), mask=torch.full((1, 4), -1, dtype=torch.int32, device=DEV), mask_row=slot.clone(),
+                out=torch.zeros_like(l), best=torch.zeros((5, 2), dtype=torch.int32, device=DEV), work=logits.scratch(5, DEV))
+    logits.process(**good)
+    host = {k: v.cpu() for k, v in good.items() if isinstance(v, torch.Tensor)}
+    host["counts"] = logits.TokenCounts.create(2, 100, "cpu")
+    host["bias"] = tuple(t.cpu() for t in good["bias"])
+    for name, value in host.items():
+        with pytest.raises(ValueError):
+            logits.process(**{**good, name: value})

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from stride_amd import cli, engine, harness, layout, logits, serving, weights
+from stride_amd import cli, engine, harness, layout, logits, serving, tc, weights
 from stride_amd.kv_pool import KvPool
 import llama_tiny
 
@@ -170,6 +170,22 @@ def test_pages_come_back(model):
     eng.pool.reserve(*eng._ints([[1], [0], [19]]))  # behind the book's back: more than there is
     with pytest.raises(Exception, match="kv pool"):
         eng.check()
+
+
+def test_engine_refusals(model):
+    eng = serving.ServingEngine(model[1], 2, 64, 16)
+    for rows in ([(2, 0, 1)], [(-1, 0, 1)], [(0, 64, 1)], [(0, -1, 1)]):
+        with pytest.raises(ValueError):
+            eng.step(rows, [0])
+    tc.set_kernel_stream(torch.cuda.current_stream().cuda_stream)
+    try:
+        with pytest.raises(ValueError, match="current stream"):
+            eng.step([(0, 0, 1)], [0])
+    finally:
+        tc.set_kernel_stream(None)
+    plain = engine.Engine(model[1], 1, 64, 16)
+    with pytest.raises(ValueError, match="ServingEngine"):
+        plain.step([(0, 0, 1)], [0], rules=eng)
 
 
 def test_captured_decode(model):

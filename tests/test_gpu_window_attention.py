@@ -485,3 +485,18 @@ def test_no_rows():
     c = Case(19, 1, 64, 2, 4, 64, 16)
     e = torch.zeros(0, dtype=torch.int32, device=DEV)
     assert harness.window_attention(torch.zeros((0, 512), device=DEV), c.kv, e, e, 2, 4, 64, 0.125).numel() == 0
+
+
+def test_arguments_of_another_device():
+    """Each argument in host memory is refused before anything is launched."""
+    c = Case(19, 2, 128, 2, 4, 64, 16)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    good = dict(q=c.queries(2), kv=c.kv, row_slot=i32(0, 1), row_pos=i32(5, 6), n_kv=2, n_q=4, head_dim=64, scale=0.125,
+                out_tiles=torch.zeros((1, 32, 16, 16), dtype=torch.int16, device=DEV), scratch=torch.zeros(4096, device=DEV))
+    harness.window_attention(**good)
+    host = dict(kv=harness.PagedKv.over(c.arena.view(torch.int16).cpu(), c.table.cpu(), 2, 64, 2, 16))
+    for name in ("q", "row_slot", "row_pos", "out_tiles", "scratch"):
+        host[name] = good[name].cpu()
+    for name, value in host.items():
+        with pytest.raises(ValueError, match="device"):
+            harness.window_attention(**{**good, name: value})
