@@ -167,9 +167,10 @@ __device__ __forceinline__ int record_floats(int n_q, int d) { return (n_q * (d 
 // operand is 16 rows of 64 bytes), the four maxima give every wave the leaf's references,
 // the weights go through LDS, and each wave sums its quarter of the dims over the leaf. The
 // next leaf's loads are in flight meanwhile.
-// SPLIT: one leaf a workgroup, its record to scratch (few rows, long contexts).
+// SPLIT: a leaf, or at head_dim 128 `each` leaves, a workgroup, their records to scratch (few
+// rows, long contexts).
 template <int D, bool SPLIT>
-__device__ __forceinline__ void one_row(const StrideWindowAttentionParams& p, int page_shift, int limit, int span, int g, int j, int begin) {
+__device__ __forceinline__ void one_row(const StrideWindowAttentionParams& p, int page_shift, int limit, int span, int g, int j, int begin, int each) {
   constexpr int kKey = D / 32;           // operands of a key row
   constexpr int kRow = D / 8;            // 16-byte pieces of a row
   constexpr int kPer = kChunk * kRow / 64;
@@ -185,7 +186,7 @@ __device__ __forceinline__ void one_row(const StrideWindowAttentionParams& p, in
   const int slot = p.row_slot[j];
   const Sight sight = sight_of(p, pos_of(p, j), limit);
   const Leaves leaves = leaves_of(sight);
-  const int end = SPLIT ? begin + 1 : leaves.count;
+  const int end = !SPLIT ? leaves.count : D < 128 ? begin + 1 : min(begin + each, leaves.count);
   if (SPLIT && begin >= leaves.count) return;
 
   const uint16_t* base = static_cast<const uint16_t*>(p.kv.arena) + p.layer * p.kv.layer_elems + g * p.kv.group_elems;
@@ -341,13 +342,13 @@ __device__ __forceinline__ void one_row(const StrideWindowAttentionParams& p, in
         }
         if (threadIdx.x < 16) *reinterpret_cast<f32x2*>(rec + p.n_q * D + 2 * col) = f32x2{ref, l[0]};
       }
-      return;
-    }
-    float a, b;
-    fold.take(ref, l[0], a, b);
+    } else {
+      float a, b;
+      fold.take(ref, l[0], a, b);
 #pragma unroll
-    for (int x = 0; x < kOut; ++x) total[x] = folded(total[x], acc[x], a, b);
-    lds_barrier();  // the staging is written again
+      for (int x = 0; x < kOut; ++x) total[x] = folded(total[x], acc[x], a, b);
+    }
+    if (it + 1 < end) lds_barrier();  // the staging is written again
   }
   if (!SPLIT && col < p.n_q) {
 #pragma unroll
@@ -360,13 +361,13 @@ __device__ __forceinline__ void one_row(const StrideWindowAttentionParams& p, in
 
 template <int D>
 __global__ __launch_bounds__(256, 2) void k_leaves(StrideWindowAttentionParams p, int page_shift, int limit, int span, const int32_t* done,
-                                                   int tile_rows, int parts) {
-  const int unit = blockIdx.x / p.n_kv, g = blockIdx.x % p.n_kv, j = unit / span, at = unit % span;
+                                                   int tile_rows, int parts, int each, int stretches) {
+  const int unit = blockIdx.x / p.n_kv, g = blockIdx.x % p.n_kv, j = unit / stretches, at = unit % stretches * (D < 128 ? 1 : each);
   if (done) {
     const Leaves leaves = leaves_of(sight_of(p, pos_of(p, j), limit));
     if (at >= leaves.count || done[(j / tile_rows * p.n_kv + g) * parts + leaves.at(at) % parts]) return;
   }
-  one_row<D, true>(p, page_shift, limit, span, g, j, at);
+  one_row<D, true>(p, page_shift, limit, span, g, j, at, each);
 }
 
 // A workgroup a unit (row, group); with tiles that k_tile may have done (done: its marks), a
@@ -385,7 +386,7 @@ template <int D>
 __global__ __launch_bounds__(256, 2) void k_rows(StrideWindowAttentionParams p, int page_shift, int limit, const int32_t* done, int tile_rows,
                                                  int parts) {
   if (!done) {
-    one_row<D, false>(p, page_shift, limit, 0, blockIdx.x % p.n_kv, blockIdx.x / p.n_kv, 0);
+    one_row<D, false>(p, page_shift, limit, 0, blockIdx.x % p.n_kv, blockIdx.x / p.n_kv, 0, 0);
     return;
   }
   __shared__ uint64_t left[4];
@@ -398,7 +399,7 @@ __global__ __launch_bounds__(256, 2) void k_rows(StrideWindowAttentionParams p, 
 #pragma unroll 1
     for (uint64_t todo = left[w]; todo; todo &= todo - 1) {
       const int unit = __builtin_amdgcn_readfirstlane((w * 64 + __builtin_ctzll(todo)) * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x));
-      one_row<D, false>(p, page_shift, limit, 0, unit % p.n_kv, unit / p.n_kv, 0);
+      one_row<D, false>(p, page_shift, limit, 0, unit % p.n_kv, unit / p.n_kv, 0, 0);
     }
 }
 
@@ -947,7 +948,10 @@ const char* plan_of(const StrideWindowAttentionParams& p, Plan& plan) {
   if (units * span > INT_MAX) return "rows, n_kv and the context are too large together";
   // Tiles where neighbouring rows may be of one sequence (a tile's copies of 64 / (head_dim / 8)
   // rows lie in one page). Leaves in workgroups of their own, and joined, where the rows or
-  // tiles alone would not fill the chip: below 512 workgroups of k_rows; of tiles below 64, a
+  // tiles alone would not fill the chip: below 512 workgroups of k_rows, or fewer where a row
+  // has fewer than ten leaves, for the second launch (1, 8, 32, 63 rows, 8 groups, head_dim 64, split
+  // and not, of 300 positions 11, 12, 12, 18 and 10, 10, 10, 12 us; of 1000 11, 11, 19, 29 and 15,
+  // 15, 19, 24; of 2000 10, 12, 29, 45 and 26, 28, 34, 41); of tiles below 64, a
   // quarter of the CUs (192 rows of one sequence at 8192, 48 tiles, head_dim 64 / 128: 118 / 168
   // us against 143 / 226 in whole tiles; 256 rows, 64 tiles: 154 / 223 against 141 / 225), and
   // with eight leaves or more, for the records and two launches more (64 rows of 2000 positions:
@@ -958,7 +962,7 @@ const char* plan_of(const StrideWindowAttentionParams& p, Plan& plan) {
   bool tiles = (p.runs == 0 || p.runs >= kRunRows) && p.l.rows >= kRunRows && tokens >= 512 / D;
   const int64_t rows_a_tile = kColumns / p.n_q, groups = (p.l.rows + rows_a_tile - 1) / rows_a_tile * p.n_kv;
   plan.split = may_split && tiles && p.runs > 0 && span >= 8 && groups < 64;
-  if (!plan.split && may_split && units < 512) plan.split = true, tiles = false;
+  if (!plan.split && may_split && units < (span < 3 ? 1 : span < 6 ? 256 : span < 10 ? 384 : 512)) plan.split = true, tiles = false;
   plan.tile_rows = tiles ? static_cast<int>(rows_a_tile) : 0;
   plan.parts = plan.split ? static_cast<int>(std::min<int64_t>((static_cast<int64_t>(plan.limit) + kLeaf - 1) / kLeaf, span + 1)) : 2;
   // As many parts as a tile may have runs, where the chip has room for them at once (128 prompts
@@ -1000,7 +1004,13 @@ int run(const StrideWindowAttentionParams& p, const Plan& plan, hipStream_t st) 
   }
   const int tile_rows = std::max(1, plan.tile_rows);
   if (plan.split) {
-    hipLaunchKernelGGL((k_leaves<D>), dim3(units * plan.span), dim3(256), 0, st, p, plan.page_shift, plan.limit, plan.span, done, tile_rows, plan.parts);
+    // At head_dim 128 a workgroup takes up to four leaves one after the other where that leaves
+    // enough of them (63 rows of 16000 positions, 8 groups of 4 heads: 824 us leaf by leaf, 770
+    // so; 4 rows of 32768, 8 heads a group: 114 and 110). At 64, 63 rows of 4000 take 87 and 88.
+    const int64_t leaves = static_cast<int64_t>(units) * plan.span;
+    const int each = D < 128 || done ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(4, leaves / 2048)));
+    const int stretches = (plan.span + each - 1) / each;
+    hipLaunchKernelGGL((k_leaves<D>), dim3(units * stretches), dim3(256), 0, st, p, plan.page_shift, plan.limit, plan.span, done, tile_rows, plan.parts, each, stretches);
     if (int rc = launched("window_attention (leaves)")) return rc;
     const int parts = (p.n_q * D + 255) / 256;
     hipLaunchKernelGGL((k_join<D>), dim3(units * parts), dim3(256), 0, st, p, plan.limit, plan.span, parts);
