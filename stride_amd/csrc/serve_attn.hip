@@ -514,11 +514,13 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
   __shared__ uint64_t starts[2];  // bit i: row i begins a run
   __shared__ int bad[2][kWaves];
   const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, cl = lane & 15, quarter = lane >> 4;
-  // The first runs' workgroups first (many of the others only leave; taken in turn with them,
-  // they left whole CUs idle: 2048 rows of window 512 70 us against 41), and later rows, which
-  // see more, before earlier ones.
+  // A tile's later runs first: most of their workgroups only leave, and a pass over a context of
+  // its own begins late otherwise (6 prompts of 300 rows at 400 to 4000 positions, head_dim 64 /
+  // 128: 95 / 164 us, 99 / 197 the other way; 3 of 333 rows at 3001, 2000, 1000 80 / 120 and 65 /
+  // 98, at 1000, 2000, 3001 65 / 98 and 73 / 111). All of them, not in turn with the others, which
+  // left whole CUs idle. Then later rows, which see more, before earlier ones.
   const int tiles = gridDim.x / p.n_kv / parts, unit = blockIdx.x / p.n_kv;
-  const int g = blockIdx.x % p.n_kv, part = unit / tiles, tile = tiles - 1 - unit % tiles;
+  const int g = blockIdx.x % p.n_kv, part = SPLIT ? unit / tiles : parts - 1 - unit / tiles, tile = tiles - 1 - unit % tiles;
   const int j0 = tile * tile_rows, nr = min(tile_rows, p.l.rows - j0);
   int32_t* mark = done + (tile * p.n_kv + g) * parts + part;
 
