@@ -166,7 +166,8 @@ __device__ __forceinline__ int record_floats(int n_q, int d) { return (n_q * (d 
 // matrix products. Wave w scores chunk w of a leaf (keys straight from memory: the 16 x 32
 // operand is 16 rows of 64 bytes), the four maxima give every wave the leaf's references,
 // the weights go through LDS, and each wave sums its quarter of the dims over the leaf. The
-// next leaf's loads are in flight meanwhile.
+// next leaf's loads are in flight meanwhile. Memory bounds it: 128 rows of window 1024, 8 groups
+// of 4 heads of 64, 57 us at 4.6 TB/s, whole contexts of 4000 at 6.1 (a 4 GiB copy: 4.8).
 // SPLIT: a leaf, or at head_dim 128 `each` leaves, a workgroup, their records to scratch (few
 // rows, long contexts).
 template <int D, bool SPLIT>
@@ -176,8 +177,8 @@ __device__ __forceinline__ void one_row(const StrideWindowAttentionParams& p, in
   constexpr int kPer = kChunk * kRow / 64;
   constexpr int kOut = (D + 63) / 64;    // 16-dim blocks of a wave
   // At head_dim 128 two leaves' registers would leave one workgroup a CU; two that take turns
-  // loading do better (128 rows of 1024 positions, 8 groups: 187 us with the next leaf's loads
-  // in flight).
+  // loading do better (128 rows of 1024 positions, 8 groups: 82 us, and 187 with the next leaf's
+  // loads in flight).
   constexpr bool kNext = !SPLIT && D < 128;
   __shared__ __align__(16) uint16_t vs[kLeaf * D];
   __shared__ __align__(16) u32x4 weights[kLeaf / 32][64];
@@ -415,8 +416,8 @@ __global__ __launch_bounds__(256, 2) void k_rows(StrideWindowAttentionParams p, 
 // C chunks at a time, a span. With two, a wave has two of each latency's work between two
 // barriers; with one, at head_dim 64, two workgroups fit on a CU (128 registers) and fill each
 // other's waits. So two at head_dim 128, or where there is at most a workgroup a CU (1024 rows
-// of one sequence at 8192, 8 groups, head_dim 64: 153 us against 183; 4096 rows: 440 against
-// 386). Spans are copied memory -> LDS one (C = 2) or two (C = 1) ahead. Key rows have their
+// of one sequence at 8192, 8 groups, head_dim 64: 155 us against 169; 4096 rows: 451 against
+// 335). Spans are copied memory -> LDS one (C = 2) or two (C = 1) ahead. Key rows have their
 // 16-byte pieces permuted by the row and value rows their 32-byte blocks, so that an operand
 // read spreads over the banks; the copy lands in order, so its source is permuted.
 //
@@ -835,8 +836,8 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
 // Joins a split row's records in ascending order. The factors of a head's leaves follow from
 // the references' running maximum, which a wave finds for 64 leaves at once; what is left in
 // order is one product and one FMA a leaf and value, a thread a value, with the values of up to
-// 32 records on their way. (With the factors formed leaf by leaf in every thread, 4 rows of 128
-// leaves at 8 heads of 128 took 17.8 us.)
+// 32 records on their way. (4 rows of 128 leaves at 8 heads of 128: 10.5 us; 17.8 with the
+// factors formed leaf by leaf in every thread.)
 template <int D>
 __global__ __launch_bounds__(256) void k_join(StrideWindowAttentionParams p, int limit, int span, int parts) {
   constexpr int kHeads = 256 / D;  // of a workgroup
@@ -954,11 +955,11 @@ const char* plan_of(const StrideWindowAttentionParams& p, Plan& plan) {
   // has fewer than ten leaves, for the second launch (1, 8, 32, 63 rows, 8 groups, head_dim 64, split
   // and not, of 300 positions 11, 12, 12, 18 and 10, 10, 10, 12 us; of 1000 11, 11, 19, 29 and 15,
   // 15, 19, 24; of 2000 10, 12, 29, 45 and 26, 28, 34, 41); of tiles below 64, a
-  // quarter of the CUs (192 rows of one sequence at 8192, 48 tiles, head_dim 64 / 128: 118 / 168
-  // us against 143 / 226 in whole tiles; 256 rows, 64 tiles: 154 / 223 against 141 / 225), and
+  // quarter of the CUs (192 rows of one sequence at 8192, 48 tiles, head_dim 64 / 128: 120 / 168
+  // us against 148 / 228 in whole tiles; 256 rows, 64 tiles: 157 / 220 against 148 / 227), and
   // with eight leaves or more, for the records and two launches more (64 rows of 2000 positions:
-  // 21 / 31 us against 42 / 64; of 600 positions 18 / 24 against 21 / 29, but 16 rows 15 / 20
-  // against 13 / 16, and 200 rows 24 / 37 against 22 / 32).
+  // 22 / 31 us against 44 / 66; of 600 positions 19 / 25 against 21 / 30, but 16 rows 16 / 19
+  // against 12 / 15, and 200 rows 25 / 36 against 22 / 31).
   const int64_t records = units * span * ((p.n_q * (D + 2) + 3) / 4 * 4);
   const bool may_split = span > 1 && records <= int64_t{1} << 28;  // a GiB
   bool tiles = (p.runs == 0 || p.runs >= kRunRows) && p.l.rows >= kRunRows && tokens >= 512 / D;

@@ -156,8 +156,8 @@ struct Few {
 // own one: item threadIdx.x, and `range` for any): an entry wants a page where `wants(entry)`,
 // and `give(i, slot, b, page)` takes it (page < 0: the entry stays). Two ways to the same outcome.
 // Few items and entries: the entries of all items in a row over the threads, each read once and
-// kept (64 items of one entry: 13.7 us the other way, which reads them twice and waits for one
-// item after the other). Else a wave an item, counts first.
+// kept (64 items of one entry: a reserve takes 5 us so, 13 the other way, which reads them twice
+// and waits for one item after the other). Else a wave an item, counts first.
 template <class Range, class Wants, class Give>
 __device__ __forceinline__ void share_out(const StrideKvPool& p, int n, uint32_t head, int* lds, Few& few, int slot0, int lo0, int hi0, Range range,
                                           Wants wants, Give give) {
@@ -363,7 +363,8 @@ __device__ __forceinline__ Runs runs_of(const StrideKvPool& p) {
   return {p.kv.layer_elems * p.elem_bytes, p.kv.which_elems * p.elem_bytes, p.kv.group_elems * p.elem_bytes, p.n_kv, p.layers * 2 * p.n_kv};
 }
 
-// Copies the first `bytes` of every run of a page; a wave takes runs r0, r0 + step, ..
+// Copies the first `bytes` of every run of a page; a wave takes runs r0, r0 + step, .. (64
+// branches, part pages of 12 tokens, 16 layers of 8 groups of 64: 7.5 us with the table, 4.5 TB/s.)
 __device__ __forceinline__ void copy_page(const StrideKvPool& p, const char* from, char* to, int bytes, int r0, int step, int lane) {
   const Runs runs = runs_of(p);
   for (int r = r0; r < runs.count; r += step) {
@@ -447,7 +448,9 @@ __global__ __launch_bounds__(kPlan) void k_compact_plan(StrideKvPool p, const in
 // what is still to be read: positions ascend and each comes from its own place or a later one,
 // so a workgroup that takes them in ascending steps, loads a step whole before it writes it,
 // overwrites only what it has read. While a step's pieces are on their way the next one's pages
-// are looked up, one position a thread, and left in LDS for the threads that share it.
+// are looked up, one position a thread, and left in LDS for the threads that share it. (8
+// sequences, 2048 of 4096 positions, 16 layers of 8 groups of 64: 212 us, 4.4 TB/s; a 4 GiB
+// copy: 4.8. 64 sequences, 4 of 16 positions: 7 us.)
 constexpr int kHold = 8;
 constexpr int kStepMax = 256;
 
