@@ -364,7 +364,7 @@ __device__ __forceinline__ Runs runs_of(const StrideKvPool& p) {
 }
 
 // Copies the first `bytes` of every run of a page; a wave takes runs r0, r0 + step, .. (64
-// branches, part pages of 12 tokens, 16 layers of 8 groups of 64: 7.5 us with the table, 4.5 TB/s.)
+// branches, part pages of 8 tokens on average, 16 layers of 8 groups of 64: 7.5 us with the table, 4.5 TB/s.)
 __device__ __forceinline__ void copy_page(const StrideKvPool& p, const char* from, char* to, int bytes, int r0, int step, int lane) {
   const Runs runs = runs_of(p);
   for (int r = r0; r < runs.count; r += step) {
