@@ -430,8 +430,10 @@ __global__ __launch_bounds__(256, 2) void k_rows(StrideWindowAttentionParams p, 
 // in turn, each column taking part in its own; a wave without a column of the run only helps
 // with the copies (64 prompts of 8 rows at 1024 positions, head_dim 64: 37 us; 62 with two parts
 // always, 74 with such waves in the products too; the rows alone 140). A tile of many short runs
-// is left to k_rows, and so is a part with a value that is not finite among positions that some
-// columns of its run must not see (0 times it is NaN). done[(tile * n_kv + g) * parts + part]:
+// is left to k_rows, and so is a part in which a row's sums are not finite: a column that must
+// not see a value gives it the weight 0, and 0 times an infinity or NaN is NaN. (Looking for such
+// values in every span that not all columns see took a barrier more: 2048 rows of window 448 29.0
+// us against 28.0, head_dim 128 62.9 against 60.3.) done[(tile * n_kv + g) * parts + part]:
 // whether it was done; with SPLIT, part = leaf % parts, otherwise run % parts.
 constexpr int kColumns = 128;
 constexpr int kRunRows = 4;  // rows a run, on average, below which a tile is left to k_rows
@@ -448,15 +450,6 @@ struct Lay {
   __device__ static __forceinline__ int k_from(int row, int at) { return at ^ k_turn(row); }
   __device__ static __forceinline__ int v_from(int row, int at) { return (((at >> 1) ^ v_turn(row)) << 1) + (at & 1); }
 };
-
-__device__ __forceinline__ bool has_nonfinite(u32x4 v) {
-  typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
-  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-  const u16x8 e = __builtin_bit_cast(u16x8, v & u32x4{0x7F807F80u, 0x7F807F80u, 0x7F807F80u, 0x7F807F80u});
-  const u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(u16x2{e[0], e[1]}, u16x2{e[2], e[3]}),
-                                            __builtin_elementwise_max(u16x2{e[4], e[5]}, u16x2{e[6], e[7]}));
-  return m[0] == 0x7F80 || m[1] == 0x7F80;
-}
 
 // The maximum over the four lanes of a column (16 apart): the row swaps leave a lane's own and
 // its partner's value.
@@ -513,7 +506,7 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
   __shared__ __align__(16) uint16_t vs[kBufs][kSpan * D];
   __shared__ int slots[kColumns], poss[kColumns];
   __shared__ uint64_t starts[2];  // bit i: row i begins a run
-  __shared__ int bad[2][kWaves];
+  __shared__ int spoiled;  // some row's sums are not finite
   const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, cl = lane & 15, quarter = lane >> 4;
   // A tile's later runs first: most of their workgroups only leave, and a pass over a context of
   // its own begins late otherwise (6 prompts of 300 rows at 400 to 4000 positions, head_dim 64 /
@@ -525,6 +518,7 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
   const int j0 = tile * tile_rows, nr = min(tile_rows, p.l.rows - j0);
   int32_t* mark = done + (tile * p.n_kv + g) * parts + part;
 
+  if (t == 0) spoiled = 0;
   if (t < kColumns) {
     const int j = j0 + min(t, nr - 1);
     slots[t] = p.row_slot[j];
@@ -574,6 +568,7 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
     v_off[u] = (lane / L::kRow * D + L::v_from(r, slot_in) * 8) * 2;
   }
 
+  bool spoil = false;
   bool taken = false;  // has this lane's column been in a run of this part's?
   int turn = SPLIT ? 0 : part;
   for (int r0 = 0, r1; r0 < nr; r0 = r1) {
@@ -664,32 +659,16 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
         return a + kSpan - 1 <= low && (a >= far.lo || a + kSpan <= near.sink_end);
       };
       // Waits until span i has arrived, and every wave has read the one before, whose buffer is
-      // filled next (the copies of the next may be under way). False: it holds a value that is not
-      // finite, and not all of the run's columns see it; nothing more is to be done here.
-      auto arrived = [&](int i, bool full, int buf) __attribute__((always_inline)) {
+      // filled next (the copies of the next may be under way).
+      auto arrived = [&]() __attribute__((always_inline)) {
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kBufs - 2) * 2 * kPer) : "memory");
         lds_barrier();
-        if (full) return true;
-        bool b = false;
-#pragma unroll
-        for (int u = 0; u < kPer; ++u) b |= has_nonfinite(*reinterpret_cast<const u32x4*>(&vs[buf][((wave * kPer + u) * 64 + lane) * 8]));
-        const bool any = __any(b);
-        if (lane == 0) bad[i & 1][wave] = any;
-        lds_barrier();
-        int sum = 0;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) sum |= bad[i & 1][w];
-        if (!__builtin_amdgcn_readfirstlane(sum)) return true;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (t == 0) *mark = 0;
-        return false;
       };
       int buf = 0, i = 0;
       // a wave without a column of this run only helps with the copies
       if (!__any(mine))
         for (; i < spans; ++i) {
-          const int a = span_at(i) * kSpan;
-          if (!arrived(i, is_full(a), buf)) __builtin_amdgcn_endpgm();
+          arrived();
           copy(i + kBufs - 1, buf == 0 ? kBufs - 1 : buf - 1);
           look(i + kBufs);
           buf = buf == kBufs - 1 ? 0 : buf + 1;
@@ -703,14 +682,7 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
         do {
           const int a = span_at(i) * kSpan;
           const bool full = is_full(a);
-          if (!arrived(i, full, buf)) {
-            // Two ways to leave, for the registers that the compiler gives the loop around them: 2048
-            // rows of window 512 take 31.5 us so and 34.4 with the return (head_dim 64), 1000 rows of
-            // three sequences of 3000 positions 108 and 116 (128); but 256 rows of 8192 positions,
-            // head_dim 64 and C == 2, 152 and 141.
-            if constexpr (D != 64 || C == 1) __builtin_amdgcn_endpgm();
-            return;
-          }
+          arrived();
           copy(i + kBufs - 1, buf == 0 ? kBufs - 1 : buf - 1);
           look(i + kBufs);
           __builtin_amdgcn_s_setprio(1);
@@ -806,6 +778,12 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
         if constexpr (SPLIT) {
           const Leaves sees = leaves_of(sight);
           const int at = leaf < sees.head ? leaf : (leaf >= sees.rest ? sees.head + leaf - sees.rest : sees.count);
+          float check = 0.0f;  // NaN where a sum is not finite
+#pragma unroll
+          for (int d = 0; d < kDims; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) check = __builtin_fmaf(acc[d][e], 0.0f, check);
+          spoil |= mine && !(check == 0.0f);
           if (live && mine && at < sees.count) {
             float* rec = p.scratch + ((static_cast<int64_t>(j0 + row) * p.n_kv + g) * span + at) * record_floats(p.n_q, D);
 #pragma unroll
@@ -825,12 +803,22 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
       lds_barrier();
     }
   }
+  if constexpr (!SPLIT) {  // (what is not finite stays so through the fold)
+    float check = 0.0f;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) check = __builtin_fmaf(total[d][e], 0.0f, check);
+    spoil = taken && !(check == 0.0f);
+  }
   if (!SPLIT && live && taken) {
     const float sum = my_pos < 0 ? 0.0f : fold.sum;
 #pragma unroll
     for (int d = 0; d < kDims; ++d) put_out(p, j0 + row, g, head, 16 * d + 4 * quarter, total[d], sum);
   }
-  if (t == 0) *mark = 1;
+  if (__any(spoil) && lane == 0) spoiled = 1;
+  lds_barrier();
+  if (t == 0) *mark = spoiled ? 0 : 1;
 }
 
 // Joins a split row's records in ascending order. The factors of a head's leaves follow from

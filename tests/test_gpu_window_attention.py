@@ -316,6 +316,23 @@ def test_a_bad_token_on_a_long_cache(D, at, poison):
     assert torch.equal(heads.view(torch.int16).reshape(rows, -1), clean)
 
 
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("rows,ctx,window", [(40, 500, 0), (40, 500, 100), (30, 2900, 0), (300, 900, 77)])
+@pytest.mark.parametrize("poison", [float("nan"), float("inf")])
+def test_a_bad_query_reaches_only_its_head(D, rows, ctx, window, poison):
+    """Tiles in which one head's scores are not finite: it alone is NaN, the others are as they were."""
+    say("query", D, rows, ctx, window, poison)
+    c = Case(D + rows, 1, ctx, 2, 4, D, 16)
+    pos = [ctx - rows + i for i in range(rows)]
+    q = c.queries(rows)
+    clean = layout.untile_lanes(c.run(q, [0] * rows, pos, window, 0, runs=rows), rows).reshape(rows, 8, D)
+    q[rows // 2, 5 * D + 3] = poison
+    got = layout.untile_lanes(c.run(q, [0] * rows, pos, window, 0, runs=rows), rows).reshape(rows, 8, D)
+    assert torch.isnan(got[rows // 2, 5].view(torch.bfloat16)).all()
+    got[rows // 2, 5] = clean[rows // 2, 5]
+    assert torch.equal(got, clean)
+
+
 def test_large_scores():
     """Scores that outrun exp's range, rising and falling along the cache, and weights that
     underflow: the references follow."""
