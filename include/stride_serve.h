@@ -29,10 +29,11 @@ extern "C" {
  * row_slot[j] at row_pos[j] = p sees position t if t <= p and (window <= 0, or p - t <
  * window, or t < sinks): the last `window` positions and the first `sinks` ones.
  *   out[h] = sum_t w_t V[t],  w = softmax over the visible t of scale * (q[h] . K[t])
- * A row that sees nothing (p < 0, as padding rows of a captured batch have it, or row_slot[j]
- * < 0) gets zeros, and so does one whose visible scores are all -inf. What lies in masked
- * places, NaN and infinities among it, has no influence; what is visible acts as in the
- * formula. A query that is not finite makes its head NaN. Pages wholly outside what any row sees are never
+ * A row that sees nothing (p < 0, as padding rows of a captured batch may have it here, or
+ * row_slot[j] < 0) gets zeros, and so does one whose visible scores are all -inf.
+ * (stride_tc_qkv has no such rows: padding needs a slot with a page of its own there.) What
+ * lies in masked places, NaN and infinities among it, has no influence; what is visible acts
+ * as in the formula. A query that is not finite makes its head NaN. Pages wholly outside what any row sees are never
  * read, so their table entries may be anything; a visible position must be held, and one
  * whose entry is negative reads as zeros; slots and entries that are not negative have to be
  * rows of the table and pages of the arena. row_pos is taken as at most max_blocks * page
