@@ -33,11 +33,12 @@ extern "C" {
  * row_slot[j] < 0) gets zeros, and so does one whose visible scores are all -inf.
  * (stride_tc_qkv has no such rows: padding needs a slot with a page of its own there.) What
  * lies in masked places, NaN and infinities among it, has no influence; what is visible acts
- * as in the formula. A query that is not finite makes its head NaN. Pages wholly outside what any row sees are never
- * read, so their table entries may be anything; a visible position must be held, and one
- * whose entry is negative reads as zeros; slots and entries that are not negative have to be
- * rows of the table and pages of the arena. row_pos is taken as at most max_blocks * page
- * tokens - 1, and 64 * max_pages - 1. Lanes of the last tile behind `rows` are left alone.
+ * as in the formula. A query that is not finite makes its head NaN. Pages wholly outside what
+ * any row sees are never read, so their table entries may be anything; a visible position must
+ * be held, and one whose entry is negative reads as zeros; slots and entries that are not
+ * negative have to be rows of the table and pages of the arena. row_pos is taken as at most
+ * max_blocks * page tokens - 1, and 64 * max_pages - 1. Lanes of the last tile behind `rows`
+ * are left alone.
  */
 typedef struct StrideWindowAttentionParams {
   StrideLanes l;
