@@ -401,6 +401,7 @@ __global__ __launch_bounds__(256, 2) void k_rows(StrideWindowAttentionParams p, 
     for (uint64_t todo = left[w]; todo; todo &= todo - 1) {
       const int unit = __builtin_amdgcn_readfirstlane((w * 64 + __builtin_ctzll(todo)) * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x));
       one_row<D, false>(p, page_shift, limit, 0, unit % p.n_kv, unit / p.n_kv, 0, 0);
+      lds_barrier();  // every wave has read the unit's staging and weights: the next unit writes there
     }
 }
 

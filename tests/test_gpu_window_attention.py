@@ -517,3 +517,35 @@ def test_arguments_of_another_device():
     for name, value in host.items():
         with pytest.raises(ValueError, match="device"):
             harness.window_attention(**{**good, name: value})
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("kind", ["pairs", "mixed", "bad value"])
+def test_units_that_share_a_workgroup(D, kind):
+    """More rows that tiles leave than workgroups, so that each does several, of several leaves:
+    hundreds of short runs; a prompt's chunk beside a large decode batch; tiles whose sums are
+    not finite. The bits of the rows form, whose workgroups have one each."""
+    n_kv, window, sinks = 8, 0, 0
+    if kind == "pairs":
+        seqs, each, first = 300, [2] * 300, lambda s: 990 + s % 50
+    elif kind == "mixed":
+        seqs, each, first = 241, [64] + [1] * 240, lambda s: 700 + 3 * (s % 100)
+    else:
+        seqs, each, first, window, sinks = 1, [300], lambda s: 740, 500, 3
+    say("units", D, kind)
+    c = Case(D + seqs, seqs, 1050, n_kv, 4, D, 16, layers=2)
+    slot = [s for s in range(seqs) for _ in range(each[s])]
+    pos = [first(s) + i for s in range(seqs) for i in range(each[s])]
+    rows = len(slot)
+    q = c.queries(rows)
+    if kind == "bad value":  # in every group, seen by the earlier rows only
+        c.arena[int(c.table[0, 300 // 16]), 1, 1, :, 300 % 16, 9] = float("inf")
+    hint = {"pairs": 0, "mixed": 64, "bad value": rows}[kind]
+    plain = c.run(q, slot, pos, window, sinks, runs=1)
+    for _ in range(3):
+        got = c.run(q, slot, pos, window, sinks, runs=hint)
+        assert torch.equal(got, plain)
+    some = list(range(0, rows, 37))
+    if kind != "bad value":
+        want, tol = c.exact(q[some], [slot[j] for j in some], [pos[j] for j in some], window, sinks)
+        assert ((layout.untile_lanes(got, rows)[some].view(torch.bfloat16).double() - want).abs() <= tol).all()

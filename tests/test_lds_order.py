@@ -40,3 +40,17 @@ def test_attention_tile_tail_weights():
     kinds = re.findall(r"(wb\[wave\]\[[^;]*\] = )|(&wb\[wave\])|(wave_phase\(\))", body)
     order = "".join("s" if store else "r" if read else "p" for store, read, _ in kinds)
     assert order == "pspr", order
+
+
+def test_attention_units_of_one_workgroup():
+    """one_row's last leaf ends with reads of all of vs and weights by every wave, and no barrier
+    behind them; it begins with writes to vs and maxima. Where a workgroup calls it in a loop, a
+    workgroup barrier stands between two calls."""
+    text = source("serve_attn.hip")
+    body = text[text.index("void one_row("):text.index("void k_leaves(")]
+    last = body.rindex("lds_barrier()")
+    assert "if (it + 1 < end)" in body[last - 40:last]  # else a call would end behind a barrier
+    loop = text[text.index("for (uint64_t todo = left[w]; todo"):]
+    loop = loop[:loop.index("\n}")]
+    order = "".join("c" if call else "b" for call, _ in re.findall(r"(one_row<)|(lds_barrier\(\))", loop))
+    assert order == "cb", order
