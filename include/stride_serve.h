@@ -66,7 +66,8 @@ typedef struct StrideWindowAttentionParams {
 int stride_serve_window_attention(const StrideWindowAttentionParams* p, void* stream);
 
 /* Floats of scratch that the call wants (0: none), from every field but the pointers;
- * -1 where the call would be refused. Its contents need no preparation. */
+ * -1 where the call would be refused. What it says for runs = 0 serves calls with any hint, for
+ * another hint calls with that hint. Its contents need no preparation. */
 int64_t stride_serve_window_attention_scratch(const StrideWindowAttentionParams* p);
 
 /* A pool of KV pages. table[slot][i] is the page that holds tokens i * page_tokens .. of a

@@ -1031,7 +1031,17 @@ extern "C" {
 int64_t stride_serve_window_attention_scratch(const StrideWindowAttentionParams* p) {
   Plan plan;
   if (!p || plan_of(*p, plan)) return -1;
-  return plan.scratch;
+  int64_t most = plan.scratch;
+  if (p->runs == 0) {
+    // What serves every hint. Hints below kRunRows plan alike, without tiles; from there on the
+    // records do not depend on the hint and a tile's parts do not grow with it.
+    StrideWindowAttentionParams hinted = *p;
+    for (const int runs : {1, kRunRows}) {
+      hinted.runs = runs;
+      if (!plan_of(hinted, plan)) most = std::max(most, plan.scratch);
+    }
+  }
+  return most;
 }
 
 int stride_serve_window_attention(const StrideWindowAttentionParams* p, void* stream) {

@@ -307,7 +307,8 @@ def here(t) -> None:
 def window_attention_scratch(rows: int, n_kv: int, n_q: int, head_dim: int, window: int, sinks: int, max_pages: int,
                              device, runs: int = 0):
     """The scratch that window_attention wants for calls of these sizes (None: none), with a
-    cache of at least 64 * max_pages positions a slot. Its contents need no preparation."""
+    cache of at least 64 * max_pages positions a slot. With runs 0 it serves calls with any
+    hint, else those with this one. Its contents need no preparation."""
     p = _lib.WindowAttentionParams()
     p.l = lanes(rows)
     p.q_stride = p.out_cols = n_kv * n_q * head_dim

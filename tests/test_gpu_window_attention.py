@@ -549,3 +549,16 @@ def test_units_that_share_a_workgroup(D, kind):
     if kind != "bad value":
         want, tol = c.exact(q[some], [slot[j] for j in some], [pos[j] for j in some], window, sinks)
         assert ((layout.untile_lanes(got, rows)[some].view(torch.bfloat16).double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("seqs,each,ctx,n_kv,n_q,D", [(3, 62, 1969, 8, 4, 128), (4, 55, 1953, 8, 1, 32), (1, 64, 2900, 8, 4, 64), (2, 2, 500, 2, 4, 64)])
+def test_a_scratch_sized_without_a_hint(seqs, each, ctx, n_kv, n_q, D):
+    """One scratch of the size for "not known" serves a call with each hint, with the same bits."""
+    c = Case(seqs * each, seqs, ctx, n_kv, n_q, D, 32)
+    slot = [s for s in range(seqs) for _ in range(each)]
+    pos = [ctx - each + i for _ in range(seqs) for i in range(each)]
+    q = c.queries(len(slot))
+    scratch = harness.window_attention_scratch(len(slot), n_kv, n_q, D, 0, 0, -(-ctx // 64), DEV)
+    plain = c.run(q, slot, pos, runs=1)
+    for runs in (0, 1, 2, 4, each, seqs * each, 1000):
+        assert torch.equal(plain, c.run(q, slot, pos, runs=runs, scratch=scratch)), runs

@@ -233,3 +233,26 @@ def test_existing_arena_is_checked():
     for a, t in ((arena[1:], table), (arena.float(), table), (arena, table.long()), (arena, table.t()), (arena, table[0])):
         with pytest.raises(ValueError):
             harness.PagedKv.over(a, t, 2, 32, 1, 16)
+
+
+def test_scratch_without_a_hint_serves_every_hint():
+    """The size for runs = 0 is no smaller than the one for any hint, over every form: short and
+    long contexts, few and many rows, tiles split or whole."""
+    size = _lib.load().stride_serve_window_attention_scratch
+    wider = 0
+    for rows in (1, 3, 4, 5, 16, 62, 100, 186, 220, 333, 1000, 2048):
+        for n_kv, n_q, D in ((8, 4, 64), (8, 4, 128), (8, 1, 32), (2, 16, 64), (1, 7, 128), (16, 2, 32)):
+            for ctx, window, sinks in ((200, 0, 0), (1500, 0, 0), (1969, 0, 0), (8192, 0, 0), (8192, 2100, 300), (40000, 0, 0), (40000, 64, 4)):
+                for page in (8, 16, 64):
+                    p = attention(l__rows=rows, l__lane_groups=(rows + 15) // 16, n_kv=n_kv, n_q=n_q, head_dim=D, kv__head_dim=D,
+                                  kv__group_elems=page * D, kv__max_blocks=-(-ctx // page), max_pages=-(-ctx // 64), window=window,
+                                  sinks=sinks, q_stride=n_kv * n_q * D, out_cols=n_kv * n_q * D)
+                    at = C.byref(p)
+                    most = size(at)
+                    for runs in (1, 2, 3, 4, 5, 7, 8, 16, 31, 55, 62, 64, 200, rows - 1, rows, rows + 1, 2 ** 31 - 1):
+                        if runs < 1:
+                            continue
+                        p.runs = runs
+                        assert size(at) <= most, (rows, n_kv, n_q, D, ctx, window, page, runs)
+                        wider += size(at) < most
+    assert wider  # a hint may want less
