@@ -27,6 +27,7 @@
 #include <type_traits>
 
 #include "../../include/stride_serve.h"
+#include "serve_sight.hpp"
 #include "tc_common.hpp"
 
 namespace stride_tc {
@@ -46,19 +47,10 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ float neg_inf() { return f32_of(0xFF800000u); }
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// What a row sees: [0, sink_end) and [lo, pos].
-struct Sight {
-  int pos, lo, sink_end;
-  __device__ __forceinline__ bool sees(int t) const { return t <= pos && (t >= lo || t < sink_end); }
-};
 // a row of no sequence is one without a position
-__device__ __forceinline__ int pos_of(const StrideWindowAttentionParams& p, int j) { return p.row_slot[j] < 0 ? -1 : p.row_pos[j]; }
+__device__ __forceinline__ int pos_of(const StrideWindowAttentionParams& p, int j) { return p.row_slot[j] < 0 ? -1 : max(p.row_pos[j], -1); }
 __device__ __forceinline__ Sight sight_of(const StrideWindowAttentionParams& p, int pos, int limit) {
-  Sight s;
-  s.pos = min(pos, limit - 1);
-  s.lo = p.window > 0 ? max(0, s.pos - p.window + 1) : 0;
-  s.sink_end = p.window > 0 ? max(0, min(p.sinks, s.pos + 1)) : 0;
-  return s;
+  return sight_at(pos, p.window, p.sinks, limit);
 }
 
 // The leaves that a row sees, ascending: `head` of them from 0, then those from `rest` on.
@@ -373,14 +365,16 @@ __global__ __launch_bounds__(256, 2) void k_leaves(StrideWindowAttentionParams p
 
 // A workgroup a unit (row, group); with tiles that k_tile may have done (done: its marks), a
 // workgroup looks at up to 256 units, spread over the batch, and takes those that are left.
-__device__ __forceinline__ bool unit_done(const StrideWindowAttentionParams& p, int unit, const int32_t* done, int tile_rows, int parts) {
+__device__ __forceinline__ bool unit_done(const StrideWindowAttentionParams& p, int unit, int limit, const int32_t* done, int tile_rows,
+                                          int parts) {
   const int j = unit / p.n_kv, tile = j / tile_rows;
   const int32_t* mark = done + (tile * p.n_kv + unit % p.n_kv) * parts;
   bool same = true;
   for (int i = 1; i < parts; ++i) same &= mark[i] == mark[0];
   if (same) return mark[0];
   int run = 0;  // the row's, in its tile
-  for (int i = tile * tile_rows + 1; i <= j; ++i) run += p.row_slot[i] != p.row_slot[i - 1];
+  for (int i = tile * tile_rows + 1; i <= j; ++i)
+    run += !one_run(p.row_slot[i - 1], min(pos_of(p, i - 1), limit - 1), p.row_slot[i], min(pos_of(p, i), limit - 1), p.window);
   return mark[run % parts];
 }
 template <int D>
@@ -392,7 +386,7 @@ __global__ __launch_bounds__(256, 2) void k_rows(StrideWindowAttentionParams p, 
   }
   __shared__ uint64_t left[4];
   const int units = p.l.rows * p.n_kv, mine = threadIdx.x * gridDim.x + blockIdx.x;
-  const uint64_t b = __ballot(mine < units && !unit_done(p, mine, done, tile_rows, parts));
+  const uint64_t b = __ballot(mine < units && !unit_done(p, mine, limit, done, tile_rows, parts));
   if ((threadIdx.x & 63) == 0) left[threadIdx.x >> 6] = b;
   __syncthreads();
 #pragma unroll 1
@@ -427,8 +421,8 @@ __global__ __launch_bounds__(256, 2) void k_rows(StrideWindowAttentionParams p, 
 // them (64 rows at 8192 positions, 8 groups, head_dim 64: 139 us otherwise, 45 so). There a
 // workgroup takes part in all of its tile's runs, one after the other.
 //
-// Rows of several sequences meet in a tile where prompts end. `parts` workgroups take its runs
-// in turn, each column taking part in its own; a wave without a column of the run only helps
+// Rows of several sequences meet in a tile where prompts end, or rows of one whose windows do
+// not touch (one_run). `parts` workgroups take its runs in turn, each column taking part in its own; a wave without a column of the run only helps
 // with the copies (64 prompts of 8 rows at 1024 positions, head_dim 64: 37 us; 62 with two parts
 // always, 74 with such waves in the products too; the rows alone 140). A tile of many short runs
 // is left to k_rows, and so is a part in which a row's sums are not finite: a column that must
@@ -527,7 +521,7 @@ __global__ __launch_bounds__(512, C == 2 ? 2 : 4) void k_tile(StrideWindowAttent
   }
   __syncthreads();
   if (t < kColumns) {
-    const uint64_t b = __ballot(t < nr && (t == 0 || slots[t] != slots[t - 1]));
+    const uint64_t b = __ballot(t < nr && (t == 0 || !one_run(slots[t - 1], poss[t - 1], slots[t], poss[t], p.window)));
     if (lane == 0) starts[wave] = b;
   }
   __syncthreads();

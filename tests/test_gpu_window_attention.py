@@ -562,3 +562,44 @@ def test_a_scratch_sized_without_a_hint(seqs, each, ctx, n_kv, n_q, D):
     plain = c.run(q, slot, pos, runs=1)
     for runs in (0, 1, 2, 4, each, seqs * each, 1000):
         assert torch.equal(plain, c.run(q, slot, pos, runs=runs, scratch=scratch)), runs
+
+
+@pytest.mark.parametrize("D,n_q", [(32, 2), (64, 4), (128, 7)])
+@pytest.mark.parametrize("window,sinks,runs", [(64, 0, 40), (64, 20, 0), (600, 3, 80), (2100, 4, 80), (2060, 0, 120)])
+def test_rows_of_one_sequence_far_apart(D, n_q, window, sinks, runs):
+    """Two pieces of one sequence's rows in one tile, and pages between their windows that are
+    gone or belong to others: no row sees them, and nothing changes."""
+    say("far apart", D, n_q, window, sinks, runs)
+    c = Case(D + window, 1, 5100, 2, n_q, D, 16)
+    pos = list(range(10, 50)) + list(range(5040, 5080))
+    slot, q = [0] * 80, c.queries(80)
+    clean = c.check(q, slot, pos, window, sinks, runs=runs)
+    assert torch.equal(clean, c.run(q, slot, pos, window, sinks, runs=1))
+    see = torch.zeros(5104, dtype=torch.bool)
+    for p in pos:
+        see[max(0, p - window + 1):p + 1] = True
+        see[:min(sinks, p + 1)] = True
+    gone = [b for b in range(5100 // 16 + 1) if not see[16 * b:16 * b + 16].any()]
+    assert len(gone) > 100
+    for b in gone:
+        c.arena[int(c.table[0, b])] = float("nan")
+    assert torch.equal(clean, c.run(q, slot, pos, window, sinks, runs=runs))
+    c.table[0, gone[::2]] = -1
+    c.table[0, gone[1::2]] = c.table[0, 0].clone()
+    assert torch.equal(clean, c.run(q, slot, pos, window, sinks, runs=runs))
+    order = [j // 2 + 40 * (j % 2) for j in range(80)]  # and where they take turns
+    got = c.run(q[order].contiguous(), slot, [pos[j] for j in order], window, sinks, runs=runs)
+    assert torch.equal(layout.untile_lanes(got, 80), layout.untile_lanes(clean, 80)[order])
+
+
+@pytest.mark.parametrize("rows,window", [(3, 0), (3, 50), (40, 50), (40, 0)])
+def test_any_negative_position_is_none(rows, window):
+    c = Case(21, 1, 300, 2, 4, 64, 16)
+    q = c.queries(rows)
+    pos = [200 + j for j in range(rows)]
+    clean = layout.untile_lanes(c.run(q, [0] * rows, pos, window, 0), rows)
+    for none in (-1, -2, -2 ** 31):
+        pos[1] = none
+        got = layout.untile_lanes(c.run(q, [0] * rows, pos, window, 0), rows)
+        assert not got[1].any()
+        assert torch.equal(got[[0] + list(range(2, rows))], clean[[0] + list(range(2, rows))])
