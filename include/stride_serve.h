@@ -84,7 +84,7 @@ int64_t stride_serve_window_attention_scratch(const StrideWindowAttentionParams*
 #define STRIDE_KV_TWICE 2        /* a slot or page to be changed came up twice, or is a source too */
 #define STRIDE_KV_NO_PAGES 4     /* fewer pages are free than the call wants */
 #define STRIDE_KV_MISSING 8      /* a position to be moved or copied has no page */
-#define STRIDE_KV_BAD_KEEP 16    /* kept positions not ascending from `first` (seen while moving: see below) */
+#define STRIDE_KV_BAD_KEEP 16    /* kept positions not ascending from `first` (one rule may be seen late: see below) */
 #define STRIDE_KV_BAD_REFS 32    /* a held page's count was not positive: the pool was written from outside */
 
 typedef struct StrideKvPool {
@@ -123,8 +123,11 @@ int stride_kv_fork(const StrideKvPool* p, const int32_t* src, const int32_t* dst
 /* Position first[i] + k of slot[i] becomes what keep[i][k] was, for k < count[i], in every
  * layer, K and V, as stored (keys keep the rotation they have). keep[i] ascends strictly
  * from first[i] or above, and count[i] is at most `width`. Pages behind the last kept position are given up, and a page that
- * others hold too is replaced before it is written. Where a list does not ascend, the moved
- * positions of that slot hold some of the slot's old entries; the other slots are right. */
+ * others hold too is replaced before it is written. With count[i] = 0 nothing is written: the
+ * page that first[i] lies in stays, shared or not. A kept position before first[i] + k or
+ * behind the table is found before anything changes, as one without a page is. Where a list
+ * does not ascend otherwise, which is seen while it is moved, the moved positions of that slot
+ * hold some of the slot's old entries; the other slots are right. */
 int stride_kv_compact(const StrideKvPool* p, const int32_t* slot, const int32_t* first, const int32_t* count,
                       const int32_t* keep, int64_t keep_stride, int32_t width, int32_t n, void* stream);
 

@@ -12,8 +12,8 @@
 ranges and lengths are int32 device tensors, one entry an item, so a call needs nothing from
 the host and can be captured in a HIP graph. Free pages are taken lowest number first, by
 ascending item and table index: the outcome is fixed. A call whose items break a rule, or that
-wants more pages than are free, changes nothing and is reported by check(), which waits for
-the device; a serving loop that counts its pages itself (pages_of) needs it only as a guard.
+wants more pages than are free, changes nothing (but see compact) and is reported by check(), which
+waits for the device; a serving loop that counts its pages itself (pages_of) needs it only as a guard.
 
 Calls on one pool are ordered by the caller (one stream, or events), captured ones among them.
 """
@@ -131,7 +131,9 @@ class KvPool:
     def compact(self, slot, first, count, keep) -> None:
         """Position first[i] + k of slot[i] becomes what position keep[i][k] was, for k <
         count[i]; what lies behind is given up. keep: int32 [n][width], count[i] <= width, each
-        row strictly ascending from first[i] or above."""
+        row strictly ascending from first[i] or above. (With count[i] 0 nothing is written, and
+        the page that first[i] lies in may still be shared.) A row that only does not ascend is
+        seen while its positions move: they then hold some of that slot's old entries."""
         n = self._items(slot, first, count)
         if keep.dtype != torch.int32 or keep.dim() != 2 or keep.shape[0] != n or (keep.shape[1] > 1 and keep.stride(1) != 1):
             raise ValueError("keep must be int32 [n][width], its rows contiguous")

@@ -374,3 +374,41 @@ def test_refusals():
     pool.fork(empty, empty, empty)
     pool.compact(i32([1]), i32([0]), i32([0]), torch.zeros((1, 0), dtype=torch.int32, device=DEV))
     pool.check()
+
+
+@pytest.mark.parametrize("count", [1, 3, 70, 5000])
+def test_a_kept_position_without_a_page_changes_nothing(count):
+    """A position whose page was given up, one before its place, one behind the table, anywhere in
+    a short or long list, the other items' lists being right: table, counts and arena are as
+    they were, though the call wants fresh pages too."""
+    pool, m = make(11, slots=6, max_ctx=6000, pages=900, layers=1, kv_heads=1, pt=16)
+    both(pool, m, "reserve", [0, 1, 3], [0, 0, 0], [375, 375, 20])
+    both(pool, m, "fork", [1], [4], [5984])  # slot 1's pages are shared
+    both(pool, m, "release", [1], [300], [301])
+    rng = np.random.default_rng(count)
+    held = [t for t in range(40, 6000) if t // 16 != 300]
+    good = sorted(rng.choice([t for t in held if t >= 40], count, replace=False).tolist())
+    other = [21, 22, 300]
+    width = max(count, 3)
+    i32row = lambda k: k + [-9] * (width - len(k))
+    for at in sorted({0, count // 2, count - 1}):
+        for bad, bit in ((4800, kv_pool.MISSING), (4815, kv_pool.MISSING), (20 + at - 1, kv_pool.BAD_KEEP), (6000, kv_pool.BAD_KEEP),
+                         (2 ** 31 - 1, kv_pool.BAD_KEEP), (-2 ** 31, kv_pool.BAD_KEEP)):
+            keep = list(good)
+            keep[at] = bad
+            args = i32([0, 1, 3]), i32([20, 20, 20]), i32([3, count, 3]), torch.tensor([i32row(other), i32row(keep), i32row(other)], dtype=torch.int32, device=DEV)
+            early = 0 <= bad < 20 + at  # place 20 + at may take positions from there on only
+            unchanged(pool, m, kv_pool.BAD_KEEP if early else bit, "compact", *args)
+    both(pool, m, "release", [4], [0], [375])  # (fresh pages for 5000 positions would be more than are left)
+    compact(pool, m, [0, 1, 3], [20, 20, 20], [other, good, other])
+
+
+def test_an_empty_list_leaves_a_shared_page():
+    """count 0 cuts a sequence off and writes nothing: the page that it ends in stays shared."""
+    pool, m = make(12)
+    both(pool, m, "reserve", [0], [0], [6])
+    both(pool, m, "fork", [0], [1], [96])
+    compact(pool, m, [1], [40], [[]])
+    assert int(pool.table[1, 2]) == int(pool.table[0, 2]) and pool.table[1, 3:].max() < 0
+    compact(pool, m, [1], [40], [[40]])  # a kept position makes it the sequence's own
+    assert int(pool.table[1, 2]) != int(pool.table[0, 2])
