@@ -8,7 +8,8 @@
     pool.copy(src, dst, tokens, into)       page contents, within a pool or into another
     pool.check()                            raises what earlier calls reported
 
-``pool.kv`` is the harness.PagedKv that tc_qkv, attention and window_attention take. Slots,
+``pool.kv`` is the harness.PagedKv that tc_qkv, attention and window_attention take (of a bf16
+pool; the exact path takes ``pool.ref``). Slots,
 ranges and lengths are int32 device tensors, one entry an item, so a call needs nothing from
 the host and can be captured in a HIP graph. Free pages are taken lowest number first, by
 ascending item and table index: the outcome is fixed. A call whose items break a rule, or that
@@ -71,8 +72,9 @@ class KvPool:
         self.work = torch.empty(ints, dtype=torch.int32, device=dev)
         group = page_tokens * head_dim
         ref = _lib.KvRef(tc.ptr(arena), tc.ptr(table), block, 2 * kv_heads * group, kv_heads * group, group, max_blocks, head_dim)
-        #: What the attention and QKV runners take.
-        self.kv = PagedKv(arena.reshape(-1), table, ref, page_tokens, max_blocks)
+        #: The cache as the C calls take it.
+        self.ref = ref
+        self._kv = PagedKv(arena.reshape(-1), table, ref, page_tokens, max_blocks) if elem == 2 else None
         self._params = _lib.KvPoolParams(ref, tc.ptr(refs), tc.ptr(self.free_bits), tc.ptr(self.errors), tc.ptr(self.work),
                                          ints, pages, slots, layers, kv_heads, elem)
         self._at = C.addressof(self._params)
@@ -87,6 +89,14 @@ class KvPool:
                             dtype=torch.float32 if fp32 else torch.int16, device=device)
         table = torch.full((slots, max_blocks), -1, dtype=torch.int32, device=device)
         return KvPool(arena, table, torch.zeros(pages, dtype=torch.int32, device=device), kv_heads, head_dim, layers, page_tokens)
+
+    @property
+    def kv(self) -> PagedKv:
+        """What the attention and QKV runners of the tensor-core path take, which read bf16: an
+        fp32 pool has none (`ref` is what the exact path's parameter blocks take)."""
+        if self._kv is None:
+            raise ValueError("the runners that take kv read bf16, and this pool holds fp32")
+        return self._kv
 
     @property
     def pages(self) -> int:
