@@ -45,7 +45,7 @@ typedef struct StrideWindowAttentionParams {
   const float* q;   /* [row][n_kv * n_q][head_dim] fp32 */
   int64_t q_stride; /* floats from one row to the next, a multiple of 4 */
   uint16_t* out;    /* bf16 x tiles [lt][ct][16][16], out_cols columns */
-  StrideKvRef kv;   /* any power-of-two page of 8 tokens or more */
+  StrideKvRef kv;   /* any power-of-two page of 8 tokens or more, a head's part of it up to 2^31 elements */
   const int32_t* row_slot;
   const int32_t* row_pos;
   float* scratch;         /* stride_serve_window_attention_scratch() floats, 16-byte aligned */
@@ -75,7 +75,8 @@ int64_t stride_serve_window_attention_scratch(const StrideWindowAttentionParams*
  * free_bits[page / 32] is set where refs is 0. Pages are taken lowest number first, by
  * ascending (item, table index), so that a call's outcome is fixed. Items are device
  * arrays of `n` int32; a slot may come up once in a call as the one to be changed. `kv`
- * carries the table, which these calls write.
+ * carries the table, which these calls write. A page has a power of two of tokens, a head's
+ * part of it at most 2^30 bytes.
  *
  * A call whose items break a rule, or that wants more pages than are free, changes nothing
  * and sets a bit of errors[0], which stays set until the caller clears it:

@@ -916,6 +916,7 @@ const char* plan_of(const StrideWindowAttentionParams& p, Plan& plan) {
     return "bad n_kv, layer, max_pages, sinks, runs or max_blocks";
   const int64_t tokens = p.kv.group_elems > 0 && p.kv.group_elems % D == 0 ? p.kv.group_elems / D : 0;
   if (tokens < 8 || (tokens & (tokens - 1)) || tokens > (int64_t{1} << 30)) return "the KV page (group_elems / head_dim) must be a power of two from 8 up";
+  if (p.kv.group_elems > int64_t{1} << 31) return "a head's part of a page must not pass 2^31 elements";  // a row's place in it has 32 bits
   if (p.kv.block_elems % 8 || p.kv.layer_elems % 8 || p.kv.which_elems % 8) return "KV strides must be multiples of 8 elements";
   const int64_t heads = static_cast<int64_t>(p.n_kv) * p.n_q * D;
   if (heads > INT_MAX || p.out_cols % 16 || p.out_cols < heads) return "out_cols must be a multiple of 16 covering every head";

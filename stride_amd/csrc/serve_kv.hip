@@ -654,6 +654,7 @@ const char* why_not(const StrideKvPool* p, int n, int& page_shift) {
   if (tokens < 1 || tokens * p->kv.head_dim != p->kv.group_elems || (tokens & (tokens - 1)) || tokens > (1 << 24))
     return "the KV page (group_elems / head_dim) must be a power of two";
   if (p->kv.head_dim * p->elem_bytes % 16 || p->kv.head_dim * p->elem_bytes > 4096) return "a head must be a multiple of 16 bytes, at most 4096";
+  if (p->kv.group_elems * p->elem_bytes > int64_t{1} << 30) return "a head's part of a page must not pass 2^30 bytes";  // counted in 32 bits
   if (p->kv.block_elems * p->elem_bytes % 16 || p->kv.layer_elems * p->elem_bytes % 16 || p->kv.which_elems * p->elem_bytes % 16)
     return "KV strides must be multiples of 16 bytes";
   page_shift = 0;

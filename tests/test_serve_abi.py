@@ -256,3 +256,26 @@ def test_scratch_without_a_hint_serves_every_hint():
                         assert size(at) <= most, (rows, n_kv, n_q, D, ctx, window, page, runs)
                         wider += size(at) < most
     assert wider  # a hint may want less
+
+
+@pytest.mark.parametrize("D,tokens,ok", [(128, 1 << 24, True), (128, 1 << 25, False), (32, 1 << 26, True), (32, 1 << 27, False), (64, 1 << 30, False)])
+def test_attention_pages_whose_offsets_pass_32_bits(D, tokens, ok):
+    """A row's offset in a head's part of a page is an int."""
+    p = attention(head_dim=D, kv__head_dim=D, kv__group_elems=tokens * D, kv__which_elems=8 * tokens * D, kv__layer_elems=16 * tokens * D,
+                  kv__block_elems=16 * tokens * D, kv__max_blocks=1, q_stride=32 * D, out_cols=32 * D)
+    want = _lib.load().stride_serve_window_attention_scratch(C.byref(p))
+    assert (want >= 0) == ok
+    if not ok:
+        assert _lib.load().stride_serve_window_attention(C.byref(p), None) == _lib.EINVAL and "2^31" in err()
+
+
+@pytest.mark.parametrize("call", POOL_CALLS)
+@pytest.mark.parametrize("D,elem,tokens,ok", [(64, 2, 1 << 23, True), (64, 2, 1 << 24, False), (64, 4, 1 << 22, True), (64, 4, 1 << 23, False)])
+def test_pool_pages_whose_bytes_pass_32_bits(call, D, elem, tokens, ok):
+    """Bytes of a head's part of a page are an int, and a copy's loop runs up to 1 KiB past them."""
+    group = tokens * D
+    p = pool(kv__head_dim=D, kv__group_elems=group, kv__which_elems=8 * group, kv__layer_elems=16 * group, kv__block_elems=32 * group,
+             elem_bytes=elem, kv__max_blocks=8)
+    assert POOL_CALLS[call](_lib.load(), C.byref(p), n=0) == (0 if ok else _lib.EINVAL)
+    if not ok:
+        assert "2^30" in err()
