@@ -129,13 +129,15 @@ class Pages:
         return released, reserved
 
     def shareable(self, src: int, length: int) -> int:
-        """`length`, or 0 where a row at `length` would see what src has given up."""
+        """`length`, or 0 where a row at `length` would see what src has given up, or src is no slot."""
+        if not 0 <= src < len(self.held):
+            return 0
         return length if 0 < self.of(length) <= self.end[src] and self.seen_from(length) >= self.gone[src] else 0
 
     def fork(self, src: int, dst: int, length: int) -> None:
         whole = length // self.page
-        if self.held[dst]:
-            raise ValueError(f"slot {dst} is in use")
+        if not 0 <= dst < len(self.held) or self.held[dst]:
+            raise ValueError(f"slot {dst} is in use, or none")
         if src == dst or self.shareable(src, length) != length:
             raise ValueError(f"slot {src} does not hold what a branch at {length} sees")
         part = length % self.page > 0 and whole in self.held[src]
@@ -152,6 +154,8 @@ class Pages:
 
     def finish(self, slot: int) -> int:
         """Gives a slot up; its entries end here."""
+        if not 0 <= slot < len(self.held):
+            raise ValueError(f"there is no slot {slot}")
         end = self.end[slot]
         self.drop(slot, list(self.held[slot]))
         self.gone[slot], self.end[slot] = self.first, 0
@@ -216,6 +220,8 @@ class ServingEngine(engine.Engine):
         named = [] if rules is None else [*(rules.bias or ()), *(rules.allowed or ())]
         if not all(0 <= t < self.cfg.vocab for t in named):
             raise ValueError("the rules name a token outside the vocabulary")
+        if shared and not 0 < shared <= len(prompt):
+            raise ValueError(f"{shared} shared tokens of a prompt of {len(prompt)}")
         if shared:
             self.book.fork(source, slot, shared)
             self.pool.fork(*self._ints([[source], [slot], [shared]]))

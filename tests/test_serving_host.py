@@ -181,3 +181,29 @@ def test_rules_and_scheduler_refusals():
 def test_longest_run():
     assert serving.longest_run([]) == 0
     assert serving.longest_run([(s, 0, 0) for s in (1, 1, 2, 2, 2, 1)]) == 3
+
+
+def test_slots_that_are_none():
+    """Python's negative indices name the last slots: a branch of slot -1 was one of the last
+    slot in the book and none on the device, whose pages the branch then lacked."""
+    eng = Model(3, 64, 40, 16, 0)
+    eng.begin(2, list(range(40)))
+    eng.step([(2, p, p) for p in range(40)], [])
+    before = eng.book.used, [dict(h) for h in eng.book.held]
+    for source in (-1, -3, 3, 100):
+        assert eng.shareable(source, 20) == 0
+        with pytest.raises(ValueError):
+            eng.begin(0, list(range(30)), None, source, 20)
+    for shared in (-5, 31):
+        with pytest.raises(ValueError):
+            eng.begin(0, list(range(30)), None, 2, shared)
+    with pytest.raises(ValueError):
+        eng.book.fork(2, -2, 20)
+    for slot in (-1, 3):
+        with pytest.raises(ValueError):
+            eng.finish(slot)
+        with pytest.raises(ValueError):
+            eng.begin(slot, [1])
+    assert before == (eng.book.used, [dict(h) for h in eng.book.held])
+    eng.begin(0, list(range(30)), None, 2, 20)
+    assert eng.pool.table[0][:1] == eng.pool.table[2][:1]
