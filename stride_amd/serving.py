@@ -74,6 +74,7 @@ class Pages:
         self.held = [{} for _ in range(slots)]  # entry -> [its holders' number], one list a page
         self.gone = [self.first] * slots        # entries [first, gone) were given up
         self.end = [0] * slots                  # entries from here on were never held
+        self.done = [0] * slots                 # tokens that steps have processed, or a branch began with
 
     def of(self, tokens: int) -> int:
         return (tokens + self.page - 1) // self.page
@@ -125,14 +126,17 @@ class Pages:
             for b in range(first, end):
                 self.held[s][b] = [1]
             self.end[s] = end
+        for s, (lo, hi) in spans.items():
+            self.done[s] = max(self.done[s], hi + 1)
         self.used += wanted
         return released, reserved
 
     def shareable(self, src: int, length: int) -> int:
-        """`length`, or 0 where a row at `length` would see what src has given up, or src is no slot."""
+        """`length`, or 0 where src has not processed as much, a row at `length` would see what it
+        has given up, or it is no slot."""
         if not 0 <= src < len(self.held):
             return 0
-        return length if 0 < self.of(length) <= self.end[src] and self.seen_from(length) >= self.gone[src] else 0
+        return length if 0 < length <= self.done[src] and self.seen_from(length) >= self.gone[src] else 0
 
     def fork(self, src: int, dst: int, length: int) -> None:
         whole = length // self.page
@@ -150,7 +154,7 @@ class Pages:
         if part:
             self.held[dst][whole] = [1]
             self.used += 1
-        self.gone[dst], self.end[dst] = self.gone[src], self.of(length)
+        self.gone[dst], self.end[dst], self.done[dst] = self.gone[src], self.of(length), length
 
     def finish(self, slot: int) -> int:
         """Gives a slot up; its entries end here."""
@@ -158,7 +162,7 @@ class Pages:
             raise ValueError(f"there is no slot {slot}")
         end = self.end[slot]
         self.drop(slot, list(self.held[slot]))
-        self.gone[slot], self.end[slot] = self.first, 0
+        self.gone[slot], self.end[slot], self.done[slot] = self.first, 0, 0
         return end
 
 
@@ -248,8 +252,9 @@ class ServingEngine(engine.Engine):
         self.rules[slot] = None
 
     def shareable(self, source: int, length: int) -> int:
-        """How many of the first `length` tokens that `source` has processed another sequence
-        can begin with: all of them, or none where the window has passed what it would see."""
+        """How many of the first `length` tokens of `source` another sequence can begin with: all of
+        them, or none where it has not processed as many, or the window has passed what the
+        other would see."""
         return self.book.shareable(source, length)
 
     def fits(self, tokens: int, others=()) -> bool:

@@ -207,3 +207,25 @@ def test_slots_that_are_none():
     assert before == (eng.book.used, [dict(h) for h in eng.book.held])
     eng.begin(0, list(range(30)), None, 2, 20)
     assert eng.pool.table[0][:1] == eng.pool.table[2][:1]
+
+
+@pytest.mark.parametrize("page", [8, 16])
+def test_what_is_not_processed_is_not_shared(page):
+    """A source that has processed part of a page: a branch at the page's end would share it with
+    places that the source has yet to write."""
+    eng = Model(3, 64, 40, page, 0)
+    eng.begin(0, list(range(40)))
+    eng.step([(0, p, p) for p in range(10)], [])
+    for length in (11, 16, 17, 40):
+        assert eng.shareable(0, length) == 0
+        with pytest.raises(ValueError):
+            eng.begin(1, list(range(40)), None, 0, length)
+    assert [eng.shareable(0, n) for n in (1, 8, 10)] == [1, 8, 10] and eng.shareable(1, 1) == 0
+    eng.begin(1, list(range(40)), None, 0, 10)
+    assert eng.shareable(1, 10) == 10 and eng.shareable(1, 11) == 0  # a branch of a branch
+    eng.step([(0, p, p) for p in range(10, 30)] + [(1, 10, 10)], [])
+    assert eng.shareable(0, 30) == 30 and eng.shareable(0, 31) == 0 and eng.shareable(1, 11) == 11
+    eng.finish(0)
+    assert eng.shareable(0, 1) == 0
+    eng.begin(0, [1, 2])
+    assert eng.shareable(0, 1) == 0
