@@ -96,10 +96,13 @@ class Pages:
                 page[0] -= 1
                 self.used -= page[0] == 0
 
+    def shared(self, slot: int, entry: int) -> bool:
+        return self.held[slot].get(entry, (1,))[0] > 1
+
     def step(self, rows):
         """(released, reserved) lists of (slot, first, end) for a step's rows [(slot, pos,
         token)], the released ones first. Raises, with nothing changed, where a row would see
-        what was given up or the pool is too small."""
+        what was given up or write what another sequence holds too, or the pool is too small."""
         spans = {}
         for s, p, *_ in rows:
             lo, hi = spans.get(s, (p, p))
@@ -109,6 +112,10 @@ class Pages:
             seen, end = self.seen_from(lo), hi // self.page + 1
             if seen < self.gone[s]:
                 raise ValueError(f"slot {s}: position {lo} sees pages that its window has passed")
+            if any(self.shared(s, b) for b in range(lo // self.page, min(end, self.end[s]))):
+                for p in (r[1] for r in rows if r[0] == s):
+                    if self.shared(s, p // self.page):
+                        raise ValueError(f"slot {s}: position {p} is in a page that another sequence holds too")
             if min(seen, self.end[s]) > self.gone[s]:
                 released.append((s, self.gone[s], min(seen, self.end[s])))
                 for b in range(*released[-1][1:]):

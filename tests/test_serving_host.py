@@ -229,3 +229,20 @@ def test_what_is_not_processed_is_not_shared(page):
     assert eng.shareable(0, 1) == 0
     eng.begin(0, [1, 2])
     assert eng.shareable(0, 1) == 0
+
+
+def test_a_shared_page_is_not_written():
+    """A position that was processed before, in a page that a branch holds too, by the source or
+    the branch: its other holder would read the new token. In a page of its own it may come again."""
+    eng = Model(3, 64, 40, 16, 0)
+    eng.begin(0, list(range(40)))
+    eng.step([(0, p, p) for p in range(40)], [])
+    eng.begin(1, list(range(40)), None, 0, 36)
+    before = eng.book.used, [dict(h) for h in eng.book.held], list(eng.book.end), list(eng.book.done)
+    for rows in ([(0, 5, 9)], [(1, 31, 9)], [(0, 40, 1), (0, 16, 9)], [(2, 0, 1), (1, 0, 9), (1, 36, 9)]):
+        with pytest.raises(ValueError, match="another sequence"):
+            eng.step(rows, [])
+    assert before == (eng.book.used, [dict(h) for h in eng.book.held], list(eng.book.end), list(eng.book.done))
+    eng.step([(0, 35, 9), (0, 40, 9), (1, 36, 8), (1, 33, 8)], [])  # the part page was copied
+    eng.finish(1)
+    eng.step([(0, 5, 5)], [])
