@@ -203,9 +203,14 @@ class ServingEngine(engine.Engine):
         t = torch.tensor([[r[i] for r in rows] for i in range(3)], dtype=torch.int32, device=self.dev)
         return t[0], t[1], t[2], None
 
-    def _attention(self, n, slot, pos, items, runs):
+    def _ready(self) -> None:
+        """What a call allocates is torch's current stream's, and may go back to it while a launch
+        on another one still reads it."""
         if tc._stream is not None:
             raise ValueError("a ServingEngine allocates for its steps, on torch's current stream: none may be set by set_kernel_stream")
+
+    def _attention(self, n, slot, pos, items, runs):
+        self._ready()
         cfg = self.cfg
         scale = float(math.pow(cfg.head_dim, -0.5))
         scratch = harness.window_attention_scratch(n, cfg.kv_heads, cfg.repeat(), cfg.head_dim, self.window, self.sinks,
@@ -226,6 +231,7 @@ class ServingEngine(engine.Engine):
     def begin(self, slot: int, prompt, rules: Rules | None = None, source: int = -1, shared: int = 0) -> None:
         """A sequence begins in a free slot, from the first `shared` tokens of slot `source`
         (at most what shareable() says), so that its first row is at position `shared`."""
+        self._ready()
         if not 0 <= slot < self.kv.slots or self.book.end[slot]:
             raise ValueError(f"slot {slot} is in use, or none")
         named = [] if rules is None else [*(rules.bias or ()), *(rules.allowed or ())]
@@ -253,6 +259,7 @@ class ServingEngine(engine.Engine):
 
     def finish(self, slot: int) -> None:
         """The slot's pages go back, and it is free."""
+        self._ready()
         end = self.book.finish(slot)
         if end:
             self.pool.release(*self._ints([[slot], [0], [end]]))
@@ -276,6 +283,7 @@ class ServingEngine(engine.Engine):
     def hold(self, rows) -> None:
         """Gives up the pages that the windows of a step's rows [(slot, pos, token)] have passed
         and takes those that the step writes. step() does so itself."""
+        self._ready()
         slots, end = self.kv.slots, self.kv.capacity
         if not all(0 <= r[0] < slots and 0 <= r[1] < end for r in rows):
             raise ValueError("a row's slot or position is outside the cache")
@@ -305,7 +313,13 @@ class ServingEngine(engine.Engine):
         return RowRules(self.counts if counted else None, row_slot, penalties, bias, self.masks if masked else None, mask_row)
 
     def step(self, rows, greedy, **how):
-        """Engine.step, with the pages that it needs and the rules of the rows' slots."""
+        """Engine.step, with the pages that it needs and the rules of the rows' slots. A step that
+        is refused, one that would write a page that another sequence holds too among them,
+        changes nothing."""
+        if not 0 < len(rows) <= self.max_rows:
+            raise ValueError(f"a step has 1 to {self.max_rows} rows, not {len(rows)}")
+        if not all(0 <= i < len(rows) for i in greedy):
+            raise ValueError("greedy names a row that the step does not have")
         self.hold(rows)
         got = super().step(rows, greedy, rules=self.row_rules([rows[i][0] for i in greedy]), runs=longest_run(rows), **how)
         for i, (token, _) in zip(greedy, got):

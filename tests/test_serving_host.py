@@ -246,3 +246,31 @@ def test_a_shared_page_is_not_written():
     eng.step([(0, 35, 9), (0, 40, 9), (1, 36, 8), (1, 33, 8)], [])  # the part page was copied
     eng.finish(1)
     eng.step([(0, 5, 5)], [])
+
+
+def test_a_refused_call_changes_no_book():
+    """Too many rows, none, a greedy row that is none, a stream of set_kernel_stream's: refused
+    before the book or the pool has changed."""
+    from stride_amd import tc
+
+    eng = Model(2, 64, 8, 16, 0)
+    eng.begin(0, [1, 2, 3])
+    eng.step([(0, 0, 1)], [])
+    state = lambda: (eng.book.used, [sorted(h) for h in eng.book.held], list(eng.book.end), list(eng.book.done), [list(t) for t in eng.pool.table])
+    before = state()
+    real = serving.ServingEngine.step
+    for rows, greedy in (([(0, p, 1) for p in range(1, 20)], []), ([], []), ([(0, 20, 1)], [1]), ([(0, 20, 1)], [-1])):
+        with pytest.raises(ValueError):
+            real(eng, rows, greedy)
+        assert state() == before
+    tc.set_kernel_stream(12345)
+    try:
+        for call in (lambda: real(eng, [(0, 20, 1)], [0]), lambda: eng.hold([(0, 20, 1)]), lambda: eng.begin(1, [1, 2], None, 0, 1),
+                     lambda: eng.begin(1, [1, 2]), lambda: eng.finish(0)):
+            with pytest.raises(ValueError, match="current stream"):
+                call()
+            assert state() == before
+    finally:
+        tc.set_kernel_stream(None)
+    eng.hold([(0, 20, 1)])
+    assert state() != before
