@@ -112,7 +112,13 @@ class KvPool:
 
     def free_pages(self) -> int:
         """How many pages are free (waits for the device)."""
+        self._wait()
         return int((self.refs == 0).sum())
+
+    def _wait(self) -> None:
+        """For every stream: the pool's calls may be on another than torch's current one."""
+        if self._device >= 0:
+            torch.cuda.synchronize(self._device)
 
     def _items(self, *items) -> int:
         n, dev = items[0].numel(), self._device
@@ -164,9 +170,11 @@ class KvPool:
     def check(self) -> None:
         """Raises StrideTcError for what calls reported since the last check (waits for the
         device)."""
+        self._wait()
         bits = int(self.errors.item())
         if bits:
             self.errors.zero_()
+            self._wait()
             raise _lib.StrideTcError("kv pool: " + "; ".join(m for b, m in MESSAGES.items() if bits & b))
 
 

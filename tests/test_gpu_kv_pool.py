@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from stride_amd import kv_pool
+from stride_amd import kv_pool, tc
 from stride_amd._lib import StrideTcError
 
 pytestmark = pytest.mark.gpu
@@ -412,3 +412,33 @@ def test_an_empty_list_leaves_a_shared_page():
     assert int(pool.table[1, 2]) == int(pool.table[0, 2]) and pool.table[1, 3:].max() < 0
     compact(pool, m, [1], [40], [[40]])  # a kept position makes it the sequence's own
     assert int(pool.table[1, 2]) != int(pool.table[0, 2])
+
+
+@pytest.mark.parametrize("how", ["current", "set"])
+def test_check_waits_for_the_stream_of_the_calls(how):
+    """Calls on a stream that is busy, which is no longer torch's current one, or never was, when
+    check and free_pages ask."""
+    pool, _ = make(13, slots=4, max_ctx=96, pages=30)
+    slot, lo, hi, bad = i32([1]), i32([0]), i32([6]), i32([9])
+    a = torch.ones((4096, 4096), device=DEV)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for call, refused, want in ((lambda: pool.reserve(slot, lo, hi), False, 24), (lambda: pool.reserve(bad, lo, hi), True, 24),
+                                (lambda: pool.release(slot, lo, hi), False, 30)):
+        with torch.cuda.stream(stream):
+            for _ in range(40):  # some 40 ms of fp32 products
+                b = a @ a
+            if how == "current":
+                call()
+        if how == "set":
+            tc.set_kernel_stream(stream)
+            try:
+                call()
+            finally:
+                tc.set_kernel_stream(None)
+        if refused:
+            with pytest.raises(StrideTcError, match="outside its bounds"):
+                pool.check()
+        assert pool.free_pages() == want
+        pool.check()
+    del b
