@@ -67,7 +67,9 @@ typedef struct StrideGemmMat {
 } StrideGemmMat;
 
 /* src/kernels.h:30-39. The page size in tokens is group_elems / head_dim
- * (64 in the reference's KvCache; any power of two here). */
+ * (64 in the reference's KvCache; any power of two here). table[slot][pos / page tokens]
+ * is the position's page in the arena; below 0 there is none: qkv does not keep such a row,
+ * attention reads page 0 for it. */
 typedef struct StrideKvRef {
   void* arena;
   const int32_t* table;

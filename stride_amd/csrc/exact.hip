@@ -210,6 +210,7 @@ struct QkvOp {  // src/kernels.cu:204-284
       const StrideKvRef& kv = p.kv;
       const int64_t tokens = kv.group_elems / kv.head_dim;  // a power of two (checked on the host)
       const int64_t block = kv.table[static_cast<int64_t>(slot) * kv.max_blocks + pos / tokens];
+      if (block < 0) return;  // no page: the row is not kept
       dst = static_cast<float*>(kv.arena) + block * kv.block_elems + p.layer * kv.layer_elems +
             (kind - 1) * kv.which_elems + head * kv.group_elems + (pos % tokens) * kv.head_dim;
     }

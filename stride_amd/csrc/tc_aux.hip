@@ -301,13 +301,14 @@ __device__ __forceinline__ void page_item(const StrideAttentionParams& p, int pa
   // used), so every load is unconditional and stays inside the row's own pages. Lane i
   // reads the KV page number of position p0 + i (src/kernel_common.h:20-25), and the
   // lanes that fetch its V row get it from there, so that two waits come before all of
-  // the page's loads. (With a table read per piece of V the compiler, short of registers
+  // the page's loads. An entry without a page, below 0, is read as page 0: a result of no
+  // meaning, but nothing outside the arena. (With a table read per piece of V the compiler, short of registers
   // at head_dim 128 in fp32, waited for every V load before the next table read: 64 rows
   // of 2900 positions, 8 groups, 619 us with the combine against 315.)
   const int last = visible - 1;
   const KvT* base = static_cast<const KvT*>(p.kv.arena) + p.layer * p.kv.layer_elems + g * p.kv.group_elems;
   const int at = min(p0 + lane, last), in_page = (1 << page_shift) - 1;
-  const int block = p.kv.table[static_cast<int64_t>(slot) * p.kv.max_blocks + (at >> page_shift)];
+  const int block = max(p.kv.table[static_cast<int64_t>(slot) * p.kv.max_blocks + (at >> page_shift)], 0);
   int vblock[kPer];
 #pragma unroll
   for (int k = 0; k < kPer; ++k) vblock[k] = __shfl(block, (k * 64 + lane) / (D / kEl));
@@ -529,7 +530,7 @@ __global__ __launch_bounds__(256, D == 64 && sizeof(KvT) == 2 ? 3 : 2) void k_at
 #pragma unroll
       for (int k = 0; k < kPer; ++k) {
         const int at = at0 + k * (256 / kRow);
-        const int64_t block = kOwn ? blk[kOwn ? k : 0] : __shfl(lane_blk, at);
+        const int64_t block = max(kOwn ? blk[kOwn ? k : 0] : __shfl(lane_blk, at), 0);
         const KvT* src = base + block * p.kv.block_elems + (pos_of(page, at) & ((1 << page_shift) - 1)) * D;
         kr[k] = load16(src);
         vr[k] = load16(src + p.kv.which_elems);
@@ -860,7 +861,7 @@ __global__ __launch_bounds__(64 * NWV) void k_attn_fused(StrideAttentionParams p
   // from LDS, so a page's loads never wait on a dependent page-table load.
   int32_t* btab = reinterpret_cast<int32_t*>(recs + p.max_pages * (RF + kHeadsPerGroup));
   const int nblk = min((last >> page_shift) + 1, (p.max_pages * kAttnPage + (1 << page_shift) - 1) >> page_shift);
-  for (int i = t; i < nblk; i += 64 * NWV) btab[i] = p.kv.table[static_cast<int64_t>(slot) * p.kv.max_blocks + i];
+  for (int i = t; i < nblk; i += 64 * NWV) btab[i] = max(p.kv.table[static_cast<int64_t>(slot) * p.kv.max_blocks + i], 0);
   const KvT* kv_base = static_cast<const KvT*>(p.kv.arena) + p.layer * p.kv.layer_elems + g * p.kv.group_elems;
   auto kv_at = [&](int which, int pos) {
     return kv_base + btab[pos >> page_shift] * p.kv.block_elems + which * p.kv.which_elems +

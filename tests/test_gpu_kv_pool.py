@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from stride_amd import kv_pool, tc
+from stride_amd import harness, kv_pool, layout, tc
 from stride_amd._lib import StrideTcError
 
 pytestmark = pytest.mark.gpu
@@ -442,3 +442,42 @@ def test_check_waits_for_the_stream_of_the_calls(how):
         assert pool.free_pages() == want
         pool.check()
     del b
+
+
+@pytest.mark.parametrize("page,D", [(16, 64), (64, 128), (8, 32)])
+def test_a_step_after_a_pool_had_no_page(page, D):
+    """reserve finds too few pages on the device, when the step's other launches are on their way:
+    qkv keeps the rows that have a page and writes nowhere else, and window_attention reads
+    zeros for the others; check() says so afterwards."""
+    n_kv, n_q, layers, H = 2, 4, 2, 256
+    pool, m = make(14, slots=3, max_ctx=64 * 4, pages=64 // page + 2, kv_heads=n_kv, D=D, layers=layers, pt=page)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    pool.reserve(i32([0]), i32([0]), i32([64 // page]))
+    pool.check()
+    m.reserve([0], [0], [64 // page])
+    w = lambda n: (torch.randn((n // 16, H // 16, 16, 16), generator=g, device=DEV) * 0.05).to(torch.bfloat16).view(torch.int16)
+    x = (torch.randn((2, H // 16, 16, 16), generator=g, device=DEV)).to(torch.bfloat16).view(torch.int16)
+    rope = torch.randn((256, D // 2, 2), generator=g, device=DEV)
+    wq, wk, wv = w(n_kv * n_q * D), w(n_kv * D), w(n_kv * D)
+    slot = i32([0] * 10 + [1] * 10)
+    pos = i32(list(range(10)) + list(range(10)))
+    pool.reserve(i32([1, 2]), i32([0, 0]), i32([2, 200 // page]))  # too many: nobody gets one
+    q = harness.qkv(wq, wk, wv, x, 20, D, rope, slot, pos, pool.kv, layer=1)
+    out = harness.window_attention(q, pool.kv, slot, pos, n_kv, n_q, D, D ** -0.5, layer=1)
+    with pytest.raises(StrideTcError, match="fewer pages"):
+        pool.check()
+    torch.cuda.synchronize()
+    got = pool.arena.cpu().numpy().reshape(m.arena.shape)
+    kept = np.zeros(m.arena.shape[:-1], dtype=bool)
+    for t in range(10):
+        kept[m.table[0, t // page], 1, :, :, t % page] = True
+    assert np.array_equal(got[~kept], m.arena[~kept]) and not np.array_equal(got[kept], m.arena[kept])
+    rows = layout.untile_lanes(out, 20)
+    assert rows[:10].any(1).all() and not rows[10:].any()
+    full = kv_pool.KvPool.create(3, 256, 100, n_kv, D, layers, page, DEV)  # the same with pages for all
+    full.reserve(i32([0, 1]), i32([0, 0]), i32([64 // page, 2]))
+    q2 = harness.qkv(wq, wk, wv, x, 20, D, rope, slot, pos, full.kv, layer=1)
+    a = harness.window_attention(q2, full.kv, slot, pos, n_kv, n_q, D, D ** -0.5, layer=1)
+    assert torch.equal(q, q2) and torch.equal(layout.untile_lanes(a, 20)[:10], rows[:10])
+    old = harness.attention(q[:10], pool.kv, slot[:10], pos[:10], n_kv, D, D ** -0.5, layer=1, max_pages=4)
+    assert torch.isfinite(layout.untile_lanes(old, 10).view(torch.bfloat16)).all()
