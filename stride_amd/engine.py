@@ -81,8 +81,7 @@ class Engine:
         self.w = weights
         cfg = self.cfg = weights.cfg
         dev = self.dev = weights.embed.device
-        if cfg.head_dim not in (32, 64, 128) or cfg.repeat() != 4:
-            raise ValueError("the tensor-core attention serves head_dim 32/64/128 with four query heads per KV head")
+        self._check_heads(cfg)
         rope_positions = int(weights.rope.shape[0])
         if max_ctx > rope_positions:
             raise ValueError(f"max_ctx {max_ctx} exceeds the RoPE table's {rope_positions} positions "
@@ -106,6 +105,10 @@ class Engine:
         self.lm_x = torch.zeros((lt, H // 16, 16, 16), dtype=torch.int16, device=dev)
         self.q = torch.zeros((max_rows, cfg.heads * D), dtype=torch.float32, device=dev)
         self.scratch = self._attention_scratch()
+
+    def _check_heads(self, cfg) -> None:
+        if cfg.head_dim not in (32, 64, 128) or cfg.repeat() != 4:
+            raise ValueError("the tensor-core attention serves head_dim 32/64/128 with four query heads per KV head")
 
     def _cache(self, slots, max_ctx, page_tokens, shuffle_seed) -> harness.PagedKv:
         cfg = self.cfg

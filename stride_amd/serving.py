@@ -189,6 +189,10 @@ class ServingEngine(engine.Engine):
         self.counts = self.masks = None
         self.lm_work = logits.scratch(max_rows, self.dev)
 
+    def _check_heads(self, cfg) -> None:
+        if cfg.head_dim not in (32, 64, 128) or cfg.heads % cfg.kv_heads or not 1 <= cfg.repeat() <= 16:
+            raise ValueError("window_attention serves head_dim 32/64/128 with 1 to 16 query heads per KV head")
+
     def _cache(self, slots, max_ctx, page_tokens, shuffle_seed):
         cfg = self.cfg
         pages = self._pages if self._pages is not None else slots * ((max_ctx + page_tokens - 1) // page_tokens)

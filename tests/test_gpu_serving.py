@@ -97,6 +97,44 @@ def test_attention_of_the_engine(model, monkeypatch, window, sinks):
     assert len(done) == 3 and len(worst) > 20
 
 
+@pytest.mark.parametrize("heads,kv_heads,D", [(2, 2, 32), (6, 2, 64), (8, 1, 64), (16, 1, 32), (4, 2, 128)])
+def test_head_layouts_of_the_engine(monkeypatch, heads, kv_heads, D):
+    """Models of 1 to 16 query heads a group: each layer's attention against the formula in 64 bits
+    (the tolerance of test_attention_of_the_engine), and the same ledger alone and together."""
+    cfg = weights.ModelConfig(hidden=256, mlp=512, layers=2, heads=heads, kv_heads=kv_heads, head_dim=D, vocab=1000)
+    w = weights.Weights.random(cfg, DEV, seed=heads, max_positions=256)
+    n_q, real, worst = heads // kv_heads, harness.window_attention, []
+
+    def checked(q, kv, slot, pos, n_kv, nq, head_dim, scale, win, snk, layer, pages, **kw):
+        tiles = real(q, kv, slot, pos, n_kv, nq, head_dim, scale, win, snk, layer, pages, **kw)
+        assert (n_kv, nq, head_dim) == (kv_heads, n_q, D)
+        got = layout.untile_lanes(tiles, q.shape[0]).view(torch.bfloat16).double()
+        for j in range(0, q.shape[0], 5):
+            s, p = int(slot[j]), int(pos[j])
+            see = [t for t in range(p + 1) if p - t < win or t < snk]
+            k, v = (kv.gather(layer, which, [s] * len(see), see, n_kv, D).view(torch.bfloat16).double().reshape(-1, n_kv, D)
+                    for which in (0, 1))
+            qj = q[j].double().reshape(n_kv, n_q, D)
+            kt, vt = k.permute(1, 2, 0).contiguous(), v.permute(1, 0, 2).contiguous()
+            weight = torch.softmax(torch.matmul(qj, kt) * scale, -1)
+            o, a = torch.matmul(weight, vt), torch.matmul(weight, vt.abs())
+            e = (2.0 ** -16 + 2.0 ** -22 * (D + 8)) * scale * torch.matmul(qj.abs(), kt.abs()).amax(-1, keepdim=True)
+            err = (2 * e + 2 * 2.0 ** -8 + 2.0 ** -20) * a
+            tol = err + 2.0 ** -8 * (o.abs() + err) + 1e-30
+            worst.append(((got[j] - o.reshape(-1)).abs() / tol.reshape(-1)).max().item())
+            assert worst[-1] <= 1, (layer, s, p, worst[-1])
+        return tiles
+
+    todo = family(heads, 4, 50)
+    monkeypatch.setattr(harness, "window_attention", checked)
+    alone = cli.Scheduler(serving.ServingEngine(w, 1, 64, 64, window=20, sinks=2), 1, 4).run(todo)
+    monkeypatch.undo()
+    assert len(worst) > 20
+    eng = serving.ServingEngine(w, 4, 64, 24, window=20, sinks=2)
+    together = cli.Scheduler(eng, 4, 4, row_shuffle=3, share_prefixes=True).run(todo)
+    assert list(cli.ledger_lines(todo, alone)) == list(cli.ledger_lines(todo, together))
+
+
 def test_rules_that_allow_everything_are_greedy(model):
     w = model[1]
     todo = family(3, 4, 60)

@@ -274,3 +274,19 @@ def test_a_refused_call_changes_no_book():
         tc.set_kernel_stream(None)
     eng.hold([(0, 20, 1)])
     assert state() != before
+
+
+def test_head_layouts():
+    """The serving engine's attention has 1 to 16 query heads a group, the plain engine's four."""
+    from stride_amd.weights import ModelConfig
+
+    serve, plain = (e._check_heads for e in (serving.ServingEngine, engine.Engine))
+    for heads, kv_heads, D, ok, four in ((8, 2, 64, True, True), (2, 2, 32, True, False), (16, 1, 128, True, False), (14, 2, 64, True, False),
+                                         (17, 1, 64, False, False), (8, 2, 80, False, False), (7, 2, 64, False, False)):
+        cfg = ModelConfig(heads=heads, kv_heads=kv_heads, head_dim=D)
+        for check, served in ((serve, ok), (plain, four)):
+            if served:
+                check(None, cfg)
+            else:
+                with pytest.raises(ValueError, match="head_dim"):
+                    check(None, cfg)
