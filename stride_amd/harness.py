@@ -304,6 +304,12 @@ def here(t) -> None:
         raise ValueError(f"tensors are on {t.device}, the current device is {torch._C._cuda_getDevice()}")
 
 
+def other_stream() -> bool:
+    """Do launches go to another stream than torch's current one? What a runner allocates belongs
+    to torch's: it would be filled there, or still be in use there, beside the launch."""
+    return tc._stream is not None and tc.kernel_stream() != torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
 def window_attention_scratch(rows: int, n_kv: int, n_q: int, head_dim: int, window: int, sinks: int, max_pages: int,
                              device, runs: int = 0):
     """The scratch that window_attention wants for calls of these sizes (None: none), with a
@@ -332,7 +338,8 @@ def window_attention(q, kv: PagedKv, row_slot, row_pos, n_kv: int, n_q: int, hea
     zeros. max_pages: no row lies behind position 64 * max_pages - 1 (default: the slots'
     capacity). runs: a hint, how many neighbouring rows are of one sequence at most (1:
     decode; 0: not known). scratch: window_attention_scratch() (default: allocated here, on
-    torch's current stream). Returns bf16 x tiles."""
+    torch's current stream; out_tiles likewise, so that with another stream set by
+    set_kernel_stream both are passed). Returns bf16 x tiles."""
     rows, cols = int(q.shape[0]), n_kv * n_q * head_dim
     here(q)
     if q.dtype != torch.float32 or q.dim() != 2 or q.shape[1] != cols or (cols > 1 and q.stride(1) != 1):
@@ -349,6 +356,8 @@ def window_attention(q, kv: PagedKv, row_slot, row_pos, n_kv: int, n_q: int, hea
         raise ValueError("layer or n_kv is not the cache's")
     T = (rows + 15) // 16
     if out_tiles is None:
+        if other_stream():
+            raise ValueError("with another stream set by set_kernel_stream, pass out_tiles and scratch")
         out_tiles = torch.zeros((T, cols // 16, 16, 16), dtype=U16, device=q.device)
     elif (out_tiles.dtype != U16 and out_tiles.dtype != torch.bfloat16) or not out_tiles.is_contiguous() \
             or out_tiles.numel() < T * 16 * cols or (out_tiles.dim() == 4 and out_tiles.shape[1] * 16 != cols):

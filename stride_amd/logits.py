@@ -22,7 +22,7 @@ import numpy as np
 import torch
 
 from . import _lib, tc
-from .harness import here
+from .harness import here, other_stream
 
 _LOGITS = Struct("<4i13Q3i4x").pack
 UNIT = 17 * 32  # scratch of a lane tile, int64
@@ -127,7 +127,8 @@ def process(logits, rows: int, vocab: int, counts: TokenCounts | None = None, ro
     frequency), with counts; bias: (offsets, tokens, values), see bias_lists; mask: bit words
     [masks][words], with mask_row int32 [rows] (below 0: no mask). out: receives the processed
     tiles (may be `logits`). work: scratch(rows) (default: one that `counts` keeps for this
-    stream, or a new one)."""
+    stream, or a new one). With another stream set by set_kernel_stream, best and work are
+    passed."""
     i32, f32 = torch.int32, torch.float32
     here(logits)
     T = (rows + 15) // 16
@@ -141,6 +142,8 @@ def process(logits, rows: int, vocab: int, counts: TokenCounts | None = None, ro
             raise ValueError("out must be tiles like logits")
         o_at = out.data_ptr()
     if best is None:
+        if other_stream():
+            raise ValueError("with another stream set by set_kernel_stream, pass best and work")
         best = torch.empty((rows, 2), dtype=i32, device=logits.device)
     elif best.get_device() != dev or best.dtype != i32 or best.numel() < 2 * rows or not best.is_contiguous():
         raise ValueError("best must be contiguous int32 [rows][2]")

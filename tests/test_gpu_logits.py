@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from stride_amd import harness, layout, logits, synth
+from stride_amd import harness, layout, logits, synth, tc
 from stride_amd._lib import StrideTcError
 
 pytestmark = pytest.mark.gpu
@@ -306,3 +306,23 @@ def test_arguments_of_another_device():
     for name, value in host.items():
         with pytest.raises(ValueError):
             logits.process(**{**good, name: value})
+
+
+def test_results_are_not_allocated_on_another_stream():
+    """With a stream of set_kernel_stream's that is not torch's current one, best and work are to be passed."""
+    l = tiles_of(np.random.default_rng(3).normal(size=(5, 100)).astype(np.float32))
+    want = logits.process(l, 5, 100)
+    best, work = torch.zeros_like(want), logits.scratch(5, DEV)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    tc.set_kernel_stream(stream)
+    try:
+        with pytest.raises(ValueError, match="best"):
+            logits.process(l, 5, 100, work=work)
+        logits.process(l, 5, 100, best=best, work=work)
+        torch.cuda.synchronize()
+        assert torch.equal(best, want)
+        tc.set_kernel_stream(torch.cuda.current_stream())
+        assert torch.equal(logits.process(l, 5, 100, work=work), want)
+    finally:
+        tc.set_kernel_stream(None)

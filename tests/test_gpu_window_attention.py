@@ -603,3 +603,27 @@ def test_any_negative_position_is_none(rows, window):
         got = layout.untile_lanes(c.run(q, [0] * rows, pos, window, 0), rows)
         assert not got[1].any()
         assert torch.equal(got[[0] + list(range(2, rows))], clean[[0] + list(range(2, rows))])
+
+
+def test_results_are_not_allocated_on_another_stream():
+    """With a stream of set_kernel_stream's that is not torch's current one, what a runner would
+    allocate would be filled beside the launch: it is to be passed."""
+    c = Case(22, 2, 300, 2, 4, 64, 16)
+    q, i = c.queries(3), torch.tensor([0, 1, 1], dtype=torch.int32, device=DEV)
+    pos = torch.tensor([250, 3, 299], dtype=torch.int32, device=DEV)
+    call = lambda **kw: harness.window_attention(q, c.kv, i, pos, 2, 4, 64, c.scale, layer=1, **kw)
+    want = call()
+    out, scratch = torch.zeros_like(want), torch.empty(1 << 20, device=DEV)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    tc.set_kernel_stream(stream)
+    try:
+        with pytest.raises(ValueError, match="out_tiles"):
+            call(scratch=scratch)
+        call(out_tiles=out, scratch=scratch)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        tc.set_kernel_stream(torch.cuda.current_stream())
+        assert torch.equal(call(scratch=scratch), want)
+    finally:
+        tc.set_kernel_stream(None)
