@@ -2,8 +2,9 @@
  * (MI355X, gfx950): attention over long or bounded contexts, a pool of KV pages that
  * sequences share, and logit processing. The reference has no counterpart; layouts and
  * conventions are those of stride_tc.h: x tiles, logits tiles, the paged KV arena
- * [page][layer][K|V][group][token][dim], one wave-parallel launch on `stream`, errors as
- * return codes with stride_tc_last_error().
+ * [page][layer][K|V][group][token][dim], launches on `stream` alone (attention one to three of
+ * them, fork and copy two, compact three, the others one), errors as return codes with
+ * stride_tc_last_error().
  *
  * Nothing here allocates, synchronizes or keeps state: workspaces are the caller's, every
  * launch can be captured in a HIP graph, and each takes its arguments from device memory
@@ -29,6 +30,9 @@ extern "C" {
  * row_slot[j] at row_pos[j] = p sees position t if t <= p and (window <= 0, or p - t <
  * window, or t < sinks): the last `window` positions and the first `sinks` ones.
  *   out[h] = sum_t w_t V[t],  w = softmax over the visible t of scale * (q[h] . K[t])
+ * Weights are rounded to bf16 before they meet V (and their sum is that of the rounded ones),
+ * queries to 16 bits, sums are fp32: where stride_tc_attention, which keeps both in fp32, serves
+ * the same rows, the two agree to the weights' rounding, not bit for bit.
  * A row that sees nothing (p < 0, as padding rows of a captured batch may have it here, or
  * row_slot[j] < 0) gets zeros, and so does one whose visible scores are all -inf.
  * (stride_tc_qkv has no such rows: padding needs a slot with a page of its own there.) What
@@ -79,7 +83,8 @@ int64_t stride_serve_window_attention_scratch(const StrideWindowAttentionParams*
  * part of it at most 2^30 bytes.
  *
  * A call whose items break a rule, or that wants more pages than are free, changes nothing
- * and sets a bit of errors[0], which stays set until the caller clears it:
+ * and sets a bit of errors[0], which stays set until the caller clears it. Launches that were
+ * on their way behind it may meet entries below 0: stride_tc_qkv does not keep such rows.
  */
 #define STRIDE_KV_BAD_ITEM 1     /* slot, range, length or page outside its bounds */
 #define STRIDE_KV_TWICE 2        /* a slot or page to be changed came up twice, or is a source too */
@@ -156,7 +161,8 @@ typedef struct StrideLogitsParams {
   const int32_t* counts;   /* [slots][vocab], or NULL: no penalties */
   const uint32_t* seen;    /* [slots][ceil(vocab / 32)]: bit set where counts is not 0 */
   const float* penalties;  /* [rows][3]: repetition (> 0), presence, frequency */
-  const int32_t* bias_offsets; /* [rows + 1], or NULL: row j has entries bias_offsets[j] .. bias_offsets[j + 1] - 1 */
+  const int32_t* bias_offsets; /* [rows + 1], or NULL: row j has entries bias_offsets[j] .. bias_offsets[j + 1] - 1, places
+                                  of the two arrays below, which the kernel takes as they are */
   const int32_t* bias_tokens;  /* ascending in a row; of equal neighbours the last counts; out of range: ignored */
   const float* bias_values;
   const uint32_t* mask;     /* [masks][ceil(vocab / 32)]: bit set where a token is allowed, or NULL */

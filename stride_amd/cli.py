@@ -17,7 +17,8 @@ the last W and the first S positions (0: all), a pool of N KV pages (0: enough
 for C sequences), pages shared between prompts that begin alike, and penalties
 for tokens that a sequence has; an input line may also have "bias": {"5": -1.5}
 and "allowed": [1, 2, 3], the tokens that may be chosen. Its ledger holds the
-processed logits.
+processed logits; its attention rounds the softmax's weights to bf16, which --path tc
+keeps in fp32, so that the two paths' ledgers differ in low bits without options too.
 
 Input lines: {"id": 0, "tokens": [1, 2, 3]}. Output lines (one per prompt, in
 input order): {"id": 0, "tokens": [...], "values": ["3f800000", ...],

@@ -481,3 +481,20 @@ def test_a_step_after_a_pool_had_no_page(page, D):
     assert torch.equal(q, q2) and torch.equal(layout.untile_lanes(a, 20)[:10], rows[:10])
     old = harness.attention(q[:10], pool.kv, slot[:10], pos[:10], n_kv, D, D ** -0.5, layer=1, max_pages=4)
     assert torch.isfinite(layout.untile_lanes(old, 10).view(torch.bfloat16)).all()
+
+
+def test_compaction_of_more_items_than_threads():
+    """1500 lists of up to 40 kept positions, and one bad position in the last of them."""
+    pool, m = make(15, slots=2000, max_ctx=64, pages=7000, kv_heads=1, layers=1, D=8, pt=16)
+    rng = np.random.default_rng(6)
+    slots = rng.permutation(2000)[:1500].tolist()
+    both(pool, m, "reserve", slots, [0] * 1500, [4] * 1500)
+    first = rng.integers(0, 20, 1500).tolist()
+    keep = [sorted(rng.choice(np.arange(f, 64), int(rng.integers(0, 40)), replace=False).tolist()) for f in first]
+    both(pool, m, "release", [slots[-1]], [3], [4])
+    keep[-1] = [first[-1], 47]
+    for bad, bit in ((48, kv_pool.MISSING), (64, kv_pool.BAD_KEEP)):
+        rows = keep[:-1] + [[first[-1], bad]]
+        unchanged(pool, m, bit, "compact", i32(slots), i32(first), i32([len(k) for k in rows]),
+                  torch.tensor([k + [0] * (40 - len(k)) for k in rows], dtype=torch.int32, device=DEV))
+    compact(pool, m, slots, first, keep)
