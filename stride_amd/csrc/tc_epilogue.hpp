@@ -258,12 +258,8 @@ struct EpiQkv {  // RoPE + q store + bf16 KV append  (src/kernels_tc.cu:347-432)
     const int32_t* row_pos;
   };
   __device__ __forceinline__ static f32x4 init(const Out&, int, int, int) { return f32x4{0.f, 0.f, 0.f, 0.f}; }
-  // Null where the table has no page for the position (a pool that had none left says so on the
-  // device, when this launch is on its way): the row is not kept.
-  __device__ __forceinline__ static uint16_t* kv_row(const Out& o, int which, int head, int slot, int pos) {
+  __device__ __forceinline__ static uint16_t* kv_row(const Out& o, int which, int head, int64_t block, int pos) {
     const StrideKvRef& kv = o.kv;
-    const int64_t block = kv.table[static_cast<int64_t>(slot) * kv.max_blocks + (pos >> o.page_shift)];
-    if (block < 0) return nullptr;
     const int token = pos & ((1 << o.page_shift) - 1);
     return static_cast<uint16_t*>(kv.arena) + block * kv.block_elems + o.layer * kv.layer_elems + which * kv.which_elems +
            head * kv.group_elems + static_cast<int64_t>(token) * kv.head_dim;
@@ -283,6 +279,10 @@ struct EpiQkv {  // RoPE + q store + bf16 KV append  (src/kernels_tc.cu:347-432)
     if (j >= g.rows) return;
     const int pos = o.row_pos[j];
     const int slot = o.row_slot[j];
+    // Without a page for the position (a pool that had none left says so on the device, when
+    // this launch is on its way) the row is not kept.
+    int block = 0;
+    if (kind != 0) block = o.kv.table[static_cast<int64_t>(slot) * o.kv.max_blocks + (pos >> o.page_shift)];
     // This lane holds dims d..d+3 (rows 4*(lane/16)+i of the tile) and, from
     // its partner, d+half..d+half+3: each half is written as one vector when
     // the destination is aligned for it.
@@ -316,10 +316,8 @@ struct EpiQkv {  // RoPE + q store + bf16 KV append  (src/kernels_tc.cu:347-432)
           q[half + i] = hi[i];
         }
       }
-    } else {
-      uint16_t* dst = kv_row(o, kind == 2 ? 1 : 0, head, slot, pos);
-      if (!dst) return;
-      dst += d;
+    } else if (block >= 0) {
+      uint16_t* dst = kv_row(o, kind == 2 ? 1 : 0, head, block, pos) + d;
       const uint32_t b0 = bf16_rne(lo[0]), b1 = bf16_rne(lo[1]), b2 = bf16_rne(lo[2]), b3 = bf16_rne(lo[3]);
       const uint32_t c0 = bf16_rne(hi[0]), c1 = bf16_rne(hi[1]), c2 = bf16_rne(hi[2]), c3 = bf16_rne(hi[3]);
       if ((reinterpret_cast<uintptr_t>(dst) & 7) == 0 && (half & 3) == 0) {

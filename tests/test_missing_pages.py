@@ -13,11 +13,9 @@ def source(name):
 
 def test_rows_without_a_page_are_not_written():
     text = source("tc_epilogue.hpp")
-    body = text[text.index("uint16_t* kv_row("):]
-    body = body[:body.index("static void apply")]
-    assert re.search(r"block = kv\.table\[[^;]*;\s*if \(block < 0\) return nullptr;", body)
-    assert len(re.findall(r"kv_row\(o,", text)) == 1
-    assert re.search(r"dst = kv_row\(o,[^;]*;\s*if \(!dst\) return;", text)
+    assert len(re.findall(r"\btable\[", text)) == 1 and len(re.findall(r"kv_row\(o,", text)) == 1
+    assert re.search(r"if \(kind != 0\) block = o\.kv\.table\[", text)
+    assert re.search(r"else if \(block >= 0\) \{\s*uint16_t\* dst = kv_row\(o,", text)
     assert re.search(r"block = kv\.table\[[^;]*;\s*if \(block < 0\) return;", source("exact.hip"))
 
 
