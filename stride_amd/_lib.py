@@ -237,6 +237,17 @@ SERVE_ENTRIES = {  # name -> (result, argument types)
     "stride_logits_reset": (C.c_int, [_VP, _VP, _VP, _I32, _VP]),
 }
 
+MX_ENTRIES = {  # include/stride_mx.h
+    "stride_mx_code_bytes": (_I64, [_I32, _I32]),
+    "stride_mx_scale_bytes": (_I64, [_I32]),
+    "stride_mx_quantize": (C.c_int, [_VP, _VP]),
+    "stride_mx_dequantize": (C.c_int, [_VP, _VP]),
+    "stride_mx_norm": (C.c_int, [_VP, _VP]),
+    "stride_mx_gemm": (C.c_int, [_VP, _VP]),
+    "stride_mx_mlp13": (C.c_int, [_VP, _VP]),
+    "stride_mx_qkv": (C.c_int, [_VP, _VP]),
+}
+
 
 def check_layout() -> None:
     """Sizes and offsets the C++ side static_asserts (reference PODs on x86-64)."""
@@ -304,7 +315,7 @@ def load(path: str = LIB_PATH) -> C.CDLL:
         fn = getattr(lib, name)
         fn.argtypes = [C.POINTER(ptype), C.c_int32, vp] if with_j else [C.POINTER(ptype), vp]
         fn.restype = C.c_int
-    for name, (result, args) in SERVE_ENTRIES.items():
+    for name, (result, args) in {**SERVE_ENTRIES, **MX_ENTRIES}.items():
         fn = getattr(lib, name)
         fn.argtypes, fn.restype = args, result
     lib.stride_tc_set_stream_config.argtypes = [C.c_int32]
@@ -344,7 +355,7 @@ def packed() -> C.CDLL:
             fn = getattr(lib, "stride_tc_" + name)
             fn.argtypes = [C.c_char_p] + [C.c_int] * ints + [C.c_void_p]
             fn.restype = C.c_int
-        for name, (result, args) in SERVE_ENTRIES.items():
+        for name, (result, args) in {**SERVE_ENTRIES, **MX_ENTRIES}.items():
             fn = getattr(lib, name)
             fn.argtypes, fn.restype = [C.c_char_p] + args[1:] if args[0] is _VP else args, result
         _packed = lib

@@ -2,7 +2,7 @@
 tools/stride_cli.cpp:
 
     python -m stride_amd.cli --model DIR --input prompts.jsonl --output out.jsonl
-        [--path tc|exact|serve] [--max-new N] [--concurrency C] [--max-rows R]
+        [--path tc|exact|serve] [--weights bf16|mx4] [--max-new N] [--concurrency C] [--max-rows R]
         [--page-tokens P] [--kv-shuffle S] [--row-shuffle S] [--use-eos]
         [--window W] [--sinks S] [--kv-pages N] [--share-prefixes]
         [--repetition-penalty X] [--presence-penalty X] [--frequency-penalty X]
@@ -19,6 +19,11 @@ for tokens that a sequence has; an input line may also have "bias": {"5": -1.5}
 and "allowed": [1, 2, 3], the tokens that may be chosen. Its ledger holds the
 processed logits; its attention rounds the softmax's weights to bf16, which --path tc
 keeps in fp32, so that the two paths' ledgers differ in low bits without options too.
+
+--weights mx4 (of --path tc and serve) runs the layers on weights in microscaled 4-bit
+blocks and activations in 8-bit ones (stride_amd.mx), made from the checkpoint's at
+loading; embedding and LM head stay bf16. Its ledger is another one than bf16's, and as
+independent of scheduling.
 
 Input lines: {"id": 0, "tokens": [1, 2, 3]}. Output lines (one per prompt, in
 input order): {"id": 0, "tokens": [...], "values": ["3f800000", ...],
@@ -202,6 +207,7 @@ def main(argv=None) -> int:
     ap.add_argument("--use-eos", action="store_true")
     ap.add_argument("--device", default="cuda:0")
     ap.add_argument("--path", choices=("tc", "exact", "serve"), default="tc")
+    ap.add_argument("--weights", choices=("bf16", "mx4"), default="bf16")
     ap.add_argument("--window", type=int, default=0)
     ap.add_argument("--sinks", type=int, default=0)
     ap.add_argument("--kv-pages", type=int, default=0)
@@ -215,6 +221,9 @@ def main(argv=None) -> int:
         ap.error("--window, --sinks, --kv-pages, --share-prefixes and the penalties belong to --path serve")
     if a.path == "serve" and a.kv_shuffle:
         ap.error("--kv-shuffle places a fixed cache; --path serve takes its pages from a pool")
+
+    if a.path == "exact" and a.weights != "bf16":
+        ap.error("--weights mx4 belongs to --path tc and serve")
 
     import torch
     from . import weights
@@ -248,6 +257,8 @@ def main(argv=None) -> int:
             w = weights.Weights.random(weights.ModelConfig(), a.device, int(a.model.split(":", 1)[1]), longest + 1)
         else:
             w = weights.Weights.load(a.model, a.device, max_positions=longest + 1)
+        if a.weights == "mx4":
+            w = w.microscaled()
         if a.path == "serve":
             eng = serving.ServingEngine(w, a.concurrency, longest, a.max_rows, a.page_tokens, a.kv_pages or None, a.window,
                                         a.sinks)

@@ -1,0 +1,299 @@
+// Blocks of 4 and 8 bits: quantisation of 16 x 16 tiles, their values, and RMSNorm with the
+// residual's addition (include/stride_mx.h). All of them move each value once and are bound by
+// memory.
+//
+// A wave has 4 rows of a chunk of 128 columns: lane l the 8 columns 8 * (l % 2) of tile l / 8, row
+// l / 2 % 4, so that eight lanes read neighbouring 16-column pieces of the rows. A block of 32 is
+// then the two tiles of lanes that differ in bits 0 and 3.
+#include <hip/hip_runtime.h>
+
+#include <climits>
+#include <cstddef>
+
+#include "mx_common.hpp"
+
+namespace stride_tc {
+namespace {
+
+struct Spot {  // a lane's place in its wave's 4 x 128 values
+  int row, tile, half;
+  __device__ __forceinline__ Spot() {
+    const int l = threadIdx.x & 63;
+    half = l & 1;
+    row = (l >> 1) & 3;
+    tile = l >> 3;
+  }
+};
+
+__device__ __forceinline__ uint32_t block_most(const float (&v)[8]) {
+  uint32_t m = mx_abs_bits(v[0]);
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = max(m, mx_abs_bits(v[i]));
+  m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 1)));
+  return max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 8)));
+}
+
+// The wave's values of chunk kc, rows `row` + ... of tile t, to codes and scales.
+template <int BITS>
+__device__ __forceinline__ void store_block(const StrideMxTiles& out, int t, int kc, int row, const Spot& s, const float (&v)[8], bool live) {
+  const int groups = mx_groups(out.cols);
+  const int byte = mx_scale_byte<BITS>(block_most(v));
+  const float inverse = mx_inverse(byte);
+  if (!live) return;
+  const int64_t chunk = static_cast<int64_t>(t) * groups * 4 + kc;
+  const int blk = s.tile >> 1;
+  if constexpr (BITS == 4) {
+    const uint32_t w = byte == 255 ? 0u : mx_pack4(v, inverse);
+    *reinterpret_cast<uint32_t*>(out.codes + chunk * kCode4Bytes + (blk * 16 + row) * 16 + (s.tile & 1) * 8 + s.half * 4) = w;
+  } else {
+    u32x2 w = {mx_pack8(v[0], v[1], v[2], v[3], inverse), mx_pack8(v[4], v[5], v[6], v[7], inverse)};
+    if (byte == 255) w = u32x2{0x7F7F7F7Fu, 0x7F7F7F7Fu};
+    *reinterpret_cast<u32x2*>(out.codes + chunk * kCode8Bytes + (s.tile * 16 + row) * 16 + s.half * 8) = w;
+  }
+  if (!s.half && !(s.tile & 1))
+    out.scales[(static_cast<int64_t>(t) * groups + (kc >> 2)) * kScaleBytes + (blk * 16 + row) * 4 + (kc & 3)] = static_cast<uint8_t>(byte);
+}
+
+template <class T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+  } else {
+    const u32x4 w = load16(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[2 * i] = f32_of(w[i] << 16), v[2 * i + 1] = f32_of(w[i] & 0xFFFF0000u);
+  }
+}
+
+// Workgroup: chunk blockIdx.x of tile blockIdx.y + ..., a wave for each four rows.
+template <int BITS, class T>
+__global__ __launch_bounds__(256) void k_quantize(const T* src, StrideMxTiles out, int rows, int chunks) {
+  const Spot s;
+  const int kc = blockIdx.x % chunks, t = blockIdx.x / chunks, row = (threadIdx.x >> 6) * 4 + s.row;
+  const int col_tiles = out.cols >> 4, ct = kc * 8 + s.tile;
+  const bool live = t * 16 + row < rows;
+  float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (live && ct < col_tiles) load8(src + (static_cast<int64_t>(t) * col_tiles + ct) * kTileElems + row * 16 + s.half * 8, v);
+  store_block<BITS>(out, t, kc, row, s, v, live);
+}
+
+// Workgroup: a chunk of a tile; a wave has four rows, a lane 8 columns of one.
+template <int BITS, class T>
+__global__ __launch_bounds__(256) void k_dequantize(StrideMxTiles in, T* out, int64_t stride, int rows, int chunks) {
+  const int kc = blockIdx.x % chunks, t = blockIdx.x / chunks, groups = mx_groups(in.cols);
+  const int l = threadIdx.x & 63, part = l & 15, row = (threadIdx.x >> 6) * 4 + (l >> 4), col = kc * kMxChunk + part * 8;
+  const int64_t at = static_cast<int64_t>(t) * 16 + row;
+  if (at >= rows || col >= in.cols) return;
+  const int64_t chunk = static_cast<int64_t>(t) * groups * 4 + kc;
+  const int blk = part >> 2;
+  const int byte = in.scales[(static_cast<int64_t>(t) * groups + (kc >> 2)) * kScaleBytes + (blk * 16 + row) * 4 + (kc & 3)];
+  float v[8];
+  if constexpr (BITS == 4) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(in.codes + chunk * kCode4Bytes + (blk * 16 + row) * 16 + (part & 3) * 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t c = (w >> (4 * i)) & 15u, e = (c >> 1) & 3u, m = c & 1u;
+      const uint32_t bits = e ? ((e + 126u) << 23) | (m << 22) : (m ? 0x3F000000u : 0u);
+      v[i] = f32_of(bits | (c >> 3) << 31);
+    }
+  } else {
+    const u32x2 w = *reinterpret_cast<const u32x2*>(in.codes + chunk * kCode8Bytes + ((part >> 1) * 16 + row) * 16 + (part & 1) * 8);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[i]), false), b = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[i]), true);
+      v[4 * i] = a[0], v[4 * i + 1] = a[1], v[4 * i + 2] = b[0], v[4 * i + 3] = b[1];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = byte == 255 ? f32_of(0x7FC00000u) : ldexpf(v[i], byte - 127);
+  T* o = out + at * stride + col;
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<f32x4*>(o)[0] = f32x4{v[0], v[1], v[2], v[3]};
+    reinterpret_cast<f32x4*>(o)[1] = f32x4{v[4], v[5], v[6], v[7]};
+  } else {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = bf16_rne(v[2 * i]) | bf16_rne(v[2 * i + 1]) << 16;
+    *reinterpret_cast<u32x4*>(o) = w;
+  }
+}
+
+// Workgroup: four rows of a lane tile. Wave w has chunks w, w + waves, ...; a lane's values stay in
+// registers between the sum and the scaling (IT chunks of 8; 0: h is read again). The order of a
+// row's sum follows from dim alone: lanes' chunks ascending, lanes by halves, waves ascending.
+template <int IT, bool ADD, bool MX>
+__global__ __launch_bounds__(1024) void k_mx_norm(StrideMxNormParams p, int chunks) {
+  __shared__ float sums[16][4];
+  const Spot s;
+  const int t = blockIdx.x >> 2, row = (blockIdx.x & 3) * 4 + s.row;
+  const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int col_tiles = p.dim >> 4;
+  const bool live = t * 16 + row < p.l.rows;
+  const int64_t at = static_cast<int64_t>(t) * col_tiles * kTileElems + row * 16 + s.half * 8;
+  float v[IT ? IT : 1][8];
+  float sum = 0.0f;
+  auto fetch = [&](int kc, float (&x)[8], bool again) {
+    const int ct = kc * 8 + s.tile;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+    if (!live || ct >= col_tiles) return;
+    float* h = p.h + at + static_cast<int64_t>(ct) * kTileElems;
+    load8(h, x);
+    if (ADD && !again) {
+      float a[8];
+      load8(p.add + at + static_cast<int64_t>(ct) * kTileElems, a);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] += a[i];
+      reinterpret_cast<f32x4*>(h)[0] = f32x4{x[0], x[1], x[2], x[3]};
+      reinterpret_cast<f32x4*>(h)[1] = f32x4{x[4], x[5], x[6], x[7]};
+    }
+  };
+  auto square = [&](const float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+  };
+  if constexpr (IT > 0) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) fetch(wave + i * waves, v[i], false);
+#pragma unroll
+    for (int i = 0; i < IT; ++i) square(v[i]);
+  } else {
+    for (int kc = wave; kc < chunks; kc += waves) {
+      fetch(kc, v[0], false);
+      square(v[0]);
+    }
+  }
+#pragma unroll
+  for (int d : {1, 8, 16, 32}) sum += __shfl_xor(sum, d);
+  if ((threadIdx.x & 63) < 8 && !s.half) sums[wave][s.row] = sum;
+  __syncthreads();
+  sum = 0.0f;
+  for (int w = 0; w < waves; ++w) sum += sums[w][s.row];
+  const float r = 1.0f / sqrtf(sum / static_cast<float>(p.dim) + p.eps);
+  auto scale = [&](int kc, float (&x)[8]) {
+    const int ct = kc * 8 + s.tile;
+    if (ct < col_tiles) {
+      float g[8];
+      load8(p.weight + ct * 16 + s.half * 8, g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = g[i] * (x[i] * r);
+    }
+    if constexpr (MX) {
+      if (kc < chunks) store_block<8>(p.out, t, kc, row, s, x, live);
+    } else if (live && ct < col_tiles) {
+      u32x4 w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = bf16_rne(x[2 * i]) | bf16_rne(x[2 * i + 1]) << 16;
+      *reinterpret_cast<u32x4*>(p.x + at + static_cast<int64_t>(ct) * kTileElems) = w;
+    }
+  };
+  if constexpr (IT > 0) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) scale(wave + i * waves, v[i]);
+  } else {
+    for (int kc = wave; kc < chunks; kc += waves) {
+      fetch(kc, v[0], true);
+      scale(kc, v[0]);
+    }
+  }
+}
+
+template <int IT>
+void launch_norm(const StrideMxNormParams& p, int chunks, int waves, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(p.l.rows) + 3) / 4)), block(waves * 64);
+  const bool mx = p.out.codes != nullptr;
+  if (p.add && mx) hipLaunchKernelGGL((k_mx_norm<IT, true, true>), grid, block, 0, st, p, chunks);
+  else if (p.add) hipLaunchKernelGGL((k_mx_norm<IT, true, false>), grid, block, 0, st, p, chunks);
+  else if (mx) hipLaunchKernelGGL((k_mx_norm<IT, false, true>), grid, block, 0, st, p, chunks);
+  else hipLaunchKernelGGL((k_mx_norm<IT, false, false>), grid, block, 0, st, p, chunks);
+}
+
+}  // namespace
+}  // namespace stride_tc
+
+using namespace stride_tc;
+
+static_assert(sizeof(StrideMxTiles) == 24, "MxTiles layout");
+static_assert(sizeof(StrideMxQuantizeParams) == 56 && sizeof(StrideMxDequantizeParams) == 64, "MxQuantizeParams layout");
+static_assert(sizeof(StrideMxNormParams) == 80 && offsetof(StrideMxNormParams, dim) == 72, "MxNormParams layout");
+
+extern "C" {
+
+int64_t stride_mx_code_bytes(int32_t cols, int32_t bits) {
+  if (cols <= 0 || cols % 16 || cols > (1 << 20) || (bits != 4 && bits != 8)) return -1;
+  return static_cast<int64_t>(mx_groups(cols)) * 4 * (bits == 4 ? kCode4Bytes : kCode8Bytes);
+}
+
+int64_t stride_mx_scale_bytes(int32_t cols) {
+  if (cols <= 0 || cols % 16 || cols > (1 << 20)) return -1;
+  return static_cast<int64_t>(mx_groups(cols)) * kScaleBytes;
+}
+
+int stride_mx_quantize(const StrideMxQuantizeParams* p, void* stream) {
+  const char* what = "mx_quantize";
+  if (!p) return mx_refused(what, "null parameters");
+  if (!mx_lanes_ok(p->l)) return mx_refused(what, "need rows >= 0 and lane_groups = ceil(rows/16)");
+  if ((p->bits != 4 && p->bits != 8) || (p->src_bytes != 2 && p->src_bytes != 4)) return mx_refused(what, "bits are 4 or 8, a source's bytes 2 or 4");
+  if (p->l.rows == 0) return 0;
+  if (const char* why = mx_why_not(p->out, p->l.lane_groups, 0)) return mx_refused(what, why);
+  if (!p->src || reinterpret_cast<uintptr_t>(p->src) % 16) return mx_refused(what, "src must be there, 16-byte aligned");
+  const int chunks = mx_groups(p->out.cols) * 4;
+  const int64_t groups = static_cast<int64_t>(chunks) * p->l.lane_groups;
+  if (groups > INT_MAX) return mx_refused(what, "rows and cols are too large together");
+  const dim3 grid(static_cast<unsigned>(groups)), block(256);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const uint16_t* half = static_cast<const uint16_t*>(p->src);
+  const float* full = static_cast<const float*>(p->src);
+  if (p->bits == 4 && p->src_bytes == 2) hipLaunchKernelGGL((k_quantize<4, uint16_t>), grid, block, 0, st, half, p->out, p->l.rows, chunks);
+  else if (p->bits == 4) hipLaunchKernelGGL((k_quantize<4, float>), grid, block, 0, st, full, p->out, p->l.rows, chunks);
+  else if (p->src_bytes == 2) hipLaunchKernelGGL((k_quantize<8, uint16_t>), grid, block, 0, st, half, p->out, p->l.rows, chunks);
+  else hipLaunchKernelGGL((k_quantize<8, float>), grid, block, 0, st, full, p->out, p->l.rows, chunks);
+  return mx_launched(what);
+}
+
+int stride_mx_dequantize(const StrideMxDequantizeParams* p, void* stream) {
+  const char* what = "mx_dequantize";
+  if (!p) return mx_refused(what, "null parameters");
+  if (!mx_lanes_ok(p->l)) return mx_refused(what, "need rows >= 0 and lane_groups = ceil(rows/16)");
+  if ((p->bits != 4 && p->bits != 8) || (p->out_bytes != 2 && p->out_bytes != 4)) return mx_refused(what, "bits are 4 or 8, a result's bytes 2 or 4");
+  if (p->l.rows == 0) return 0;
+  if (const char* why = mx_why_not(p->in, p->l.lane_groups, 0)) return mx_refused(what, why);
+  if (!p->out || reinterpret_cast<uintptr_t>(p->out) % 16) return mx_refused(what, "out must be there, 16-byte aligned");
+  if (p->out_stride < p->in.cols || p->out_stride % 8) return mx_refused(what, "out_stride must be a multiple of 8, at least cols");
+  const int chunks = (p->in.cols + kMxChunk - 1) / kMxChunk;
+  const int64_t groups = static_cast<int64_t>(chunks) * p->l.lane_groups;
+  if (groups > INT_MAX) return mx_refused(what, "rows and cols are too large together");
+  const dim3 grid(static_cast<unsigned>(groups)), block(256);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  uint16_t* half = static_cast<uint16_t*>(p->out);
+  float* full = static_cast<float*>(p->out);
+  if (p->bits == 4 && p->out_bytes == 2) hipLaunchKernelGGL((k_dequantize<4, uint16_t>), grid, block, 0, st, p->in, half, p->out_stride, p->l.rows, chunks);
+  else if (p->bits == 4) hipLaunchKernelGGL((k_dequantize<4, float>), grid, block, 0, st, p->in, full, p->out_stride, p->l.rows, chunks);
+  else if (p->out_bytes == 2) hipLaunchKernelGGL((k_dequantize<8, uint16_t>), grid, block, 0, st, p->in, half, p->out_stride, p->l.rows, chunks);
+  else hipLaunchKernelGGL((k_dequantize<8, float>), grid, block, 0, st, p->in, full, p->out_stride, p->l.rows, chunks);
+  return mx_launched(what);
+}
+
+int stride_mx_norm(const StrideMxNormParams* p, void* stream) {
+  const char* what = "mx_norm";
+  if (!p) return mx_refused(what, "null parameters");
+  if (!mx_lanes_ok(p->l)) return mx_refused(what, "need rows >= 0 and lane_groups = ceil(rows/16)");
+  if (p->dim <= 0 || p->dim % 16 || p->dim > 65536) return mx_refused(what, "dim must be a positive multiple of 16, at most 65536");
+  if (p->l.rows == 0) return 0;
+  if (!p->h || !p->weight || !p->out.codes == !p->x) return mx_refused(what, "need h, weight and one of out and x");
+  if (p->out.codes)
+    if (const char* why = mx_why_not(p->out, p->l.lane_groups, p->dim)) return mx_refused(what, why);
+  if ((reinterpret_cast<uintptr_t>(p->h) | reinterpret_cast<uintptr_t>(p->add) | reinterpret_cast<uintptr_t>(p->weight) | reinterpret_cast<uintptr_t>(p->x)) % 16)
+    return mx_refused(what, "pointers must be 16-byte aligned");
+  const int chunks = mx_groups(p->dim) * 4, waves = chunks < 16 ? chunks : 16, rounds = (chunks + waves - 1) / waves;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (rounds == 1) launch_norm<1>(*p, chunks, waves, st);
+  else if (rounds == 2) launch_norm<2>(*p, chunks, waves, st);
+  else if (rounds <= 4) launch_norm<4>(*p, chunks, waves, st);
+  else launch_norm<0>(*p, chunks, waves, st);
+  return mx_launched(what);
+}
+
+}  // extern "C"

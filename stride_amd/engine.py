@@ -27,7 +27,7 @@ import math
 import numpy as np
 import torch
 
-from . import harness, layout, tc
+from . import harness, layout, mx, tc
 from .weights import ModelConfig
 from .weights import Weights as PackedWeights
 
@@ -101,7 +101,11 @@ class Engine:
         self.h = torch.zeros((lt, H // 16, 16, 16), dtype=torch.float32, device=dev)
         self.x = torch.zeros((lt, H // 16, 16, 16), dtype=torch.int16, device=dev)
         self.attn = torch.zeros((lt, cfg.heads * D // 16, 16, 16), dtype=torch.int16, device=dev)
-        self.z = torch.zeros((lt, cfg.mlp // 16, 16, 16), dtype=torch.int16, device=dev)
+        if weights.bits == 4:  # 8-bit activations and the products that the next norm adds to h
+            self.x8, self.attn8, self.z8 = (mx.Tiles.create(max_rows, k, 8, dev) for k in (H, cfg.heads * D, cfg.mlp))
+            self.y = torch.zeros((lt, H // 16, 16, 16), dtype=torch.int16, device=dev)
+        else:
+            self.z = torch.zeros((lt, cfg.mlp // 16, 16, 16), dtype=torch.int16, device=dev)
         self.lm_x = torch.zeros((lt, H // 16, 16, 16), dtype=torch.int16, device=dev)
         self.q = torch.zeros((max_rows, cfg.heads * D), dtype=torch.float32, device=dev)
         self.scratch = self._attention_scratch()
@@ -135,6 +139,21 @@ class Engine:
         harness.best_reset(best)
         harness.lm_greedy(self.w.lm, x, count, self.cfg.vocab, best=best)
 
+    def _microscaled_layers(self, n: int, slot, pos, attend) -> None:
+        """The layers of a step and the final norm on microscaled weights: a product's result is
+        added to h by the norm behind it."""
+        cfg, w, add = self.cfg, self.w, None
+        for li, L in enumerate(w.layers):
+            mx.norm(self.h, n, L["norm_attn"], cfg.rms_eps, add=add, out=self.x8)
+            mx.qkv(L["q"], L["k"], L["v"], self.x8, n, cfg.head_dim, w.rope, slot, pos, self.kv, layer=li, q_out=self.q)
+            attend(li)
+            mx.quantize(self.attn, n, bits=8, out=self.attn8)
+            mx.gemm(L["o"], self.attn8, n, out=self.y)
+            mx.norm(self.h, n, L["norm_mlp"], cfg.rms_eps, add=self.y, out=self.x8)
+            mx.mlp13(L["w1"], L["w3"], self.x8, n, out=self.z8)
+            add = mx.gemm(L["w2"], self.z8, n, out=self.y)
+        mx.norm(self.h, n, w.norm_final, cfg.rms_eps, add=add, out=self.x, bits=16)
+
     def launch(self, n: int, slot, pos, tok, items, greedy=None, best=None, rules=None, runs: int = 0) -> None:
         """Enqueue one step over n rows described by device tensors (row slots,
         positions, tokens, attention items); no host synchronization, so it can
@@ -144,16 +163,19 @@ class Engine:
         cfg, w = self.cfg, self.w
         attend = self._attention(n, slot, pos, items, runs)
         harness.embed(w.embed, tok, n, cfg.hidden, h_out=self.h)
-        for li, L in enumerate(w.layers):
-            harness.norm(self.h, n, L["norm_attn"], cfg.rms_eps, x_out=self.x)
-            harness.qkv(L["q"], L["k"], L["v"], self.x, n, cfg.head_dim, w.rope, slot, pos, self.kv, layer=li,
-                        q_out=self.q)
-            attend(li)
-            harness.gemm_residual(L["o"], self.attn, self.h, n)
-            harness.norm(self.h, n, L["norm_mlp"], cfg.rms_eps, x_out=self.x)
-            harness.mlp13(L["w1"], L["w3"], self.x, n, out=self.z)
-            harness.gemm_residual(L["w2"], self.z, self.h, n)
-        harness.norm(self.h, n, w.norm_final, cfg.rms_eps, x_out=self.x)
+        if w.bits == 4:
+            self._microscaled_layers(n, slot, pos, attend)
+        else:
+            for li, L in enumerate(w.layers):
+                harness.norm(self.h, n, L["norm_attn"], cfg.rms_eps, x_out=self.x)
+                harness.qkv(L["q"], L["k"], L["v"], self.x, n, cfg.head_dim, w.rope, slot, pos, self.kv, layer=li,
+                            q_out=self.q)
+                attend(li)
+                harness.gemm_residual(L["o"], self.attn, self.h, n)
+                harness.norm(self.h, n, L["norm_mlp"], cfg.rms_eps, x_out=self.x)
+                harness.mlp13(L["w1"], L["w3"], self.x, n, out=self.z)
+                harness.gemm_residual(L["w2"], self.z, self.h, n)
+            harness.norm(self.h, n, w.norm_final, cfg.rms_eps, x_out=self.x)
         if best is None:
             return
         count = n if greedy is None else int(greedy.numel())

@@ -1,0 +1,233 @@
+"""Operators for models in microscaled 4-bit weights (include/stride_mx.h): blocks of 32 neighbours
+along K that share a scale, a power of two; weights in 4 bits (e2m1), activations in 8 (e4m3).
+
+    w = quantize(tiles, bits=4)                    packed weight tiles (layout.pack_tiles) -> Tiles
+    x = norm(h, rows, gains, eps, add=y)           h += y, RMSNorm(h) * gains in 8 bits
+    q = qkv(wq, wk, wv, x, rows, head_dim, rope, row_slot, row_pos, kv, layer)
+    a = quantize(attn, rows, bits=8)               attention's x tiles -> Tiles
+    y = gemm(wo, a, rows)                          W x in bf16 tiles, which the next norm adds to h
+    z = mlp13(w1, w3, x, rows)                     silu(W1 x) * (W3 x) in 8 bits
+
+A row's result depends on the row and the weights only, whatever the batch. Results go to `out`
+(default: allocated here, on torch's current stream, so that with another one set by
+set_kernel_stream it is passed), where rows behind `rows` are left as they were. Everything is
+read when the launch runs, so it can be captured in a HIP graph.
+"""
+from __future__ import annotations
+
+from struct import Struct
+
+import torch
+
+from . import _lib, tc
+from .harness import PagedKv, here, other_stream
+
+_TILES = Struct("<2Q2i").pack
+_QUANTIZE = Struct("<4iQ24s2i").pack
+_DEQUANTIZE = Struct("<4i24sQq2i").pack
+_NORM = Struct("<4i3Q24sQif").pack
+_GEMM = Struct("<4i24s24sQ").pack
+_MLP13 = Struct("<4i24s24s24s24s").pack
+_QKV = Struct("<4i24s24s24s24sQq56s3Q2i").pack
+_NONE = _TILES(0, 0, 0, 0)
+
+BLOCK, CHUNK, GROUP = 32, 128, 512  # columns of a scale, of a matrix instruction, of a lane's word of scales
+_PARTS = {4: (4, 16, 16), 8: (2, 4, 16, 16)}  # a chunk's codes
+
+
+class Tiles:
+    """Rows of `cols` columns in blocks of 4 or 8 bits, by tiles of 16 rows: codes and scales as
+    include/stride_mx.h lays them out, uint8 [tiles][4 groups][4][16][16] (8 bits: [2][4][16][16])
+    and [tiles][groups][4][16][4] with groups = ceil(cols / 512)."""
+
+    def __init__(self, codes, scales, cols: int, bits: int):
+        if bits not in (4, 8) or cols <= 0 or cols % 16 or cols > 1 << 20:
+            raise ValueError("blocks have 4 or 8 bits, and cols is a positive multiple of 16, at most 2^20")
+        tiles, groups = int(codes.shape[0]), (cols + GROUP - 1) // GROUP
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.device != scales.device \
+                or not (codes.is_contiguous() and scales.is_contiguous()):
+            raise ValueError("codes and scales must be contiguous uint8 on one device")
+        if tuple(codes.shape) != (tiles, 4 * groups, *_PARTS[bits]) or tuple(scales.shape) != (tiles, groups, 4, 16, 4):
+            raise ValueError(f"codes must be [tiles][{4 * groups}]{list(_PARTS[bits])} and scales [tiles][{groups}][4][16][4]")
+        self.codes, self.scales, self.cols, self.bits, self.tiles = codes, scales, int(cols), bits, tiles
+        self._ref, self._device = _TILES(codes.data_ptr(), scales.data_ptr(), tiles, int(cols)), codes.get_device()
+
+    @staticmethod
+    def create(rows: int, cols: int, bits: int, device) -> "Tiles":
+        """For `rows` rows, all zeros."""
+        if bits not in _PARTS or rows < 0 or cols <= 0:
+            raise ValueError("blocks have 4 or 8 bits; rows and cols are counts")
+        tiles, groups = (rows + 15) // 16, (cols + GROUP - 1) // GROUP
+        return Tiles(torch.zeros((tiles, 4 * groups, *_PARTS[bits]), dtype=torch.uint8, device=device),
+                     torch.zeros((tiles, groups, 4, 16, 4), dtype=torch.uint8, device=device), cols, bits)
+
+    @property
+    def rows(self) -> int:
+        return self.tiles * 16
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+
+def _check(rc: int) -> None:
+    if rc:
+        _lib.check(rc)
+
+
+def _operand(t, bits: int, rows: int, dev: int, cols: int, name: str) -> bytes:
+    """A Tiles argument's block, looked over (cols 0: any)."""
+    if not isinstance(t, Tiles) or t.bits != bits or t._device != dev or t.tiles * 16 < rows or (cols and t.cols != cols):
+        raise ValueError(f"{name} must be Tiles in {bits} bits with the rows and columns of the call, on its device")
+    return t._ref
+
+
+def _result(out, rows: int, cols: int, device) -> Tiles:
+    if out is None:
+        _allocates()
+        return Tiles.create(rows, cols, 8, device)
+    return out
+
+
+def _allocates() -> None:
+    if other_stream():
+        raise ValueError("with another stream set by set_kernel_stream, pass out")
+
+
+def _tile_shape(t, rows: int, name: str):
+    if t.dim() != 4 or t.shape[2] != 16 or t.shape[3] != 16 or not t.is_contiguous() or t.shape[0] * 16 < rows or t.shape[1] < 1:
+        raise ValueError(f"{name} must be contiguous tiles [ceil(rows / 16)][cols / 16][16][16]")
+
+
+def _y_tiles(out, rows: int, cols: int, device, dev: int):
+    """bf16 x tiles that are written."""
+    T = (rows + 15) // 16
+    if out is None:
+        _allocates()
+        return torch.zeros((T, cols // 16, 16, 16), dtype=torch.int16, device=device)
+    if out.dtype not in (torch.int16, torch.bfloat16) or out.get_device() != dev:
+        raise ValueError("out must be 16-bit tiles on the call's device")
+    _tile_shape(out, rows, "out")
+    if out.shape[1] * 16 != cols:
+        raise ValueError(f"out must have {cols} columns")
+    return out
+
+
+def quantize(tiles, rows: int | None = None, bits: int = 4, out: Tiles | None = None) -> Tiles:
+    """Tiles [t][ct][16][16] of 16-bit (bf16, or its bits in int16) or fp32 values to blocks of 4
+    or 8 bits, for the first `rows` rows (default: all)."""
+    if tiles.dtype in (torch.int16, torch.bfloat16):
+        size = 2
+    elif tiles.dtype == torch.float32:
+        size = 4
+    else:
+        raise ValueError("tiles must hold bf16 or fp32")
+    if bits not in (4, 8):
+        raise ValueError("blocks have 4 or 8 bits")
+    here(tiles)
+    rows = tiles.shape[0] * 16 if rows is None else rows
+    _tile_shape(tiles, rows, "tiles")
+    cols, dev = tiles.shape[1] * 16, tiles.get_device()
+    if out is None:
+        _allocates()
+        out = Tiles.create(rows, cols, bits, tiles.device)
+    p = _QUANTIZE(rows, (rows + 15) // 16, 0, 0, tiles.data_ptr(), _operand(out, bits, rows, dev, cols, "out"), bits, size)
+    _check(_lib.packed().stride_mx_quantize(p, tc.kernel_stream()))
+    return out
+
+
+def dequantize(t: Tiles, rows: int | None = None, dtype=torch.bfloat16, out=None):
+    """The values of the first `rows` rows, row-major [rows][cols] in bf16 or fp32."""
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("values come in bf16 or fp32")
+    here(t.codes)
+    rows = t.rows if rows is None else rows
+    if out is None:
+        _allocates()
+        out = torch.empty((rows, t.cols), dtype=dtype, device=t.codes.device)
+    elif out.dtype != dtype or out.dim() != 2 or out.shape[0] < rows or out.shape[1] != t.cols or out.stride(1) != 1 or out.get_device() != t._device:
+        raise ValueError("out must be [rows][cols] of that type on the same device, its rows contiguous")
+    p = _DEQUANTIZE(rows, (rows + 15) // 16, 0, 0, _operand(t, t.bits, rows, t._device, 0, "t"), out.data_ptr(),
+                    out.stride(0) if rows > 1 else t.cols, t.bits, 2 if dtype == torch.bfloat16 else 4)
+    _check(_lib.packed().stride_mx_dequantize(p, tc.kernel_stream()))
+    return out
+
+
+def norm(h, rows: int, weight, eps: float, add=None, out=None, bits: int = 8):
+    """h += add (bf16 tiles, where given), then RMSNorm(h) * weight: in 8 bits (Tiles), or with
+    bits=16 in bf16 x tiles. h: fp32 tiles [lt][ct][16][16]."""
+    here(h)
+    if h.dtype != torch.float32:
+        raise ValueError("h must be fp32 tiles")
+    _tile_shape(h, rows, "h")
+    cols, dev = h.shape[1] * 16, h.get_device()
+    if weight.dtype != torch.float32 or weight.numel() != cols or not weight.is_contiguous() or weight.get_device() != dev:
+        raise ValueError("weight must be contiguous fp32 of h's columns, on its device")
+    a = 0
+    if add is not None:
+        if add.dtype not in (torch.int16, torch.bfloat16) or add.get_device() != dev:
+            raise ValueError("add must be bf16 tiles on h's device")
+        _tile_shape(add, rows, "add")
+        if add.shape[1] * 16 != cols:
+            raise ValueError("add must have h's columns")
+        a = add.data_ptr()
+    if bits == 8:
+        out = _result(out, rows, cols, h.device)
+        ref, x = _operand(out, 8, rows, dev, cols, "out"), 0
+    elif bits == 16:
+        out = _y_tiles(out, rows, cols, h.device, dev)
+        ref, x = _NONE, out.data_ptr()
+    else:
+        raise ValueError("a norm's result has 8 or 16 bits")
+    p = _NORM(rows, (rows + 15) // 16, 0, 0, h.data_ptr(), a, weight.data_ptr(), ref, x, cols, eps)
+    _check(_lib.packed().stride_mx_norm(p, tc.kernel_stream()))
+    return out
+
+
+def gemm(w: Tiles, x: Tiles, rows: int, out=None):
+    """y = W x for the first `rows` rows of x, in bf16 x tiles."""
+    here(x.codes)
+    dev = x._device
+    out = _y_tiles(out, rows, w.tiles * 16, x.codes.device, dev)
+    p = _GEMM(rows, (rows + 15) // 16, 0, 0, _operand(x, 8, rows, dev, 0, "x"), _operand(w, 4, 1, dev, x.cols, "w"), out.data_ptr())
+    _check(_lib.packed().stride_mx_gemm(p, tc.kernel_stream()))
+    return out
+
+
+def mlp13(w1: Tiles, w3: Tiles, x: Tiles, rows: int, out: Tiles | None = None) -> Tiles:
+    """z = silu(W1 x) * (W3 x) in 8 bits."""
+    here(x.codes)
+    dev = x._device
+    out = _result(out, rows, w1.tiles * 16, x.codes.device)
+    p = _MLP13(rows, (rows + 15) // 16, 0, 0, _operand(x, 8, rows, dev, 0, "x"), _operand(w1, 4, 1, dev, x.cols, "w1"),
+               _operand(w3, 4, w1.tiles * 16, dev, x.cols, "w3"), _operand(out, 8, rows, dev, w1.tiles * 16, "out"))
+    _check(_lib.packed().stride_mx_mlp13(p, tc.kernel_stream()))
+    return out
+
+
+def qkv(wq: Tiles, wk: Tiles, wv: Tiles, x: Tiles, rows: int, head_dim: int, rope, row_slot, row_pos, kv: PagedKv, layer: int = 0,
+        q_out=None):
+    """harness.qkv on these weights (rows in layout.rope_rows' order): q with RoPE in fp32 rows, K
+    and V appended to the paged bf16 cache."""
+    here(x.codes)
+    dev, nq = x._device, wq.tiles * 16
+    if row_slot.dtype != torch.int32 or row_pos.dtype != torch.int32 or row_slot.numel() < rows or row_pos.numel() < rows \
+            or not (row_slot.is_contiguous() and row_pos.is_contiguous()):
+        raise ValueError("row_slot and row_pos must be contiguous int32, one for each row")
+    if rope.dtype != torch.float32 or not rope.is_contiguous() or rope.dim() != 3 or rope.shape[1] * 2 != head_dim or rope.shape[2] != 2:
+        raise ValueError("rope must be contiguous fp32 [positions][head_dim / 2][2]")
+    if not row_slot.get_device() == row_pos.get_device() == rope.get_device() == kv.table.get_device() == dev:
+        raise ValueError("the arguments are on different devices")
+    if not 0 <= layer < kv.ref.block_elems // kv.ref.layer_elems or kv.ref.which_elems * head_dim != wk.tiles * 16 * kv.ref.group_elems:
+        raise ValueError("layer or the number of KV heads is not the cache's")
+    if q_out is None:
+        _allocates()
+        q_out = torch.zeros((max(rows, 1), nq), dtype=torch.float32, device=x.codes.device)
+    elif q_out.dtype != torch.float32 or q_out.dim() != 2 or q_out.shape[0] < rows or q_out.shape[1] != nq or q_out.stride(1) != 1 \
+            or q_out.get_device() != dev:
+        raise ValueError("q_out must be fp32 [rows][q columns], its rows contiguous")
+    ws = [_operand(w, 4, 1, dev, x.cols, name) for w, name in ((wq, "wq"), (wk, "wk"), (wv, "wv"))]
+    p = _QKV(rows, (rows + 15) // 16, 0, 0, _operand(x, 8, rows, dev, 0, "x"), *ws, q_out.data_ptr(), q_out.stride(0) if rows > 1 else nq,
+             bytes(kv.ref), rope.data_ptr(), row_slot.data_ptr(), row_pos.data_ptr(), layer, head_dim)
+    _check(_lib.packed().stride_mx_qkv(p, tc.kernel_stream()))
+    return q_out

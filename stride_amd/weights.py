@@ -26,7 +26,7 @@ import os
 import numpy as np
 import torch
 
-from . import layout
+from . import layout, mx
 
 MAX_HEAD_DIM = 256  # src/kernels.h kMaxHeadDim
 
@@ -177,12 +177,23 @@ class Checkpoint:
 class Weights:
     """Device-resident packed weights in the layout the tensor-core operators
     consume: `embed` and `lm` tiles (the same tensor when tied), per layer q, k,
-    v, o, w1, w3, w2 tiles and fp32 norm gains, `norm_final`, and `rope`."""
+    v, o, w1, w3, w2 tiles and fp32 norm gains, `norm_final`, and `rope`. `bits`: 16,
+    or 4 where the layers' matrices are microscaled (stride_amd.mx.Tiles)."""
 
     def __init__(self, cfg: ModelConfig, embed, lm, layers, norm_final, rope):
         self.cfg, self.embed, self.lm, self.layers, self.norm_final, self.rope = cfg, embed, lm, layers, norm_final, rope
-        self.bytes_per_pass = sum(int(t.numel()) * 2 for L in layers for k, t in L.items() if k not in
-                                  ("norm_attn", "norm_mlp")) + cfg.vocab * cfg.hidden * 2
+        self.bits = 4 if layers and isinstance(layers[0]["q"], mx.Tiles) else 16
+        self.bytes_per_pass = sum(t.nbytes if self.bits == 4 else int(t.numel()) * 2 for L in layers for k, t in L.items()
+                                  if k not in ("norm_attn", "norm_mlp")) + cfg.vocab * cfg.hidden * 2
+
+    def microscaled(self) -> "Weights":
+        """The model with its layers' matrices in blocks of 4 bits (stride_amd.mx), which engine.Engine
+        and serving.ServingEngine run as they run this one. Embedding, LM head and gains stay as they
+        are; with a microscaled model there is nothing left to do."""
+        if self.bits == 4:
+            return self
+        layers = [{k: t if k in ("norm_attn", "norm_mlp") else mx.quantize(t) for k, t in L.items()} for L in self.layers]
+        return Weights(self.cfg, self.embed, self.lm, layers, self.norm_final, self.rope)
 
     @staticmethod
     def load(model_dir: str, device, cfg: ModelConfig | None = None, max_positions: int = 4097) -> "Weights":
