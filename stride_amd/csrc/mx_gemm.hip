@@ -1,11 +1,11 @@
 // The linear layers' products on microscaled operands (include/stride_mx.h): e2m1 weights by e4m3
 // activations, v_mfma_scale_f32_16x16x128_f8f6f4, fp32 sums.
 //
-// Every kernel evaluates the same expression: chunks of 128 columns chain in ascending order within
-// each split of K, and the splits' sums are added in ascending order, so a row has the same bits
-// whatever the batch and the kernel.
+// Every kernel evaluates the same expression: the chunks of 128 columns chain in ascending order from
+// zero on, so a row has the same bits whatever the batch and the kernel.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cstddef>
 
@@ -15,15 +15,12 @@
 namespace stride_tc {
 namespace {
 
-constexpr int kSplits = 4;
-
 // Up to three matrices over the same x, their row tiles end to end (q, k, v), or gate and up.
 struct MxGeometry {
   const uint8_t *xc, *xs;
   const uint8_t *wc[3], *ws[3];
   int32_t tiles[3];
   int32_t groups;  // of 512 columns
-  int32_t per;     // groups of a split
   int32_t rows, lane_groups;
 };
 
@@ -44,7 +41,7 @@ struct EpiY {
     uint16_t* y;
     int32_t row_tiles;
   };
-  __device__ __forceinline__ static void apply(const Out& o, const MxGeometry& g, int rt, int lt, const f32x4 (&y)[1][1], int lane) {
+  __device__ __forceinline__ static void finish(const Out& o, const MxGeometry& g, int rt, int lt, const f32x4 (&y)[1][1], int lane) {
     if (lt * 16 + (lane & 15) >= g.rows) return;
     const f32x4 v = y[0][0];
     *reinterpret_cast<u32x2*>(o.y + (static_cast<int64_t>(lt) * o.row_tiles + rt) * kTileElems + (lane & 15) * 16 + (lane >> 4) * 4) =
@@ -55,13 +52,20 @@ struct EpiY {
 struct EpiRope {
   static constexpr int kMats = 1, kUnit = 1;
   using Out = EpiQkv::Out;
-  __device__ __forceinline__ static void apply(const Out& o, const MxGeometry& g, int rt, int lt, const f32x4 (&y)[1][1], int lane) {
+  __device__ __forceinline__ static void finish(const Out& o, const MxGeometry& g, int rt, int lt, const f32x4 (&y)[1][1], int lane) {
     Geometry rows{};
     rows.rows = g.rows;
     const int which = mx_matrix(g, rt);
     EpiQkv::apply(o, rows, which, rt, lt, y[0], lane);
   }
 };
+
+// x / (1 + e^-x) with the hardware's exponential and reciprocal, each good to an ulp or so: the result
+// is rounded to four bits. (2048 rows of 2 x 8192 x 2048: 70 us, 93 with the exact division and the
+// polynomial that the bf16 path has for its bits.)
+__device__ __forceinline__ float silu(float x) {
+  return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504088896341f));
+}
 
 // z's block: two row tiles, whose 32 values of a batch row four lanes hold. Where z's columns end
 // inside a group of 512, what fills it up is written as zeros.
@@ -80,97 +84,309 @@ struct EpiZ {
     if (quarter == 0)
       o.z.scales[(static_cast<int64_t>(lt) * groups + (kc >> 2)) * kScaleBytes + (blk * 16 + row) * 4 + (kc & 3)] = static_cast<uint8_t>(byte);
   }
-  __device__ __forceinline__ static void apply(const Out& o, const MxGeometry& g, int rt, int lt, const f32x4 (&y)[2][2], int lane) {
+  __device__ __forceinline__ static void finish(const Out& o, const MxGeometry& g, int unit, int lt, const f32x4 (&y)[2][2], int lane) {
     float v[2][4];
     uint32_t most = 0;
 #pragma unroll
     for (int r = 0; r < 2; ++r)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        v[r][i] = rt + r < g.tiles[0] ? det_silu(y[0][r][i]) * y[1][r][i] : 0.0f;
+        v[r][i] = unit * 2 + r < g.tiles[0] ? silu(y[0][r][i]) * y[1][r][i] : 0.0f;
         most = max(most, mx_abs_bits(v[r][i]));
       }
-    most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16)));
-    most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32)));
+    const auto halves = __builtin_amdgcn_permlane32_swap(most, most, false, false);
+    most = max(halves[0], halves[1]);
+    const auto quarters = __builtin_amdgcn_permlane16_swap(most, most, false, false);
+    most = max(quarters[0], quarters[1]);
     const int byte = mx_scale_byte<8>(most);
     const float inverse = mx_inverse(byte);
     u32x2 w = {mx_pack8(v[0][0], v[0][1], v[0][2], v[0][3], inverse), mx_pack8(v[1][0], v[1][1], v[1][2], v[1][3], inverse)};
     if (byte == 255) w = u32x2{0x7F7F7F7Fu, 0x7F7F7F7Fu};
-    store(o, g, rt >> 1, lt, w, byte, lane);
+    store(o, g, unit, lt, w, byte, lane);
   }
 };
 
-// Workgroup: one unit of row tiles by one lane tile, a wave for each split.
+// Pointers of tile `rt` of the matrices end to end (UNIT 1) or of matrix m (UNIT 2), clamped to what
+// is there.
 template <class Epi>
-__global__ __launch_bounds__(256) void k_mx_simple(MxGeometry g, typename Epi::Out o, int units) {
-  constexpr int M = Epi::kMats, U = Epi::kUnit;
-  __shared__ f32x4 part[kSplits][M][U][kWave];
-  const int lane = threadIdx.x & 63, split = threadIdx.x >> 6;
-  const int unit = blockIdx.x % units, lt = blockIdx.x / units;
-  if constexpr (U == 2) {
-    if (unit * U >= g.tiles[0]) {
-      if (split == 0) Epi::store(o, g, unit, lt, u32x2{0u, 0u}, 0, lane);
-      return;
-    }
+__device__ __forceinline__ void mx_source(const MxGeometry& g, int m, int rt, const uint8_t*& codes, const uint8_t*& scales) {
+  int which = m;
+  if constexpr (Epi::kMats == 1) {
+    rt = min(rt, g.tiles[0] + g.tiles[1] + g.tiles[2] - 1);
+    which = mx_matrix(g, rt);
+  } else {
+    rt = min(rt, g.tiles[0] - 1);
   }
+  codes = (which == 0 ? g.wc[0] : which == 1 ? g.wc[1] : g.wc[2]) + static_cast<int64_t>(rt) * g.groups * 4 * kCode4Bytes;
+  scales = (which == 0 ? g.ws[0] : which == 1 ? g.ws[1] : g.ws[2]) + static_cast<int64_t>(rt) * g.groups * kScaleBytes;
+}
+
+// One lane tile: workgroup of W waves, one unit. Wave w loads the w-th part of K at once; the sums
+// go from wave to wave through LDS, so that the products chain in ascending order.
+template <class Epi, int W>
+__global__ __launch_bounds__(64 * W) void k_mx_row(MxGeometry g, typename Epi::Out o, int units) {
+  constexpr int M = Epi::kMats, U = Epi::kUnit;
+  __shared__ f32x4 sums[M][U][kWave];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int unit = blockIdx.x % units, lt = blockIdx.x / units;
   const uint8_t *wc[M][U], *ws[M][U];
 #pragma unroll
   for (int m = 0; m < M; ++m)
 #pragma unroll
-    for (int r = 0; r < U; ++r) {
-      int rt = unit * U + r, which = m;
-      if constexpr (U == 1) which = mx_matrix(g, rt);
-      else rt = min(rt, g.tiles[0] - 1);
-      wc[m][r] = (which == 0 ? g.wc[0] : which == 1 ? g.wc[1] : g.wc[2]) + static_cast<int64_t>(rt) * g.groups * 4 * kCode4Bytes + lane * 16;
-      ws[m][r] = (which == 0 ? g.ws[0] : which == 1 ? g.ws[1] : g.ws[2]) + static_cast<int64_t>(rt) * g.groups * kScaleBytes + lane * 4;
-    }
-  const uint8_t* xc = g.xc + static_cast<int64_t>(lt) * g.groups * 4 * kCode8Bytes + lane * 16;
-  const uint8_t* xs = g.xs + static_cast<int64_t>(lt) * g.groups * kScaleBytes + lane * 4;
+    for (int u = 0; u < U; ++u) mx_source<Epi>(g, m, unit * U + u, wc[m][u], ws[m][u]);
+  const uint8_t* xc = g.xc + static_cast<int64_t>(lt) * g.groups * 4 * kCode8Bytes;
+  const uint8_t* xs = g.xs + static_cast<int64_t>(lt) * g.groups * kScaleBytes;
+  const uint32_t at16 = lane * 16, at4 = lane * 4;
   f32x4 acc[M][U];
 #pragma unroll
   for (int m = 0; m < M; ++m)
 #pragma unroll
-    for (int r = 0; r < U; ++r) acc[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int end = min((split + 1) * g.per, g.groups);
-  for (int i = split * g.per; i < end; ++i) {
-    const uint32_t sx = *reinterpret_cast<const uint32_t*>(xs + i * kScaleBytes);
-    uint32_t sw[M][U];
-#pragma unroll
-    for (int m = 0; m < M; ++m)
-#pragma unroll
-      for (int r = 0; r < U; ++r) sw[m][r] = *reinterpret_cast<const uint32_t*>(ws[m][r] + i * kScaleBytes);
-    unroll<4>([&](auto c) {
-      const int kc = i * 4 + c;
-      const u32x4 x0 = load16(xc + static_cast<int64_t>(kc) * kCode8Bytes), x1 = load16(xc + static_cast<int64_t>(kc) * kCode8Bytes + 1024);
+    for (int u = 0; u < U; ++u) acc[m][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int round = 0; round < g.groups; round += W) {
+    const int i = round + wave;
+    u32x4 w[4][M][U], x[4][2];
+    uint32_t sw[M][U], sx = 0;
+    if (i < g.groups) {
+      sx = *reinterpret_cast<const uint32_t*>(xs + static_cast<int64_t>(i) * kScaleBytes + at4);
 #pragma unroll
       for (int m = 0; m < M; ++m)
 #pragma unroll
-        for (int r = 0; r < U; ++r)
-          acc[m][r] = mx_mfma<c>(load16(wc[m][r] + static_cast<int64_t>(kc) * kCode4Bytes), x0, x1, acc[m][r], sw[m][r], sx);
-    });
+        for (int u = 0; u < U; ++u) sw[m][u] = *reinterpret_cast<const uint32_t*>(ws[m][u] + static_cast<int64_t>(i) * kScaleBytes + at4);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int64_t kc = static_cast<int64_t>(i) * 4 + c;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) x[c][h] = load16(xc + kc * kCode8Bytes + h * 1024 + at16);
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int u = 0; u < U; ++u) w[c][m][u] = load16(wc[m][u] + kc * kCode4Bytes + at16);
+      }
+    }
+    for (int turn = 0; turn < W; ++turn) {
+      if (turn == wave && i < g.groups) {
+        if (i > 0) {
+#pragma unroll
+          for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int u = 0; u < U; ++u) acc[m][u] = sums[m][u][lane];
+        }
+        unroll<4>([&](auto c) {
+#pragma unroll
+          for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int u = 0; u < U; ++u) acc[m][u] = mx_mfma<c>(w[c][m][u], x[c][0], x[c][1], acc[m][u], sw[m][u], sx);
+        });
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int u = 0; u < U; ++u) sums[m][u][lane] = acc[m][u];
+      }
+      __syncthreads();
+    }
   }
+  if (wave) return;
 #pragma unroll
   for (int m = 0; m < M; ++m)
 #pragma unroll
-    for (int r = 0; r < U; ++r) part[split][m][r][lane] = acc[m][r];
-  __syncthreads();
-  if (split) return;
-  const int splits = (g.groups + g.per - 1) / g.per;
-  for (int s = 1; s < splits; ++s)
+    for (int u = 0; u < U; ++u) acc[m][u] = sums[m][u][lane];
+  Epi::finish(o, g, unit, lt, acc, lane);
+}
+
+// A wave's 64 x 16 or 64 x 4 bytes from base + offset to LDS at `to` on, in lane order. In assembly,
+// since the compiler would wait for every such copy before any read of LDS; wait_copies() does it.
+__device__ __forceinline__ void copy16(uint32_t to, uint32_t offset, const uint8_t* base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void copy4(uint32_t to, uint32_t offset, const uint8_t* base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory", "m0");
+}
+// Until at most N of the wave's copies are on their way.
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)p));
+}
+
+// Many rows: workgroup of WM x WN waves, A weight tiles by L lane tiles a wave. A chunk's operands
+// (weights 1 KiB, activations 2 KiB a tile) go to a ring of four stages in LDS by
+// global_load_lds, a group's scales beside its first chunk; a wave reads a chunk's fragments while
+// it multiplies the one before.
+template <class Epi, int A, int L, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_pipe(MxGeometry g, typename Epi::Out o, int units, int unit_blocks, int lane_blocks) {
+  constexpr int M = Epi::kMats, U = Epi::kUnit, NW = WM * WN, NS = 4;
+  constexpr int T = A / M;                  // row tiles of a wave
+  constexpr int WA = WM * A, WL = WN * L;   // weight and lane tiles of the workgroup
+  constexpr int kCodes = WA + 2 * WL;       // KiB of a stage
+  constexpr int kScales = WA + WL;          // quarter KiB of a group
+  static_assert(kCodes % NW == 0 && kScales % NW == 0, "copies must split evenly over the waves");
+  constexpr int PC = kCodes / NW, PS = kScales / NW;
+  __shared__ u32x4 ring[NS][kCodes][kWave];
+  __shared__ uint32_t scales[2][kScales][kWave];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  // eight blocks of rows walk the lane blocks together, so that an XCD's workgroups share operands in its L2
+  const int b = xcd_remap(blockIdx.x, gridDim.x);
+  constexpr int G = 8;
+  const int gang = b / (G * lane_blocks), size = min(G, unit_blocks - gang * G), within = b % (G * lane_blocks);
+  const int ub = gang * G + within % size, lb = within / size;
+  const int rt0 = ub * WM * T, lt0 = lb * WL;  // of the workgroup
+
+  const uint8_t *src[PC], *ssrc[PS];
 #pragma unroll
-    for (int m = 0; m < M; ++m)
+  for (int i = 0; i < PC; ++i) {
+    const int j = wave + i * NW;
+    if (j < WA) {
+      const int m = j / (WM * T), t = j % (WM * T);
+      const uint8_t* unused;
+      mx_source<Epi>(g, m, rt0 + t, src[i], unused);
+    } else {
+      const int lt = min(lt0 + (j - WA) / 2, g.lane_groups - 1);
+      src[i] = g.xc + static_cast<int64_t>(lt) * g.groups * 4 * kCode8Bytes + (j - WA) % 2 * 1024;
+    }
+  }
 #pragma unroll
-      for (int r = 0; r < U; ++r) acc[m][r] += part[s][m][r][lane];
-  Epi::apply(o, g, unit * U, lt, acc, lane);
+  for (int i = 0; i < PS; ++i) {
+    const int j = wave + i * NW;
+    if (j < WA) {
+      const int m = j / (WM * T), t = j % (WM * T);
+      const uint8_t* unused;
+      mx_source<Epi>(g, m, rt0 + t, unused, ssrc[i]);
+    } else {
+      ssrc[i] = g.xs + static_cast<int64_t>(min(lt0 + j - WA, g.lane_groups - 1)) * g.groups * kScaleBytes;
+    }
+  }
+  const uint32_t at16 = lane * 16, at4 = lane * 4;
+  const uint32_t ring_at = lds_at(&ring[0][0][0]) + wave * 1024, scales_at = lds_at(&scales[0][0][0]) + wave * 256;
+  auto issue = [&](int stage, auto slot) {
+    if constexpr (slot == 0) {
+#pragma unroll
+      for (int i = 0; i < PS; ++i)
+        copy4(scales_at + ((stage >> 2) & 1) * (kScales * 256) + i * NW * 256, at4, ssrc[i] + static_cast<int64_t>(stage >> 2) * kScaleBytes);
+    }
+#pragma unroll
+    for (int i = 0; i < PC; ++i) {
+      const int64_t step = static_cast<int64_t>(stage) * (wave + i * NW < WA ? kCode4Bytes : kCode8Bytes);
+      copy16(ring_at + (slot * kCodes + i * NW) * 1024, at16, src[i] + step);
+    }
+  };
+
+  f32x4 acc[A][L];
+  u32x4 fa[A], fb[2][L][2];
+  uint32_t sa[2][A], sb[2][L];
+#pragma unroll
+  for (int a = 0; a < A; ++a)
+#pragma unroll
+    for (int l = 0; l < L; ++l) acc[a][l] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // weight tile a of a wave: matrix a / T, row tile a % T
+  auto tile = [&](int a) { return a / T * (WM * T) + wm * T + a % T; };
+  auto read_x = [&](auto buf, auto slot) {
+#pragma unroll
+    for (int l = 0; l < L; ++l) {
+      fb[buf][l][0] = ring[slot][WA + (wn * L + l) * 2][lane];
+      fb[buf][l][1] = ring[slot][WA + (wn * L + l) * 2 + 1][lane];
+    }
+  };
+  auto read_scales = [&](int buf, int group) {
+#pragma unroll
+    for (int a = 0; a < A; ++a) sa[buf][a] = scales[group & 1][tile(a)][lane];
+#pragma unroll
+    for (int l = 0; l < L; ++l) sb[buf][l] = scales[group & 1][WA + wn * L + l][lane];
+  };
+  auto sync = [] {
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  unroll<NS>([&](auto s) { issue(s, s); });
+  wait_copies<3 * PC>();
+  sync();
+#pragma unroll
+  for (int a = 0; a < A; ++a) fa[a] = ring[0][tile(a)][lane];
+  read_x(std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{});
+  read_scales(0, 0);
+
+  // Chunks 4 i .. 4 i + 3 of group i, without a branch, so that the products stay where they are
+  // written.
+  auto group = [&](int i, auto last) {
+    unroll<4>([&](auto c) {
+      constexpr int cur = c & 1, nxt = cur ^ 1;
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      // stage + 1 has landed, and what is being refilled has been read, by every wave
+      if constexpr (!last) {
+        wait_copies<2 * PC + (c == 1 || c == 2 ? PS : 0)>();
+        sync();
+        issue(i * 4 + c + NS, c);
+      } else if constexpr (c < 3) {
+        wait_copies<c == 0 ? 2 * PC : c == 1 ? PC : 0>();
+        sync();
+      }
+      constexpr bool more = !last || c < 3;
+      if constexpr (more) read_x(std::integral_constant<int, nxt>{}, std::integral_constant<int, (c + 1) & 3>{});
+      if constexpr (!last && c == 3) read_scales(1, i + 1);
+      // a weight fragment's register takes the next chunk's behind its last product
+#pragma unroll
+      for (int a = 0; a < A; ++a) {
+#pragma unroll
+        for (int l = 0; l < L; ++l) acc[a][l] = mx_mfma<c>(fa[a], fb[cur][l][0], fb[cur][l][1], acc[a][l], sa[0][a], sb[0][l]);
+        if constexpr (more) fa[a] = ring[(c + 1) & 3][tile(a)][lane];
+      }
+      constexpr int kFirst = more ? 2 * L + (c == 3 ? A + L : 0) : 0;  // x's fragments and scales, among the first products
+      unroll<A>([&](auto q) {
+        __builtin_amdgcn_sched_group_barrier(0x008, L, 0);
+        if constexpr (more) __builtin_amdgcn_sched_group_barrier(0x100, 1 + (q < A / 2 ? (kFirst * 2 + A - 1) / A : 0), 0);
+      });
+    });
+    if constexpr (!last) {
+#pragma unroll
+      for (int a = 0; a < A; ++a) sa[0][a] = sa[1][a];
+#pragma unroll
+      for (int l = 0; l < L; ++l) sb[0][l] = sb[1][l];
+    }
+  };
+  const int end = g.groups - 1;
+  for (int i = 0; i < end; ++i) group(i, std::false_type{});
+  group(end, std::true_type{});
+  // The products end here: without a use in this place the compiler moves them into the branches
+  // below. (The wait covers the longest of them; what follows is no instruction.)
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7");
+#pragma unroll
+  for (int a = 0; a < A; ++a)
+#pragma unroll
+    for (int l = 0; l < L; ++l) asm volatile("" : "+a"(acc[a][l]));
+
+  unroll<T / U>([&](auto r) {
+    unroll<L>([&](auto l) {
+      const int unit = (rt0 + wm * T) / U + r, lt = lt0 + wn * L + l;
+      if (unit >= units || lt >= g.lane_groups) return;
+      f32x4 v[M][U];
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[m][u] = acc[m * T + r * U + u][l];
+      Epi::finish(o, g, unit, lt, v, lane);
+    });
+  });
+}
+
+template <class Epi, int A, int L, int WM, int WN>
+void launch_pipe(const MxGeometry& g, const typename Epi::Out& o, int units, hipStream_t st) {
+  constexpr int per = WM * A / Epi::kMats / Epi::kUnit;
+  const int unit_blocks = (units + per - 1) / per, lane_blocks = (g.lane_groups + WN * L - 1) / (WN * L);
+  hipLaunchKernelGGL((k_mx_pipe<Epi, A, L, WM, WN>), dim3(unit_blocks * lane_blocks), dim3(64 * WM * WN), 0, st, g, o, units, unit_blocks, lane_blocks);
 }
 
 template <class Epi>
 int run(const char* what, const MxGeometry& g, const typename Epi::Out& o, int row_tiles, hipStream_t st) {
   // z is written to the end of its last group of 512 columns
   const int units = Epi::kUnit == 2 ? mx_groups(row_tiles * 16) * (kMxGroup / kMxBlock) : row_tiles;
-  const int64_t groups = static_cast<int64_t>(units) * g.lane_groups;
-  if (groups > INT_MAX) return mx_refused(what, "rows and weights are too large together");
-  hipLaunchKernelGGL((k_mx_simple<Epi>), dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, g, o, units);
+  if (static_cast<int64_t>(units) * g.lane_groups > INT_MAX) return mx_refused(what, "rows and weights are too large together");
+  if (g.lane_groups >= 32) launch_pipe<Epi, 8, 4, 2, 2>(g, o, units, st);
+  else hipLaunchKernelGGL((k_mx_row<Epi, 4>), dim3(units * g.lane_groups), dim3(256), 0, st, g, o, units);
   return mx_launched(what);
 }
 
@@ -187,7 +403,6 @@ const char* operands(const StrideLanes& l, const StrideMxTiles& x, const StrideM
     if (w[i]->tiles > (1 << 26)) return "too many row tiles";
   }
   g.groups = mx_groups(x.cols);
-  g.per = (g.groups + kSplits - 1) / kSplits;
   g.rows = l.rows;
   g.lane_groups = l.lane_groups;
   return nullptr;
