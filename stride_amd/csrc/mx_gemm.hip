@@ -121,13 +121,12 @@ __device__ __forceinline__ void mx_source(const MxGeometry& g, int m, int rt, co
   scales = (which == 0 ? g.ws[0] : which == 1 ? g.ws[1] : g.ws[2]) + static_cast<int64_t>(rt) * g.groups * kScaleBytes;
 }
 
-// One lane tile: workgroup of W waves, one unit. Wave w loads the w-th part of K at once; the sums
-// go from wave to wave through LDS, so that the products chain in ascending order.
-template <class Epi, int W>
-__global__ __launch_bounds__(64 * W) void k_mx_row(MxGeometry g, typename Epi::Out o, int units) {
+// Few output tiles: a wave has one unit by one lane tile, operands straight to registers, P groups of
+// K in use and P on their way.
+template <class Epi, int P>
+__global__ __launch_bounds__(64) void k_mx_row(MxGeometry g, typename Epi::Out o, int units) {
   constexpr int M = Epi::kMats, U = Epi::kUnit;
-  __shared__ f32x4 sums[M][U][kWave];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x;
   const int unit = blockIdx.x % units, lt = blockIdx.x / units;
   const uint8_t *wc[M][U], *ws[M][U];
 #pragma unroll
@@ -142,64 +141,66 @@ __global__ __launch_bounds__(64 * W) void k_mx_row(MxGeometry g, typename Epi::O
   for (int m = 0; m < M; ++m)
 #pragma unroll
     for (int u = 0; u < U; ++u) acc[m][u] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int round = 0; round < g.groups; round += W) {
-    const int i = round + wave;
-    u32x4 w[4][M][U], x[4][2];
-    uint32_t sw[M][U], sx = 0;
-    if (i < g.groups) {
-      sx = *reinterpret_cast<const uint32_t*>(xs + static_cast<int64_t>(i) * kScaleBytes + at4);
+  struct Part {
+    u32x4 w[P][4][M][U], x[P][4][2];
+    uint32_t sw[P][M][U], sx[P];
+  };
+  Part part[2];
+  auto load = [&](Part& t, int first) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const int64_t i = min(first + p, g.groups - 1);
+      t.sx[p] = *reinterpret_cast<const uint32_t*>(xs + i * kScaleBytes + at4);
 #pragma unroll
       for (int m = 0; m < M; ++m)
 #pragma unroll
-        for (int u = 0; u < U; ++u) sw[m][u] = *reinterpret_cast<const uint32_t*>(ws[m][u] + static_cast<int64_t>(i) * kScaleBytes + at4);
+        for (int u = 0; u < U; ++u) t.sw[p][m][u] = *reinterpret_cast<const uint32_t*>(ws[m][u] + i * kScaleBytes + at4);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const int64_t kc = static_cast<int64_t>(i) * 4 + c;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) x[c][h] = load16(xc + kc * kCode8Bytes + h * 1024 + at16);
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
-          for (int u = 0; u < U; ++u) w[c][m][u] = load16(wc[m][u] + kc * kCode4Bytes + at16);
+          for (int u = 0; u < U; ++u) t.w[p][c][m][u] = load16(wc[m][u] + (i * 4 + c) * kCode4Bytes + at16);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) t.x[p][c][h] = load16(xc + (i * 4 + c) * kCode8Bytes + h * 1024 + at16);
       }
     }
-    for (int turn = 0; turn < W; ++turn) {
-      if (turn == wave && i < g.groups) {
-        if (i > 0) {
-#pragma unroll
-          for (int m = 0; m < M; ++m)
-#pragma unroll
-            for (int u = 0; u < U; ++u) acc[m][u] = sums[m][u][lane];
-        }
-        unroll<4>([&](auto c) {
-#pragma unroll
-          for (int m = 0; m < M; ++m)
-#pragma unroll
-            for (int u = 0; u < U; ++u) acc[m][u] = mx_mfma<c>(w[c][m][u], x[c][0], x[c][1], acc[m][u], sw[m][u], sx);
-        });
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto products = [&](const Part& t, int first) {
+    unroll<P>([&](auto p) {
+      if (p > 0 && first + p >= g.groups) return;
+      unroll<4>([&](auto c) {
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
-          for (int u = 0; u < U; ++u) sums[m][u][lane] = acc[m][u];
-      }
-      __syncthreads();
-    }
+          for (int u = 0; u < U; ++u) acc[m][u] = mx_mfma<c>(t.w[p][c][m][u], t.x[p][c][0], t.x[p][c][1], acc[m][u], t.sw[p][m][u], t.sx[p]);
+      });
+    });
+  };
+  load(part[0], 0);
+  for (int i = 0; i < g.groups; i += 2 * P) {
+    if (i + P < g.groups) load(part[1], i + P);
+    products(part[0], i);
+    if (i + 2 * P < g.groups) load(part[0], i + 2 * P);
+    if (i + P < g.groups) products(part[1], i + P);
   }
-  if (wave) return;
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7");
 #pragma unroll
   for (int m = 0; m < M; ++m)
 #pragma unroll
-    for (int u = 0; u < U; ++u) acc[m][u] = sums[m][u][lane];
+    for (int u = 0; u < U; ++u) asm volatile("" : "+v"(acc[m][u]));
   Epi::finish(o, g, unit, lt, acc, lane);
 }
 
 // A wave's 64 x 16 or 64 x 4 bytes from base + offset to LDS at `to` on, in lane order. In assembly,
 // since the compiler would wait for every such copy before any read of LDS; wait_copies() does it.
 __device__ __forceinline__ void copy16(uint32_t to, uint32_t offset, const uint8_t* base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(offset), "s"(base) : "memory", "m0");
 }
 __device__ __forceinline__ void copy4(uint32_t to, uint32_t offset, const uint8_t* base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(offset), "s"(base) : "memory", "m0");
 }
 // Until at most N of the wave's copies are on their way.
 template <int N>
@@ -214,9 +215,9 @@ __device__ __forceinline__ uint32_t lds_at(const void* p) {
 // (weights 1 KiB, activations 2 KiB a tile) go to a ring of four stages in LDS by
 // global_load_lds, a group's scales beside its first chunk; a wave reads a chunk's fragments while
 // it multiplies the one before.
-template <class Epi, int A, int L, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_pipe(MxGeometry g, typename Epi::Out o, int units, int unit_blocks, int lane_blocks) {
-  constexpr int M = Epi::kMats, U = Epi::kUnit, NW = WM * WN, NS = 4;
+template <class Epi, int A, int L, int WM, int WN, int NS, int OCC>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void k_mx_pipe(MxGeometry g, typename Epi::Out o, int units, int unit_blocks, int lane_blocks) {
+  constexpr int M = Epi::kMats, U = Epi::kUnit, NW = WM * WN;
   constexpr int T = A / M;                  // row tiles of a wave
   constexpr int WA = WM * A, WL = WN * L;   // weight and lane tiles of the workgroup
   constexpr int kCodes = WA + 2 * WL;       // KiB of a stage
@@ -260,8 +261,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_pipe(MxGeometry g, typen
   }
   const uint32_t at16 = lane * 16, at4 = lane * 4;
   const uint32_t ring_at = lds_at(&ring[0][0][0]) + wave * 1024, scales_at = lds_at(&scales[0][0][0]) + wave * 256;
-  auto issue = [&](int stage, auto slot) {
-    if constexpr (slot == 0) {
+  auto issue = [&](int stage, int slot, auto with_scales) {
+    if constexpr (with_scales) {
 #pragma unroll
       for (int i = 0; i < PS; ++i)
         copy4(scales_at + ((stage >> 2) & 1) * (kScales * 256) + i * NW * 256, at4, ssrc[i] + static_cast<int64_t>(stage >> 2) * kScaleBytes);
@@ -282,7 +283,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_pipe(MxGeometry g, typen
     for (int l = 0; l < L; ++l) acc[a][l] = f32x4{0.f, 0.f, 0.f, 0.f};
   // weight tile a of a wave: matrix a / T, row tile a % T
   auto tile = [&](int a) { return a / T * (WM * T) + wm * T + a % T; };
-  auto read_x = [&](auto buf, auto slot) {
+  auto read_x = [&](auto buf, int slot) {
 #pragma unroll
     for (int l = 0; l < L; ++l) {
       fb[buf][l][0] = ring[slot][WA + (wn * L + l) * 2][lane];
@@ -300,39 +301,42 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_pipe(MxGeometry g, typen
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  unroll<NS>([&](auto s) { issue(s, s); });
-  wait_copies<3 * PC>();
+  unroll<NS>([&](auto s) { issue(s, s, std::bool_constant<s % 4 == 0>{}); });
+  wait_copies<(NS - 1) * PC>();
   sync();
 #pragma unroll
   for (int a = 0; a < A; ++a) fa[a] = ring[0][tile(a)][lane];
-  read_x(std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{});
+  read_x(std::integral_constant<int, 0>{}, 0);
   read_scales(0, 0);
 
   // Chunks 4 i .. 4 i + 3 of group i, without a branch, so that the products stay where they are
   // written.
+  int at = 0;  // the slot of the stage, where it doesn't follow from c
   auto group = [&](int i, auto last) {
     unroll<4>([&](auto c) {
       constexpr int cur = c & 1, nxt = cur ^ 1;
+      const int slot = 4 % NS == 0 ? c % NS : at, after = 4 % NS == 0 ? (c + 1) % NS : (at + 1 == NS ? 0 : at + 1);
+      at = after;
+      // copies behind those of stage + 1: NS - 2 stages, a group's scales among them
+      constexpr int behind = last ? std::min(NS - 2, std::max(0, 2 - c)) : NS - 2;
+      constexpr bool scaled = !last && c < 4 && c + 2 <= 4 && c + NS - 1 >= 4;
       __builtin_amdgcn_sched_barrier(0);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       // stage + 1 has landed, and what is being refilled has been read, by every wave
-      if constexpr (!last) {
-        wait_copies<2 * PC + (c == 1 || c == 2 ? PS : 0)>();
-        sync();
-        issue(i * 4 + c + NS, c);
-      } else if constexpr (c < 3) {
-        wait_copies<c == 0 ? 2 * PC : c == 1 ? PC : 0>();
+      if constexpr (!last || c < 3) {
+        wait_copies<behind * PC + (scaled ? PS : 0)>();
         sync();
       }
+      if constexpr (!last || c + NS < 4) issue(i * 4 + c + NS, slot, std::bool_constant<(c + NS) % 4 == 0>{});
       constexpr bool more = !last || c < 3;
-      if constexpr (more) read_x(std::integral_constant<int, nxt>{}, std::integral_constant<int, (c + 1) & 3>{});
+      if constexpr (more) read_x(std::integral_constant<int, nxt>{}, after);
       if constexpr (!last && c == 3) read_scales(1, i + 1);
       // a weight fragment's register takes the next chunk's behind its last product
 #pragma unroll
       for (int a = 0; a < A; ++a) {
 #pragma unroll
         for (int l = 0; l < L; ++l) acc[a][l] = mx_mfma<c>(fa[a], fb[cur][l][0], fb[cur][l][1], acc[a][l], sa[0][a], sb[0][l]);
-        if constexpr (more) fa[a] = ring[(c + 1) & 3][tile(a)][lane];
+        if constexpr (more) fa[a] = ring[after][tile(a)][lane];
       }
       constexpr int kFirst = more ? 2 * L + (c == 3 ? A + L : 0) : 0;  // x's fragments and scales, among the first products
       unroll<A>([&](auto q) {
@@ -373,11 +377,138 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_pipe(MxGeometry g, typen
   });
 }
 
-template <class Epi, int A, int L, int WM, int WN>
+// In between: workgroup of WM x WN waves, A weight tiles by L lane tiles a wave; a group of 512
+// columns is a stage, NS - 1 of them on their way.
+template <class Epi, int A, int L, int WM, int WN, int NS>
+__global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxGeometry g, typename Epi::Out o, int units, int unit_blocks, int lane_blocks) {
+  constexpr int M = Epi::kMats, U = Epi::kUnit, NW = WM * WN;
+  constexpr int T = A / M;
+  constexpr int WA = WM * A, WL = WN * L;
+  constexpr int kCodes = 4 * (WA + 2 * WL), kScales = WA + WL;
+  constexpr int PC = (kCodes + NW - 1) / NW, PS = (kScales + NW - 1) / NW;
+  static_assert(kCodes % NW == 0, "copies must split evenly over the waves");
+  __shared__ u32x4 ring[NS][kCodes][kWave];
+  __shared__ uint32_t scales[NS][kScales][kWave];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int b = xcd_remap(blockIdx.x, gridDim.x);
+  const int ub = b / lane_blocks, lb = b % lane_blocks;  // an XCD reads a weight tile once
+  const int rt0 = ub * WM * T, lt0 = lb * WL;
+  const uint8_t *src[PC], *ssrc[PS];
+#pragma unroll
+  for (int i = 0; i < PC; ++i) {
+    const int j = wave + i * NW;
+    if (j < 4 * WA) {
+      const int w = j / 4, m = w / (WM * T), t = w % (WM * T);
+      const uint8_t* unused;
+      mx_source<Epi>(g, m, rt0 + t, src[i], unused);
+      src[i] += j % 4 * kCode4Bytes;
+    } else {
+      const int x = (j - 4 * WA) / 8;
+      src[i] = g.xc + static_cast<int64_t>(min(lt0 + x, g.lane_groups - 1)) * g.groups * 4 * kCode8Bytes + (j - 4 * WA) % 8 * 1024;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PS; ++i) {
+    const int j = min(wave + i * NW, kScales - 1);  // a copy too many goes where it was
+    if (j < WA) {
+      const int m = j / (WM * T), t = j % (WM * T);
+      const uint8_t* unused;
+      mx_source<Epi>(g, m, rt0 + t, unused, ssrc[i]);
+    } else {
+      ssrc[i] = g.xs + static_cast<int64_t>(min(lt0 + j - WA, g.lane_groups - 1)) * g.groups * kScaleBytes;
+    }
+  }
+  const uint32_t at16 = lane * 16, at4 = lane * 4;
+  const uint32_t ring_at = lds_at(&ring[0][0][0]), scales_at = lds_at(&scales[0][0][0]);
+  auto issue = [&](int stage, int slot) {
+#pragma unroll
+    for (int i = 0; i < PS; ++i)
+      copy4(scales_at + (slot * kScales + min(wave + i * NW, kScales - 1)) * 256, at4, ssrc[i] + static_cast<int64_t>(stage) * kScaleBytes);
+#pragma unroll
+    for (int i = 0; i < PC; ++i) {
+      const int64_t step = static_cast<int64_t>(stage) * 4 * (wave + i * NW < 4 * WA ? kCode4Bytes : kCode8Bytes);
+      copy16(ring_at + (slot * kCodes + wave + i * NW) * 1024, at16, src[i] + step);
+    }
+  };
+  f32x4 acc[A][L];
+#pragma unroll
+  for (int a = 0; a < A; ++a)
+#pragma unroll
+    for (int l = 0; l < L; ++l) acc[a][l] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto tile = [&](int a) { return a / T * (WM * T) + wm * T + a % T; };
+  const int first = min(NS - 1, g.groups);
+  for (int i = 0; i < first; ++i) issue(i, i);
+  int slot = 0, next = NS - 1;  // of stage i, of stage i + NS - 1
+  for (int i = 0; i < g.groups; ++i) {
+    // stage i has landed; what is being refilled has been read, by every wave
+    const int ahead = min(NS - 2, g.groups - 1 - i);
+    if (ahead >= NS - 2) wait_copies<(NS - 2) * (PC + PS)>();
+    else if (NS > 4 && ahead == 2) wait_copies<2 * (PC + PS)>();
+    else if (NS > 3 && ahead == 1) wait_copies<PC + PS>();
+    else wait_copies<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (i + NS - 1 < g.groups) issue(i + NS - 1, next);
+    uint32_t sa[A], sb[L];
+#pragma unroll
+    for (int a = 0; a < A; ++a) sa[a] = scales[slot][tile(a)][lane];
+#pragma unroll
+    for (int l = 0; l < L; ++l) sb[l] = scales[slot][WA + wn * L + l][lane];
+    unroll<4>([&](auto c) {
+      u32x4 fa[A], fb[L][2];
+#pragma unroll
+      for (int l = 0; l < L; ++l)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) fb[l][h] = ring[slot][4 * WA + (wn * L + l) * 8 + c * 2 + h][lane];
+#pragma unroll
+      for (int a = 0; a < A; ++a) fa[a] = ring[slot][tile(a) * 4 + c][lane];
+#pragma unroll
+      for (int a = 0; a < A; ++a)
+#pragma unroll
+        for (int l = 0; l < L; ++l) acc[a][l] = mx_mfma<c>(fa[a], fb[l][0], fb[l][1], acc[a][l], sa[a], sb[l]);
+    });
+    slot = slot + 1 == NS ? 0 : slot + 1;
+    next = next + 1 == NS ? 0 : next + 1;
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7");
+#pragma unroll
+  for (int a = 0; a < A; ++a)
+#pragma unroll
+    for (int l = 0; l < L; ++l) asm volatile("" : "+v"(acc[a][l]));
+  unroll<T / U>([&](auto r) {
+    unroll<L>([&](auto l) {
+      const int unit = (rt0 + wm * T) / U + r, lt = lt0 + wn * L + l;
+      if (unit >= units || lt >= g.lane_groups) return;
+      f32x4 v[M][U];
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[m][u] = acc[m * T + r * U + u][l];
+      Epi::finish(o, g, unit, lt, v, lane);
+    });
+  });
+}
+
+template <class Epi, int P>
+void launch_row(const MxGeometry& g, const typename Epi::Out& o, int units, hipStream_t st) {
+  hipLaunchKernelGGL((k_mx_row<Epi, P>), dim3(units * g.lane_groups), dim3(64), 0, st, g, o, units);
+}
+
+template <class Epi, int A, int L, int WM, int WN, int NS, int OCC>
 void launch_pipe(const MxGeometry& g, const typename Epi::Out& o, int units, hipStream_t st) {
   constexpr int per = WM * A / Epi::kMats / Epi::kUnit;
   const int unit_blocks = (units + per - 1) / per, lane_blocks = (g.lane_groups + WN * L - 1) / (WN * L);
-  hipLaunchKernelGGL((k_mx_pipe<Epi, A, L, WM, WN>), dim3(unit_blocks * lane_blocks), dim3(64 * WM * WN), 0, st, g, o, units, unit_blocks, lane_blocks);
+  hipLaunchKernelGGL((k_mx_pipe<Epi, A, L, WM, WN, NS, OCC>), dim3(unit_blocks * lane_blocks), dim3(64 * WM * WN), 0, st, g, o, units, unit_blocks, lane_blocks);
+}
+
+template <class Epi, int A, int L, int WM, int WN, int NS>
+void launch_tile(const MxGeometry& g, const typename Epi::Out& o, int units, hipStream_t st) {
+  constexpr int per = WM * A / Epi::kMats / Epi::kUnit;
+  const int unit_blocks = (units + per - 1) / per, lane_blocks = (g.lane_groups + WN * L - 1) / (WN * L);
+  hipLaunchKernelGGL((k_mx_tile<Epi, A, L, WM, WN, NS>), dim3(unit_blocks * lane_blocks), dim3(64 * WM * WN), 0, st, g, o, units, unit_blocks, lane_blocks);
 }
 
 template <class Epi>
@@ -385,8 +516,24 @@ int run(const char* what, const MxGeometry& g, const typename Epi::Out& o, int r
   // z is written to the end of its last group of 512 columns
   const int units = Epi::kUnit == 2 ? mx_groups(row_tiles * 16) * (kMxGroup / kMxBlock) : row_tiles;
   if (static_cast<int64_t>(units) * g.lane_groups > INT_MAX) return mx_refused(what, "rows and weights are too large together");
-  if (g.lane_groups >= 32) launch_pipe<Epi, 8, 4, 2, 2>(g, o, units, st);
-  else hipLaunchKernelGGL((k_mx_row<Epi, 4>), dim3(units * g.lane_groups), dim3(256), 0, st, g, o, units);
+  // configuration
+  // By the number of 16 x 16 products, of which the card's 256 CUs want four each before tiles pay.
+  // Measured at 1 to 4096 rows of weights from 512 x 512 to 14336 x 4096, us here / as the next form:
+  //   waves of their own to 768 (gate and up, whose waves have four products: 2048), 1536 where K is
+  //     short: 2048 x 8192 at 1 / 64 rows 5.5 / 6.9 against 10 / 8.2 as 32 x 32 tiles, at 128 rows
+  //     9.5 against 8.4; 8192 x 2048 at 32 rows 4.1 against 4.9
+  //   32 x 32 to 1536: 4096 x 14336 at 64 rows 12.1 against 19 as 64 x 64
+  //   64 x 64 to 6144: 2048 x 8192 at 512 rows 13 against 17.4 as 128 x 64, 4096 x 4096 12.2 against 12.1
+  //   128 x 64 to 20480: 2048 x 8192 at 1024 rows 20.8 against 32.7 as 128 x 128, 8192 x 2048 22.2
+  //     against 21.3 at 32768
+  //   128 x 128: 14336 x 4096 at 2048 rows 105 against 113
+  const int64_t products = static_cast<int64_t>(row_tiles) * Epi::kMats * g.lane_groups;
+  if (products <= (Epi::kMats == 2 ? 2048 : g.groups <= 4 ? 1536 : 768)) launch_row<Epi, 4 / Epi::kMats>(g, o, units, st);
+  else if (Epi::kMats == 1 && products <= 1536) {
+    if constexpr (Epi::kMats == 1) launch_tile<Epi, 1, 1, 2, 2, 3>(g, o, units, st);
+  } else if (products <= 6144) launch_pipe<Epi, 4, 1, 1, 4, 4, 2>(g, o, units, st);
+  else if (products <= 20480) launch_pipe<Epi, 4, 2, 2, 2, 4, 2>(g, o, units, st);
+  else launch_pipe<Epi, 4, 4, 2, 2, 3, 2>(g, o, units, st);
   return mx_launched(what);
 }
 
