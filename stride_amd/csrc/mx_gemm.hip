@@ -261,17 +261,18 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_mx_pipe(MxGeometry g, typ
   }
   const uint32_t at16 = lane * 16, at4 = lane * 4;
   const uint32_t ring_at = lds_at(&ring[0][0][0]) + wave * 1024, scales_at = lds_at(&scales[0][0][0]) + wave * 256;
-  auto issue = [&](int stage, int slot, auto with_scales) {
-    if constexpr (with_scales) {
-#pragma unroll
-      for (int i = 0; i < PS; ++i)
-        copy4(scales_at + ((stage >> 2) & 1) * (kScales * 256) + i * NW * 256, at4, ssrc[i] + static_cast<int64_t>(stage >> 2) * kScaleBytes);
-    }
-#pragma unroll
-    for (int i = 0; i < PC; ++i) {
-      const int64_t step = static_cast<int64_t>(stage) * (wave + i * NW < WA ? kCode4Bytes : kCode8Bytes);
-      copy16(ring_at + (slot * kCodes + i * NW) * 1024, at16, src[i] + step);
-    }
+  // copies [FROM, TO) of a stage, the scales' first where a group begins
+  auto issue = [&](int stage, int slot, auto with_scales, auto from, auto to) {
+    constexpr int lead = with_scales ? PS : 0;
+    unroll<to - from>([&](auto n) {
+      constexpr int i = from + n - lead;
+      if constexpr (i < 0) {
+        copy4(scales_at + ((stage >> 2) & 1) * (kScales * 256) + (i + lead) * NW * 256, at4, ssrc[i + lead] + static_cast<int64_t>(stage >> 2) * kScaleBytes);
+      } else {
+        const int64_t step = static_cast<int64_t>(stage) * (wave + i * NW < WA ? kCode4Bytes : kCode8Bytes);
+        copy16(ring_at + (slot * kCodes + i * NW) * 1024, at16, src[i] + step);
+      }
+    });
   };
 
   f32x4 acc[A][L];
@@ -283,31 +284,28 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_mx_pipe(MxGeometry g, typ
     for (int l = 0; l < L; ++l) acc[a][l] = f32x4{0.f, 0.f, 0.f, 0.f};
   // weight tile a of a wave: matrix a / T, row tile a % T
   auto tile = [&](int a) { return a / T * (WM * T) + wm * T + a % T; };
-  auto read_x = [&](auto buf, int slot) {
-#pragma unroll
-    for (int l = 0; l < L; ++l) {
-      fb[buf][l][0] = ring[slot][WA + (wn * L + l) * 2][lane];
-      fb[buf][l][1] = ring[slot][WA + (wn * L + l) * 2 + 1][lane];
-    }
-  };
-  auto read_scales = [&](int buf, int group) {
-#pragma unroll
-    for (int a = 0; a < A; ++a) sa[buf][a] = scales[group & 1][tile(a)][lane];
-#pragma unroll
-    for (int l = 0; l < L; ++l) sb[buf][l] = scales[group & 1][WA + wn * L + l][lane];
+  // the n-th fragment of x, the n-th word of scales
+  auto read_x = [&](auto buf, int slot, auto n) { fb[buf][n / 2][n % 2] = ring[slot][WA + wn * L * 2 + n][lane]; };
+  auto read_scale = [&](int buf, int group, auto n) {
+    if constexpr (n < A) sa[buf][n] = scales[group & 1][tile(n)][lane];
+    else sb[buf][n - A] = scales[group & 1][WA + wn * L + n - A][lane];
   };
   auto sync = [] {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  unroll<NS>([&](auto s) { issue(s, s, std::bool_constant<s % 4 == 0>{}); });
+  using Zero = std::integral_constant<int, 0>;
+  unroll<NS>([&](auto s) {
+    constexpr bool first = s % 4 == 0;
+    issue(s, s, std::bool_constant<first>{}, Zero{}, std::integral_constant<int, PC + (first ? PS : 0)>{});
+  });
   wait_copies<(NS - 1) * PC>();
   sync();
+  unroll<2 * L>([&](auto n) { read_x(Zero{}, 0, n); });
+  unroll<A + L>([&](auto n) { read_scale(0, 0, n); });
 #pragma unroll
   for (int a = 0; a < A; ++a) fa[a] = ring[0][tile(a)][lane];
-  read_x(std::integral_constant<int, 0>{}, 0);
-  read_scales(0, 0);
 
   // Chunks 4 i .. 4 i + 3 of group i, without a branch, so that the products stay where they are
   // written.
@@ -320,29 +318,41 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_mx_pipe(MxGeometry g, typ
       // copies behind those of stage + 1: NS - 2 stages, a group's scales among them
       constexpr int behind = last ? std::min(NS - 2, std::max(0, 2 - c)) : NS - 2;
       constexpr bool scaled = !last && c < 4 && c + 2 <= 4 && c + NS - 1 >= 4;
-      __builtin_amdgcn_sched_barrier(0);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      // stage + 1 has landed, and what is being refilled has been read, by every wave
-      if constexpr (!last || c < 3) {
-        wait_copies<behind * PC + (scaled ? PS : 0)>();
-        sync();
-      }
-      if constexpr (!last || c + NS < 4) issue(i * 4 + c + NS, slot, std::bool_constant<(c + NS) % 4 == 0>{});
-      constexpr bool more = !last || c < 3;
-      if constexpr (more) read_x(std::integral_constant<int, nxt>{}, after);
-      if constexpr (!last && c == 3) read_scales(1, i + 1);
-      // a weight fragment's register takes the next chunk's behind its last product
-#pragma unroll
-      for (int a = 0; a < A; ++a) {
+      constexpr bool more = !last || c < 3, copies = !last || c + NS < 4, starts = (c + NS) % 4 == 0;
+      // A step has the products of a weight fragment. Behind the first ones lies the barrier, and in
+      // the others the next chunk's fragments are read and a stage is copied to the slot of this one,
+      // a few at a time, so that the matrix unit never waits for long.
+      constexpr int kOpen = A / 4, kSteps = A - kOpen;
+      unroll<A>([&](auto a) {
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (a == kOpen && more) {
+          // stage + 1 has landed, and what is being refilled has been read, by every wave
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          wait_copies<behind * PC + (scaled ? PS : 0)>();
+          sync();
+        }
+        if constexpr (a >= kOpen) {
+          constexpr int n = a - kOpen;
+          if constexpr (more) {
+            constexpr int x0 = 2 * L * n / kSteps, x1 = 2 * L * (n + 1) / kSteps;
+            unroll<x1 - x0>([&](auto i) { read_x(std::integral_constant<int, nxt>{}, after, std::integral_constant<int, x0 + i>{}); });
+            constexpr int w0 = n == 0 ? 0 : a - 1;
+            unroll<a - w0>([&](auto i) { fa[w0 + i] = ring[after][tile(w0 + i)][lane]; });
+          }
+          if constexpr (!last && c == 3) {
+            constexpr int s0 = (A + L) * n / kSteps, s1 = (A + L) * (n + 1) / kSteps;
+            unroll<s1 - s0>([&](auto q) { read_scale(1, i + 1, std::integral_constant<int, s0 + q>{}); });
+          }
+          if constexpr (copies) {
+            constexpr int all = PC + (starts ? PS : 0);
+            issue(i * 4 + c + NS, slot, std::bool_constant<starts>{}, std::integral_constant<int, all * n / kSteps>{},
+                  std::integral_constant<int, all * (n + 1) / kSteps>{});
+          }
+        }
 #pragma unroll
         for (int l = 0; l < L; ++l) acc[a][l] = mx_mfma<c>(fa[a], fb[cur][l][0], fb[cur][l][1], acc[a][l], sa[0][a], sb[0][l]);
-        if constexpr (more) fa[a] = ring[after][tile(a)][lane];
-      }
-      constexpr int kFirst = more ? 2 * L + (c == 3 ? A + L : 0) : 0;  // x's fragments and scales, among the first products
-      unroll<A>([&](auto q) {
-        __builtin_amdgcn_sched_group_barrier(0x008, L, 0);
-        if constexpr (more) __builtin_amdgcn_sched_group_barrier(0x100, 1 + (q < A / 2 ? (kFirst * 2 + A - 1) / A : 0), 0);
       });
+      if constexpr (more) fa[A - 1] = ring[after][tile(A - 1)][lane];
     });
     if constexpr (!last) {
 #pragma unroll
@@ -450,24 +460,27 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxGeometry g, typename
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (i + NS - 1 < g.groups) issue(i + NS - 1, next);
     uint32_t sa[A], sb[L];
+    u32x4 fa[4][A], fb[4][L][2];
 #pragma unroll
     for (int a = 0; a < A; ++a) sa[a] = scales[slot][tile(a)][lane];
 #pragma unroll
     for (int l = 0; l < L; ++l) sb[l] = scales[slot][WA + wn * L + l][lane];
-    unroll<4>([&](auto c) {
-      u32x4 fa[A], fb[L][2];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
 #pragma unroll
       for (int l = 0; l < L; ++l)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) fb[l][h] = ring[slot][4 * WA + (wn * L + l) * 8 + c * 2 + h][lane];
+        for (int h = 0; h < 2; ++h) fb[c][l][h] = ring[slot][4 * WA + (wn * L + l) * 8 + c * 2 + h][lane];
 #pragma unroll
-      for (int a = 0; a < A; ++a) fa[a] = ring[slot][tile(a) * 4 + c][lane];
+      for (int a = 0; a < A; ++a) fa[c][a] = ring[slot][tile(a) * 4 + c][lane];
+    }
+    if (i + NS - 1 < g.groups) issue(i + NS - 1, next);  // while the fragments are on their way
+    unroll<4>([&](auto c) {
 #pragma unroll
       for (int a = 0; a < A; ++a)
 #pragma unroll
-        for (int l = 0; l < L; ++l) acc[a][l] = mx_mfma<c>(fa[a], fb[l][0], fb[l][1], acc[a][l], sa[a], sb[l]);
+        for (int l = 0; l < L; ++l) acc[a][l] = mx_mfma<c>(fa[c][a], fb[c][l][0], fb[c][l][1], acc[a][l], sa[a], sb[l]);
     });
     slot = slot + 1 == NS ? 0 : slot + 1;
     next = next + 1 == NS ? 0 : next + 1;
@@ -521,19 +534,23 @@ int run(const char* what, const MxGeometry& g, const typename Epi::Out& o, int r
   // Measured at 1 to 4096 rows of weights from 512 x 512 to 14336 x 4096, us here / as the next form:
   //   waves of their own to 768 (gate and up, whose waves have four products: 2048), 1536 where K is
   //     short: 2048 x 8192 at 1 / 64 rows 5.5 / 6.9 against 10 / 8.2 as 32 x 32 tiles, at 128 rows
-  //     9.5 against 8.4; 8192 x 2048 at 32 rows 4.1 against 4.9
+  //     9.6 against 8.3; 8192 x 2048 at 32 rows 4.1 against 4.9
   //   32 x 32 to 1536: 4096 x 14336 at 64 rows 12.1 against 19 as 64 x 64
-  //   64 x 64 to 6144: 2048 x 8192 at 512 rows 13 against 17.4 as 128 x 64, 4096 x 4096 12.2 against 12.1
-  //   128 x 64 to 20480: 2048 x 8192 at 1024 rows 20.8 against 32.7 as 128 x 128, 8192 x 2048 22.2
-  //     against 21.3 at 32768
-  //   128 x 128: 14336 x 4096 at 2048 rows 105 against 113
+  //   64 x 64 to 6144: 2048 x 8192 at 512 rows 13.6 against 15.5 as 128 x 64, at 1024 22.2 against 17.6
+  //   128 x 64 to 20480: 2048 x 8192 at 2048 rows 32.6 against 36.5 as 128 x 128, 8192 x 2048 40.7
+  //     against 37.4
+  //   128 x 128, two workgroups a CU whose ends hide each other: gate and up 8192 x 2048 at 2048 rows
+  //     62 against 68 as 256 x 128
+  //   256 x 128 where K is long and every CU has one: the fewest bytes a product, by which the clock
+  //     stays up: 2048 x 8192 at 4096 rows 54 against 60 as 128 x 128, 4096 x 14336 166 against 192
   const int64_t products = static_cast<int64_t>(row_tiles) * Epi::kMats * g.lane_groups;
   if (products <= (Epi::kMats == 2 ? 2048 : g.groups <= 4 ? 1536 : 768)) launch_row<Epi, 4 / Epi::kMats>(g, o, units, st);
   else if (Epi::kMats == 1 && products <= 1536) {
     if constexpr (Epi::kMats == 1) launch_tile<Epi, 1, 1, 2, 2, 3>(g, o, units, st);
   } else if (products <= 6144) launch_pipe<Epi, 4, 1, 1, 4, 4, 2>(g, o, units, st);
   else if (products <= 20480) launch_pipe<Epi, 4, 2, 2, 2, 4, 2>(g, o, units, st);
-  else launch_pipe<Epi, 4, 4, 2, 2, 3, 2>(g, o, units, st);
+  else if (products < 32768 || g.groups < 16) launch_pipe<Epi, 4, 4, 2, 2, 3, 2>(g, o, units, st);
+  else launch_pipe<Epi, 8, 4, 2, 2, 4, 1>(g, o, units, st);
   return mx_launched(what);
 }
 

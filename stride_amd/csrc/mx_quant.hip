@@ -2,9 +2,9 @@
 // residual's addition (include/stride_mx.h). All of them move each value once and are bound by
 // memory.
 //
-// A wave has 4 rows of a chunk of 128 columns: lane l the 8 columns 8 * (l % 2) of tile l / 8, row
-// l / 2 % 4, so that eight lanes read neighbouring 16-column pieces of the rows. A block of 32 is
-// then the two tiles of lanes that differ in bits 0 and 3.
+// A wave has R = 1, 2 or 4 rows of 4 / R chunks of 128 columns: a lane has 8 columns, half l % 2 of
+// tile l / (2 R), row l / 2 % R, so that 2 R lanes read neighbouring 16-column pieces of the rows. A
+// block of 32 is then the two tiles of lanes that differ in bits 0 and 2 R.
 #include <hip/hip_runtime.h>
 
 #include <climits>
@@ -15,29 +15,32 @@
 namespace stride_tc {
 namespace {
 
-struct Spot {  // a lane's place in its wave's 4 x 128 values
-  int row, tile, half;
+template <int R>
+struct Spot {  // a lane's place in its wave's values
+  int row, chunk, tile, half;
   __device__ __forceinline__ Spot() {
     const int l = threadIdx.x & 63;
     half = l & 1;
-    row = (l >> 1) & 3;
-    tile = l >> 3;
+    row = (l >> 1) % R;
+    tile = l / (2 * R) & 7;
+    chunk = l / (16 * R);
   }
 };
 
+template <int R>
 __device__ __forceinline__ uint32_t block_most(const float (&v)[8]) {
   uint32_t m = mx_abs_bits(v[0]);
 #pragma unroll
   for (int i = 1; i < 8; ++i) m = max(m, mx_abs_bits(v[i]));
   m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 1)));
-  return max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 8)));
+  return max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 2 * R)));
 }
 
-// The wave's values of chunk kc, rows `row` + ... of tile t, to codes and scales.
-template <int BITS>
-__device__ __forceinline__ void store_block(const StrideMxTiles& out, int t, int kc, int row, const Spot& s, const float (&v)[8], bool live) {
+// A lane's values of chunk kc, row `row` of tile t, to codes and scales. Whole waves call it.
+template <int BITS, int R>
+__device__ __forceinline__ void store_block(const StrideMxTiles& out, int t, int kc, int row, const Spot<R>& s, const float (&v)[8], bool live) {
   const int groups = mx_groups(out.cols);
-  const int byte = mx_scale_byte<BITS>(block_most(v));
+  const int byte = mx_scale_byte<BITS>(block_most<R>(v));
   const float inverse = mx_inverse(byte);
   if (!live) return;
   const int64_t chunk = static_cast<int64_t>(t) * groups * 4 + kc;
@@ -70,7 +73,7 @@ __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
 // Workgroup: chunk blockIdx.x of tile blockIdx.y + ..., a wave for each four rows.
 template <int BITS, class T>
 __global__ __launch_bounds__(256) void k_quantize(const T* src, StrideMxTiles out, int rows, int chunks) {
-  const Spot s;
+  const Spot<4> s;
   const int kc = blockIdx.x % chunks, t = blockIdx.x / chunks, row = (threadIdx.x >> 6) * 4 + s.row;
   const int col_tiles = out.cols >> 4, ct = kc * 8 + s.tile;
   const bool live = t * 16 + row < rows;
@@ -116,24 +119,27 @@ __global__ __launch_bounds__(256) void k_dequantize(StrideMxTiles in, T* out, in
     u32x4 w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = bf16_rne(v[2 * i]) | bf16_rne(v[2 * i + 1]) << 16;
-    *reinterpret_cast<u32x4*>(o) = w;
+    __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(o));
   }
 }
 
-// Workgroup: four rows of a lane tile. Wave w has chunks w, w + waves, ...; a lane's values stay in
-// registers between the sum and the scaling (IT chunks of 8; 0: h is read again). The order of a
-// row's sum follows from dim alone: lanes' chunks ascending, lanes by halves, waves ascending.
-template <int IT, bool ADD, bool MX>
+// Workgroup: R rows of a lane tile; a lane's values stay in registers between the sum and the
+// scaling (IT places; 0: h is read again). A row's sum has the same order for every R: a chunk's
+// pieces of 8 by halves and tiles, then its chunks 16 apart ascending, and those by halves again.
+template <int R, int IT, bool ADD, bool MX>
 __global__ __launch_bounds__(1024) void k_mx_norm(StrideMxNormParams p, int chunks) {
-  __shared__ float sums[16][4];
-  const Spot s;
-  const int t = blockIdx.x >> 2, row = (blockIdx.x & 3) * 4 + s.row;
-  const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  extern __shared__ float sums[];  // [R][chunks]
+  const Spot<R> s;
+  constexpr int per = 4 / R;  // chunks of a wave
+  const int t = blockIdx.x / (16 / R), row = blockIdx.x % (16 / R) * R + s.row;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int col_tiles = p.dim >> 4;
   const bool live = t * 16 + row < p.l.rows;
   const int64_t at = static_cast<int64_t>(t) * col_tiles * kTileElems + row * 16 + s.half * 8;
   float v[IT ? IT : 1][8];
-  float sum = 0.0f;
+  constexpr bool kEarly = IT == 1 || IT == 2;  // the gains come beside the values
+  float gain[kEarly ? IT : 1][8];
+  auto chunk_of = [&](int i) { return (wave + i * waves) * per + s.chunk; };
   auto fetch = [&](int kc, float (&x)[8], bool again) {
     const int ct = kc * 8 + s.tile;
 #pragma unroll
@@ -150,38 +156,44 @@ __global__ __launch_bounds__(1024) void k_mx_norm(StrideMxNormParams p, int chun
       reinterpret_cast<f32x4*>(h)[1] = f32x4{x[4], x[5], x[6], x[7]};
     }
   };
-  auto square = [&](const float (&x)[8]) {
+  auto square = [&](int kc, const float (&x)[8]) {
+    float sum = x[0] * x[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+    for (int i = 1; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+#pragma unroll
+    for (int d : {1, 2 * R, 4 * R, 8 * R}) sum += __shfl_xor(sum, d);
+    if (!s.half && s.tile == 0 && kc < chunks) sums[s.row * chunks + kc] = sum;
   };
   if constexpr (IT > 0) {
 #pragma unroll
-    for (int i = 0; i < IT; ++i) fetch(wave + i * waves, v[i], false);
+    for (int i = 0; i < IT; ++i) fetch(chunk_of(i), v[i], false);
+    if constexpr (kEarly) {
 #pragma unroll
-    for (int i = 0; i < IT; ++i) square(v[i]);
+      for (int i = 0; i < IT; ++i) load8(p.weight + min(chunk_of(i) * 8 + s.tile, col_tiles - 1) * 16 + s.half * 8, gain[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < IT; ++i) square(chunk_of(i), v[i]);
   } else {
-    for (int kc = wave; kc < chunks; kc += waves) {
-      fetch(kc, v[0], false);
-      square(v[0]);
+    for (int i = 0; i * waves * per < chunks; ++i) {
+      fetch(chunk_of(i), v[0], false);
+      square(chunk_of(i), v[0]);
     }
   }
-#pragma unroll
-  for (int d : {1, 8, 16, 32}) sum += __shfl_xor(sum, d);
-  if ((threadIdx.x & 63) < 8 && !s.half) sums[wave][s.row] = sum;
   __syncthreads();
-  sum = 0.0f;
-  for (int w = 0; w < waves; ++w) sum += sums[w][s.row];
-  const float r = 1.0f / sqrtf(sum / static_cast<float>(p.dim) + p.eps);
-  auto scale = [&](int kc, float (&x)[8]) {
+  float sum = 0.0f;  // sixteen lanes a row
+  for (int c = lane & 15; c < chunks; c += 16) sum += sums[((lane >> 4) % R) * chunks + c];
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor(sum, d);
+  const float inverse = __shfl(1.0f / sqrtf(sum / static_cast<float>(p.dim) + p.eps), s.row * 16);
+  auto scale = [&](int kc, float (&x)[8], float (&g)[8]) {
     const int ct = kc * 8 + s.tile;
     if (ct < col_tiles) {
-      float g[8];
-      load8(p.weight + ct * 16 + s.half * 8, g);
+      if constexpr (!kEarly) load8(p.weight + ct * 16 + s.half * 8, g);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = g[i] * (x[i] * r);
+      for (int i = 0; i < 8; ++i) x[i] = g[i] * (x[i] * inverse);
     }
     if constexpr (MX) {
-      if (kc < chunks) store_block<8>(p.out, t, kc, row, s, x, live);
+      store_block<8>(p.out, t, kc, row, s, x, live && kc < chunks);
     } else if (live && ct < col_tiles) {
       u32x4 w;
 #pragma unroll
@@ -191,23 +203,33 @@ __global__ __launch_bounds__(1024) void k_mx_norm(StrideMxNormParams p, int chun
   };
   if constexpr (IT > 0) {
 #pragma unroll
-    for (int i = 0; i < IT; ++i) scale(wave + i * waves, v[i]);
+    for (int i = 0; i < IT; ++i) scale(chunk_of(i), v[i], gain[kEarly ? i : 0]);
   } else {
-    for (int kc = wave; kc < chunks; kc += waves) {
-      fetch(kc, v[0], true);
-      scale(kc, v[0]);
+    for (int i = 0; i * waves * per < chunks; ++i) {
+      fetch(chunk_of(i), v[0], true);
+      scale(chunk_of(i), v[0], gain[0]);
     }
   }
 }
 
-template <int IT>
+template <int R, int IT>
 void launch_norm(const StrideMxNormParams& p, int chunks, int waves, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(p.l.rows) + 3) / 4)), block(waves * 64);
+  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(p.l.rows) + R - 1) / R)), block(waves * 64);
+  const unsigned lds = R * chunks * sizeof(float);
   const bool mx = p.out.codes != nullptr;
-  if (p.add && mx) hipLaunchKernelGGL((k_mx_norm<IT, true, true>), grid, block, 0, st, p, chunks);
-  else if (p.add) hipLaunchKernelGGL((k_mx_norm<IT, true, false>), grid, block, 0, st, p, chunks);
-  else if (mx) hipLaunchKernelGGL((k_mx_norm<IT, false, true>), grid, block, 0, st, p, chunks);
-  else hipLaunchKernelGGL((k_mx_norm<IT, false, false>), grid, block, 0, st, p, chunks);
+  if (p.add && mx) hipLaunchKernelGGL((k_mx_norm<R, IT, true, true>), grid, block, lds, st, p, chunks);
+  else if (p.add) hipLaunchKernelGGL((k_mx_norm<R, IT, true, false>), grid, block, lds, st, p, chunks);
+  else if (mx) hipLaunchKernelGGL((k_mx_norm<R, IT, false, true>), grid, block, lds, st, p, chunks);
+  else hipLaunchKernelGGL((k_mx_norm<R, IT, false, false>), grid, block, lds, st, p, chunks);
+}
+
+template <int R>
+void launch_norm(const StrideMxNormParams& p, int chunks, hipStream_t st) {
+  const int places = (chunks * R + 3) / 4, waves = places < 16 ? places : 16, rounds = (places + waves - 1) / waves;
+  if (rounds == 1) launch_norm<R, 1>(p, chunks, waves, st);
+  else if (rounds == 2) launch_norm<R, 2>(p, chunks, waves, st);
+  else if (rounds <= 4) launch_norm<R, 4>(p, chunks, waves, st);
+  else launch_norm<R, 0>(p, chunks, waves, st);
 }
 
 }  // namespace
@@ -287,12 +309,14 @@ int stride_mx_norm(const StrideMxNormParams* p, void* stream) {
     if (const char* why = mx_why_not(p->out, p->l.lane_groups, p->dim)) return mx_refused(what, why);
   if ((reinterpret_cast<uintptr_t>(p->h) | reinterpret_cast<uintptr_t>(p->add) | reinterpret_cast<uintptr_t>(p->weight) | reinterpret_cast<uintptr_t>(p->x)) % 16)
     return mx_refused(what, "pointers must be 16-byte aligned");
-  const int chunks = mx_groups(p->dim) * 4, waves = chunks < 16 ? chunks : 16, rounds = (chunks + waves - 1) / waves;
+  const int chunks = mx_groups(p->dim) * 4;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (rounds == 1) launch_norm<1>(*p, chunks, waves, st);
-  else if (rounds == 2) launch_norm<2>(*p, chunks, waves, st);
-  else if (rounds <= 4) launch_norm<4>(*p, chunks, waves, st);
-  else launch_norm<0>(*p, chunks, waves, st);
+  // A row a workgroup where rows are few, more where the reads are many, since neighbouring rows share
+  // their lines (us at R = 1 / 2 / 4 with an addition: 1 x 2048 2.7 / 2.9 / 3.7, 333 x 8192 15.9 / 9.7 /
+  // 12, 1024 x 2048 11.5 / 7.7 / 6.9, 4096 x 2048 37 / 24.6 / 19.9, 92 MB: 4.7 TB/s, a 4 GiB copy's 4.8).
+  if (p->l.rows <= 32) launch_norm<1>(*p, chunks, st);
+  else if (p->l.rows <= 512) launch_norm<2>(*p, chunks, st);
+  else launch_norm<4>(*p, chunks, st);
   return mx_launched(what);
 }
 

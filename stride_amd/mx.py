@@ -20,7 +20,7 @@ from struct import Struct
 import torch
 
 from . import _lib, tc
-from .harness import PagedKv, here, other_stream
+from .harness import PagedKv, other_stream
 
 _TILES = Struct("<2Q2i").pack
 _QUANTIZE = Struct("<4iQ24s2i").pack
@@ -32,6 +32,7 @@ _QKV = Struct("<4i24s24s24s24sQq56s3Q2i").pack
 _NONE = _TILES(0, 0, 0, 0)
 
 BLOCK, CHUNK, GROUP = 32, 128, 512  # columns of a scale, of a matrix instruction, of a lane's word of scales
+_BF16 = (torch.int16, torch.bfloat16)  # or its bits
 _PARTS = {4: (4, 16, 16), 8: (2, 4, 16, 16)}  # a chunk's codes
 
 
@@ -75,6 +76,13 @@ def _check(rc: int) -> None:
         _lib.check(rc)
 
 
+def _here(dev: int) -> int:
+    """The stream of a launch for tensors of device `dev`, which has to be the current one."""
+    if dev != torch._C._cuda_getDevice() or dev < 0:
+        raise ValueError(f"tensors are on device {dev}, the current one is {torch._C._cuda_getDevice()}")
+    return torch._C._cuda_getCurrentRawStream(dev) if tc._stream is None else tc.kernel_stream()
+
+
 def _operand(t, bits: int, rows: int, dev: int, cols: int, name: str) -> bytes:
     """A Tiles argument's block, looked over (cols 0: any)."""
     if not isinstance(t, Tiles) or t.bits != bits or t._device != dev or t.tiles * 16 < rows or (cols and t.cols != cols):
@@ -94,29 +102,28 @@ def _allocates() -> None:
         raise ValueError("with another stream set by set_kernel_stream, pass out")
 
 
-def _tile_shape(t, rows: int, name: str):
-    if t.dim() != 4 or t.shape[2] != 16 or t.shape[3] != 16 or not t.is_contiguous() or t.shape[0] * 16 < rows or t.shape[1] < 1:
+def _tile_cols(t, rows: int, name: str) -> int:
+    """Columns of tiles [ceil(rows / 16)][cols / 16][16][16]."""
+    shape = t.shape
+    if len(shape) != 4 or shape[2] != 16 or shape[3] != 16 or shape[0] * 16 < rows or shape[1] < 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous tiles [ceil(rows / 16)][cols / 16][16][16]")
+    return shape[1] * 16
 
 
 def _y_tiles(out, rows: int, cols: int, device, dev: int):
     """bf16 x tiles that are written."""
-    T = (rows + 15) // 16
     if out is None:
         _allocates()
-        return torch.zeros((T, cols // 16, 16, 16), dtype=torch.int16, device=device)
-    if out.dtype not in (torch.int16, torch.bfloat16) or out.get_device() != dev:
-        raise ValueError("out must be 16-bit tiles on the call's device")
-    _tile_shape(out, rows, "out")
-    if out.shape[1] * 16 != cols:
-        raise ValueError(f"out must have {cols} columns")
+        return torch.zeros(((rows + 15) // 16, cols // 16, 16, 16), dtype=torch.int16, device=device)
+    if out.dtype not in _BF16 or out.get_device() != dev or _tile_cols(out, rows, "out") != cols:
+        raise ValueError(f"out must be 16-bit tiles of {cols} columns on the call's device")
     return out
 
 
 def quantize(tiles, rows: int | None = None, bits: int = 4, out: Tiles | None = None) -> Tiles:
     """Tiles [t][ct][16][16] of 16-bit (bf16, or its bits in int16) or fp32 values to blocks of 4
     or 8 bits, for the first `rows` rows (default: all)."""
-    if tiles.dtype in (torch.int16, torch.bfloat16):
+    if tiles.dtype in _BF16:
         size = 2
     elif tiles.dtype == torch.float32:
         size = 4
@@ -124,15 +131,15 @@ def quantize(tiles, rows: int | None = None, bits: int = 4, out: Tiles | None = 
         raise ValueError("tiles must hold bf16 or fp32")
     if bits not in (4, 8):
         raise ValueError("blocks have 4 or 8 bits")
-    here(tiles)
+    dev = tiles.get_device()
+    stream = _here(dev)
     rows = tiles.shape[0] * 16 if rows is None else rows
-    _tile_shape(tiles, rows, "tiles")
-    cols, dev = tiles.shape[1] * 16, tiles.get_device()
+    cols = _tile_cols(tiles, rows, "tiles")
     if out is None:
         _allocates()
         out = Tiles.create(rows, cols, bits, tiles.device)
     p = _QUANTIZE(rows, (rows + 15) // 16, 0, 0, tiles.data_ptr(), _operand(out, bits, rows, dev, cols, "out"), bits, size)
-    _check(_lib.packed().stride_mx_quantize(p, tc.kernel_stream()))
+    _check(_lib.packed().stride_mx_quantize(p, stream))
     return out
 
 
@@ -140,7 +147,7 @@ def dequantize(t: Tiles, rows: int | None = None, dtype=torch.bfloat16, out=None
     """The values of the first `rows` rows, row-major [rows][cols] in bf16 or fp32."""
     if dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("values come in bf16 or fp32")
-    here(t.codes)
+    stream = _here(t._device)
     rows = t.rows if rows is None else rows
     if out is None:
         _allocates()
@@ -149,27 +156,24 @@ def dequantize(t: Tiles, rows: int | None = None, dtype=torch.bfloat16, out=None
         raise ValueError("out must be [rows][cols] of that type on the same device, its rows contiguous")
     p = _DEQUANTIZE(rows, (rows + 15) // 16, 0, 0, _operand(t, t.bits, rows, t._device, 0, "t"), out.data_ptr(),
                     out.stride(0) if rows > 1 else t.cols, t.bits, 2 if dtype == torch.bfloat16 else 4)
-    _check(_lib.packed().stride_mx_dequantize(p, tc.kernel_stream()))
+    _check(_lib.packed().stride_mx_dequantize(p, stream))
     return out
 
 
 def norm(h, rows: int, weight, eps: float, add=None, out=None, bits: int = 8):
     """h += add (bf16 tiles, where given), then RMSNorm(h) * weight: in 8 bits (Tiles), or with
     bits=16 in bf16 x tiles. h: fp32 tiles [lt][ct][16][16]."""
-    here(h)
+    dev = h.get_device()
+    stream = _here(dev)
     if h.dtype != torch.float32:
         raise ValueError("h must be fp32 tiles")
-    _tile_shape(h, rows, "h")
-    cols, dev = h.shape[1] * 16, h.get_device()
+    cols = _tile_cols(h, rows, "h")
     if weight.dtype != torch.float32 or weight.numel() != cols or not weight.is_contiguous() or weight.get_device() != dev:
         raise ValueError("weight must be contiguous fp32 of h's columns, on its device")
     a = 0
     if add is not None:
-        if add.dtype not in (torch.int16, torch.bfloat16) or add.get_device() != dev:
-            raise ValueError("add must be bf16 tiles on h's device")
-        _tile_shape(add, rows, "add")
-        if add.shape[1] * 16 != cols:
-            raise ValueError("add must have h's columns")
+        if add.dtype not in _BF16 or add.get_device() != dev or _tile_cols(add, rows, "add") != cols:
+            raise ValueError("add must be bf16 tiles of h's columns on its device")
         a = add.data_ptr()
     if bits == 8:
         out = _result(out, rows, cols, h.device)
@@ -180,28 +184,28 @@ def norm(h, rows: int, weight, eps: float, add=None, out=None, bits: int = 8):
     else:
         raise ValueError("a norm's result has 8 or 16 bits")
     p = _NORM(rows, (rows + 15) // 16, 0, 0, h.data_ptr(), a, weight.data_ptr(), ref, x, cols, eps)
-    _check(_lib.packed().stride_mx_norm(p, tc.kernel_stream()))
+    _check(_lib.packed().stride_mx_norm(p, stream))
     return out
 
 
 def gemm(w: Tiles, x: Tiles, rows: int, out=None):
     """y = W x for the first `rows` rows of x, in bf16 x tiles."""
-    here(x.codes)
     dev = x._device
+    stream = _here(dev)
     out = _y_tiles(out, rows, w.tiles * 16, x.codes.device, dev)
     p = _GEMM(rows, (rows + 15) // 16, 0, 0, _operand(x, 8, rows, dev, 0, "x"), _operand(w, 4, 1, dev, x.cols, "w"), out.data_ptr())
-    _check(_lib.packed().stride_mx_gemm(p, tc.kernel_stream()))
+    _check(_lib.packed().stride_mx_gemm(p, stream))
     return out
 
 
 def mlp13(w1: Tiles, w3: Tiles, x: Tiles, rows: int, out: Tiles | None = None) -> Tiles:
     """z = silu(W1 x) * (W3 x) in 8 bits."""
-    here(x.codes)
     dev = x._device
+    stream = _here(dev)
     out = _result(out, rows, w1.tiles * 16, x.codes.device)
     p = _MLP13(rows, (rows + 15) // 16, 0, 0, _operand(x, 8, rows, dev, 0, "x"), _operand(w1, 4, 1, dev, x.cols, "w1"),
                _operand(w3, 4, w1.tiles * 16, dev, x.cols, "w3"), _operand(out, 8, rows, dev, w1.tiles * 16, "out"))
-    _check(_lib.packed().stride_mx_mlp13(p, tc.kernel_stream()))
+    _check(_lib.packed().stride_mx_mlp13(p, stream))
     return out
 
 
@@ -209,8 +213,8 @@ def qkv(wq: Tiles, wk: Tiles, wv: Tiles, x: Tiles, rows: int, head_dim: int, rop
         q_out=None):
     """harness.qkv on these weights (rows in layout.rope_rows' order): q with RoPE in fp32 rows, K
     and V appended to the paged bf16 cache."""
-    here(x.codes)
     dev, nq = x._device, wq.tiles * 16
+    stream = _here(dev)
     if row_slot.dtype != torch.int32 or row_pos.dtype != torch.int32 or row_slot.numel() < rows or row_pos.numel() < rows \
             or not (row_slot.is_contiguous() and row_pos.is_contiguous()):
         raise ValueError("row_slot and row_pos must be contiguous int32, one for each row")
@@ -229,5 +233,5 @@ def qkv(wq: Tiles, wk: Tiles, wv: Tiles, x: Tiles, rows: int, head_dim: int, rop
     ws = [_operand(w, 4, 1, dev, x.cols, name) for w, name in ((wq, "wq"), (wk, "wk"), (wv, "wv"))]
     p = _QKV(rows, (rows + 15) // 16, 0, 0, _operand(x, 8, rows, dev, 0, "x"), *ws, q_out.data_ptr(), q_out.stride(0) if rows > 1 else nq,
              bytes(kv.ref), rope.data_ptr(), row_slot.data_ptr(), row_pos.data_ptr(), layer, head_dim)
-    _check(_lib.packed().stride_mx_qkv(p, tc.kernel_stream()))
+    _check(_lib.packed().stride_mx_qkv(p, stream))
     return q_out
