@@ -33,6 +33,7 @@ _NONE = _TILES(0, 0, 0, 0)
 
 BLOCK, CHUNK, GROUP = 32, 128, 512  # columns of a scale, of a matrix instruction, of a lane's word of scales
 _BF16 = (torch.int16, torch.bfloat16)  # or its bits
+_device, _stream_of = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _PARTS = {4: (4, 16, 16), 8: (2, 4, 16, 16)}  # a chunk's codes
 
 
@@ -50,7 +51,7 @@ class Tiles:
             raise ValueError("codes and scales must be contiguous uint8 on one device")
         if tuple(codes.shape) != (tiles, 4 * groups, *_PARTS[bits]) or tuple(scales.shape) != (tiles, groups, 4, 16, 4):
             raise ValueError(f"codes must be [tiles][{4 * groups}]{list(_PARTS[bits])} and scales [tiles][{groups}][4][16][4]")
-        self.codes, self.scales, self.cols, self.bits, self.tiles = codes, scales, int(cols), bits, tiles
+        self.codes, self.scales, self.cols, self.bits, self.tiles, self.rows = codes, scales, int(cols), bits, tiles, tiles * 16
         self._ref, self._device = _TILES(codes.data_ptr(), scales.data_ptr(), tiles, int(cols)), codes.get_device()
 
     @staticmethod
@@ -63,37 +64,28 @@ class Tiles:
                      torch.zeros((tiles, groups, 4, 16, 4), dtype=torch.uint8, device=device), cols, bits)
 
     @property
-    def rows(self) -> int:
-        return self.tiles * 16
-
-    @property
     def nbytes(self) -> int:
         return self.codes.numel() + self.scales.numel()
 
 
-def _check(rc: int) -> None:
-    if rc:
-        _lib.check(rc)
-
-
 def _here(dev: int) -> int:
     """The stream of a launch for tensors of device `dev`, which has to be the current one."""
-    if dev != torch._C._cuda_getDevice() or dev < 0:
-        raise ValueError(f"tensors are on device {dev}, the current one is {torch._C._cuda_getDevice()}")
-    return torch._C._cuda_getCurrentRawStream(dev) if tc._stream is None else tc.kernel_stream()
+    if dev != _device() or dev < 0:
+        raise ValueError(f"tensors are on device {dev}, the current one is {_device()}")
+    return _stream_of(dev) if tc._stream is None else tc.kernel_stream()
 
 
 def _operand(t, bits: int, rows: int, dev: int, cols: int, name: str) -> bytes:
     """A Tiles argument's block, looked over (cols 0: any)."""
-    if not isinstance(t, Tiles) or t.bits != bits or t._device != dev or t.tiles * 16 < rows or (cols and t.cols != cols):
+    if type(t) is not Tiles or t.bits != bits or t._device != dev or t.rows < rows or (cols and t.cols != cols):
         raise ValueError(f"{name} must be Tiles in {bits} bits with the rows and columns of the call, on its device")
     return t._ref
 
 
-def _result(out, rows: int, cols: int, device) -> Tiles:
+def _result(out, rows: int, cols: int, like) -> Tiles:
     if out is None:
         _allocates()
-        return Tiles.create(rows, cols, 8, device)
+        return Tiles.create(rows, cols, 8, getattr(like, "codes", like).device)
     return out
 
 
@@ -104,17 +96,18 @@ def _allocates() -> None:
 
 def _tile_cols(t, rows: int, name: str) -> int:
     """Columns of tiles [ceil(rows / 16)][cols / 16][16][16]."""
-    shape = t.shape
-    if len(shape) != 4 or shape[2] != 16 or shape[3] != 16 or shape[0] * 16 < rows or shape[1] < 1 or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous tiles [ceil(rows / 16)][cols / 16][16][16]")
-    return shape[1] * 16
+    if t.dim() == 4 and t.is_contiguous():
+        tiles, col_tiles, a, b = t.shape
+        if a == 16 and b == 16 and tiles * 16 >= rows and col_tiles:
+            return col_tiles * 16
+    raise ValueError(f"{name} must be contiguous tiles [ceil(rows / 16)][cols / 16][16][16]")
 
 
-def _y_tiles(out, rows: int, cols: int, device, dev: int):
-    """bf16 x tiles that are written."""
+def _y_tiles(out, rows: int, cols: int, like, dev: int):
+    """bf16 x tiles that are written (on the device of `like`, a tensor or Tiles)."""
     if out is None:
         _allocates()
-        return torch.zeros(((rows + 15) // 16, cols // 16, 16, 16), dtype=torch.int16, device=device)
+        return torch.zeros(((rows + 15) // 16, cols // 16, 16, 16), dtype=torch.int16, device=getattr(like, "codes", like).device)
     if out.dtype not in _BF16 or out.get_device() != dev or _tile_cols(out, rows, "out") != cols:
         raise ValueError(f"out must be 16-bit tiles of {cols} columns on the call's device")
     return out
@@ -139,7 +132,9 @@ def quantize(tiles, rows: int | None = None, bits: int = 4, out: Tiles | None = 
         _allocates()
         out = Tiles.create(rows, cols, bits, tiles.device)
     p = _QUANTIZE(rows, (rows + 15) // 16, 0, 0, tiles.data_ptr(), _operand(out, bits, rows, dev, cols, "out"), bits, size)
-    _check(_lib.packed().stride_mx_quantize(p, stream))
+    rc = _lib.packed().stride_mx_quantize(p, stream)
+    if rc:
+        _lib.check(rc)
     return out
 
 
@@ -156,7 +151,9 @@ def dequantize(t: Tiles, rows: int | None = None, dtype=torch.bfloat16, out=None
         raise ValueError("out must be [rows][cols] of that type on the same device, its rows contiguous")
     p = _DEQUANTIZE(rows, (rows + 15) // 16, 0, 0, _operand(t, t.bits, rows, t._device, 0, "t"), out.data_ptr(),
                     out.stride(0) if rows > 1 else t.cols, t.bits, 2 if dtype == torch.bfloat16 else 4)
-    _check(_lib.packed().stride_mx_dequantize(p, stream))
+    rc = _lib.packed().stride_mx_dequantize(p, stream)
+    if rc:
+        _lib.check(rc)
     return out
 
 
@@ -176,15 +173,17 @@ def norm(h, rows: int, weight, eps: float, add=None, out=None, bits: int = 8):
             raise ValueError("add must be bf16 tiles of h's columns on its device")
         a = add.data_ptr()
     if bits == 8:
-        out = _result(out, rows, cols, h.device)
+        out = _result(out, rows, cols, h)
         ref, x = _operand(out, 8, rows, dev, cols, "out"), 0
     elif bits == 16:
-        out = _y_tiles(out, rows, cols, h.device, dev)
+        out = _y_tiles(out, rows, cols, h, dev)
         ref, x = _NONE, out.data_ptr()
     else:
         raise ValueError("a norm's result has 8 or 16 bits")
     p = _NORM(rows, (rows + 15) // 16, 0, 0, h.data_ptr(), a, weight.data_ptr(), ref, x, cols, eps)
-    _check(_lib.packed().stride_mx_norm(p, stream))
+    rc = _lib.packed().stride_mx_norm(p, stream)
+    if rc:
+        _lib.check(rc)
     return out
 
 
@@ -192,9 +191,11 @@ def gemm(w: Tiles, x: Tiles, rows: int, out=None):
     """y = W x for the first `rows` rows of x, in bf16 x tiles."""
     dev = x._device
     stream = _here(dev)
-    out = _y_tiles(out, rows, w.tiles * 16, x.codes.device, dev)
+    out = _y_tiles(out, rows, w.rows, x, dev)
     p = _GEMM(rows, (rows + 15) // 16, 0, 0, _operand(x, 8, rows, dev, 0, "x"), _operand(w, 4, 1, dev, x.cols, "w"), out.data_ptr())
-    _check(_lib.packed().stride_mx_gemm(p, stream))
+    rc = _lib.packed().stride_mx_gemm(p, stream)
+    if rc:
+        _lib.check(rc)
     return out
 
 
@@ -202,10 +203,12 @@ def mlp13(w1: Tiles, w3: Tiles, x: Tiles, rows: int, out: Tiles | None = None) -
     """z = silu(W1 x) * (W3 x) in 8 bits."""
     dev = x._device
     stream = _here(dev)
-    out = _result(out, rows, w1.tiles * 16, x.codes.device)
+    out = _result(out, rows, w1.rows, x)
     p = _MLP13(rows, (rows + 15) // 16, 0, 0, _operand(x, 8, rows, dev, 0, "x"), _operand(w1, 4, 1, dev, x.cols, "w1"),
-               _operand(w3, 4, w1.tiles * 16, dev, x.cols, "w3"), _operand(out, 8, rows, dev, w1.tiles * 16, "out"))
-    _check(_lib.packed().stride_mx_mlp13(p, stream))
+               _operand(w3, 4, w1.rows, dev, x.cols, "w3"), _operand(out, 8, rows, dev, w1.rows, "out"))
+    rc = _lib.packed().stride_mx_mlp13(p, stream)
+    if rc:
+        _lib.check(rc)
     return out
 
 
@@ -213,7 +216,7 @@ def qkv(wq: Tiles, wk: Tiles, wv: Tiles, x: Tiles, rows: int, head_dim: int, rop
         q_out=None):
     """harness.qkv on these weights (rows in layout.rope_rows' order): q with RoPE in fp32 rows, K
     and V appended to the paged bf16 cache."""
-    dev, nq = x._device, wq.tiles * 16
+    dev, nq = x._device, wq.rows
     stream = _here(dev)
     if row_slot.dtype != torch.int32 or row_pos.dtype != torch.int32 or row_slot.numel() < rows or row_pos.numel() < rows \
             or not (row_slot.is_contiguous() and row_pos.is_contiguous()):
@@ -222,7 +225,7 @@ def qkv(wq: Tiles, wk: Tiles, wv: Tiles, x: Tiles, rows: int, head_dim: int, rop
         raise ValueError("rope must be contiguous fp32 [positions][head_dim / 2][2]")
     if not row_slot.get_device() == row_pos.get_device() == rope.get_device() == kv.table.get_device() == dev:
         raise ValueError("the arguments are on different devices")
-    if not 0 <= layer < kv.ref.block_elems // kv.ref.layer_elems or kv.ref.which_elems * head_dim != wk.tiles * 16 * kv.ref.group_elems:
+    if not 0 <= layer < kv.ref.block_elems // kv.ref.layer_elems or kv.ref.which_elems * head_dim != wk.rows * kv.ref.group_elems:
         raise ValueError("layer or the number of KV heads is not the cache's")
     if q_out is None:
         _allocates()
@@ -233,5 +236,7 @@ def qkv(wq: Tiles, wk: Tiles, wv: Tiles, x: Tiles, rows: int, head_dim: int, rop
     ws = [_operand(w, 4, 1, dev, x.cols, name) for w, name in ((wq, "wq"), (wk, "wk"), (wv, "wv"))]
     p = _QKV(rows, (rows + 15) // 16, 0, 0, _operand(x, 8, rows, dev, 0, "x"), *ws, q_out.data_ptr(), q_out.stride(0) if rows > 1 else nq,
              bytes(kv.ref), rope.data_ptr(), row_slot.data_ptr(), row_pos.data_ptr(), layer, head_dim)
-    _check(_lib.packed().stride_mx_qkv(p, stream))
+    rc = _lib.packed().stride_mx_qkv(p, stream)
+    if rc:
+        _lib.check(rc)
     return q_out
