@@ -463,3 +463,47 @@ def test_no_rows():
     assert mx.gemm(w, x, 0).shape == (0, 4, 16, 16) and mx.mlp13(w, w, x, 0).tiles == 0
     h = torch.zeros((0, 32, 16, 16), device=DEV)
     assert mx.norm(h, 0, torch.ones(512, device=DEV), 1e-5).tiles == 0 and mx.quantize(h).tiles == 0 and mx.dequantize(x).shape == (0, 512)
+
+
+def rows_alone(x, first, n):
+    """Rows first * 16 .. of Tiles, as Tiles of their own."""
+    return mx.Tiles(x.codes[first:first + n].contiguous(), x.scales[first:first + n].contiguous(), x.cols, x.bits)
+
+
+@pytest.mark.parametrize("m,n,k", [
+    (40, 2048, 512), (100, 256, 8192), (150, 2048, 4096), (200, 1024, 1024), (600, 2048, 1024), (1000, 1552, 528),
+    (1400, 4096, 512), (1400, 2064, 2064), (2100, 4096, 8192)])
+def test_each_form_has_the_same_bits(m, n, k):
+    """From waves of their own to 256 x 128 tiles, ragged ones among them: every row as in a batch of
+    16, which is a wave's of its own; lanes behind the rows stay as they were."""
+    say("forms", m, n, k)
+    gen = torch.Generator(device=DEV).manual_seed(m + n + k)
+    rand = lambda *s: torch.randn(s, generator=gen, device=DEV)
+    ws = [mx.quantize(layout.lane_tiles((rand(n, k) * 0.05).to(torch.bfloat16))) for _ in range(2)]
+    x = mx.quantize(layout.lane_tiles(rand(m, k).to(torch.bfloat16)), m, bits=8)
+    T = (m + 15) // 16
+    y = torch.full((T, n // 16, 16, 16), 99, dtype=torch.int16, device=DEV)
+    z = marked(m, n, 8)
+    mx.gemm(ws[0], x, m, out=y)
+    mx.mlp13(*ws, x, m, out=z)
+    D, kv_heads = 32, n // 64
+    slots = torch.zeros(m, dtype=torch.int32, device=DEV)
+    pos = torch.randperm(m, generator=gen, device=DEV).to(torch.int32)
+    rope = rand(m, D // 2, 2)
+    caches = [harness.PagedKv.create(1, m, kv_heads, D, 1, 16, DEV) for _ in range(2)]
+    w_qkv = (ws[0], *(mx.Tiles(w.codes[: kv_heads * 2].contiguous(), w.scales[: kv_heads * 2].contiguous(), k, 4) for w in ws))
+    q = torch.zeros((m, n), device=DEV) if n % D == 0 else None
+    if q is not None:
+        mx.qkv(*w_qkv, x, m, D, rope, slots, pos, caches[0], q_out=q)
+    for t in range(T):
+        rows = min(16, m - 16 * t)
+        part = rows_alone(x, t, 1)
+        y1 = torch.full((1, n // 16, 16, 16), 99, dtype=torch.int16, device=DEV)
+        z1 = marked(rows, n, 8)
+        mx.gemm(ws[0], part, rows, out=y1)
+        mx.mlp13(*ws, part, rows, out=z1)
+        assert torch.equal(y[t], y1[0]) and torch.equal(z.codes[t], z1.codes[0]) and torch.equal(z.scales[t], z1.scales[0]), t
+        if q is not None:
+            q1 = mx.qkv(*w_qkv, part, rows, D, rope, slots[:rows], pos[16 * t:16 * t + rows].contiguous(), caches[1])
+            assert torch.equal(q[16 * t:16 * t + rows], q1), t
+    assert torch.equal(caches[0].arena, caches[1].arena)
