@@ -121,48 +121,37 @@ __device__ __forceinline__ void mx_source(const MxGeometry& g, int m, int rt, co
   scales = (which == 0 ? g.ws[0] : which == 1 ? g.ws[1] : g.ws[2]) + static_cast<int64_t>(rt) * g.groups * kScaleBytes;
 }
 
-// Few output tiles: a wave has one unit by one lane tile, operands straight to registers, P groups of
-// K in use and P on their way.
+// Few output tiles: a wave has one weight tile by one lane tile, operands straight to registers, P
+// groups of K in use and P on their way. The tiles of a unit meet in LDS.
 template <class Epi, int P>
-__global__ __launch_bounds__(64) void k_mx_row(MxGeometry g, typename Epi::Out o, int units) {
+__global__ __launch_bounds__(64 * Epi::kMats * Epi::kUnit) void k_mx_row(MxGeometry g, typename Epi::Out o, int units) {
   constexpr int M = Epi::kMats, U = Epi::kUnit;
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int unit = blockIdx.x % units, lt = blockIdx.x / units;
-  const uint8_t *wc[M][U], *ws[M][U];
-#pragma unroll
-  for (int m = 0; m < M; ++m)
-#pragma unroll
-    for (int u = 0; u < U; ++u) mx_source<Epi>(g, m, unit * U + u, wc[m][u], ws[m][u]);
+  const uint8_t *wc, *ws;
+  mx_source<Epi>(g, wave / U, unit * U + wave % U, wc, ws);
   const uint8_t* xc = g.xc + static_cast<int64_t>(lt) * g.groups * 4 * kCode8Bytes;
   const uint8_t* xs = g.xs + static_cast<int64_t>(lt) * g.groups * kScaleBytes;
-  const uint32_t at16 = lane * 16, at4 = lane * 4;
-  f32x4 acc[M][U];
-#pragma unroll
-  for (int m = 0; m < M; ++m)
-#pragma unroll
-    for (int u = 0; u < U; ++u) acc[m][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // lanes without a row take the last one's: for one row a quarter of the lines
+  const int row = min(lane & 15, g.rows - 1 - lt * 16);
+  const uint32_t at16 = lane * 16, at4 = lane * 4, x16 = ((lane & 48) + row) * 16, x4 = x16 / 4;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   struct Part {
-    u32x4 w[P][4][M][U], x[P][4][2];
-    uint32_t sw[P][M][U], sx[P];
+    u32x4 w[P][4], x[P][4][2];
+    uint32_t sw[P], sx[P];
   };
   Part part[2];
   auto load = [&](Part& t, int first) {
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       const int64_t i = min(first + p, g.groups - 1);
-      t.sx[p] = *reinterpret_cast<const uint32_t*>(xs + i * kScaleBytes + at4);
-#pragma unroll
-      for (int m = 0; m < M; ++m)
-#pragma unroll
-        for (int u = 0; u < U; ++u) t.sw[p][m][u] = *reinterpret_cast<const uint32_t*>(ws[m][u] + i * kScaleBytes + at4);
+      t.sx[p] = *reinterpret_cast<const uint32_t*>(xs + i * kScaleBytes + x4);
+      t.sw[p] = *reinterpret_cast<const uint32_t*>(ws + i * kScaleBytes + at4);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
+        t.w[p][c] = load16(wc + (i * 4 + c) * kCode4Bytes + at16);
 #pragma unroll
-        for (int m = 0; m < M; ++m)
-#pragma unroll
-          for (int u = 0; u < U; ++u) t.w[p][c][m][u] = load16(wc[m][u] + (i * 4 + c) * kCode4Bytes + at16);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) t.x[p][c][h] = load16(xc + (i * 4 + c) * kCode8Bytes + h * 1024 + at16);
+        for (int h = 0; h < 2; ++h) t.x[p][c][h] = load16(xc + (i * 4 + c) * kCode8Bytes + h * 1024 + x16);
       }
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -170,12 +159,7 @@ __global__ __launch_bounds__(64) void k_mx_row(MxGeometry g, typename Epi::Out o
   auto products = [&](const Part& t, int first) {
     unroll<P>([&](auto p) {
       if (p > 0 && first + p >= g.groups) return;
-      unroll<4>([&](auto c) {
-#pragma unroll
-        for (int m = 0; m < M; ++m)
-#pragma unroll
-          for (int u = 0; u < U; ++u) acc[m][u] = mx_mfma<c>(t.w[p][c][m][u], t.x[p][c][0], t.x[p][c][1], acc[m][u], t.sw[p][m][u], t.sx[p]);
-      });
+      unroll<4>([&](auto c) { acc = mx_mfma<c>(t.w[p][c], t.x[p][c][0], t.x[p][c][1], acc, t.sw[p], t.sx[p]); });
     });
   };
   load(part[0], 0);
@@ -187,11 +171,21 @@ __global__ __launch_bounds__(64) void k_mx_row(MxGeometry g, typename Epi::Out o
   }
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7");
+  asm volatile("" : "+v"(acc));
+  f32x4 y[M][U];
+  if constexpr (M * U > 1) {
+    __shared__ f32x4 tiles[M * U][kWave];
+    tiles[wave][lane] = acc;
+    __syncthreads();
+    if (wave) return;
 #pragma unroll
-  for (int m = 0; m < M; ++m)
+    for (int m = 0; m < M; ++m)
 #pragma unroll
-    for (int u = 0; u < U; ++u) asm volatile("" : "+v"(acc[m][u]));
-  Epi::finish(o, g, unit, lt, acc, lane);
+      for (int u = 0; u < U; ++u) y[m][u] = tiles[m * U + u][lane];
+  } else {
+    y[0][0] = acc;
+  }
+  Epi::finish(o, g, unit, lt, y, lane);
 }
 
 // A wave's 64 x 16 or 64 x 4 bytes from base + offset to LDS at `to` on, in lane order. In assembly,
@@ -507,7 +501,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxGeometry g, typename
 
 template <class Epi, int P>
 void launch_row(const MxGeometry& g, const typename Epi::Out& o, int units, hipStream_t st) {
-  hipLaunchKernelGGL((k_mx_row<Epi, P>), dim3(units * g.lane_groups), dim3(64), 0, st, g, o, units);
+  hipLaunchKernelGGL((k_mx_row<Epi, P>), dim3(units * g.lane_groups), dim3(64 * Epi::kMats * Epi::kUnit), 0, st, g, o, units);
 }
 
 template <class Epi, int A, int L, int WM, int WN, int NS, int OCC>
@@ -532,9 +526,10 @@ int run(const char* what, const MxGeometry& g, const typename Epi::Out& o, int r
   // configuration
   // By the number of 16 x 16 products, of which the card's 256 CUs want four each before tiles pay.
   // Measured at 1 to 4096 rows of weights from 512 x 512 to 14336 x 4096, us here / as the next form:
-  //   waves of their own to 768 (gate and up, whose waves have four products: 2048), 1536 where K is
-  //     short: 2048 x 8192 at 1 / 64 rows 5.5 / 6.9 against 10 / 8.2 as 32 x 32 tiles, at 128 rows
-  //     9.6 against 8.3; 8192 x 2048 at 32 rows 4.1 against 4.9
+  //   a wave a tile to 768 (1536 where K is short; gate and up, which have no 32 x 32: 1280): 2048 x
+  //     8192 at 1 / 64 rows 5.2 / 6.9 against 10 / 8.2 as 32 x 32, at 128 rows 9.6 against 8.3; 8192 x
+  //     2048 at 32 rows 4.1 against 4.9; gate and up 8192 x 2048 at 16 / 32 rows 5.6 / 7.1 against
+  //     6.2 / 6.3 as 64 x 64
   //   32 x 32 to 1536: 4096 x 14336 at 64 rows 12.1 against 19 as 64 x 64
   //   64 x 64 to 6144: 2048 x 8192 at 512 rows 13.6 against 15.5 as 128 x 64, at 1024 22.2 against 17.6
   //   128 x 64 to 20480: 2048 x 8192 at 2048 rows 32.6 against 36.5 as 128 x 128, 8192 x 2048 40.7
@@ -544,7 +539,7 @@ int run(const char* what, const MxGeometry& g, const typename Epi::Out& o, int r
   //   256 x 128 where K is long and every CU has one: the fewest bytes a product, by which the clock
   //     stays up: 2048 x 8192 at 4096 rows 54 against 60 as 128 x 128, 4096 x 14336 166 against 192
   const int64_t products = static_cast<int64_t>(row_tiles) * Epi::kMats * g.lane_groups;
-  if (products <= (Epi::kMats == 2 ? 2048 : g.groups <= 4 ? 1536 : 768)) launch_row<Epi, 4 / Epi::kMats>(g, o, units, st);
+  if (products <= (Epi::kMats == 2 ? 1280 : g.groups <= 4 ? 1536 : 768)) launch_row<Epi, 4 / Epi::kMats>(g, o, units, st);
   else if (Epi::kMats == 1 && products <= 1536) {
     if constexpr (Epi::kMats == 1) launch_tile<Epi, 1, 1, 2, 2, 3>(g, o, units, st);
   } else if (products <= 6144) launch_pipe<Epi, 4, 1, 1, 4, 4, 2>(g, o, units, st);
