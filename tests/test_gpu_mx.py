@@ -507,3 +507,19 @@ def test_each_form_has_the_same_bits(m, n, k):
             q1 = mx.qkv(*w_qkv, part, rows, D, rope, slots[:rows], pos[16 * t:16 * t + rows].contiguous(), caches[1])
             assert torch.equal(q[16 * t:16 * t + rows], q1), t
     assert torch.equal(caches[0].arena, caches[1].arena)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_many_values(bits):
+    """Where a workgroup takes a whole group: the values that the same tiles have in small calls."""
+    gen = torch.Generator(device=DEV).manual_seed(bits)
+    m, k = 5003, 1552
+    t = mx.quantize(layout.lane_tiles(torch.randn((m, k), generator=gen, device=DEV) * 3), m, bits=bits)
+    for dtype in (torch.bfloat16, torch.float32):
+        out = torch.full((m + 1, k + 48), 7.0, dtype=dtype, device=DEV)
+        mx.dequantize(t, m, dtype=dtype, out=out[:, :k])
+        assert (out[m:] == 7).all() and (out[:, k:] == 7).all()
+        for first in range(0, t.tiles, 40):
+            part = rows_alone(t, first, 40)
+            rows = min(part.rows, m - 16 * first)
+            assert torch.equal(out[16 * first:16 * first + rows, :k], mx.dequantize(part, rows, dtype=dtype))
