@@ -137,6 +137,9 @@ __global__ __launch_bounds__(256) void k_dequantize(StrideMxTiles in, T* out, in
   }
 }
 
+// bf16_rne, and NaN whatever its payload (h may hold any).
+__device__ __forceinline__ uint32_t bf16_of(float v) { return v != v ? 0x7FC0u : bf16_rne(v); }
+
 // Workgroup: R rows of a lane tile; a lane's values stay in registers between the sum and the
 // scaling (IT places; 0: h is read again). A row's sum has the same order for every R: a chunk's
 // pieces of 8 by halves and tiles, then its chunks 16 apart ascending, and those by halves again.
@@ -211,7 +214,7 @@ __global__ __launch_bounds__(1024) void k_mx_norm(StrideMxNormParams p, int chun
     } else if (live && ct < col_tiles) {
       u32x4 w;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = bf16_rne(x[2 * i]) | bf16_rne(x[2 * i + 1]) << 16;
+      for (int i = 0; i < 4; ++i) w[i] = bf16_of(x[2 * i]) | bf16_of(x[2 * i + 1]) << 16;
       *reinterpret_cast<u32x4*>(p.x + at + static_cast<int64_t>(ct) * kTileElems) = w;
     }
   };

@@ -209,6 +209,17 @@ def test_norm_rows_that_are_zero_or_not_finite():
     assert np.isnan(got[2, 96:128]).all() and (got[2, :96] == 0).all()
 
 
+def test_norm_of_any_nan():
+    """NaN of every payload and sign stays NaN in both results, in its own row."""
+    bits = torch.tensor([0x7FFFFFFF, -1, 0x7F800001, 0x7FC00000, -0x3FFFFF], dtype=torch.int32, device=DEV)
+    h = torch.ones((1, 32, 16, 16), device=DEV)
+    h.view(torch.int32)[0, 3, :5, 7] = bits
+    for b in (8, 16):
+        t = mx.norm(h, 16, torch.ones(512, device=DEV), 1e-5, bits=b)
+        v = mx.dequantize(t).float() if b == 8 else layout.untile_lanes(t, 16).view(torch.bfloat16).float()
+        assert v[:5].isnan().all() and (v[5:] == 1).all()
+
+
 # --- products -----------------------------------------------------------------
 
 SHAPES = [(1, 16, 16), (1, 256, 512), (16, 48, 528), (17, 512, 2048), (33, 1040, 1040), (5, 2048, 8192), (64, 512, 2560), (130, 256, 4112),
