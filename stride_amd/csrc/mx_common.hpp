@@ -16,6 +16,8 @@ constexpr int kMxChunk = 128;    // columns of a matrix instruction
 constexpr int kMxGroup = 512;    // columns whose scales a lane reads as one word
 constexpr int kCode4Bytes = 1024, kCode8Bytes = 2048, kScaleBytes = 256;  // a tile's chunk; a tile's group
 
+constexpr int64_t kMxMostGroups = (int64_t{1} << 32) / 1024 - 1;  // of up to 1024 threads, all of which a launch counts in 32 bits
+
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 __host__ __device__ constexpr int mx_groups(int cols) { return (cols + kMxGroup - 1) / kMxGroup; }

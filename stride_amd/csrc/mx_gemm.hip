@@ -534,7 +534,7 @@ template <class Epi>
 int run(const char* what, const MxGeometry& g, const typename Epi::Out& o, int row_tiles, hipStream_t st) {
   // z is written to the end of its last group of 512 columns
   const int units = Epi::kUnit == 2 ? mx_groups(row_tiles * 16) * (kMxGroup / kMxBlock) : row_tiles;
-  if (static_cast<int64_t>(units) * g.lane_groups > INT_MAX) return mx_refused(what, "rows and weights are too large together");
+  if (static_cast<int64_t>(units) * g.lane_groups > kMxMostGroups) return mx_refused(what, "rows and weights are too large together");
   // configuration
   // By the number of 16 x 16 products, of which the card's 256 CUs want four each before tiles pay.
   // Measured at 1 to 4096 rows of weights from 512 x 512 to 14336 x 4096, us here / as the next form:

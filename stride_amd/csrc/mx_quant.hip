@@ -288,7 +288,7 @@ int stride_mx_quantize(const StrideMxQuantizeParams* p, void* stream) {
   if (!p->src || reinterpret_cast<uintptr_t>(p->src) % 16) return mx_refused(what, "src must be there, 16-byte aligned");
   const int chunks = mx_groups(p->out.cols) * 4;
   const int64_t all = static_cast<int64_t>(chunks) * p->l.lane_groups;
-  if (all > INT_MAX) return mx_refused(what, "rows and cols are too large together");
+  if (all > 4 * kMxMostGroups) return mx_refused(what, "rows and cols are too large together");
   const dim3 grid(static_cast<unsigned>(all)), block(256);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const uint16_t* half = static_cast<const uint16_t*>(p->src);
@@ -310,7 +310,7 @@ int stride_mx_dequantize(const StrideMxDequantizeParams* p, void* stream) {
   if (!p->out || reinterpret_cast<uintptr_t>(p->out) % 16) return mx_refused(what, "out must be there, 16-byte aligned");
   if (p->out_stride < p->in.cols || p->out_stride % 8) return mx_refused(what, "out_stride must be a multiple of 8, at least cols");
   const int groups = mx_groups(p->in.cols);
-  if (static_cast<int64_t>(groups) * 4 * p->l.lane_groups > INT_MAX) return mx_refused(what, "rows and cols are too large together");
+  if (static_cast<int64_t>(groups) * 4 * p->l.lane_groups > 4 * kMxMostGroups) return mx_refused(what, "rows and cols are too large together");
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (p->bits == 4 && p->out_bytes == 2) launch_values<4, uint16_t>(*p, groups, st);
   else if (p->bits == 4) launch_values<4, float>(*p, groups, st);
@@ -324,6 +324,7 @@ int stride_mx_norm(const StrideMxNormParams* p, void* stream) {
   if (!p) return mx_refused(what, "null parameters");
   if (!mx_lanes_ok(p->l)) return mx_refused(what, "need rows >= 0 and lane_groups = ceil(rows/16)");
   if (p->dim <= 0 || p->dim % 16 || p->dim > 65536) return mx_refused(what, "dim must be a positive multiple of 16, at most 65536");
+  if (p->l.rows / 4 > kMxMostGroups - 1) return mx_refused(what, "too many rows");
   if (p->l.rows == 0) return 0;
   if (!p->h || !p->weight || !p->out.codes == !p->x) return mx_refused(what, "need h, weight and one of out and x");
   if (p->out.codes)

@@ -93,6 +93,16 @@ def test_nothing_to_do_and_nothing_given():
         assert call(name, None) == _lib.EINVAL and "null" in err()
 
 
+def test_launches_beyond_32_bits_of_threads():
+    """A launch counts its threads in 32 bits: what would not fit is refused."""
+    rows = 2 ** 31 - 16
+    t, w = tiles(1 << 27, 1 << 20), tiles(1 << 10, 1 << 20)
+    for name, block in (("quantize", mx._QUANTIZE(rows, rows // 16, 0, 0, BUF, t, 4, 2)), ("dequantize", mx._DEQUANTIZE(rows, rows // 16, 0, 0, t, BUF, 1 << 20, 4, 2)),
+                        ("norm", mx._NORM(rows, rows // 16, 0, 0, BUF, 0, BUF, tiles(1 << 27), 0, 512, 1e-5)), ("gemm", mx._GEMM(rows, rows // 16, 0, 0, t, w, BUF)),
+                        ("mlp13", mx._MLP13(rows, rows // 16, 0, 0, t, w, w, tiles(1 << 27, 1 << 14, BUF + 64)))):
+        assert call(name, block) == _lib.EINVAL and "too " in err(), name
+
+
 @pytest.mark.parametrize("block,why", [
     (mx._QUANTIZE(5, 1, 0, 0, BUF, tiles(), 6, 2), "bits"), (mx._QUANTIZE(5, 1, 0, 0, BUF, tiles(), 4, 3), "bytes"),
     (mx._QUANTIZE(5, 1, 0, 0, 0, tiles(), 4, 2), "src"), (mx._QUANTIZE(5, 1, 0, 0, BUF + 8, tiles(), 4, 2), "src"),
