@@ -61,8 +61,15 @@ struct EpiRope {
   static constexpr int kMats = 1, kUnit = 1;
   using Out = EpiQkv::Out;
   __device__ __forceinline__ static void finish(const Out& o, const MxGeometry& g, int rt, int lt, const f32x4 (&y)[1][1], int lane) {
+    // a lane whose row has no place in the cache has none here either
+    const int j = lt * 16 + (lane & 15);
+    bool live = j < g.rows;
+    if (live) {
+      const int pos = o.row_pos[j];
+      live = pos >= 0 && (pos >> o.page_shift) < o.kv.max_blocks && o.row_slot[j] >= 0;
+    }
     Geometry rows{};
-    rows.rows = g.rows;
+    rows.rows = live ? g.rows : 0;
     const int which = mx_matrix(g, rt);
     EpiQkv::apply(o, rows, which, rt, lt, y[0], lane);
   }

@@ -33,7 +33,7 @@ _NONE = _TILES(0, 0, 0, 0)
 
 BLOCK, CHUNK, GROUP = 32, 128, 512  # columns of a scale, of a matrix instruction, of a lane's word of scales
 _BF16 = (torch.int16, torch.bfloat16)  # or its bits
-_device, _stream_of = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_device, _stream_of = (getattr(torch._C, name, None) for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"))
 _PARTS = {4: (4, 16, 16), 8: (2, 4, 16, 16)}  # a chunk's codes
 
 
@@ -215,7 +215,8 @@ def mlp13(w1: Tiles, w3: Tiles, x: Tiles, rows: int, out: Tiles | None = None) -
 def qkv(wq: Tiles, wk: Tiles, wv: Tiles, x: Tiles, rows: int, head_dim: int, rope, row_slot, row_pos, kv: PagedKv, layer: int = 0,
         q_out=None):
     """harness.qkv on these weights (rows in layout.rope_rows' order): q with RoPE in fp32 rows, K
-    and V appended to the paged bf16 cache."""
+    and V appended to the paged bf16 cache. A row whose slot or position is below 0, or whose position
+    lies behind the table, is left out, its q as it was."""
     dev, nq = x._device, wq.rows
     stream = _here(dev)
     if row_slot.dtype != torch.int32 or row_pos.dtype != torch.int32 or row_slot.numel() < rows or row_pos.numel() < rows \

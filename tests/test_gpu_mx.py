@@ -1,7 +1,6 @@
 """stride_amd.mx against plain forms in 64 bits (mx_plain): blocks bit for bit, the norm and the
 products within the roundings that they take; rows that do not depend on their batch; capture,
 streams, refusals."""
-import ctypes as C
 
 import numpy as np
 import pytest
@@ -322,6 +321,53 @@ def test_qkv(m, heads, kv_heads, D, k, page):
     for which in (0, 1):
         kv.fill_dense(1, which, torch.zeros((3, kv_heads, 200, D), dtype=torch.int16, device=DEV))
     assert torch.equal(kv.arena, before)
+
+
+@pytest.mark.parametrize("m", [5, 200, 1500])
+def test_qkv_rows_without_a_place(m):
+    """Padding rows of a captured batch (slot or position below 0), positions behind the table and
+    entries without a page: the others' bits are as without them, in the cache and in q."""
+    rng = np.random.default_rng(m)
+    ws, _, x, kv, slot, pos, rope = qkv_case(rng, m, 8, 2, 64, 512, slots=8)
+    rope = np.concatenate([rope, rope])
+    q = torch.full((m, 512), 99.0, device=DEV)
+    mx.qkv(*ws, x, m, 64, dev(rope), dev(slot), dev(pos), kv, layer=1, q_out=q)
+    want_q, want = q.clone(), kv.arena.clone()
+    bad = rng.permutation(m)[: m // 2]
+    slot2, pos2 = slot.copy(), pos.copy()
+    for i, j in enumerate(bad):
+        if i % 4 == 0:
+            slot2[j] = -1 - i
+        elif i % 4 == 1:
+            pos2[j] = -2 ** 31 + i
+        elif i % 4 == 2:
+            pos2[j] = 208 + i % 100
+        else:
+            slot2[j], pos2[j] = -2 ** 31, 2 ** 31 - 1
+    kv.arena.zero_()
+    q.fill_(99.0)
+    args = (*ws, x, m, 64, dev(rope), dev(slot2), dev(pos2), kv)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mx.qkv(*args, layer=1, q_out=q)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        mx.gemm(ws[0], x, m)
+        rest = np.setdiff1d(np.arange(m), bad)
+        assert torch.equal(q[dev(rest)], want_q[dev(rest)]) and (q[dev(bad)] == 99).all()
+    for j in bad:  # what the whole call kept of them, taken away
+        base = int(kv.table[slot[j], pos[j] // 16]) * kv.ref.block_elems + kv.ref.layer_elems + int(pos[j] % 16) * 64
+        for which in (0, 1):
+            for h in (0, 1):
+                at = base + which * kv.ref.which_elems + h * kv.ref.group_elems
+                want[at:at + 64] = 0
+    assert torch.equal(kv.arena, want)
+    kv.table.fill_(-1)
+    kv.arena.zero_()
+    mx.qkv(*ws, x, m, 64, dev(rope), dev(slot), dev(pos), kv, layer=1, q_out=q)
+    assert torch.equal(q, want_q) and not kv.arena.any()
 
 
 def test_rows_do_not_depend_on_their_batch():
