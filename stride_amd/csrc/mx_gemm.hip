@@ -524,10 +524,12 @@ void launch_row(const MxGeometry& g, const typename Epi::Out& o, int units, hipS
 }
 
 template <class Epi, int A, int L, int WM, int WN, int NS, int OCC>
-void launch_pipe(const MxGeometry& g, const typename Epi::Out& o, int units, hipStream_t st) {
+bool launch_pipe(const MxGeometry& g, const typename Epi::Out& o, int units, hipStream_t st) {
   constexpr int per = WM * A / Epi::kMats / Epi::kUnit;
   const int unit_blocks = (units + per - 1) / per, lane_blocks = (g.lane_groups + WN * L - 1) / (WN * L);
+  if (static_cast<int64_t>(unit_blocks) * lane_blocks > kMxMostGroups * 1024 / (64 * WM * WN)) return false;
   hipLaunchKernelGGL((k_mx_pipe<Epi, A, L, WM, WN, NS, OCC>), dim3(unit_blocks * lane_blocks), dim3(64 * WM * WN), 0, st, g, o, units, unit_blocks, lane_blocks);
+  return true;
 }
 
 template <class Epi, int A, int L, int WM, int WN, int NS>
@@ -541,7 +543,6 @@ template <class Epi>
 int run(const char* what, const MxGeometry& g, const typename Epi::Out& o, int row_tiles, hipStream_t st) {
   // z is written to the end of its last group of 512 columns
   const int units = Epi::kUnit == 2 ? mx_groups(row_tiles * 16) * (kMxGroup / kMxBlock) : row_tiles;
-  if (static_cast<int64_t>(units) * g.lane_groups > kMxMostGroups) return mx_refused(what, "rows and weights are too large together");
   // configuration
   // By the number of 16 x 16 products, of which the card's 256 CUs want four each before tiles pay.
   // Measured at 1 to 4096 rows of weights from 512 x 512 to 14336 x 4096, us here / as the next form:
@@ -558,13 +559,15 @@ int run(const char* what, const MxGeometry& g, const typename Epi::Out& o, int r
   //   256 x 128 where K is long and every CU has one: the fewest bytes a product, by which the clock
   //     stays up: 2048 x 8192 at 4096 rows 54 against 60 as 128 x 128, 4096 x 14336 166 against 192
   const int64_t products = static_cast<int64_t>(row_tiles) * Epi::kMats * g.lane_groups;
+  bool fits = true;  // the few of the first two do
   if (products <= (Epi::kMats == 2 ? 1280 : g.groups <= 4 ? 1536 : 768)) launch_row<Epi, 4 / Epi::kMats>(g, o, units, st);
   else if (Epi::kMats == 1 && products <= 1536) {
     if constexpr (Epi::kMats == 1) launch_tile<Epi, 1, 1, 2, 2, 3>(g, o, units, st);
-  } else if (products <= 6144) launch_pipe<Epi, 4, 1, 1, 4, 4, 2>(g, o, units, st);
-  else if (products <= 20480) launch_pipe<Epi, 4, 2, 2, 2, 4, 2>(g, o, units, st);
-  else if (products < 32768 || g.groups < 16) launch_pipe<Epi, 4, 4, 2, 2, 3, 2>(g, o, units, st);
-  else launch_pipe<Epi, 8, 4, 2, 2, 4, 1>(g, o, units, st);
+  } else if (products <= 6144) fits = launch_pipe<Epi, 4, 1, 1, 4, 4, 2>(g, o, units, st);
+  else if (products <= 20480) fits = launch_pipe<Epi, 4, 2, 2, 2, 4, 2>(g, o, units, st);
+  else if (products < 32768 || g.groups < 16) fits = launch_pipe<Epi, 4, 4, 2, 2, 3, 2>(g, o, units, st);
+  else fits = launch_pipe<Epi, 8, 4, 2, 2, 4, 1>(g, o, units, st);
+  if (!fits) return mx_refused(what, "rows and weights are too large together");
   return mx_launched(what);
 }
 

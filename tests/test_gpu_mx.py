@@ -566,6 +566,62 @@ def test_each_form_has_the_same_bits(m, n, k):
     assert torch.equal(caches[0].arena, caches[1].arena)
 
 
+LONG = 2 ** 18 + 37  # rows of 16384 values: offsets beyond 32 bits, in bytes and in elements
+
+
+def random_tiles(rows, cols, bits):
+    t = mx.Tiles.create(rows, cols, bits, DEV)
+    t.codes.random_(0, 256 if bits == 4 else 0x70)
+    t.scales.random_(115, 125)
+    return t
+
+
+def tail(t, first):
+    """The last tiles of a tensor or Tiles, in memory of their own."""
+    if isinstance(t, mx.Tiles):
+        return mx.Tiles(t.codes[first:].clone(), t.scales[first:].clone(), t.cols, t.bits)
+    return t[first:].clone()
+
+
+def same_ends(whole, part, first):
+    """The last tiles of a long result are those of a call on these rows alone."""
+    for a, b in ([(whole.codes, part.codes), (whole.scales, part.scales)] if isinstance(whole, mx.Tiles) else [(whole, part)]):
+        assert torch.equal(a[first:], b)
+
+
+def test_long_products():
+    first, rows = 2 ** 14 - 3, 37 + 48
+    say("x of 4 GiB")
+    x, w = random_tiles(LONG, 16384, 8), random_tiles(48, 16384, 4)
+    same_ends(mx.gemm(w, x, LONG), mx.gemm(w, tail(x, first), rows), first)
+    say("y of 8 GiB")
+    x, w = random_tiles(LONG, 512, 8), random_tiles(16384, 512, 4)
+    same_ends(mx.gemm(w, x, LONG), mx.gemm(w, tail(x, first), rows), first)
+    say("z of 4 GiB")
+    w3 = random_tiles(16384, 512, 4)
+    same_ends(mx.mlp13(w, w3, x, LONG), mx.mlp13(w, w3, tail(x, first), rows), first)
+
+
+def test_long_values():
+    first, rows = 2 ** 14 - 3, 37 + 48
+    say("h of 16 GiB")
+    h = torch.empty((2 ** 14 + 3, 1024, 16, 16), dtype=torch.float32, device=DEV).normal_()
+    add = torch.empty(h.shape, dtype=torch.bfloat16, device=DEV).normal_()
+    gains = torch.rand(16384, device=DEV)
+    part = tail(h, first)
+    same_ends(mx.norm(h, LONG, gains, 1e-5, add=add), mx.norm(part, rows, gains, 1e-5, add=tail(add, first)), first)
+    live = torch.arange(h[first:].numel(), device=DEV).view(part.shape)
+    live = (live // (1024 * 256) * 16 + live // 16 % 16) < rows
+    assert torch.equal(h[first:][live], part[live])
+    del h, part, live
+    for bits in (4, 8):
+        say("to", bits, "bits")
+        t = mx.quantize(add, LONG, bits=bits)
+        small = mx.quantize(tail(add, first), rows, bits=bits)
+        same_ends(t, small, first)
+        assert torch.equal(mx.dequantize(t, LONG)[first * 16:], mx.dequantize(small, rows))
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 def test_many_values(bits):
     """Where a workgroup takes a whole group: the values that the same tiles have in small calls."""
