@@ -51,8 +51,18 @@ class Tiles:
             raise ValueError("codes and scales must be contiguous uint8 on one device")
         if tuple(codes.shape) != (tiles, 4 * groups, *_PARTS[bits]) or tuple(scales.shape) != (tiles, groups, 4, 16, 4):
             raise ValueError(f"codes must be [tiles][{4 * groups}]{list(_PARTS[bits])} and scales [tiles][{groups}][4][16][4]")
-        self.codes, self.scales, self.cols, self.bits, self.tiles, self.rows = codes, scales, int(cols), bits, tiles, tiles * 16
+        self._codes, self._scales, self._cols, self._bits = codes, scales, int(cols), bits
+        self.tiles, self.rows = tiles, tiles * 16
         self._ref, self._device = _TILES(codes.data_ptr(), scales.data_ptr(), tiles, int(cols)), codes.get_device()
+
+    # what _ref stands for is not exchanged afterwards
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
+    cols = property(lambda self: self._cols)
+    bits = property(lambda self: self._bits)
+
+    def __reduce__(self):  # a copy has addresses of its own
+        return Tiles, (self._codes, self._scales, self._cols, self._bits)
 
     @staticmethod
     def create(rows: int, cols: int, bits: int, device) -> "Tiles":
@@ -77,7 +87,7 @@ def _here(dev: int) -> int:
 
 def _operand(t, bits: int, rows: int, dev: int, cols: int, name: str) -> bytes:
     """A Tiles argument's block, looked over (cols 0: any)."""
-    if type(t) is not Tiles or t.bits != bits or t._device != dev or t.rows < rows or (cols and t.cols != cols):
+    if type(t) is not Tiles or t._bits != bits or t._device != dev or t.rows < rows or (cols and t._cols != cols):
         raise ValueError(f"{name} must be Tiles in {bits} bits with the rows and columns of the call, on its device")
     return t._ref
 
@@ -192,7 +202,7 @@ def gemm(w: Tiles, x: Tiles, rows: int, out=None):
     dev = x._device
     stream = _here(dev)
     out = _y_tiles(out, rows, w.rows, x, dev)
-    p = _GEMM(rows, (rows + 15) // 16, 0, 0, _operand(x, 8, rows, dev, 0, "x"), _operand(w, 4, 1, dev, x.cols, "w"), out.data_ptr())
+    p = _GEMM(rows, (rows + 15) // 16, 0, 0, _operand(x, 8, rows, dev, 0, "x"), _operand(w, 4, 1, dev, x._cols, "w"), out.data_ptr())
     rc = _lib.packed().stride_mx_gemm(p, stream)
     if rc:
         _lib.check(rc)
@@ -204,8 +214,8 @@ def mlp13(w1: Tiles, w3: Tiles, x: Tiles, rows: int, out: Tiles | None = None) -
     dev = x._device
     stream = _here(dev)
     out = _result(out, rows, w1.rows, x)
-    p = _MLP13(rows, (rows + 15) // 16, 0, 0, _operand(x, 8, rows, dev, 0, "x"), _operand(w1, 4, 1, dev, x.cols, "w1"),
-               _operand(w3, 4, w1.rows, dev, x.cols, "w3"), _operand(out, 8, rows, dev, w1.rows, "out"))
+    p = _MLP13(rows, (rows + 15) // 16, 0, 0, _operand(x, 8, rows, dev, 0, "x"), _operand(w1, 4, 1, dev, x._cols, "w1"),
+               _operand(w3, 4, w1.rows, dev, x._cols, "w3"), _operand(out, 8, rows, dev, w1.rows, "out"))
     rc = _lib.packed().stride_mx_mlp13(p, stream)
     if rc:
         _lib.check(rc)
@@ -234,7 +244,7 @@ def qkv(wq: Tiles, wk: Tiles, wv: Tiles, x: Tiles, rows: int, head_dim: int, rop
     elif q_out.dtype != torch.float32 or q_out.dim() != 2 or q_out.shape[0] < rows or q_out.shape[1] != nq or q_out.stride(1) != 1 \
             or q_out.get_device() != dev:
         raise ValueError("q_out must be fp32 [rows][q columns], its rows contiguous")
-    ws = [_operand(w, 4, 1, dev, x.cols, name) for w, name in ((wq, "wq"), (wk, "wk"), (wv, "wv"))]
+    ws = [_operand(w, 4, 1, dev, x._cols, name) for w, name in ((wq, "wq"), (wk, "wk"), (wv, "wv"))]
     p = _QKV(rows, (rows + 15) // 16, 0, 0, _operand(x, 8, rows, dev, 0, "x"), *ws, q_out.data_ptr(), q_out.stride(0) if rows > 1 else nq,
              bytes(kv.ref), rope.data_ptr(), row_slot.data_ptr(), row_pos.data_ptr(), layer, head_dim)
     rc = _lib.packed().stride_mx_qkv(p, stream)

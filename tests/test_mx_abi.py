@@ -1,7 +1,9 @@
 """The microscaled operators' C ABI (include/stride_mx.h) without a GPU: exports, struct layouts,
 packed blocks, sizes, and every refusal that comes before a launch; the plain forms of the tests."""
+import copy
 import ctypes as C
 import os
+import pickle
 import re
 import struct
 import subprocess
@@ -91,6 +93,20 @@ def test_nothing_to_do_and_nothing_given():
                         ("mlp13", mx._MLP13(0, 0, 0, 0, t, t, t, t)), ("qkv", mx._QKV(0, 0, 0, 0, t, t, t, t, 0, 16, kv, 0, 0, 0, 0, 16))):
         assert call(name, block) == 0, name
         assert call(name, None) == _lib.EINVAL and "null" in err()
+
+
+def test_copies_of_tiles_have_their_own_memory():
+    """What a copied, pickled or loaded Tiles hands to a call is its own memory's address, and the
+    tensors behind an address are not exchanged."""
+    t = mx.Tiles.create(20, 528, 4, "cpu")
+    t.codes.fill_(3)
+    for other in (copy.deepcopy(t), pickle.loads(pickle.dumps(t)), copy.copy(t)):
+        assert other._ref == mx._TILES(other.codes.data_ptr(), other.scales.data_ptr(), 2, 528)
+        assert torch.equal(other.codes, t.codes) and (other.cols, other.bits, other.rows) == (528, 4, 32)
+    assert copy.deepcopy(t).codes.data_ptr() != t.codes.data_ptr()
+    for name in ("codes", "scales", "cols", "bits"):
+        with pytest.raises(AttributeError):
+            setattr(t, name, getattr(t, name))
 
 
 def test_launches_beyond_32_bits_of_threads():
