@@ -11,6 +11,7 @@
 #include <cstddef>
 
 #include "mx_common.hpp"
+#include "tc_epilogue.hpp"
 
 namespace stride_tc {
 namespace {
@@ -148,7 +149,8 @@ __global__ __launch_bounds__(1024) void k_mx_norm(StrideMxNormParams p, int chun
   extern __shared__ float sums[];  // [R][chunks]
   const Spot<R> s;
   constexpr int per = 4 / R;  // chunks of a wave
-  const int t = blockIdx.x / (16 / R), row = blockIdx.x % (16 / R) * R + s.row;
+  const int b = R < 4 ? xcd_remap(blockIdx.x, gridDim.x) : blockIdx.x;  // rows that share lines, on one XCD
+  const int t = b / (16 / R), row = b % (16 / R) * R + s.row;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int col_tiles = p.dim >> 4;
   const bool live = t * 16 + row < p.l.rows;
@@ -333,10 +335,12 @@ int stride_mx_norm(const StrideMxNormParams* p, void* stream) {
     return mx_refused(what, "pointers must be 16-byte aligned");
   const int chunks = mx_groups(p->dim) * 4;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  // A row a workgroup where rows are few, more where the reads are many, since neighbouring rows share
-  // their lines (us at R = 1 / 2 / 4 with an addition: 1 x 2048 2.7 / 2.9 / 3.7, 333 x 8192 15.9 / 9.7 /
-  // 12, 1024 x 2048 11.5 / 7.7 / 6.9, 4096 x 2048 37 / 24.6 / 19.9, 92 MB: 4.7 TB/s, a 4 GiB copy's 4.8).
-  if (p->l.rows <= 32) launch_norm<1>(*p, chunks, st);
+  // A row a workgroup while each can have a CU, and two while two rows can, four where the memory is
+  // full either way: neighbouring rows share their lines, from one XCD's L2 or in one workgroup (us at
+  // R = 1 / 2 / 4 with an addition: 1 x 2048 2.7 / 2.9 / 3.6, 256 x 8192 7.6 / 9.1 / 11.8, 333 x 8192 11.0 /
+  // 9.8 / 12.2, 512 x 4096 7.5 / 7.4 / 8.2, 1024 x 4096 12.2 / 11.4 / 10.1, 4096 x 2048 25.2 / 22.7 / 19.9,
+  // 92 MB: 4.7 TB/s, a 4 GiB copy's 4.8; dealt out over the XCDs in turn 256 x 8192 takes 11.8 at R = 1).
+  if (p->l.rows <= 256) launch_norm<1>(*p, chunks, st);
   else if (p->l.rows <= 512) launch_norm<2>(*p, chunks, st);
   else launch_norm<4>(*p, chunks, st);
   return mx_launched(what);
