@@ -551,22 +551,25 @@ int run(const char* what, const MxGeometry& g, const typename Epi::Out& o, int r
   //     2048 at 32 rows 4.1 against 4.9; gate and up 8192 x 2048 at 16 / 32 rows 5.6 / 7.1 against
   //     6.2 / 6.3 as 64 x 64
   //   32 x 32 to 1536: 4096 x 14336 at 64 rows 12.1 against 19 as 64 x 64
-  //   64 x 64 to 6144: 2048 x 8192 at 512 rows 13.6 against 15.5 as 128 x 64, at 1024 22.2 against 17.6
-  //   128 x 64 to 20480: 2048 x 8192 at 2048 rows 32.6 against 36.5 as 128 x 128, 8192 x 2048 40.7
-  //     against 37.4
-  //   128 x 128, two workgroups a CU whose ends hide each other: gate and up 8192 x 2048 at 2048 rows
-  //     62 against 68 as 256 x 128
-  //   256 x 128 where K is long and every CU has one: the fewest bytes a product, by which the clock
-  //     stays up: 2048 x 8192 at 4096 rows 54 against 60 as 128 x 128, 4096 x 14336 166 against 192
+  //   64 x 64 to 6144: 2048 x 8192 at 512 rows 13.6 against 15.4 as 128 x 64, at 1024 21.3 against 17.9
+  //   128 x 64 to 9216: 2048 x 8192 at 1024 rows 17.9 against 23.1 as 128 x 128, at 1280 27.2 against 24.4
+  //   128 x 128 of eight waves, by a workgroup a CU while 256 do: 2048 x 8192 at 2048 rows 29 against 32
+  //     by two and 40 as 256 x 128; by four waves 35
+  //   beyond, where K is short, by two workgroups a CU, whose ends hide each other: 8192 x 2048 at 2048
+  //     rows 33.6 against 35.2 as 256 x 128, gate and up 57.5 against 59; by four waves 36.7 and 60.5
+  //   256 x 128 where K is long: the fewest bytes a product, of which a CU reads 75 to 80 a ns from its
+  //     L2, and by which the clock stays up: 2048 x 8192 at 4096 rows 50.4 against 57.3 as 128 x 128, 4096
+  //     x 14336 160 against 181; by four waves, one a SIMD, 52.4 and 165
   const int64_t products = static_cast<int64_t>(row_tiles) * Epi::kMats * g.lane_groups;
   bool fits = true;  // the few of the first two do
   if (products <= (Epi::kMats == 2 ? 1280 : g.groups <= 4 ? 1536 : 768)) launch_row<Epi, 4 / Epi::kMats>(g, o, units, st);
   else if (Epi::kMats == 1 && products <= 1536) {
     if constexpr (Epi::kMats == 1) launch_tile<Epi, 1, 1, 2, 2, 3>(g, o, units, st);
   } else if (products <= 6144) fits = launch_pipe<Epi, 4, 1, 1, 4, 4, 2>(g, o, units, st);
-  else if (products <= 20480) fits = launch_pipe<Epi, 4, 2, 2, 2, 4, 2>(g, o, units, st);
-  else if (products < 32768 || g.groups < 16) fits = launch_pipe<Epi, 4, 4, 2, 2, 3, 2>(g, o, units, st);
-  else fits = launch_pipe<Epi, 8, 4, 2, 2, 4, 1>(g, o, units, st);
+  else if (products <= 9216) fits = launch_pipe<Epi, 4, 2, 2, 2, 4, 2>(g, o, units, st);
+  else if (products <= 16384) fits = launch_pipe<Epi, 4, 2, 2, 4, 4, 2>(g, o, units, st);
+  else if (g.groups < 8) fits = launch_pipe<Epi, 4, 2, 2, 4, 3, 4>(g, o, units, st);
+  else fits = launch_pipe<Epi, 8, 2, 2, 4, 4, 2>(g, o, units, st);
   if (!fits) return mx_refused(what, "rows and weights are too large together");
   return mx_launched(what);
 }

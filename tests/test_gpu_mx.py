@@ -529,7 +529,7 @@ def rows_alone(x, first, n):
 
 @pytest.mark.parametrize("m,n,k", [
     (40, 2048, 512), (100, 256, 8192), (150, 2048, 4096), (200, 1024, 1024), (600, 2048, 1024), (1000, 1552, 528),
-    (1400, 4096, 512), (1400, 2064, 2064), (2100, 4096, 8192)])
+    (1400, 4096, 512), (1400, 2064, 2064), (2100, 4096, 8192), (440, 2064, 528), (870, 2064, 1040), (2600, 2064, 4112)])
 def test_each_form_has_the_same_bits(m, n, k):
     """From waves of their own to 256 x 128 tiles, ragged ones among them: every row as in a batch of
     16, which is a wave's of its own; lanes behind the rows stay as they were."""
