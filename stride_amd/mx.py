@@ -106,8 +106,9 @@ def _allocates() -> None:
 
 def _tile_cols(t, rows: int, name: str) -> int:
     """Columns of tiles [ceil(rows / 16)][cols / 16][16][16]."""
-    if t.dim() == 4 and t.is_contiguous():
-        tiles, col_tiles, a, b = t.shape
+    shape = t.shape
+    if len(shape) == 4 and t.is_contiguous():
+        tiles, col_tiles, a, b = shape
         if a == 16 and b == 16 and tiles * 16 >= rows and col_tiles:
             return col_tiles * 16
     raise ValueError(f"{name} must be contiguous tiles [ceil(rows / 16)][cols / 16][16][16]")
