@@ -106,7 +106,8 @@ int stride_mx_mlp13(const StrideMxMlp13Params* p, void* stream);
 /* stride_tc_qkv on these weights (rows in the RoPE order): q in fp32, K and V into the bf16
  * cache. A row whose slot or position is below 0, or whose position lies behind the table's blocks,
  * is left out: nothing of it is kept, and its q stays as it was. Otherwise row_slot is a row of the
- * table, row_pos one of the rope table, and a table entry below 0 keeps nothing of K and V.
+ * table, row_pos one of the rope table (stride_mx_qkv_within looks), and a table entry below 0 keeps
+ * nothing of K and V; the others are pages of the arena.
  * Of two rows at one place of the cache either may be kept, or parts of both. */
 typedef struct StrideMxQkvParams {
   StrideLanes l;
@@ -122,6 +123,10 @@ typedef struct StrideMxQkvParams {
 } StrideMxQkvParams;
 
 int stride_mx_qkv(const StrideMxQkvParams* p, void* stream);
+
+/* The same with a page table of `slots` rows and a rope table of `positions`: rows beyond either are
+ * left out too, so that no row_slot or row_pos is read or written behind an end. */
+int stride_mx_qkv_within(const StrideMxQkvParams* p, int32_t slots, int32_t positions, void* stream);
 
 #ifdef __cplusplus
 }

@@ -246,6 +246,7 @@ MX_ENTRIES = {  # include/stride_mx.h
     "stride_mx_gemm": (C.c_int, [_VP, _VP]),
     "stride_mx_mlp13": (C.c_int, [_VP, _VP]),
     "stride_mx_qkv": (C.c_int, [_VP, _VP]),
+    "stride_mx_qkv_within": (C.c_int, [_VP, _I32, _I32, _VP]),
 }
 
 

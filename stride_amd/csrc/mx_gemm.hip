@@ -59,14 +59,17 @@ struct EpiY {
 
 struct EpiRope {
   static constexpr int kMats = 1, kUnit = 1;
-  using Out = EpiQkv::Out;
+  struct Out : EpiQkv::Out {
+    int32_t slots, positions;  // rows of the page table and of the rope table
+  };
   __device__ __forceinline__ static void finish(const Out& o, const MxGeometry& g, int rt, int lt, const f32x4 (&y)[1][1], int lane) {
-    // a lane whose row has no place in the cache has none here either
+    // A lane whose row has no place in the cache has none here either: past this neither table is read
+    // behind its end (the cache's last page may hold positions that rope has no row for).
     const int j = lt * 16 + (lane & 15);
     bool live = j < g.rows;
     if (live) {
-      const int pos = o.row_pos[j];
-      live = pos >= 0 && (pos >> o.page_shift) < o.kv.max_blocks && o.row_slot[j] >= 0;
+      const int pos = o.row_pos[j], slot = o.row_slot[j];
+      live = pos >= 0 && pos < o.positions && (pos >> o.page_shift) < o.kv.max_blocks && slot >= 0 && slot < o.slots;
     }
     Geometry rows{};
     rows.rows = live ? g.rows : 0;
@@ -629,10 +632,13 @@ int stride_mx_mlp13(const StrideMxMlp13Params* p, void* stream) {
   return run<EpiZ>(what, g, EpiZ::Out{p->z}, p->w1.tiles, static_cast<hipStream_t>(stream));
 }
 
-int stride_mx_qkv(const StrideMxQkvParams* p, void* stream) {
+int stride_mx_qkv(const StrideMxQkvParams* p, void* stream) { return stride_mx_qkv_within(p, INT_MAX, INT_MAX, stream); }
+
+int stride_mx_qkv_within(const StrideMxQkvParams* p, int32_t slots, int32_t positions, void* stream) {
   const char* what = "mx_qkv";
   if (!p) return mx_refused(what, "null parameters");
   if (!mx_lanes_ok(p->l)) return mx_refused(what, "need rows >= 0 and lane_groups = ceil(rows/16)");
+  if (slots < 0 || positions < 0) return mx_refused(what, "slots and positions are counts");
   if (p->l.rows == 0) return 0;
   MxGeometry g;
   const StrideMxTiles* w[] = {&p->q, &p->k, &p->v};
@@ -649,7 +655,9 @@ int stride_mx_qkv(const StrideMxQkvParams* p, void* stream) {
   int shift = 0;
   while ((int64_t{1} << shift) < page) ++shift;
   if ((int64_t{1} << shift) != page) return mx_refused(what, "KV page size (group_elems/head_dim) must be a power of two");
-  EpiQkv::Out o{};
+  EpiRope::Out o{};
+  o.slots = slots;
+  o.positions = positions;
   o.q_out = p->q_out;
   o.q_stride = static_cast<int32_t>(p->q_stride);
   o.layer = p->layer;

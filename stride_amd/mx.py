@@ -226,8 +226,8 @@ def mlp13(w1: Tiles, w3: Tiles, x: Tiles, rows: int, out: Tiles | None = None) -
 def qkv(wq: Tiles, wk: Tiles, wv: Tiles, x: Tiles, rows: int, head_dim: int, rope, row_slot, row_pos, kv: PagedKv, layer: int = 0,
         q_out=None):
     """harness.qkv on these weights (rows in layout.rope_rows' order): q with RoPE in fp32 rows, K
-    and V appended to the paged bf16 cache. A row whose slot or position is below 0, or whose position
-    lies behind the table, is left out, its q as it was."""
+    and V appended to the paged bf16 cache. A row is left out, its q as it was, where its slot is no row
+    of kv.table or its position lies behind the cache's last page or behind rope."""
     dev, nq = x._device, wq.rows
     stream = _here(dev)
     if row_slot.dtype != torch.int32 or row_pos.dtype != torch.int32 or row_slot.numel() < rows or row_pos.numel() < rows \
@@ -248,7 +248,7 @@ def qkv(wq: Tiles, wk: Tiles, wv: Tiles, x: Tiles, rows: int, head_dim: int, rop
     ws = [_operand(w, 4, 1, dev, x._cols, name) for w, name in ((wq, "wq"), (wk, "wk"), (wv, "wv"))]
     p = _QKV(rows, (rows + 15) // 16, 0, 0, _operand(x, 8, rows, dev, 0, "x"), *ws, q_out.data_ptr(), q_out.stride(0) if rows > 1 else nq,
              bytes(kv.ref), rope.data_ptr(), row_slot.data_ptr(), row_pos.data_ptr(), layer, head_dim)
-    rc = _lib.packed().stride_mx_qkv(p, stream)
+    rc = _lib.packed().stride_mx_qkv_within(p, kv.table.shape[0], rope.shape[0], stream)
     if rc:
         _lib.check(rc)
     return q_out
