@@ -20,6 +20,8 @@
  *   8-bit codes  [tile][4 G][2 halves][4 parts of 16 columns][16 rows][16 bytes]
  *   scales       [tile][G][4 blocks of a chunk][16 rows][4 chunks]
  * All of a tile's rows below `rows` are written, their filling too; the others are left alone.
+ * A result lies on no other argument of its call, and what shares memory with values, blocks or weights
+ * is refused; only a norm's x may be its add.
  *
  * Batch invariance: a row's result depends on the row and the weights only. A product's K is
  * summed in chunks of 128 columns, one scaled matrix instruction each, that chain in ascending

@@ -2,6 +2,7 @@
 // (include/stride_mx.h has the formats and layouts).
 #pragma once
 
+#include <initializer_list>
 #include <string>
 
 #include "../../include/stride_mx.h"
@@ -74,6 +75,26 @@ inline const char* mx_why_not(const StrideMxTiles& t, int64_t tiles, int cols) {
   if (!t.codes || !t.scales) return "missing pointer";
   if (reinterpret_cast<uintptr_t>(t.codes) % 16 || reinterpret_cast<uintptr_t>(t.scales) % 4) return "codes must be 16-byte and scales 4-byte aligned";
   return nullptr;
+}
+
+// Host: memory that a call reads or writes, and whether a result shares some with another operand: other
+// workgroups read that one at any time.
+struct MxSpan {
+  const void* at;
+  int64_t bytes;
+};
+inline MxSpan mx_codes(const StrideMxTiles& t, int64_t tiles, int bits) {
+  return {t.codes, tiles * mx_groups(t.cols) * 4 * (bits == 4 ? kCode4Bytes : kCode8Bytes)};
+}
+inline MxSpan mx_scales(const StrideMxTiles& t, int64_t tiles) { return {t.scales, tiles * mx_groups(t.cols) * kScaleBytes}; }
+
+inline bool mx_overlap(std::initializer_list<MxSpan> results, std::initializer_list<MxSpan> operands) {
+  for (const MxSpan& r : results)
+    for (const MxSpan& o : operands) {
+      const uintptr_t a = reinterpret_cast<uintptr_t>(r.at), b = reinterpret_cast<uintptr_t>(o.at);
+      if (a && b && a < b + o.bytes && b < a + r.bytes) return true;
+    }
+  return false;
 }
 
 inline int mx_refused(const char* what, const char* why) { return fail(STRIDE_TC_EINVAL, std::string(what) + ": " + why); }

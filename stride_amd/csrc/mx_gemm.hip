@@ -527,12 +527,13 @@ void launch_row(const MxGeometry& g, const typename Epi::Out& o, int units, hipS
 }
 
 template <class Epi, int A, int L, int WM, int WN, int NS, int OCC>
-bool launch_pipe(const MxGeometry& g, const typename Epi::Out& o, int units, hipStream_t st) {
+const char* launch_pipe(const MxGeometry& g, const typename Epi::Out& o, int units, const char* clash, hipStream_t st) {
   constexpr int per = WM * A / Epi::kMats / Epi::kUnit;
   const int unit_blocks = (units + per - 1) / per, lane_blocks = (g.lane_groups + WN * L - 1) / (WN * L);
-  if (static_cast<int64_t>(unit_blocks) * lane_blocks > kMxMostGroups * 1024 / (64 * WM * WN)) return false;
+  if (static_cast<int64_t>(unit_blocks) * lane_blocks > kMxMostGroups * 1024 / (64 * WM * WN)) return "rows and weights are too large together";
+  if (clash) return clash;
   hipLaunchKernelGGL((k_mx_pipe<Epi, A, L, WM, WN, NS, OCC>), dim3(unit_blocks * lane_blocks), dim3(64 * WM * WN), 0, st, g, o, units, unit_blocks, lane_blocks);
-  return true;
+  return nullptr;
 }
 
 template <class Epi, int A, int L, int WM, int WN, int NS>
@@ -542,8 +543,16 @@ void launch_tile(const MxGeometry& g, const typename Epi::Out& o, int units, hip
   hipLaunchKernelGGL((k_mx_tile<Epi, A, L, WM, WN, NS>), dim3(unit_blocks * lane_blocks), dim3(64 * WM * WN), 0, st, g, o, units, unit_blocks, lane_blocks);
 }
 
+// Host: does a result lie on x or on one of the weights? (Other workgroups read them until the end.)
+bool overlaps(std::initializer_list<MxSpan> results, const StrideLanes& l, const StrideMxTiles& x, const StrideMxTiles* const* w, int n) {
+  bool any = mx_overlap(results, {mx_codes(x, l.lane_groups, 8), mx_scales(x, l.lane_groups)});
+  for (int i = 0; i < n; ++i) any = any || mx_overlap(results, {mx_codes(*w[i], w[i]->tiles, 4), mx_scales(*w[i], w[i]->tiles)});
+  return any;
+}
+
+// `clash`: why the memory of the call's arguments is refused, or NULL.
 template <class Epi>
-int run(const char* what, const MxGeometry& g, const typename Epi::Out& o, int row_tiles, hipStream_t st) {
+int run(const char* what, const MxGeometry& g, const typename Epi::Out& o, int row_tiles, const char* clash, hipStream_t st) {
   // z is written to the end of its last group of 512 columns
   const int units = Epi::kUnit == 2 ? mx_groups(row_tiles * 16) * (kMxGroup / kMxBlock) : row_tiles;
   // configuration
@@ -564,16 +573,17 @@ int run(const char* what, const MxGeometry& g, const typename Epi::Out& o, int r
   //     L2, and by which the clock stays up: 2048 x 8192 at 4096 rows 50.4 against 57.3 as 128 x 128, 4096
   //     x 14336 160 against 181; by four waves, one a SIMD, 52.4 and 165
   const int64_t products = static_cast<int64_t>(row_tiles) * Epi::kMats * g.lane_groups;
-  bool fits = true;  // the few of the first two do
+  if (clash && products <= 1536) return mx_refused(what, clash);  // a launch of these fits
+  const char* why = nullptr;
   if (products <= (Epi::kMats == 2 ? 1280 : g.groups <= 4 ? 1536 : 768)) launch_row<Epi, 4 / Epi::kMats>(g, o, units, st);
   else if (Epi::kMats == 1 && products <= 1536) {
     if constexpr (Epi::kMats == 1) launch_tile<Epi, 1, 1, 2, 2, 3>(g, o, units, st);
-  } else if (products <= 6144) fits = launch_pipe<Epi, 4, 1, 1, 4, 4, 2>(g, o, units, st);
-  else if (products <= 9216) fits = launch_pipe<Epi, 4, 2, 2, 2, 4, 2>(g, o, units, st);
-  else if (products <= 16384) fits = launch_pipe<Epi, 4, 2, 2, 4, 4, 2>(g, o, units, st);
-  else if (g.groups < 8) fits = launch_pipe<Epi, 4, 2, 2, 4, 3, 4>(g, o, units, st);
-  else fits = launch_pipe<Epi, 8, 2, 2, 4, 4, 2>(g, o, units, st);
-  if (!fits) return mx_refused(what, "rows and weights are too large together");
+  } else if (products <= 6144) why = launch_pipe<Epi, 4, 1, 1, 4, 4, 2>(g, o, units, clash, st);
+  else if (products <= 9216) why = launch_pipe<Epi, 4, 2, 2, 2, 4, 2>(g, o, units, clash, st);
+  else if (products <= 16384) why = launch_pipe<Epi, 4, 2, 2, 4, 4, 2>(g, o, units, clash, st);
+  else if (g.groups < 8) why = launch_pipe<Epi, 4, 2, 2, 4, 3, 4>(g, o, units, clash, st);
+  else why = launch_pipe<Epi, 8, 2, 2, 4, 4, 2>(g, o, units, clash, st);
+  if (why) return mx_refused(what, why);
   return mx_launched(what);
 }
 
@@ -614,7 +624,8 @@ int stride_mx_gemm(const StrideMxGemmParams* p, void* stream) {
   const StrideMxTiles* w[] = {&p->w};
   if (const char* why = operands(p->l, p->x, w, 1, g)) return mx_refused(what, why);
   if (!p->y || reinterpret_cast<uintptr_t>(p->y) % 16) return mx_refused(what, "y must be there, 16-byte aligned");
-  return run<EpiY>(what, g, EpiY::Out{p->y, p->w.tiles}, p->w.tiles, static_cast<hipStream_t>(stream));
+  const bool clash = overlaps({{p->y, p->l.lane_groups * int64_t{2} * kTileElems * p->w.tiles}}, p->l, p->x, w, 1);
+  return run<EpiY>(what, g, EpiY::Out{p->y, p->w.tiles}, p->w.tiles, clash ? "y must not overlap x or w" : nullptr, static_cast<hipStream_t>(stream));
 }
 
 int stride_mx_mlp13(const StrideMxMlp13Params* p, void* stream) {
@@ -629,7 +640,8 @@ int stride_mx_mlp13(const StrideMxMlp13Params* p, void* stream) {
   if (p->w1.tiles > (1 << 16)) return mx_refused(what, "too many row tiles");
   if (const char* why = mx_why_not(p->z, p->l.lane_groups, p->w1.tiles * 16)) return mx_refused(what, why);
   if (p->z.codes == p->x.codes) return mx_refused(what, "z must not be x");
-  return run<EpiZ>(what, g, EpiZ::Out{p->z}, p->w1.tiles, static_cast<hipStream_t>(stream));
+  const bool clash = overlaps({mx_codes(p->z, p->l.lane_groups, 8), mx_scales(p->z, p->l.lane_groups)}, p->l, p->x, w, 2);
+  return run<EpiZ>(what, g, EpiZ::Out{p->z}, p->w1.tiles, clash ? "z must not overlap x, w1 or w3" : nullptr, static_cast<hipStream_t>(stream));
 }
 
 int stride_mx_qkv(const StrideMxQkvParams* p, void* stream) { return stride_mx_qkv_within(p, INT_MAX, INT_MAX, stream); }
@@ -667,7 +679,11 @@ int stride_mx_qkv_within(const StrideMxQkvParams* p, int32_t slots, int32_t posi
   o.rope = p->rope;
   o.row_slot = p->row_slot;
   o.row_pos = p->row_pos;
-  return run<EpiRope>(what, g, o, p->q.tiles + p->k.tiles + p->v.tiles, static_cast<hipStream_t>(stream));
+  const int64_t q_cols = static_cast<int64_t>(p->q.tiles) * 16;
+  const MxSpan q = {p->q_out, ((p->l.rows - 1) * p->q_stride + q_cols) * 4}, rope = {p->rope, positions == INT_MAX ? 0 : positions * int64_t{4} * D};
+  const int64_t words = p->l.rows * int64_t{4};
+  const bool clash = overlaps({q}, p->l, p->x, w, 3) || mx_overlap({q}, {{p->row_slot, words}, {p->row_pos, words}, rope});
+  return run<EpiRope>(what, g, o, p->q.tiles + p->k.tiles + p->v.tiles, clash ? "q_out must not overlap x, the weights or what describes the rows" : nullptr, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -291,6 +291,9 @@ int stride_mx_quantize(const StrideMxQuantizeParams* p, void* stream) {
   const int chunks = mx_groups(p->out.cols) * 4;
   const int64_t all = static_cast<int64_t>(chunks) * p->l.lane_groups;
   if (all > 4 * kMxMostGroups) return mx_refused(what, "rows and cols are too large together");
+  const int64_t lt = p->l.lane_groups;
+  if (mx_overlap({mx_codes(p->out, lt, p->bits), mx_scales(p->out, lt)}, {{p->src, lt * kTileElems * (p->out.cols / 16) * p->src_bytes}}))
+    return mx_refused(what, "out and src must not overlap");
   const dim3 grid(static_cast<unsigned>(all)), block(256);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const uint16_t* half = static_cast<const uint16_t*>(p->src);
@@ -311,8 +314,12 @@ int stride_mx_dequantize(const StrideMxDequantizeParams* p, void* stream) {
   if (const char* why = mx_why_not(p->in, p->l.lane_groups, 0)) return mx_refused(what, why);
   if (!p->out || reinterpret_cast<uintptr_t>(p->out) % 16) return mx_refused(what, "out must be there, 16-byte aligned");
   if (p->out_stride < p->in.cols || p->out_stride % 8) return mx_refused(what, "out_stride must be a multiple of 8, at least cols");
+  if (p->out_stride > INT64_MAX / 8 / p->l.rows) return mx_refused(what, "out_stride is too large for the rows");
   const int groups = mx_groups(p->in.cols);
   if (static_cast<int64_t>(groups) * 4 * p->l.lane_groups > 4 * kMxMostGroups) return mx_refused(what, "rows and cols are too large together");
+  const int64_t lt = p->l.lane_groups;
+  if (mx_overlap({{p->out, ((p->l.rows - 1) * p->out_stride + p->in.cols) * p->out_bytes}}, {mx_codes(p->in, lt, p->bits), mx_scales(p->in, lt)}))
+    return mx_refused(what, "out and in must not overlap");
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (p->bits == 4 && p->out_bytes == 2) launch_values<4, uint16_t>(*p, groups, st);
   else if (p->bits == 4) launch_values<4, float>(*p, groups, st);
@@ -333,6 +340,13 @@ int stride_mx_norm(const StrideMxNormParams* p, void* stream) {
     if (const char* why = mx_why_not(p->out, p->l.lane_groups, p->dim)) return mx_refused(what, why);
   if ((reinterpret_cast<uintptr_t>(p->h) | reinterpret_cast<uintptr_t>(p->add) | reinterpret_cast<uintptr_t>(p->weight) | reinterpret_cast<uintptr_t>(p->x)) % 16)
     return mx_refused(what, "pointers must be 16-byte aligned");
+  const int64_t lt = p->l.lane_groups, values = lt * kTileElems * (p->dim / 16);
+  const MxSpan h = {p->h, values * 4}, add = {p->add, values * 2}, weight = {p->weight, p->dim * int64_t{4}}, x = {p->x, values * 2};
+  const MxSpan codes = mx_codes(p->out, lt, 8), scales = mx_scales(p->out, lt);
+  // x in add's place is served: a thread reads its own values of it before it writes them
+  if (mx_overlap({h}, {add, weight}) || mx_overlap({codes, scales, x}, {h, weight}) || mx_overlap({codes, scales}, {add}) ||
+      (p->x != p->add && mx_overlap({x}, {add})))
+    return mx_refused(what, "h, add, weight and the result must not overlap");
   const int chunks = mx_groups(p->dim) * 4;
   hipStream_t st = static_cast<hipStream_t>(stream);
   // A row a workgroup while each can have a CU, and two while two rows can, four where the memory is

@@ -1,11 +1,12 @@
 """Calls of stride_amd.mx at the borders of what they were given: rows beyond the page table or the rope
-table."""
+table, results beside and on their operands."""
 import numpy as np
 import pytest
 import torch
 
 import test_gpu_mx as plain
-from stride_amd import harness, mx
+from stride_amd import harness, layout, mx
+from stride_amd._lib import StrideTcError
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -50,3 +51,62 @@ def test_qkv_rows_beyond_the_tables(m):
     whole = harness.PagedKv.over(kv.arena, kv.table._base if kv.table._base is not None else kv.table, 2, 64, 2, 16)
     mx.qkv(*ws, x, m, 64, long_rope, plain.dev(slot), plain.dev(pos), whole, layer=1, q_out=q)
     assert whole.slots == 11 and not (q == 99).all(1).any()
+
+
+def carved(buf, at, rows, cols, bits):
+    """Tiles in a buffer of bytes from `at` on, codes then scales; and where they end."""
+    like = mx.Tiles.create(rows, cols, bits, "cpu")
+    c, s = like.codes.numel(), like.scales.numel()
+    return mx.Tiles(buf[at:at + c].view(like.codes.shape), buf[at + c:at + c + s].view(like.scales.shape), cols, bits), at + c + s
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 96, 528), (300, 1040, 528)])
+def test_results_beside_their_operands(m, n, k):
+    """Operands and results end to end in one buffer, as a workspace is dealt out, have the bits that
+    they have in buffers of their own; a byte less and they are refused."""
+    print("beside", m, n, k, flush=True)
+    rng = np.random.default_rng(m)
+    w, w3, x = plain.held(plain.weights_of(rng, n, k), 4), plain.held(plain.weights_of(rng, n, k), 4), plain.held(plain.acts_of(rng, m, k), 8)
+    want_y, want_z = mx.gemm(w, x, m), mx.mlp13(w, w3, x, m)
+    T = (m + 15) // 16
+    buf = torch.zeros(64 << 20, dtype=torch.uint8, device=DEV)
+    bx, at = carved(buf, 0, m, k, 8)
+    bz, at = carved(buf, at, m, n, 8)
+    bw, at = carved(buf, at, n, k, 4)
+    y = buf[at:at + T * 16 * n * 2].view(torch.int16).view(T, n // 16, 16, 16)
+    at += T * 16 * n * 2
+    bw3, at = carved(buf, at, n, k, 4)
+    for t, of in ((bx, x), (bw, w), (bw3, w3)):
+        t.codes.copy_(of.codes)
+        t.scales.copy_(of.scales)
+    mx.gemm(bw, bx, m, out=y)
+    mx.mlp13(bw, bw3, bx, m, out=bz)
+    live = lambda a: layout.untile_lanes(a.cpu(), m)
+    assert torch.equal(live(y), live(want_y))
+    for a, b in ((bz, want_z),):
+        got, want = plain.mx_plain.unpack(a.codes.cpu().numpy(), a.scales.cpu().numpy(), 8), plain.mx_plain.unpack(b.codes.cpu().numpy(), b.scales.cpu().numpy(), 8)
+        assert all(np.array_equal(p[:m], q[:m]) for p, q in zip(got, want))
+    back = mx.dequantize(bx, m, out=buf[at:at + m * k * 2].view(torch.bfloat16).view(m, k))
+    assert torch.equal(back, mx.dequantize(x, m))
+    last, _ = carved(buf, x.nbytes - 16, m, n, 8)
+    with pytest.raises(StrideTcError, match="overlap"):
+        mx.mlp13(bw, bw3, bx, m, out=last)
+    with pytest.raises(StrideTcError, match="overlap"):
+        mx.gemm(bw, bx, m, out=buf[x.nbytes - 16:x.nbytes - 16 + y.numel() * 2].view(torch.int16).view(y.shape))
+
+
+@pytest.mark.parametrize("m,dim", [(5, 528), (300, 2064), (600, 8208), (5, 33296)])
+def test_norm_in_the_place_of_its_addition(m, dim):
+    """bf16 x tiles written over `add`: the bits of a result of its own."""
+    print("in place", m, dim, flush=True)
+    gen = torch.Generator(device=DEV).manual_seed(dim)
+    T = (m + 15) // 16
+    h = torch.randn((T, dim // 16, 16, 16), generator=gen, device=DEV)
+    add = torch.randn(h.shape, generator=gen, device=DEV).to(torch.bfloat16)
+    gain = torch.rand(dim, generator=gen, device=DEV)
+    h2 = h.clone()
+    want = mx.norm(h, m, gain, 1e-5, add=add, bits=16)
+    got = mx.norm(h2, m, gain, 1e-5, add=add, out=add, bits=16).view(torch.int16)
+    assert torch.equal(h, h2) and torch.equal(layout.untile_lanes(got.cpu(), m), layout.untile_lanes(want.cpu(), m))
+    with pytest.raises(StrideTcError, match="overlap"):
+        mx.norm(h, m, gain, 1e-5, out=h.view(torch.int16).view(-1)[:add.numel()].view(add.shape), bits=16)
