@@ -85,9 +85,22 @@ def _here(dev: int) -> int:
     return _stream_of(dev) if tc._stream is None else tc.kernel_stream()
 
 
+def _tiles(t, name: str) -> int:
+    """The device of a Tiles argument."""
+    if type(t) is not Tiles:
+        raise ValueError(f"{name} must be Tiles")
+    return t._device
+
+
+def _tensor(t, name: str):
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a tensor")
+    return t
+
+
 def _operand(t, bits: int, rows: int, dev: int, cols: int, name: str) -> bytes:
     """A Tiles argument's block, looked over (cols 0: any)."""
-    if type(t) is not Tiles or t._bits != bits or t._device != dev or t.rows < rows or (cols and t._cols != cols):
+    if type(t) is not Tiles or t._bits != bits or t._device != dev or not 0 <= rows <= t.rows or (cols and t._cols != cols):
         raise ValueError(f"{name} must be Tiles in {bits} bits with the rows and columns of the call, on its device")
     return t._ref
 
@@ -109,7 +122,7 @@ def _tile_cols(t, rows: int, name: str) -> int:
     shape = t.shape
     if len(shape) == 4 and t.is_contiguous():
         tiles, col_tiles, a, b = shape
-        if a == 16 and b == 16 and tiles * 16 >= rows and col_tiles:
+        if a == 16 and b == 16 and 0 <= rows <= tiles * 16 and col_tiles:
             return col_tiles * 16
     raise ValueError(f"{name} must be contiguous tiles [ceil(rows / 16)][cols / 16][16][16]")
 
@@ -119,7 +132,7 @@ def _y_tiles(out, rows: int, cols: int, like, dev: int):
     if out is None:
         _allocates()
         return torch.zeros(((rows + 15) // 16, cols // 16, 16, 16), dtype=torch.int16, device=getattr(like, "codes", like).device)
-    if out.dtype not in _BF16 or out.get_device() != dev or _tile_cols(out, rows, "out") != cols:
+    if _tensor(out, "out").dtype not in _BF16 or out.get_device() != dev or _tile_cols(out, rows, "out") != cols:
         raise ValueError(f"out must be 16-bit tiles of {cols} columns on the call's device")
     return out
 
@@ -127,7 +140,7 @@ def _y_tiles(out, rows: int, cols: int, like, dev: int):
 def quantize(tiles, rows: int | None = None, bits: int = 4, out: Tiles | None = None) -> Tiles:
     """Tiles [t][ct][16][16] of 16-bit (bf16, or its bits in int16) or fp32 values to blocks of 4
     or 8 bits, for the first `rows` rows (default: all)."""
-    if tiles.dtype in _BF16:
+    if _tensor(tiles, "tiles").dtype in _BF16:
         size = 2
     elif tiles.dtype == torch.float32:
         size = 4
@@ -137,7 +150,7 @@ def quantize(tiles, rows: int | None = None, bits: int = 4, out: Tiles | None = 
         raise ValueError("blocks have 4 or 8 bits")
     dev = tiles.get_device()
     stream = _here(dev)
-    rows = tiles.shape[0] * 16 if rows is None else rows
+    rows = len(tiles) * 16 if rows is None and tiles.dim() else rows
     cols = _tile_cols(tiles, rows, "tiles")
     if out is None:
         _allocates()
@@ -153,15 +166,15 @@ def dequantize(t: Tiles, rows: int | None = None, dtype=torch.bfloat16, out=None
     """The values of the first `rows` rows, row-major [rows][cols] in bf16 or fp32."""
     if dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("values come in bf16 or fp32")
-    stream = _here(t._device)
+    stream = _here(_tiles(t, "t"))
     rows = t.rows if rows is None else rows
+    ref = _operand(t, t.bits, rows, t._device, 0, "t")
     if out is None:
         _allocates()
         out = torch.empty((rows, t.cols), dtype=dtype, device=t.codes.device)
-    elif out.dtype != dtype or out.dim() != 2 or out.shape[0] < rows or out.shape[1] != t.cols or out.stride(1) != 1 or out.get_device() != t._device:
+    elif _tensor(out, "out").dtype != dtype or out.dim() != 2 or out.shape[0] < rows or out.shape[1] != t.cols or out.stride(1) != 1 or out.get_device() != t._device:
         raise ValueError("out must be [rows][cols] of that type on the same device, its rows contiguous")
-    p = _DEQUANTIZE(rows, (rows + 15) // 16, 0, 0, _operand(t, t.bits, rows, t._device, 0, "t"), out.data_ptr(),
-                    out.stride(0) if rows > 1 else t.cols, t.bits, 2 if dtype == torch.bfloat16 else 4)
+    p = _DEQUANTIZE(rows, (rows + 15) // 16, 0, 0, ref, out.data_ptr(), out.stride(0) if rows > 1 else t.cols, t.bits, 2 if dtype == torch.bfloat16 else 4)
     rc = _lib.packed().stride_mx_dequantize(p, stream)
     if rc:
         _lib.check(rc)
@@ -171,16 +184,16 @@ def dequantize(t: Tiles, rows: int | None = None, dtype=torch.bfloat16, out=None
 def norm(h, rows: int, weight, eps: float, add=None, out=None, bits: int = 8):
     """h += add (bf16 tiles, where given), then RMSNorm(h) * weight: in 8 bits (Tiles), or with
     bits=16 in bf16 x tiles. h: fp32 tiles [lt][ct][16][16]."""
-    dev = h.get_device()
+    dev = _tensor(h, "h").get_device()
     stream = _here(dev)
     if h.dtype != torch.float32:
         raise ValueError("h must be fp32 tiles")
     cols = _tile_cols(h, rows, "h")
-    if weight.dtype != torch.float32 or weight.numel() != cols or not weight.is_contiguous() or weight.get_device() != dev:
+    if _tensor(weight, "weight").dtype != torch.float32 or weight.numel() != cols or not weight.is_contiguous() or weight.get_device() != dev:
         raise ValueError("weight must be contiguous fp32 of h's columns, on its device")
     a = 0
     if add is not None:
-        if add.dtype not in _BF16 or add.get_device() != dev or _tile_cols(add, rows, "add") != cols:
+        if _tensor(add, "add").dtype not in _BF16 or add.get_device() != dev or _tile_cols(add, rows, "add") != cols:
             raise ValueError("add must be bf16 tiles of h's columns on its device")
         a = add.data_ptr()
     if bits == 8:
@@ -200,10 +213,11 @@ def norm(h, rows: int, weight, eps: float, add=None, out=None, bits: int = 8):
 
 def gemm(w: Tiles, x: Tiles, rows: int, out=None):
     """y = W x for the first `rows` rows of x, in bf16 x tiles."""
-    dev = x._device
+    dev = _tiles(x, "x")
     stream = _here(dev)
+    xr, wr = _operand(x, 8, rows, dev, 0, "x"), _operand(w, 4, 1, dev, x._cols, "w")
     out = _y_tiles(out, rows, w.rows, x, dev)
-    p = _GEMM(rows, (rows + 15) // 16, 0, 0, _operand(x, 8, rows, dev, 0, "x"), _operand(w, 4, 1, dev, x._cols, "w"), out.data_ptr())
+    p = _GEMM(rows, (rows + 15) // 16, 0, 0, xr, wr, out.data_ptr())
     rc = _lib.packed().stride_mx_gemm(p, stream)
     if rc:
         _lib.check(rc)
@@ -212,11 +226,12 @@ def gemm(w: Tiles, x: Tiles, rows: int, out=None):
 
 def mlp13(w1: Tiles, w3: Tiles, x: Tiles, rows: int, out: Tiles | None = None) -> Tiles:
     """z = silu(W1 x) * (W3 x) in 8 bits."""
-    dev = x._device
+    dev = _tiles(x, "x")
     stream = _here(dev)
+    xr, r1 = _operand(x, 8, rows, dev, 0, "x"), _operand(w1, 4, 1, dev, x._cols, "w1")
+    r3 = _operand(w3, 4, w1.rows, dev, x._cols, "w3")
     out = _result(out, rows, w1.rows, x)
-    p = _MLP13(rows, (rows + 15) // 16, 0, 0, _operand(x, 8, rows, dev, 0, "x"), _operand(w1, 4, 1, dev, x._cols, "w1"),
-               _operand(w3, 4, w1.rows, dev, x._cols, "w3"), _operand(out, 8, rows, dev, w1.rows, "out"))
+    p = _MLP13(rows, (rows + 15) // 16, 0, 0, xr, r1, r3, _operand(out, 8, rows, dev, w1.rows, "out"))
     rc = _lib.packed().stride_mx_mlp13(p, stream)
     if rc:
         _lib.check(rc)
@@ -228,25 +243,31 @@ def qkv(wq: Tiles, wk: Tiles, wv: Tiles, x: Tiles, rows: int, head_dim: int, rop
     """harness.qkv on these weights (rows in layout.rope_rows' order): q with RoPE in fp32 rows, K
     and V appended to the paged bf16 cache. A row is left out, its q as it was, where its slot is no row
     of kv.table or its position lies behind the cache's last page or behind rope."""
-    dev, nq = x._device, wq.rows
+    dev = _tiles(x, "x")
     stream = _here(dev)
+    xr = _operand(x, 8, rows, dev, 0, "x")
+    ws = [_operand(w, 4, 1, dev, x._cols, name) for w, name in ((wq, "wq"), (wk, "wk"), (wv, "wv"))]
+    nq = wq.rows
+    for t, name in ((rope, "rope"), (row_slot, "row_slot"), (row_pos, "row_pos")):
+        _tensor(t, name)
+    if not isinstance(kv, PagedKv):
+        raise ValueError("kv must be a PagedKv")
     if row_slot.dtype != torch.int32 or row_pos.dtype != torch.int32 or row_slot.numel() < rows or row_pos.numel() < rows \
             or not (row_slot.is_contiguous() and row_pos.is_contiguous()):
         raise ValueError("row_slot and row_pos must be contiguous int32, one for each row")
     if rope.dtype != torch.float32 or not rope.is_contiguous() or rope.dim() != 3 or rope.shape[1] * 2 != head_dim or rope.shape[2] != 2:
         raise ValueError("rope must be contiguous fp32 [positions][head_dim / 2][2]")
-    if not row_slot.get_device() == row_pos.get_device() == rope.get_device() == kv.table.get_device() == dev:
+    if not row_slot.get_device() == row_pos.get_device() == rope.get_device() == kv.table.get_device() == kv.arena.get_device() == dev:
         raise ValueError("the arguments are on different devices")
     if not 0 <= layer < kv.ref.block_elems // kv.ref.layer_elems or kv.ref.which_elems * head_dim != wk.rows * kv.ref.group_elems:
         raise ValueError("layer or the number of KV heads is not the cache's")
     if q_out is None:
         _allocates()
         q_out = torch.zeros((max(rows, 1), nq), dtype=torch.float32, device=x.codes.device)
-    elif q_out.dtype != torch.float32 or q_out.dim() != 2 or q_out.shape[0] < rows or q_out.shape[1] != nq or q_out.stride(1) != 1 \
+    elif _tensor(q_out, "q_out").dtype != torch.float32 or q_out.dim() != 2 or q_out.shape[0] < rows or q_out.shape[1] != nq or q_out.stride(1) != 1 \
             or q_out.get_device() != dev:
         raise ValueError("q_out must be fp32 [rows][q columns], its rows contiguous")
-    ws = [_operand(w, 4, 1, dev, x._cols, name) for w, name in ((wq, "wq"), (wk, "wk"), (wv, "wv"))]
-    p = _QKV(rows, (rows + 15) // 16, 0, 0, _operand(x, 8, rows, dev, 0, "x"), *ws, q_out.data_ptr(), q_out.stride(0) if rows > 1 else nq,
+    p = _QKV(rows, (rows + 15) // 16, 0, 0, xr, *ws, q_out.data_ptr(), q_out.stride(0) if rows > 1 else nq,
              bytes(kv.ref), rope.data_ptr(), row_slot.data_ptr(), row_pos.data_ptr(), layer, head_dim)
     rc = _lib.packed().stride_mx_qkv_within(p, kv.table.shape[0], rope.shape[0], stream)
     if rc:

@@ -110,3 +110,28 @@ def test_norm_in_the_place_of_its_addition(m, dim):
     assert torch.equal(h, h2) and torch.equal(layout.untile_lanes(got.cpu(), m), layout.untile_lanes(want.cpu(), m))
     with pytest.raises(StrideTcError, match="overlap"):
         mx.norm(h, m, gain, 1e-5, out=h.view(torch.int16).view(-1)[:add.numel()].view(add.shape), bits=16)
+
+
+def test_arguments_of_another_kind_are_refused_by_a_message():
+    """As without a GPU, for the arguments that are looked at after the device; and rows that an operand
+    does not have are refused before a result of their size is made."""
+    x, w, y = mx.Tiles.create(20, 512, 8, DEV), mx.Tiles.create(64, 512, 4, DEV), torch.zeros((2, 4, 16, 16), dtype=torch.int16, device=DEV)
+    h, gain, z = torch.zeros((2, 32, 16, 16), device=DEV), torch.ones(512, device=DEV), mx.Tiles.create(20, 64, 8, DEV)
+    kv = harness.PagedKv.create(1, 32, 1, 32, 1, 16, DEV)
+    narrow = mx.Tiles.create(32, 512, 4, DEV)
+    rope, at = torch.zeros((32, 16, 2), device=DEV), torch.zeros(20, dtype=torch.int32, device=DEV)
+    good = dict(wq=w, wk=narrow, wv=narrow, x=x, rows=20, head_dim=32, rope=rope, row_slot=at, row_pos=at, kv=kv)
+    mx.qkv(**good)
+    for bad, why in ((lambda: mx.gemm(h, x, 20), "w must"), (lambda: mx.gemm(w, x, 20, out=z), "out must"), (lambda: mx.gemm(w, x, 20, out=[y]), "out must"),
+                     (lambda: mx.mlp13(h, w, x, 20), "w1 must"), (lambda: mx.mlp13(w, None, x, 20), "w3 must"), (lambda: mx.mlp13(w, w, x, 20, out=y), "out must"),
+                     (lambda: mx.quantize(h, out=h), "out must"), (lambda: mx.dequantize(x, out=x), "out must"), (lambda: mx.norm(h, 20, x, 1e-5), "weight must"),
+                     (lambda: mx.norm(h, 20, gain, 1e-5, add=x), "add must"), (lambda: mx.norm(h, 20, gain, 1e-5, bits=16, out=x), "out must"),
+                     (lambda: mx.norm(h, 20, gain, 1e-5, out=y), "out must"), (lambda: mx.qkv(**{**good, "wq": h}), "wq must"),
+                     (lambda: mx.qkv(**{**good, "rope": x}), "rope must"), (lambda: mx.qkv(**{**good, "row_pos": [0] * 20}), "row_pos must"),
+                     (lambda: mx.qkv(**{**good, "kv": kv.ref}), "kv must"), (lambda: mx.qkv(**{**good, "q_out": x}), "q_out must"),
+                     *((call, "must be") for rows in (-1, -100, 33, 10 ** 12) for call in (
+                         lambda rows=rows: mx.gemm(w, x, rows), lambda rows=rows: mx.mlp13(w, w, x, rows), lambda rows=rows: mx.quantize(h, rows, bits=8),
+                         lambda rows=rows: mx.dequantize(x, rows), lambda rows=rows: mx.norm(h, rows, gain, 1e-5),
+                         lambda rows=rows: mx.norm(h, rows, gain, 1e-5, bits=16), lambda rows=rows: mx.qkv(**{**good, "rows": rows})))):
+        with pytest.raises(ValueError, match=why):
+            bad()

@@ -1,8 +1,9 @@
 """Calls of the microscaled operators that have to be refused, or that have to leave rows alone, without
 a GPU: what the C ABI refuses before a launch."""
 import pytest
+import torch
 
-from stride_amd import _lib, mx
+from stride_amd import _lib, harness, mx
 
 BUF = 0x7F0000000000  # an address that nothing may touch: every call here is refused
 
@@ -73,3 +74,14 @@ def test_qkv_results_that_lie_on_an_operand(q_out, slot):
                     q_out, 256, ref, FAR + (6 << 30), slot, FAR + (7 << 30), 0, 64)
     for call in (lambda: _lib.packed().stride_mx_qkv(block, None), lambda: _lib.packed().stride_mx_qkv_within(block, 8, 8, None)):
         assert call() == _lib.EINVAL and "overlap" in err(), err()
+
+
+def test_arguments_of_another_kind_are_refused_by_a_message():
+    """What trips over a missing attribute is no refusal: a tensor where Tiles belong and the other way."""
+    x, w, t = mx.Tiles.create(20, 512, 8, "cpu"), mx.Tiles.create(64, 512, 4, "cpu"), torch.zeros((2, 32, 16, 16))
+    kv = harness.PagedKv.create(1, 16, 1, 32, 1, 16, "cpu")
+    for bad, name in ((lambda: mx.gemm(w, t, 20), "x"), (lambda: mx.gemm(w, None, 20), "x"), (lambda: mx.mlp13(w, w, t, 20), "x"),
+                      (lambda: mx.qkv(w, w, w, t, 20, 32, t, t, t, kv), "x"), (lambda: mx.dequantize(t), "t"), (lambda: mx.quantize(x), "tiles"),
+                      (lambda: mx.quantize([1.0]), "tiles"), (lambda: mx.norm(x, 20, t, 1e-5), "h"), (lambda: mx.norm(None, 20, t, 1e-5), "h")):
+        with pytest.raises(ValueError, match=f"^{name} must"):
+            bad()
