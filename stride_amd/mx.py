@@ -140,6 +140,16 @@ def _y_tiles(out, rows: int, cols: int, like, dev: int):
 def quantize(tiles, rows: int | None = None, bits: int = 4, out: Tiles | None = None) -> Tiles:
     """Tiles [t][ct][16][16] of 16-bit (bf16, or its bits in int16) or fp32 values to blocks of 4
     or 8 bits, for the first `rows` rows (default: all)."""
+    return _quantize(tiles, rows, bits, out, True)
+
+
+def microscaled(tiles) -> Tiles:
+    """quantize(tiles) on torch's current stream, whatever set_kernel_stream says: there a model's
+    weights are packed and its buffers made."""
+    return _quantize(tiles, None, 4, None, False)
+
+
+def _quantize(tiles, rows, bits, out, kernel_stream: bool) -> Tiles:
     if _tensor(tiles, "tiles").dtype in _BF16:
         size = 2
     elif tiles.dtype == torch.float32:
@@ -152,8 +162,11 @@ def quantize(tiles, rows: int | None = None, bits: int = 4, out: Tiles | None = 
     stream = _here(dev)
     rows = len(tiles) * 16 if rows is None and tiles.dim() else rows
     cols = _tile_cols(tiles, rows, "tiles")
-    if out is None:
+    if not kernel_stream:
+        stream = _stream_of(dev)
+    elif out is None:
         _allocates()
+    if out is None:
         out = Tiles.create(rows, cols, bits, tiles.device)
     p = _QUANTIZE(rows, (rows + 15) // 16, 0, 0, tiles.data_ptr(), _operand(out, bits, rows, dev, cols, "out"), bits, size)
     rc = _lib.packed().stride_mx_quantize(p, stream)

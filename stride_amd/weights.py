@@ -192,7 +192,7 @@ class Weights:
         are; with a microscaled model there is nothing left to do."""
         if self.bits == 4:
             return self
-        layers = [{k: t if k in ("norm_attn", "norm_mlp") else mx.quantize(t) for k, t in L.items()} for L in self.layers]
+        layers = [{k: t if k in ("norm_attn", "norm_mlp") else mx.microscaled(t) for k, t in L.items()} for L in self.layers]
         return Weights(self.cfg, self.embed, self.lm, layers, self.norm_final, self.rope)
 
     @staticmethod
