@@ -253,12 +253,11 @@ def main(argv=None) -> int:
         eng = ExactCliEngine(model, a.concurrency, longest, a.max_rows, a.kv_shuffle, a.device)
         cfg = model.cfg
     else:
+        bits = 4 if a.weights == "mx4" else 16
         if a.model.startswith("random:"):
-            w = weights.Weights.random(weights.ModelConfig(), a.device, int(a.model.split(":", 1)[1]), longest + 1)
+            w = weights.Weights.random(weights.ModelConfig(), a.device, int(a.model.split(":", 1)[1]), longest + 1, bits)
         else:
-            w = weights.Weights.load(a.model, a.device, max_positions=longest + 1)
-        if a.weights == "mx4":
-            w = w.microscaled()
+            w = weights.Weights.load(a.model, a.device, max_positions=longest + 1, bits=bits)
         if a.path == "serve":
             eng = serving.ServingEngine(w, a.concurrency, longest, a.max_rows, a.page_tokens, a.kv_pages or None, a.window,
                                         a.sinks)

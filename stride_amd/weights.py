@@ -174,6 +174,13 @@ class Checkpoint:
         return t
 
 
+def _as_held(bits: int):
+    """What becomes of a layer's packed matrix."""
+    if bits not in (4, 16):
+        raise ValueError("a model's matrices have 4 or 16 bits")
+    return mx.microscaled if bits == 4 else lambda t: t
+
+
 class Weights:
     """Device-resident packed weights in the layout the tensor-core operators
     consume: `embed` and `lm` tiles (the same tensor when tied), per layer q, k,
@@ -189,14 +196,17 @@ class Weights:
     def microscaled(self) -> "Weights":
         """The model with its layers' matrices in blocks of 4 bits (stride_amd.mx), which engine.Engine
         and serving.ServingEngine run as they run this one. Embedding, LM head and gains stay as they
-        are; with a microscaled model there is nothing left to do."""
+        are; with a microscaled model there is nothing left to do. This one's matrices stay as well:
+        load(..., bits=4) holds one at a time."""
         if self.bits == 4:
             return self
         layers = [{k: t if k in ("norm_attn", "norm_mlp") else mx.microscaled(t) for k, t in L.items()} for L in self.layers]
         return Weights(self.cfg, self.embed, self.lm, layers, self.norm_final, self.rope)
 
     @staticmethod
-    def load(model_dir: str, device, cfg: ModelConfig | None = None, max_positions: int = 4097) -> "Weights":
+    def load(model_dir: str, device, cfg: ModelConfig | None = None, max_positions: int = 4097, bits: int = 16) -> "Weights":
+        """A checkpoint's weights; with bits=4 what microscaled() makes of them, each matrix as it is read."""
+        packed = _as_held(bits)
         cfg = cfg or ModelConfig.load(model_dir)
         ck = Checkpoint(model_dir)
         D = cfg.head_dim
@@ -206,8 +216,7 @@ class Weights:
             n, k = t.shape
             if n % 16 or k % 16:
                 raise RuntimeError("matrix shape incompatible with the packed kernels")
-            bits = t.view(torch.int16).to(device)
-            return layout.pack_tiles(bits, layout.rope_rows(n, D) if rope else None)
+            return packed(layout.pack_tiles(t.view(torch.int16).to(device), layout.rope_rows(n, D) if rope else None))
 
         def gains(name):
             return ck.get(name).float().to(device)
@@ -233,9 +242,10 @@ class Weights:
         return Weights(cfg, embed, lm, layers, gains("model.norm.weight"), rope)
 
     @staticmethod
-    def random(cfg: ModelConfig, device, seed: int = 0, max_positions: int = 4097) -> "Weights":
+    def random(cfg: ModelConfig, device, seed: int = 0, max_positions: int = 4097, bits: int = 16) -> "Weights":
         """Random-init weights ~N(0, 0.02) in bf16 with unit norm gains and a tied
-        LM head (no checkpoint)."""
+        LM head (no checkpoint); `bits` as load() takes it."""
+        packed = _as_held(bits)
         g = torch.Generator(device=device).manual_seed(seed)
         D, H = cfg.head_dim, cfg.hidden
 
@@ -247,10 +257,10 @@ class Weights:
         layers = []
         for _ in range(cfg.layers):
             layers.append(dict(
-                q=w(cfg.heads * D, H, layout.rope_rows(cfg.heads * D, D)),
-                k=w(cfg.kv_heads * D, H, layout.rope_rows(cfg.kv_heads * D, D)),
-                v=w(cfg.kv_heads * D, H, layout.rope_rows(cfg.kv_heads * D, D)),
-                o=w(H, cfg.heads * D), w1=w(cfg.mlp, H), w3=w(cfg.mlp, H), w2=w(H, cfg.mlp),
+                q=packed(w(cfg.heads * D, H, layout.rope_rows(cfg.heads * D, D))),
+                k=packed(w(cfg.kv_heads * D, H, layout.rope_rows(cfg.kv_heads * D, D))),
+                v=packed(w(cfg.kv_heads * D, H, layout.rope_rows(cfg.kv_heads * D, D))),
+                o=packed(w(H, cfg.heads * D)), w1=packed(w(cfg.mlp, H)), w3=packed(w(cfg.mlp, H)), w2=packed(w(H, cfg.mlp)),
                 norm_attn=torch.ones(H, device=device), norm_mlp=torch.ones(H, device=device)))
         rope = torch.from_numpy(build_rope_table(cfg, max_positions)).to(device)
         return Weights(cfg, embed, embed, layers, torch.ones(H, device=device), rope)
