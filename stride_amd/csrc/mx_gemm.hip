@@ -402,123 +402,74 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_mx_pipe(MxGeometry g, typ
   });
 }
 
-// In between: workgroup of WM x WN waves, A weight tiles by L lane tiles a wave; a group of 512
-// columns is a stage, NS - 1 of them on their way (a chunk a stage as above has too little on its way
-// for such small tiles: 2048 x 8192 at 128 rows 17 us as 128 x 64, 8.3 here).
-template <class Epi, int A, int L, int WM, int WN, int NS>
-__global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxGeometry g, typename Epi::Out o, int units, int unit_blocks, int lane_blocks) {
-  constexpr int M = Epi::kMats, U = Epi::kUnit, NW = WM * WN;
-  constexpr int T = A / M;
-  constexpr int WA = WM * A, WL = WN * L;
-  constexpr int kCodes = 4 * (WA + 2 * WL), kScales = WA + WL;
-  constexpr int PC = (kCodes + NW - 1) / NW, PS = (kScales + NW - 1) / NW;
-  static_assert(kCodes % NW == 0, "copies must split evenly over the waves");
-  __shared__ u32x4 ring[NS][kCodes][kWave];
-  __shared__ uint32_t scales[NS][kScales][kWave];
+// In between: workgroup of 2 x 2 waves, a weight tile by a lane tile each; a group of 512 columns is a
+// stage of a ring of three, two of them on their way (a chunk a stage as above has too little on its way
+// for such small tiles: 2048 x 8192 at 128 rows 17 us as 128 x 64, 8.3 here). One matrix at a time:
+// gate and up, whose unit is 32 x 32 of each, go from waves of their own to 64 x 64.
+template <class Epi>
+__global__ __launch_bounds__(256) void k_mx_tile(MxGeometry g, typename Epi::Out o, int units, int lane_blocks) {
+  static_assert(Epi::kMats == 1 && Epi::kUnit == 1, "a wave has a weight tile");
+  constexpr int NS = 3;
+  constexpr int PC = 6;  // KiB of codes that a wave copies of a stage's 24: a chunk of each weight tile, four halves of x's
+  __shared__ u32x4 ring[NS][4 * PC][kWave];
+  __shared__ uint32_t scales[NS][4][kWave];  // of both weight tiles, of both lane tiles
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / WN, wn = wave % WN;
+  const int wm = wave >> 1, wn = wave & 1;
   const int b = xcd_remap(blockIdx.x, gridDim.x);
-  const int ub = b / lane_blocks, lb = b % lane_blocks;  // an XCD reads a weight tile once
-  const int rt0 = ub * WM * T, lt0 = lb * WL;
-  const uint8_t *src[PC], *ssrc[PS];
+  const int rt0 = b / lane_blocks * 2, lt0 = b % lane_blocks * 2;  // an XCD reads a weight tile once
+  auto x_tile = [&](int i) { return static_cast<int64_t>(min(lt0 + i, g.lane_groups - 1)); };
+  const uint8_t *src[PC], *ssrc, *unused;
 #pragma unroll
   for (int i = 0; i < PC; ++i) {
-    const int j = wave + i * NW;
-    if (j < 4 * WA) {
-      const int w = j / 4, m = w / (WM * T), t = w % (WM * T);
-      const uint8_t* unused;
-      mx_source<Epi>(g, m, rt0 + t, src[i], unused);
-      src[i] += j % 4 * kCode4Bytes;
+    if (i < 2) {
+      mx_source<Epi>(g, 0, rt0 + i, src[i], unused);
+      src[i] += wave * kCode4Bytes;
     } else {
-      const int x = (j - 4 * WA) / 8;
-      src[i] = g.xc + static_cast<int64_t>(min(lt0 + x, g.lane_groups - 1)) * g.groups * 4 * kCode8Bytes + (j - 4 * WA) % 8 * 1024;
+      const int j = wave + (i - 2) * 4;
+      src[i] = g.xc + x_tile(j / 8) * g.groups * 4 * kCode8Bytes + j % 8 * 1024;
     }
   }
-#pragma unroll
-  for (int i = 0; i < PS; ++i) {
-    const int j = min(wave + i * NW, kScales - 1);  // a copy too many goes where it was
-    if (j < WA) {
-      const int m = j / (WM * T), t = j % (WM * T);
-      const uint8_t* unused;
-      mx_source<Epi>(g, m, rt0 + t, unused, ssrc[i]);
-    } else {
-      ssrc[i] = g.xs + static_cast<int64_t>(min(lt0 + j - WA, g.lane_groups - 1)) * g.groups * kScaleBytes;
-    }
-  }
+  if (wave < 2) mx_source<Epi>(g, 0, rt0 + wave, unused, ssrc);
+  else ssrc = g.xs + x_tile(wave - 2) * g.groups * kScaleBytes;
   const uint32_t at16 = lane * 16, at4 = lane * 4;
-  const uint32_t ring_at = lds_at(&ring[0][0][0]), scales_at = lds_at(&scales[0][0][0]);
+  const uint32_t ring_at = lds_at(&ring[0][0][0]) + wave * 1024, scales_at = lds_at(&scales[0][0][0]) + wave * 256;
   auto issue = [&](int stage, int slot) {
+    copy4(scales_at + slot * 1024, at4, ssrc + static_cast<int64_t>(stage) * kScaleBytes);
 #pragma unroll
-    for (int i = 0; i < PS; ++i)
-      copy4(scales_at + (slot * kScales + min(wave + i * NW, kScales - 1)) * 256, at4, ssrc[i] + static_cast<int64_t>(stage) * kScaleBytes);
-#pragma unroll
-    for (int i = 0; i < PC; ++i) {
-      const int64_t step = static_cast<int64_t>(stage) * 4 * (wave + i * NW < 4 * WA ? kCode4Bytes : kCode8Bytes);
-      copy16(ring_at + (slot * kCodes + wave + i * NW) * 1024, at16, src[i] + step);
-    }
+    for (int i = 0; i < PC; ++i)
+      copy16(ring_at + (slot * PC + i) * 4096, at16, src[i] + static_cast<int64_t>(stage) * 4 * (i < 2 ? kCode4Bytes : kCode8Bytes));
   };
-  f32x4 acc[A][L];
-#pragma unroll
-  for (int a = 0; a < A; ++a)
-#pragma unroll
-    for (int l = 0; l < L; ++l) acc[a][l] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto tile = [&](int a) { return a / T * (WM * T) + wm * T + a % T; };
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   const int first = min(NS - 1, g.groups);
   for (int i = 0; i < first; ++i) issue(i, i);
   int slot = 0, next = NS - 1;  // of stage i, of stage i + NS - 1
   for (int i = 0; i < g.groups; ++i) {
-    // stage i has landed; what is being refilled has been read, by every wave
-    const int ahead = min(NS - 2, g.groups - 1 - i);
-    if (ahead >= NS - 2) wait_copies<(NS - 2) * (PC + PS)>();
-    else if (NS > 4 && ahead == 2) wait_copies<2 * (PC + PS)>();
-    else if (NS > 3 && ahead == 1) wait_copies<PC + PS>();
+    // stage i has landed (the one behind it may be on its way); what is being refilled has been read, by every wave
+    if (i + 1 < g.groups) wait_copies<PC + 1>();
     else wait_copies<0>();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    uint32_t sa[A], sb[L];
-    u32x4 fa[4][A], fb[4][L][2];
-#pragma unroll
-    for (int a = 0; a < A; ++a) sa[a] = scales[slot][tile(a)][lane];
-#pragma unroll
-    for (int l = 0; l < L; ++l) sb[l] = scales[slot][WA + wn * L + l][lane];
+    const uint32_t sa = scales[slot][wm][lane], sb = scales[slot][2 + wn][lane];
+    u32x4 fa[4], fb[4][2];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
 #pragma unroll
-      for (int l = 0; l < L; ++l)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) fb[c][l][h] = ring[slot][4 * WA + (wn * L + l) * 8 + c * 2 + h][lane];
-#pragma unroll
-      for (int a = 0; a < A; ++a) fa[c][a] = ring[slot][tile(a) * 4 + c][lane];
+      for (int h = 0; h < 2; ++h) fb[c][h] = ring[slot][8 + wn * 8 + c * 2 + h][lane];
+      fa[c] = ring[slot][wm * 4 + c][lane];
     }
     if (i + NS - 1 < g.groups) issue(i + NS - 1, next);  // while the fragments are on their way
-    unroll<4>([&](auto c) {
-#pragma unroll
-      for (int a = 0; a < A; ++a)
-#pragma unroll
-        for (int l = 0; l < L; ++l) acc[a][l] = mx_mfma<c>(fa[c][a], fb[c][l][0], fb[c][l][1], acc[a][l], sa[a], sb[l]);
-    });
+    unroll<4>([&](auto c) { acc = mx_mfma<c>(fa[c], fb[c][0], fb[c][1], acc, sa, sb); });
     slot = slot + 1 == NS ? 0 : slot + 1;
     next = next + 1 == NS ? 0 : next + 1;
   }
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7");
-#pragma unroll
-  for (int a = 0; a < A; ++a)
-#pragma unroll
-    for (int l = 0; l < L; ++l) asm volatile("" : "+v"(acc[a][l]));
-  unroll<T / U>([&](auto r) {
-    unroll<L>([&](auto l) {
-      const int unit = (rt0 + wm * T) / U + r, lt = lt0 + wn * L + l;
-      if (unit >= units || lt >= g.lane_groups) return;
-      f32x4 v[M][U];
-#pragma unroll
-      for (int m = 0; m < M; ++m)
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[m][u] = acc[m * T + r * U + u][l];
-      Epi::finish(o, g, unit, lt, v, lane);
-    });
-  });
+  asm volatile("" : "+v"(acc));
+  const int unit = rt0 + wm, lt = lt0 + wn;
+  if (unit >= units || lt >= g.lane_groups) return;
+  const f32x4 v[1][1] = {{acc}};
+  Epi::finish(o, g, unit, lt, v, lane);
 }
 
 template <class Epi, int P>
@@ -536,11 +487,10 @@ const char* launch_pipe(const MxGeometry& g, const typename Epi::Out& o, int uni
   return nullptr;
 }
 
-template <class Epi, int A, int L, int WM, int WN, int NS>
+template <class Epi>
 void launch_tile(const MxGeometry& g, const typename Epi::Out& o, int units, hipStream_t st) {
-  constexpr int per = WM * A / Epi::kMats / Epi::kUnit;
-  const int unit_blocks = (units + per - 1) / per, lane_blocks = (g.lane_groups + WN * L - 1) / (WN * L);
-  hipLaunchKernelGGL((k_mx_tile<Epi, A, L, WM, WN, NS>), dim3(unit_blocks * lane_blocks), dim3(64 * WM * WN), 0, st, g, o, units, unit_blocks, lane_blocks);
+  const int unit_blocks = (units + 1) / 2, lane_blocks = (g.lane_groups + 1) / 2;
+  hipLaunchKernelGGL(k_mx_tile<Epi>, dim3(unit_blocks * lane_blocks), dim3(256), 0, st, g, o, units, lane_blocks);
 }
 
 // Host: does a result lie on x or on one of the weights? (Other workgroups read them until the end.)
@@ -577,7 +527,7 @@ int run(const char* what, const MxGeometry& g, const typename Epi::Out& o, int r
   const char* why = nullptr;
   if (products <= (Epi::kMats == 2 ? 1280 : g.groups <= 4 ? 1536 : 768)) launch_row<Epi, 4 / Epi::kMats>(g, o, units, st);
   else if (Epi::kMats == 1 && products <= 1536) {
-    if constexpr (Epi::kMats == 1) launch_tile<Epi, 1, 1, 2, 2, 3>(g, o, units, st);
+    if constexpr (Epi::kMats == 1) launch_tile<Epi>(g, o, units, st);
   } else if (products <= 6144) why = launch_pipe<Epi, 4, 1, 1, 4, 4, 2>(g, o, units, clash, st);
   else if (products <= 9216) why = launch_pipe<Epi, 4, 2, 2, 2, 4, 2>(g, o, units, clash, st);
   else if (products <= 16384) why = launch_pipe<Epi, 4, 2, 2, 4, 4, 2>(g, o, units, clash, st);
