@@ -85,17 +85,14 @@ def _here(dev: int) -> int:
     return _stream_of(dev) if tc._stream is None else tc.kernel_stream()
 
 
-def _tiles(t, name: str) -> int:
-    """The device of a Tiles argument."""
-    if type(t) is not Tiles:
-        raise ValueError(f"{name} must be Tiles")
-    return t._device
-
-
-def _tensor(t, name: str):
-    if not isinstance(t, torch.Tensor):
-        raise ValueError(f"{name} must be a tensor")
-    return t
+def _kind(error: AttributeError, tiles=(), tensors=(), given=()) -> Exception:
+    """Why a check has met an argument without the attribute that it reads: the first that is no Tiles or
+    no tensor (`given`: None is none either), by name."""
+    for args, kind, what in ((tiles, Tiles, "Tiles"), (tensors, torch.Tensor, "a tensor"), (given, torch.Tensor, "a tensor")):
+        for name, t in args:
+            if not isinstance(t, kind) and not (args is given and t is None):
+                return ValueError(f"{name} must be {what}")
+    return error
 
 
 def _operand(t, bits: int, rows: int, dev: int, cols: int, name: str) -> bytes:
@@ -132,7 +129,7 @@ def _y_tiles(out, rows: int, cols: int, like, dev: int):
     if out is None:
         _allocates()
         return torch.zeros(((rows + 15) // 16, cols // 16, 16, 16), dtype=torch.int16, device=getattr(like, "codes", like).device)
-    if _tensor(out, "out").dtype not in _BF16 or out.get_device() != dev or _tile_cols(out, rows, "out") != cols:
+    if out.dtype not in _BF16 or out.get_device() != dev or _tile_cols(out, rows, "out") != cols:
         raise ValueError(f"out must be 16-bit tiles of {cols} columns on the call's device")
     return out
 
@@ -140,36 +137,41 @@ def _y_tiles(out, rows: int, cols: int, like, dev: int):
 def quantize(tiles, rows: int | None = None, bits: int = 4, out: Tiles | None = None) -> Tiles:
     """Tiles [t][ct][16][16] of 16-bit (bf16, or its bits in int16) or fp32 values to blocks of 4
     or 8 bits, for the first `rows` rows (default: all)."""
-    return _quantize(tiles, rows, bits, out, True)
+    try:
+        if tiles.dtype in _BF16:
+            size = 2
+        elif tiles.dtype == torch.float32:
+            size = 4
+        else:
+            raise ValueError("tiles must hold bf16 or fp32")
+        if bits not in (4, 8):
+            raise ValueError("blocks have 4 or 8 bits")
+        dev = tiles.get_device()
+        stream = _here(dev)
+        rows = len(tiles) * 16 if rows is None and tiles.dim() else rows
+        cols = _tile_cols(tiles, rows, "tiles")
+        if out is None:
+            _allocates()
+            out = Tiles.create(rows, cols, bits, tiles.device)
+        p = _QUANTIZE(rows, (rows + 15) // 16, 0, 0, tiles.data_ptr(), _operand(out, bits, rows, dev, cols, "out"), bits, size)
+    except AttributeError as e:
+        raise _kind(e, tensors=(("tiles", tiles),))
+    rc = _lib.packed().stride_mx_quantize(p, stream)
+    if rc:
+        _lib.check(rc)
+    return out
 
 
 def microscaled(tiles) -> Tiles:
-    """quantize(tiles) on torch's current stream, whatever set_kernel_stream says: there a model's
-    weights are packed and its buffers made."""
-    return _quantize(tiles, None, 4, None, False)
-
-
-def _quantize(tiles, rows, bits, out, kernel_stream: bool) -> Tiles:
-    if _tensor(tiles, "tiles").dtype in _BF16:
-        size = 2
-    elif tiles.dtype == torch.float32:
-        size = 4
-    else:
-        raise ValueError("tiles must hold bf16 or fp32")
-    if bits not in (4, 8):
-        raise ValueError("blocks have 4 or 8 bits")
+    """quantize(tiles) of bf16 weights on torch's current stream, whatever set_kernel_stream says: there a
+    model's weights are packed and its buffers made."""
+    if tiles.dtype not in _BF16:
+        raise ValueError("weights are bf16")
     dev = tiles.get_device()
-    stream = _here(dev)
-    rows = len(tiles) * 16 if rows is None and tiles.dim() else rows
-    cols = _tile_cols(tiles, rows, "tiles")
-    if not kernel_stream:
-        stream = _stream_of(dev)
-    elif out is None:
-        _allocates()
-    if out is None:
-        out = Tiles.create(rows, cols, bits, tiles.device)
-    p = _QUANTIZE(rows, (rows + 15) // 16, 0, 0, tiles.data_ptr(), _operand(out, bits, rows, dev, cols, "out"), bits, size)
-    rc = _lib.packed().stride_mx_quantize(p, stream)
+    _here(dev)
+    out = Tiles.create(len(tiles) * 16, _tile_cols(tiles, 0, "tiles"), 4, tiles.device)
+    p = _QUANTIZE(out.rows, out.tiles, 0, 0, tiles.data_ptr(), out._ref, 4, 2)
+    rc = _lib.packed().stride_mx_quantize(p, _stream_of(dev))
     if rc:
         _lib.check(rc)
     return out
@@ -179,14 +181,17 @@ def dequantize(t: Tiles, rows: int | None = None, dtype=torch.bfloat16, out=None
     """The values of the first `rows` rows, row-major [rows][cols] in bf16 or fp32."""
     if dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("values come in bf16 or fp32")
-    stream = _here(_tiles(t, "t"))
-    rows = t.rows if rows is None else rows
-    ref = _operand(t, t.bits, rows, t._device, 0, "t")
-    if out is None:
-        _allocates()
-        out = torch.empty((rows, t.cols), dtype=dtype, device=t.codes.device)
-    elif _tensor(out, "out").dtype != dtype or out.dim() != 2 or out.shape[0] < rows or out.shape[1] != t.cols or out.stride(1) != 1 or out.get_device() != t._device:
-        raise ValueError("out must be [rows][cols] of that type on the same device, its rows contiguous")
+    try:
+        stream = _here(t._device)
+        rows = t.rows if rows is None else rows
+        ref = _operand(t, t._bits, rows, t._device, 0, "t")
+        if out is None:
+            _allocates()
+            out = torch.empty((rows, t.cols), dtype=dtype, device=t.codes.device)
+        elif out.dtype != dtype or out.dim() != 2 or out.shape[0] < rows or out.shape[1] != t.cols or out.stride(1) != 1 or out.get_device() != t._device:
+            raise ValueError("out must be [rows][cols] of that type on the same device, its rows contiguous")
+    except AttributeError as e:
+        raise _kind(e, tiles=(("t", t),), given=(("out", out),))
     p = _DEQUANTIZE(rows, (rows + 15) // 16, 0, 0, ref, out.data_ptr(), out.stride(0) if rows > 1 else t.cols, t.bits, 2 if dtype == torch.bfloat16 else 4)
     rc = _lib.packed().stride_mx_dequantize(p, stream)
     if rc:
@@ -197,26 +202,29 @@ def dequantize(t: Tiles, rows: int | None = None, dtype=torch.bfloat16, out=None
 def norm(h, rows: int, weight, eps: float, add=None, out=None, bits: int = 8):
     """h += add (bf16 tiles, where given), then RMSNorm(h) * weight: in 8 bits (Tiles), or with
     bits=16 in bf16 x tiles. h: fp32 tiles [lt][ct][16][16]."""
-    dev = _tensor(h, "h").get_device()
-    stream = _here(dev)
-    if h.dtype != torch.float32:
-        raise ValueError("h must be fp32 tiles")
-    cols = _tile_cols(h, rows, "h")
-    if _tensor(weight, "weight").dtype != torch.float32 or weight.numel() != cols or not weight.is_contiguous() or weight.get_device() != dev:
-        raise ValueError("weight must be contiguous fp32 of h's columns, on its device")
-    a = 0
-    if add is not None:
-        if _tensor(add, "add").dtype not in _BF16 or add.get_device() != dev or _tile_cols(add, rows, "add") != cols:
-            raise ValueError("add must be bf16 tiles of h's columns on its device")
-        a = add.data_ptr()
-    if bits == 8:
-        out = _result(out, rows, cols, h)
-        ref, x = _operand(out, 8, rows, dev, cols, "out"), 0
-    elif bits == 16:
-        out = _y_tiles(out, rows, cols, h, dev)
-        ref, x = _NONE, out.data_ptr()
-    else:
-        raise ValueError("a norm's result has 8 or 16 bits")
+    try:
+        dev = h.get_device()
+        stream = _here(dev)
+        if h.dtype != torch.float32:
+            raise ValueError("h must be fp32 tiles")
+        cols = _tile_cols(h, rows, "h")
+        if weight.dtype != torch.float32 or weight.numel() != cols or not weight.is_contiguous() or weight.get_device() != dev:
+            raise ValueError("weight must be contiguous fp32 of h's columns, on its device")
+        a = 0
+        if add is not None:
+            if add.dtype not in _BF16 or add.get_device() != dev or _tile_cols(add, rows, "add") != cols:
+                raise ValueError("add must be bf16 tiles of h's columns on its device")
+            a = add.data_ptr()
+        if bits == 8:
+            out = _result(out, rows, cols, h)
+            ref, x = _operand(out, 8, rows, dev, cols, "out"), 0
+        elif bits == 16:
+            out = _y_tiles(out, rows, cols, h, dev)
+            ref, x = _NONE, out.data_ptr()
+        else:
+            raise ValueError("a norm's result has 8 or 16 bits")
+    except AttributeError as e:
+        raise _kind(e, tensors=(("h", h), ("weight", weight)), given=(("add", add), ("out", out)))
     p = _NORM(rows, (rows + 15) // 16, 0, 0, h.data_ptr(), a, weight.data_ptr(), ref, x, cols, eps)
     rc = _lib.packed().stride_mx_norm(p, stream)
     if rc:
@@ -226,10 +234,13 @@ def norm(h, rows: int, weight, eps: float, add=None, out=None, bits: int = 8):
 
 def gemm(w: Tiles, x: Tiles, rows: int, out=None):
     """y = W x for the first `rows` rows of x, in bf16 x tiles."""
-    dev = _tiles(x, "x")
-    stream = _here(dev)
-    xr, wr = _operand(x, 8, rows, dev, 0, "x"), _operand(w, 4, 1, dev, x._cols, "w")
-    out = _y_tiles(out, rows, w.rows, x, dev)
+    try:
+        dev = x._device
+        stream = _here(dev)
+        xr, wr = _operand(x, 8, rows, dev, 0, "x"), _operand(w, 4, 1, dev, x._cols, "w")
+        out = _y_tiles(out, rows, w.rows, x, dev)
+    except AttributeError as e:
+        raise _kind(e, tiles=(("x", x), ("w", w)), given=(("out", out),))
     p = _GEMM(rows, (rows + 15) // 16, 0, 0, xr, wr, out.data_ptr())
     rc = _lib.packed().stride_mx_gemm(p, stream)
     if rc:
@@ -239,12 +250,15 @@ def gemm(w: Tiles, x: Tiles, rows: int, out=None):
 
 def mlp13(w1: Tiles, w3: Tiles, x: Tiles, rows: int, out: Tiles | None = None) -> Tiles:
     """z = silu(W1 x) * (W3 x) in 8 bits."""
-    dev = _tiles(x, "x")
-    stream = _here(dev)
-    xr, r1 = _operand(x, 8, rows, dev, 0, "x"), _operand(w1, 4, 1, dev, x._cols, "w1")
-    r3 = _operand(w3, 4, w1.rows, dev, x._cols, "w3")
-    out = _result(out, rows, w1.rows, x)
-    p = _MLP13(rows, (rows + 15) // 16, 0, 0, xr, r1, r3, _operand(out, 8, rows, dev, w1.rows, "out"))
+    try:
+        dev = x._device
+        stream = _here(dev)
+        xr, r1 = _operand(x, 8, rows, dev, 0, "x"), _operand(w1, 4, 1, dev, x._cols, "w1")
+        r3 = _operand(w3, 4, w1.rows, dev, x._cols, "w3")
+        out = _result(out, rows, w1.rows, x)
+        p = _MLP13(rows, (rows + 15) // 16, 0, 0, xr, r1, r3, _operand(out, 8, rows, dev, w1.rows, "out"))
+    except AttributeError as e:
+        raise _kind(e, tiles=(("x", x),))
     rc = _lib.packed().stride_mx_mlp13(p, stream)
     if rc:
         _lib.check(rc)
@@ -256,30 +270,31 @@ def qkv(wq: Tiles, wk: Tiles, wv: Tiles, x: Tiles, rows: int, head_dim: int, rop
     """harness.qkv on these weights (rows in layout.rope_rows' order): q with RoPE in fp32 rows, K
     and V appended to the paged bf16 cache. A row is left out, its q as it was, where its slot is no row
     of kv.table or its position lies behind the cache's last page or behind rope."""
-    dev = _tiles(x, "x")
-    stream = _here(dev)
-    xr = _operand(x, 8, rows, dev, 0, "x")
-    ws = [_operand(w, 4, 1, dev, x._cols, name) for w, name in ((wq, "wq"), (wk, "wk"), (wv, "wv"))]
-    nq = wq.rows
-    for t, name in ((rope, "rope"), (row_slot, "row_slot"), (row_pos, "row_pos")):
-        _tensor(t, name)
-    if not isinstance(kv, PagedKv):
-        raise ValueError("kv must be a PagedKv")
-    if row_slot.dtype != torch.int32 or row_pos.dtype != torch.int32 or row_slot.numel() < rows or row_pos.numel() < rows \
-            or not (row_slot.is_contiguous() and row_pos.is_contiguous()):
-        raise ValueError("row_slot and row_pos must be contiguous int32, one for each row")
-    if rope.dtype != torch.float32 or not rope.is_contiguous() or rope.dim() != 3 or rope.shape[1] * 2 != head_dim or rope.shape[2] != 2:
-        raise ValueError("rope must be contiguous fp32 [positions][head_dim / 2][2]")
-    if not row_slot.get_device() == row_pos.get_device() == rope.get_device() == kv.table.get_device() == kv.arena.get_device() == dev:
-        raise ValueError("the arguments are on different devices")
-    if not 0 <= layer < kv.ref.block_elems // kv.ref.layer_elems or kv.ref.which_elems * head_dim != wk.rows * kv.ref.group_elems:
-        raise ValueError("layer or the number of KV heads is not the cache's")
-    if q_out is None:
-        _allocates()
-        q_out = torch.zeros((max(rows, 1), nq), dtype=torch.float32, device=x.codes.device)
-    elif _tensor(q_out, "q_out").dtype != torch.float32 or q_out.dim() != 2 or q_out.shape[0] < rows or q_out.shape[1] != nq or q_out.stride(1) != 1 \
-            or q_out.get_device() != dev:
-        raise ValueError("q_out must be fp32 [rows][q columns], its rows contiguous")
+    try:
+        dev = x._device
+        stream = _here(dev)
+        xr = _operand(x, 8, rows, dev, 0, "x")
+        ws = [_operand(w, 4, 1, dev, x._cols, name) for w, name in ((wq, "wq"), (wk, "wk"), (wv, "wv"))]
+        nq = wq.rows
+        if not isinstance(kv, PagedKv):
+            raise ValueError("kv must be a PagedKv")
+        if row_slot.dtype != torch.int32 or row_pos.dtype != torch.int32 or row_slot.numel() < rows or row_pos.numel() < rows \
+                or not (row_slot.is_contiguous() and row_pos.is_contiguous()):
+            raise ValueError("row_slot and row_pos must be contiguous int32, one for each row")
+        if rope.dtype != torch.float32 or not rope.is_contiguous() or rope.dim() != 3 or rope.shape[1] * 2 != head_dim or rope.shape[2] != 2:
+            raise ValueError("rope must be contiguous fp32 [positions][head_dim / 2][2]")
+        if not row_slot.get_device() == row_pos.get_device() == rope.get_device() == kv.table.get_device() == kv.arena.get_device() == dev:
+            raise ValueError("the arguments are on different devices")
+        if not 0 <= layer < kv.ref.block_elems // kv.ref.layer_elems or kv.ref.which_elems * head_dim != wk.rows * kv.ref.group_elems:
+            raise ValueError("layer or the number of KV heads is not the cache's")
+        if q_out is None:
+            _allocates()
+            q_out = torch.zeros((max(rows, 1), nq), dtype=torch.float32, device=x.codes.device)
+        elif q_out.dtype != torch.float32 or q_out.dim() != 2 or q_out.shape[0] < rows or q_out.shape[1] != nq or q_out.stride(1) != 1 \
+                or q_out.get_device() != dev:
+            raise ValueError("q_out must be fp32 [rows][q columns], its rows contiguous")
+    except AttributeError as e:
+        raise _kind(e, tiles=(("x", x),), tensors=(("rope", rope), ("row_slot", row_slot), ("row_pos", row_pos)), given=(("q_out", q_out),))
     p = _QKV(rows, (rows + 15) // 16, 0, 0, xr, *ws, q_out.data_ptr(), q_out.stride(0) if rows > 1 else nq,
              bytes(kv.ref), rope.data_ptr(), row_slot.data_ptr(), row_pos.data_ptr(), layer, head_dim)
     rc = _lib.packed().stride_mx_qkv_within(p, kv.table.shape[0], rope.shape[0], stream)
