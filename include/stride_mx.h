@@ -99,7 +99,8 @@ typedef struct StrideMxGemmParams {
 
 int stride_mx_gemm(const StrideMxGemmParams* p, void* stream);
 
-/* z = silu(W1 x) * (W3 x) in 8 bits, 16 * w1.tiles columns. */
+/* z = silu(W1 x) * (W3 x) in 8 bits, 16 * w1.tiles columns. silu is 0 where 1 + e^-x leaves fp32 (below
+ * -88.7; from -87.3 on, where 1 / (1 + e^-x) is no normal number, it may be). */
 typedef struct StrideMxMlp13Params {
   StrideLanes l;
   StrideMxTiles x, w1, w3, z;
