@@ -3,14 +3,19 @@
 //
 // Every kernel evaluates the same expression: the chunks of 128 columns chain in ascending order from
 // zero on, so a row has the same bits whatever the batch and the kernel. One chain and no splits of K:
-// few rows leave a chain of K / 128 products to a wave (1 us at K = 8192, of 5), and in exchange many
-// rows keep one accumulator a tile; with four splits and their running sums the registers spilled
-// (2048 x 8192 at 4096 rows 172 us, 54 without).
+// few rows leave a chain of K / 128 products to a wave (1 us at K = 8192, of 5.2), and in exchange many
+// rows keep one accumulator a tile. (Four splits and their running sums were measured in the four-wave
+// form of 256 x 128 alone, whose 128 accumulators a lane they made spill: 172 us against 54 at 4096 rows
+// of 2048 x 8192. The eight-wave form that is here now has 64, and has not been measured with splits.)
 //
-// What bounds them: few rows the reads of weights and the launch (2048 x 8192 at one row 5.2 us, of
-// which an empty launch is 2), the middle the x that each tile of weights reads again from L2, many rows
-// the matrix units and the power that they draw: 2.85 PFLOP/s at 2048 x 8192 and 4096 rows, 85 % of the
-// units' cycles within the loop at 1.7 to 1.95 GHz, where a library's 8192^3 product in 8 bits reaches 2.96.
+// Times beside the kernels are us a call in a graph of calls on up to eight different matrices.
+//
+// What bounds them: few rows what one wave a CU has on its way, and the launch (2048 x 8192 at one row
+// 5.2 us, of which an empty launch is 2: 128 waves read 68 KiB each, in two rounds of four groups), the
+// middle the x that each tile of weights reads again from L2, many rows the matrix units and the power that
+// they draw: 2.7 PFLOP/s at 2048 x 8192 and 4096 rows (51.7 us; 2.8 in calls one by one), with the units at
+// work for 76 % of the cycles, of which there are 1.7 a ns, where a library's 8192^3 product in 8 bits
+// reaches 2.96.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -79,8 +84,9 @@ struct EpiRope {
 };
 
 // x / (1 + e^-x) with the hardware's exponential and reciprocal, each good to an ulp or so: the result
-// is rounded to four bits. (2048 rows of 2 x 8192 x 2048: 70 us, 93 with the exact division and the
-// polynomial that the bf16 path has for its bits.)
+// is rounded to four bits. 0 where 1 / (1 + e^-x) is no normal number, x below -87.3. (2048 rows of
+// 2 x 8192 x 2048: 58.6 us, 68.7 with the exact division and the polynomial that the bf16 path has for its
+// bits.)
 __device__ __forceinline__ float silu(float x) {
   return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504088896341f));
 }
@@ -140,7 +146,7 @@ __device__ __forceinline__ void mx_source(const MxGeometry& g, int m, int rt, co
 }
 
 // Few output tiles: a wave has one weight tile by one lane tile, operands straight to registers, P
-// groups of K in use and P on their way (2048 x 8192 at one row with P = 4 / 2: 5.2 / 6.4 us). The tiles
+// groups of K in use and P on their way (2048 x 8192 at one row with P = 4 / 2: 5.2 / 6.5 us). The tiles
 // of a unit meet in LDS.
 template <class Epi, int P>
 __global__ __launch_bounds__(64 * Epi::kMats * Epi::kUnit) void k_mx_row(MxGeometry g, typename Epi::Out o, int units) {
@@ -227,9 +233,10 @@ __device__ __forceinline__ uint32_t lds_at(const void* p) {
 // Many rows: workgroup of WM x WN waves, A weight tiles by L lane tiles a wave. A chunk's operands
 // (weights 1 KiB, activations 2 KiB a tile) go to a ring of NS stages in LDS by global_load_lds, a
 // group's scales beside its first chunk; a wave reads a chunk's fragments while it multiplies the one
-// before. Copies and reads lie between the products: issued together behind the barrier they cost 1760
-// cycles a chunk of 256 x 128 tiles, spread 1200, of which the matrix units work 1024. (A raised wave
-// priority in the loop changed nothing.)
+// before. Copies and reads lie between the products: issued together behind the barrier a chunk of 256 x 128
+// by four waves took 1760 cycles, spread 1200, of which the matrix units work 1024; by eight waves, which
+// cover each other's waits too, the whole product takes 51.7 us against 53.0. (A raised wave priority in the
+// loop changed nothing.)
 template <class Epi, int A, int L, int WM, int WN, int NS, int OCC>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void k_mx_pipe(MxGeometry g, typename Epi::Out o, int units, int unit_blocks, int lane_blocks) {
   constexpr int M = Epi::kMats, U = Epi::kUnit, NW = WM * WN;
@@ -404,7 +411,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_mx_pipe(MxGeometry g, typ
 
 // In between: workgroup of 2 x 2 waves, a weight tile by a lane tile each; a group of 512 columns is a
 // stage of a ring of three, two of them on their way (a chunk a stage as above has too little on its way
-// for such small tiles: 2048 x 8192 at 128 rows 17 us as 128 x 64, 8.3 here). One matrix at a time:
+// for such small tiles: 2048 x 8192 at 128 rows 12.5 us as 64 x 64, 8.1 here). One matrix at a time:
 // gate and up, whose unit is 32 x 32 of each, go from waves of their own to 64 x 64.
 template <class Epi>
 __global__ __launch_bounds__(256) void k_mx_tile(MxGeometry g, typename Epi::Out o, int units, int lane_blocks) {
@@ -506,22 +513,28 @@ int run(const char* what, const MxGeometry& g, const typename Epi::Out& o, int r
   // z is written to the end of its last group of 512 columns
   const int units = Epi::kUnit == 2 ? mx_groups(row_tiles * 16) * (kMxGroup / kMxBlock) : row_tiles;
   // configuration
-  // By the number of 16 x 16 products, of which the card's 256 CUs want four each before tiles pay.
-  // Measured at 1 to 4096 rows of weights from 512 x 512 to 14336 x 4096, us here / as the next form:
+  // By the number of 16 x 16 products, of which the card's 256 CUs want four each before tiles pay. us
+  // here / as the other forms, with 4 groups at K = 2048, 16 at 8192 and 28 at 14336; where a border lies
+  // between two sizes measured, it may be a few per cent off for sizes near it:
   //   a wave a tile to 768 (1536 where K is short; gate and up, which have no 32 x 32: 1280): 2048 x
-  //     8192 at 1 / 64 rows 5.2 / 6.9 against 10 / 8.2 as 32 x 32, at 128 rows 9.6 against 8.3; 8192 x
-  //     2048 at 32 rows 4.1 against 4.9; gate and up 8192 x 2048 at 16 / 32 rows 5.6 / 7.1 against
-  //     6.2 / 6.3 as 64 x 64
-  //   32 x 32 to 1536: 4096 x 14336 at 64 rows 12.1 against 19 as 64 x 64
-  //   64 x 64 to 6144: 2048 x 8192 at 512 rows 13.6 against 15.4 as 128 x 64, at 1024 21.3 against 17.9
-  //   128 x 64 to 9216: 2048 x 8192 at 1024 rows 17.9 against 23.1 as 128 x 128, at 1280 27.2 against 24.4
-  //   128 x 128 of eight waves, by a workgroup a CU while 256 do: 2048 x 8192 at 2048 rows 29 against 32
-  //     by two and 40 as 256 x 128; by four waves 35
-  //   beyond, where K is short, by two workgroups a CU, whose ends hide each other: 8192 x 2048 at 2048
-  //     rows 33.6 against 35.2 as 256 x 128, gate and up 57.5 against 59; by four waves 36.7 and 60.5
+  //     8192 at 1 / 64 rows (128, 512 products) 5.2 / 6.9 against 7.6 / 7.7 as 32 x 32, at 128 rows (1024) 9.7
+  //     against 8.1; 8192 x 2048 at 32 rows (1024) 4.0 against 4.9, 2048 x 2048 at 128 / 192 rows (1024, 1536)
+  //     4.0 / 6.0 against 4.2 / 5.2; gate and up 8192 x 2048 at 16 / 32 rows (1024, 2048) 5.6 / 6.9 against
+  //     6.1 / 6.3 as 64 x 64
+  //   32 x 32 to 1536: 2048 x 8192 at 128 / 192 rows (1024, 1536) 8.1 / 11.3 against 12.5 as 64 x 64, at
+  //     256 / 384 rows 12.1 / 17.1 against 12.6 / 13.1; 4096 x 14336 at 64 rows (1024) 12.4 against 19.4
+  //   64 x 64 to 6144: 8192 x 2048 at 96 rows 6.1 against 7.4 as 32 x 32; 2048 x 8192 at 512 rows (4096) 13.9
+  //     against 15.6 as 128 x 64, but at 768 (6144) 19.4 against 16.3, and at 1024 20.9 against 17.6
+  //   128 x 64 to 9216: 2048 x 8192 at 1024 rows (8192) 17.6 against 21.6 as 128 x 128, at 1280 25.8 against
+  //     22.6; gate and up 8192 x 2048 at 128 rows (8192) 7.6 against 8.0 as 64 x 64
+  //   128 x 128 of eight waves, by a workgroup a CU while 256 do: 2048 x 8192 at 2048 rows (16384) 29.9 against
+  //     31.2 by two, 33.6 as 128 x 64 and 40.7 as 256 x 128; gate and up at 256 rows 10.3 against 10.5 by two
+  //   beyond, where K is short, by two workgroups a CU, whose ends hide each other: 8192 x 2048 at 2048 / 4096
+  //     rows 35.8 / 68.8 against 35.9 / 70.9 as 256 x 128, gate and up at 2048 rows 58.6 against 60.7; by four
+  //     waves 46.7 and 73.1
   //   256 x 128 where K is long: the fewest bytes a product, of which a CU reads 75 to 80 a ns from its
-  //     L2, and by which the clock stays up: 2048 x 8192 at 4096 rows 50.4 against 57.3 as 128 x 128, 4096
-  //     x 14336 160 against 181; by four waves, one a SIMD, 52.4 and 165
+  //     L2, and by which the clock stays up: 2048 x 8192 at 4096 rows 51.7 against 58.4 as 128 x 128, 4096
+  //     x 14336 163 against 184; by four waves, one a SIMD, 53.0 and 164
   const int64_t products = static_cast<int64_t>(row_tiles) * Epi::kMats * g.lane_groups;
   if (clash && products <= 1536) return mx_refused(what, clash);  // a launch of these fits
   const char* why = nullptr;

@@ -85,8 +85,8 @@ __global__ __launch_bounds__(256) void k_quantize(const T* src, StrideMxTiles ou
 }
 
 // Workgroup: C chunks of a tile, a whole group or one; a wave has four rows, a lane 8 columns of one in
-// each. (16384 x 2048 from 4 bits to bf16 with C = 4 / 1: 17.6 / 20.2 us, 4.8 TB/s; 1008 x 1040 4.2 /
-// 3.7: a group's worth of stores pays where workgroups are many.)
+// each. (16384 x 2048 from 4 bits to bf16 with C = 4 / 1: 17.6 / 20.2 us of GPU, 4.8 TB/s; 1008 x 1040 4.2 /
+// 3.7 a call in a graph: a group's worth of stores pays where workgroups are many.)
 template <int BITS, class T, int C>
 __global__ __launch_bounds__(256) void k_dequantize(StrideMxTiles in, T* out, int64_t stride, int rows, int groups) {
   const int all = groups * (4 / C), g = blockIdx.x % all / (4 / C), first = blockIdx.x % (4 / C), t = blockIdx.x / all;
@@ -350,10 +350,13 @@ int stride_mx_norm(const StrideMxNormParams* p, void* stream) {
   const int chunks = mx_groups(p->dim) * 4;
   hipStream_t st = static_cast<hipStream_t>(stream);
   // A row a workgroup while each can have a CU, and two while two rows can, four where the memory is
-  // full either way: neighbouring rows share their lines, from one XCD's L2 or in one workgroup (us at
-  // R = 1 / 2 / 4 with an addition: 1 x 2048 2.7 / 2.9 / 3.6, 256 x 8192 7.6 / 9.1 / 11.8, 333 x 8192 11.0 /
-  // 9.8 / 12.2, 512 x 4096 7.5 / 7.4 / 8.2, 1024 x 4096 12.2 / 11.4 / 10.1, 4096 x 2048 25.2 / 22.7 / 19.9,
-  // 92 MB: 4.7 TB/s, a 4 GiB copy's 4.8; dealt out over the XCDs in turn 256 x 8192 takes 11.8 at R = 1).
+  // full either way: neighbouring rows share their lines, from one XCD's L2 or in one workgroup (us a call
+  // in a graph of calls on other rows, at R = 1 / 2 / 4 with an addition: 1 x 2048 2.7 / 2.9 / 3.6, 256 x 8192
+  // 7.6 / 9.1 / 11.8, 333 x 8192 11.0 / 9.8 / 12.2, 512 x 4096 7.5 / 7.4 / 8.2, 1024 x 4096 12.2 / 11.4 / 10.1,
+  // 4096 x 2048 25.2 / 22.7 / 19.9, 92 MB: 4.7 TB/s, a 4 GiB copy's 4.8; dealt out over the XCDs in turn
+  // 256 x 8192 takes 11.8 at R = 1). More than 512 rows of more than 8192 columns leave no registers at
+  // R = 4, and h is read twice: 1024 x 16384 49.5 us of GPU, where its bytes take 38.6; two rows a workgroup
+  // would hold 16384 columns, and are not measured there.
   if (p->l.rows <= 256) launch_norm<1>(*p, chunks, st);
   else if (p->l.rows <= 512) launch_norm<2>(*p, chunks, st);
   else launch_norm<4>(*p, chunks, st);
