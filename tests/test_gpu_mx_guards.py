@@ -135,3 +135,25 @@ def test_arguments_of_another_kind_are_refused_by_a_message():
                          lambda rows=rows: mx.norm(h, rows, gain, 1e-5, bits=16), lambda rows=rows: mx.qkv(**{**good, "rows": rows})))):
         with pytest.raises(ValueError, match=why):
             bad()
+
+
+@pytest.mark.parametrize("m,n", [(3, 48), (260, 1040), (520, 1040), (1100, 2064)])
+def test_the_longest_rows(m, n):
+    """K = 2^20 in each kind of product: small whole numbers, whose sums fp32 holds exactly (2^20 products of
+    at most 18, of either sign: far below 2^24), so that y is the exact sum rounded once; and their blocks
+    there and back."""
+    print("longest", m, n, flush=True)
+    k = 1 << 20
+    gen = torch.Generator(device=DEV).manual_seed(m)
+    ints = lambda rows, most: torch.randint(-most, most + 1, (rows, k), generator=gen, device=DEV, dtype=torch.int8)
+    a, b = ints(n, 3), ints(m, 6)  # e2m1 has all of these, e4m3 too
+    tiles = lambda v: layout.lane_tiles(v.to(torch.bfloat16))
+    w, x = mx.quantize(tiles(a)), mx.quantize(tiles(b), m, bits=8)
+    y = layout.untile_lanes(mx.gemm(w, x, m), m).view(torch.bfloat16)
+    want = torch.zeros((m, n), dtype=torch.float64, device=DEV)
+    for at in range(0, k, 1 << 15):  # float32 holds each part exactly
+        want += (b[:, at:at + (1 << 15)].float() @ a[:, at:at + (1 << 15)].float().t()).double()
+    assert want.abs().max() < 2 ** 24 and torch.equal(y, want.float().to(torch.bfloat16))
+    for t, v in ((w, a), (x, b)):
+        rows = min(64, len(v))
+        assert torch.equal(mx.dequantize(t, rows), v[:rows].to(torch.bfloat16))
