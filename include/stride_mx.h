@@ -130,7 +130,7 @@ typedef struct StrideMxQkvParams {
 int stride_mx_qkv(const StrideMxQkvParams* p, void* stream);
 
 /* The same with a page table of `slots` rows and a rope table of `positions`: rows beyond either are
- * left out too, so that no row_slot or row_pos is read or written behind an end. */
+ * left out too, so that neither table is read behind its end. */
 int stride_mx_qkv_within(const StrideMxQkvParams* p, int32_t slots, int32_t positions, void* stream);
 
 #ifdef __cplusplus
